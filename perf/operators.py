@@ -1,0 +1,293 @@
+"""The measured cases of three operators: layer norm, the linear layer with bias, activation and residual in its epilogue, and the
+Muon update (momentum, orthogonalisation by Newton-Schulz products, step).
+
+`own` false: the operators from elementary torch operations in 32 bits.  `own` true: the framework's entry points (fneus.ops)."""
+import functools
+import math
+import os
+import sys
+
+import torch
+
+own = False
+
+TYPES = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
+BYTES = {"fp32": 4, "bf16": 2, "fp16": 2}
+EPS = 1e-5                                   # layer norm
+NS = (3.4445, -4.7750, 2.0315)               # the quintic's coefficients
+NS_EPS, MOMENTUM, LR, DECAY = 1e-7, 0.95, 0.02, 0.01
+
+
+def _ln(name, direction, dtype, rows, n):
+    return dict(name=name, op="layer_norm", direction=direction, dtype=dtype, rows=rows, n=n)
+
+
+def _lin(name, direction, dtype, rows, n_in, n_out, act, residual):
+    return dict(name=name, op="linear", direction=direction, dtype=dtype, rows=rows, n_in=n_in, n_out=n_out, act=act, residual=residual)
+
+
+def listed():
+    return [
+        _ln("ln_fwd_row", "fwd", "bf16", 1, 4096),                     # one token of a wide model: the call's latency
+        _ln("ln_fwd_wide", "fwd", "bf16", 8192, 8192),                 # a long batch of wide rows: bandwidth
+        _ln("ln_train_samples", "train", "fp32", 65536, 256),          # 512 rays x 128 samples of this framework's width
+        _ln("ln_train_odd", "train", "fp16", 4099, 1031),              # a ragged batch of odd width
+        _lin("lin_fwd_row", "fwd", "bf16", 1, 4096, 4096, "silu", True),             # one token: reading the weight
+        _lin("lin_train_layer", "train", "fp32", 512, 512, 512, "relu", True),       # a hidden layer of IndirectLight, 512 rays
+        _lin("lin_train_samples", "train", "fp32", 65536, 256, 256, "relu", True),   # every sample of a 512-ray batch
+        _lin("lin_train_odd", "train", "fp16", 1999, 777, 1111, "gelu", False),      # odd in every direction
+        _lin("lin_train_large", "train", "bf16", 8192, 4096, 8192, "gelu", True),    # a wide layer of a large model
+        dict(name="muon_stack", op="muon", dtype="fp32", count=8, rows=256, cols=256),      # the SDF network's hidden layers
+        dict(name="ns_tall", op="newton_schulz", dtype="bf16", count=4, rows=4096, cols=1024),  # projections of a large model
+        dict(name="muon_large", op="muon", dtype="fp32", count=1, rows=4096, cols=4096),    # one square layer of a large model
+    ]
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    op = rng.choice(["layer_norm", "layer_norm", "linear", "linear", "linear", "muon", "newton_schulz"])
+    dtype = rng.choice(["fp32", "bf16", "fp16"])
+    direction = rng.choice(["fwd", "train"])
+    if op == "layer_norm":
+        n = _log(rng, 16, 16384)
+        return dict(op=op, direction=direction, dtype=dtype, rows=_log(rng, 1, min(262144, 64 * 2 ** 20 // n)), n=n)
+    if op == "linear":
+        rows, n_in = _log(rng, 1, 65536), _log(rng, 1, 8192)
+        n_out = _log(rng, 1, max(1, min(8192, 2 ** 34 // (rows * n_in), 2 ** 26 // rows)))
+        return dict(op=op, direction=direction, dtype=dtype, rows=rows, n_in=n_in, n_out=n_out,
+                    act=rng.choice(["none", "relu", "leaky", "sigmoid", "softplus", "gelu", "silu"]), residual=rng.random() < 0.5)
+    rows, cols = _log(rng, 2, 4096), _log(rng, 2, 4096)
+    count = _log(rng, 1, max(1, min(24, 2 ** 23 // (rows * cols))))
+    return dict(op=op, dtype="fp32" if op == "muon" else rng.choice(["fp32", "bf16"]), count=count, rows=rows, cols=cols)
+
+
+def work(case):
+    w = BYTES[case["dtype"]]
+    if case["op"] == "layer_norm":
+        e, n = case["rows"] * case["n"], case["n"]
+        if case["direction"] == "fwd":
+            return {"bytes": 2 * e * w + 2 * n * w + 8 * case["rows"], "flops": 8 * e}
+        return {"bytes": 4 * e * w + 4 * n * w + 8 * case["rows"], "flops": 22 * e}
+    if case["op"] == "linear":
+        m, k, n = case["rows"], case["n_in"], case["n_out"]
+        fwd = m * k + n * k + n + m * n * (2 if case["residual"] else 1)
+        if case["direction"] == "fwd":
+            return {"bytes": w * fwd, "flops": 2 * m * n * k}
+        return {"bytes": w * (fwd + m * n + m * k + n * k + n), "flops": 6 * m * n * k}
+    s, l = sorted((case["rows"], case["cols"]))
+    e = case["count"] * s * l
+    flops = 5 * case["count"] * (s * s * l + s * s * s + 2 * s * s * l)      # the two symmetric products by half
+    return {"bytes": (5 if case["op"] == "muon" else 2) * w * e, "flops": flops}
+
+
+def _gradient(g, count, rows, cols, device):
+    """a gradient's spectrum: noise whose rows and columns differ in scale by an order of magnitude"""
+    r = torch.randn(count, rows, 1, generator=g, device=device) * 0.7
+    c = torch.randn(count, 1, cols, generator=g, device=device) * 0.7
+    return torch.randn(count, rows, cols, generator=g, device=device) * torch.exp(r + c) * 1e-3
+
+
+def prepare(case, seed):
+    dev = torch.device("cuda")
+    g = torch.Generator(device=dev)
+    g.manual_seed(int(seed))
+    t = TYPES[case["dtype"]]
+    rnd = lambda *s: torch.randn(*s, generator=g, device=dev)  # noqa: E731
+    s = dict(case)
+    if case["op"] == "layer_norm":
+        rows, n = case["rows"], case["n"]
+        s["x"] = (rnd(rows, n) * (0.5 + torch.rand(rows, 1, generator=g, device=dev)) + 0.5 * rnd(rows, 1)).to(t)
+        s["weight"], s["bias"] = (1.0 + 0.2 * rnd(n)).to(t), (0.2 * rnd(n)).to(t)
+        if case["direction"] == "train":
+            s["dy"] = rnd(rows, n).to(t)
+    elif case["op"] == "linear":
+        m, k, n = case["rows"], case["n_in"], case["n_out"]
+        s["x"], s["weight"], s["bias"] = rnd(m, k).to(t), (rnd(n, k) / math.sqrt(k)).to(t), (0.2 * rnd(n)).to(t)
+        s["residual_in"] = rnd(m, n).to(t) if case["residual"] else None
+        if case["direction"] == "train":
+            s["dy"] = rnd(m, n).to(t)
+    else:
+        count, rows, cols = case["count"], case["rows"], case["cols"]
+        s["grad"] = _gradient(g, count, rows, cols, dev).to(t)
+        if case["op"] == "muon":
+            s["param"] = (rnd(count, rows, cols) / math.sqrt(cols)).to(t)
+            s["momentum"] = _gradient(g, count, rows, cols, dev).to(t)
+            s["lr"] = torch.full((), LR, device=dev)
+            for k in ("grad", "param", "momentum"):
+                s[k + "s"] = list(s[k].unbind(0))
+    return s
+
+
+# ---- plain forms: 32 bits, rounded once ------------------------------------------------------------------------------------
+def _act(z, act):
+    if act == "relu":
+        return torch.where(z > 0, z, torch.zeros_like(z))
+    if act == "leaky":
+        return torch.where(z > 0, z, 0.2 * z)
+    if act == "sigmoid":
+        return torch.sigmoid(z)
+    if act == "softplus":
+        return torch.clamp(z, min=0) + torch.log1p(torch.exp(-100.0 * z.abs())) / 100.0
+    if act == "gelu":
+        return 0.5 * z * (1.0 + torch.erf(z * math.sqrt(0.5)))
+    if act == "silu":
+        return z * torch.sigmoid(z)
+    return z
+
+
+def _dact(z, act):
+    if act == "relu":
+        return (z > 0).to(z.dtype)
+    if act == "leaky":
+        return torch.where(z > 0, torch.ones_like(z), torch.full_like(z, 0.2))
+    if act == "sigmoid":
+        s = torch.sigmoid(z)
+        return s * (1.0 - s)
+    if act == "softplus":
+        return torch.sigmoid(100.0 * z)
+    if act == "gelu":
+        return 0.5 * (1.0 + torch.erf(z * math.sqrt(0.5))) + z * torch.exp(-0.5 * z * z) * (1.0 / math.sqrt(2.0 * math.pi))
+    if act == "silu":
+        s = torch.sigmoid(z)
+        return s * (1.0 + z * (1.0 - s))
+    return torch.ones_like(z)
+
+
+def _plain_layer_norm(s):
+    t = TYPES[s["dtype"]]
+    x, w, b = s["x"].float(), s["weight"].float(), s["bias"].float()
+    mean = x.mean(dim=1, keepdim=True)
+    xc = x - mean
+    rstd = torch.rsqrt((xc * xc).mean(dim=1, keepdim=True) + EPS)
+    xh = xc * rstd
+    y = (xh * w + b).to(t)
+    if s["direction"] == "fwd":
+        return y, mean[:, 0], rstd[:, 0]
+    dy = s["dy"].float()
+    g = dy * w
+    dx = rstd * (g - g.mean(dim=1, keepdim=True) - xh * (g * xh).mean(dim=1, keepdim=True))
+    return y, mean[:, 0], rstd[:, 0], dx.to(t), (dy * xh).sum(dim=0).to(t), dy.sum(dim=0).to(t)
+
+
+def _plain_linear(s):
+    t = TYPES[s["dtype"]]
+    x, w = s["x"].float(), s["weight"].float()
+    z = x @ w.t() + s["bias"].float()
+    y = _act(z, s["act"])
+    if s["residual_in"] is not None:
+        y = y + s["residual_in"].float()
+    if s["direction"] == "fwd":
+        return (y.to(t),)
+    d = s["dy"].float() * _dact(z, s["act"])
+    return y.to(t), (d @ w).to(t), (d.t() @ x).to(t), d.sum(dim=0).to(t)
+
+
+def _ns_step(x):
+    a = x @ x.transpose(1, 2)
+    return NS[0] * x + (NS[1] * a + NS[2] * (a @ a)) @ x
+
+
+def _plain_ns(u):
+    x = u / torch.clamp(torch.sqrt((u * u).sum(dim=(1, 2), keepdim=True)), min=NS_EPS)
+    x = x.transpose(1, 2) if u.shape[1] > u.shape[2] else x
+    x = _ns_step(_ns_step(_ns_step(_ns_step(_ns_step(x)))))
+    return x.transpose(1, 2) if u.shape[1] > u.shape[2] else x
+
+
+def _adjust(rows, cols):
+    return 0.2 * math.sqrt(max(rows, cols))              # the update's rms as Adam's
+
+
+def _plain_muon(s):
+    g, p, m = s["grad"].float(), s["param"], s["momentum"]
+    m.copy_(MOMENTUM * m.float() + (1.0 - MOMENTUM) * g)
+    o = _plain_ns((1.0 - MOMENTUM) * g + MOMENTUM * m.float())
+    p.copy_(p.float() * (1.0 - s["lr"] * DECAY) - s["lr"] * _adjust(s["rows"], s["cols"]) * o)
+    return p, m
+
+
+# ---- the framework's entry points ------------------------------------------------------------------------------------------
+@functools.lru_cache(maxsize=None)
+def _ops():
+    at = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "factored-neus_amd")
+    if at not in sys.path:
+        sys.path.insert(1, at)
+    from fneus import ops
+    return ops
+
+
+def _own(s):
+    ops = _ops()
+    if s["op"] == "layer_norm":
+        y, mean, rstd = ops.layer_norm_fwd(s["x"], s["weight"], s["bias"], EPS)
+        if s["direction"] == "fwd":
+            return y, mean, rstd
+        return (y, mean, rstd) + ops.layer_norm_bwd(s["dy"], s["x"], s["weight"], mean, rstd)
+    if s["op"] == "linear":
+        train = s["direction"] == "train"
+        y, z = ops.linear_fwd(s["x"], s["weight"], s["bias"], act=s["act"], residual=s["residual_in"], train=train)
+        if not train:
+            return (y,)
+        return (y,) + ops.linear_bwd(s["dy"], s["x"], s["weight"], z, act=s["act"])
+    if s["op"] == "newton_schulz":
+        return ops.newton_schulz(s["grad"], coefficients=NS, steps=5, eps=NS_EPS)
+    ops.muon_step(s["params"], s["grads"], s["momentums"], s["lr"], momentum=MOMENTUM, nesterov=True, weight_decay=DECAY,
+                  adjust="match_rms", coefficients=NS, steps=5, eps=NS_EPS)
+    return s["param"], s["momentum"]
+
+
+def run(state):
+    if own:
+        return _own(state)
+    if state["op"] == "layer_norm":
+        return _plain_layer_norm(state)
+    if state["op"] == "linear":
+        return _plain_linear(state)
+    if state["op"] == "newton_schulz":
+        return _plain_ns(state["grad"].float()).to(TYPES[state["dtype"]])
+    return _plain_muon(state)
+
+
+# ---- 64 bits, from the definitions: gradients by differentiation, the orthogonalisation through the other Gram matrix ------------
+def _exact_act(z, act):
+    f = torch.nn.functional
+    return {"none": lambda: z, "relu": lambda: f.relu(z), "leaky": lambda: f.leaky_relu(z, 0.2), "sigmoid": lambda: torch.sigmoid(z),
+            "softplus": lambda: torch.logaddexp(torch.zeros_like(z), 100.0 * z) / 100.0,
+            "gelu": lambda: z * torch.special.ndtr(z), "silu": lambda: z / (1.0 + torch.exp(-z))}[act]()
+
+
+def _exact_ns(u):
+    x = u / torch.clamp(torch.linalg.matrix_norm(u, keepdim=True), min=NS_EPS)
+    if u.shape[1] < u.shape[2]:
+        x = x.transpose(1, 2)
+    eye = torch.eye(x.shape[2], dtype=x.dtype, device=x.device)
+    for _ in range(5):
+        gram = x.transpose(1, 2) @ x
+        x = x @ (NS[0] * eye + gram @ (NS[1] * eye + NS[2] * gram))
+    return x.transpose(1, 2) if u.shape[1] < u.shape[2] else x
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    d = lambda k: s[k].double()  # noqa: E731
+    if case["op"] == "layer_norm":
+        x, w, b = d("x").requires_grad_(), d("weight").requires_grad_(), d("bias").requires_grad_()
+        var, mean = torch.var_mean(x, dim=1, correction=0, keepdim=True)
+        y = (x - mean) / torch.sqrt(var + EPS) * w + b
+        first = (y.detach(), mean.detach()[:, 0], 1.0 / torch.sqrt(var.detach()[:, 0] + EPS))
+        return first if case["direction"] == "fwd" else first + torch.autograd.grad(y, (x, w, b), d("dy"))
+    if case["op"] == "linear":
+        x, w, b = d("x").requires_grad_(), d("weight").requires_grad_(), d("bias").requires_grad_()
+        y = _exact_act(torch.addmm(b, x, w.t()), case["act"])
+        if s["residual_in"] is not None:
+            y = y + d("residual_in")
+        return (y.detach(),) if case["direction"] == "fwd" else (y.detach(),) + torch.autograd.grad(y, (x, w, b), d("dy"))
+    if case["op"] == "newton_schulz":
+        return _exact_ns(d("grad"))
+    m = MOMENTUM * d("momentum") + (1.0 - MOMENTUM) * d("grad")
+    lr = float(s["lr"])
+    o = _exact_ns((1.0 - MOMENTUM) * d("grad") + MOMENTUM * m)
+    return d("param") * (1.0 - lr * DECAY) - lr * _adjust(case["rows"], case["cols"]) * o, m
