@@ -1,0 +1,93 @@
+// Activations of the linear layer's epilogue and their derivatives, in fp32 (linear_kernels.hip).
+// Codes: 0 none, 1 ReLU, 2 LeakyReLU(0.2), 3 sigmoid (fneus_mlp_*'s), 4 softplus(beta 100) (the SDF network's), 5 GELU (erf), 6 SiLU.
+#pragma once
+#include "fneus_types.h"
+
+namespace fneus {
+
+constexpr int kLinActs = 7;
+
+FN_DEV float lin_sigmoid(float z) { return 1.0f / (1.0f + expf(-z)); }
+
+FN_DEV float lin_act(float z, int act) {
+    switch (act) {
+        case 1: return z > 0.0f ? z : (z != z ? z : 0.0f);
+        case 2: return z > 0.0f ? z : 0.2f * z;
+        case 3: return lin_sigmoid(z);
+        case 4: return fmaxf(z, 0.0f) + log1pf(expf(-100.0f * fabsf(z))) * 0.01f + (z != z ? z : 0.0f);
+        case 5: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+        case 6: return z * lin_sigmoid(z);
+        default: return z;
+    }
+}
+
+// act'(z); at 0 the ReLUs take the slope of the negative side
+FN_DEV float lin_dact(float z, int act) {
+    switch (act) {
+        case 1: return z > 0.0f ? 1.0f : 0.0f;
+        case 2: return z > 0.0f ? 1.0f : 0.2f;
+        case 3: { const float s = lin_sigmoid(z); return s * (1.0f - s); }
+        case 4: return lin_sigmoid(100.0f * z);
+        case 5: return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * (0.39894228040143268f * expf(-0.5f * z * z));
+        case 6: { const float s = lin_sigmoid(z); return s * (1.0f + z * (1.0f - s)); }
+        default: return 1.0f;
+    }
+}
+
+// Operands of the 32x32x16 / 16x16x32 matrix instructions: 8 consecutive values of the contraction a lane.  bf16 and fp16 enter as
+// they are.  An fp32 value enters as THREE bf16 terms x = t0 + t1 + t2 (each the rounding of what is left: 24 bits, the whole range of
+// fp32), a product as the six term pairs down to 2^-24 of it, smallest first: fp32's accuracy at 6 bf16 MFMAs (16 k in 192 cycles; the
+// fp32 MFMA takes 512).  An infinity has NaN as its second term, so it comes out as NaN.
+template <class T> struct LinFrag;
+template <> struct LinFrag<__bf16> { bf16x8 t; };
+template <> struct LinFrag<_Float16> { fn_f16x8 t; };
+template <> struct LinFrag<float> { bf16x8 t0, t1, t2; };
+
+FN_DEV void lin_frag(const float (&v)[8], LinFrag<__bf16>& f) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f.t[k] = (__bf16)v[k];
+}
+FN_DEV void lin_frag(const float (&v)[8], LinFrag<_Float16>& f) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f.t[k] = (_Float16)v[k];
+}
+FN_DEV void lin_frag(const float (&v)[8], LinFrag<float>& f) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        f.t0[k] = (__bf16)v[k];
+        const float r = v[k] - (float)f.t0[k];
+        f.t1[k] = (__bf16)r;
+        f.t2[k] = (__bf16)(r - (float)f.t1[k]);
+    }
+}
+
+FN_DEV f32x16 lin_mfma32(const LinFrag<__bf16>& a, const LinFrag<__bf16>& b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.t, b.t, c, 0, 0, 0);
+}
+FN_DEV f32x16 lin_mfma32(const LinFrag<_Float16>& a, const LinFrag<_Float16>& b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a.t, b.t, c, 0, 0, 0);
+}
+FN_DEV f32x16 lin_mfma32(const LinFrag<float>& a, const LinFrag<float>& b, f32x16 c) {
+    c = mfma32(a.t2, b.t0, c);
+    c = mfma32(a.t0, b.t2, c);
+    c = mfma32(a.t1, b.t1, c);
+    c = mfma32(a.t1, b.t0, c);
+    c = mfma32(a.t0, b.t1, c);
+    return mfma32(a.t0, b.t0, c);
+}
+FN_DEV f32x4 lin_mfma16(const LinFrag<__bf16>& a, const LinFrag<__bf16>& b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.t, b.t, c, 0, 0, 0);
+}
+FN_DEV f32x4 lin_mfma16(const LinFrag<_Float16>& a, const LinFrag<_Float16>& b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a.t, b.t, c, 0, 0, 0);
+}
+FN_DEV f32x4 lin_mfma16(const LinFrag<float>& a, const LinFrag<float>& b, f32x4 c) {
+    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.t2, b.t0, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.t0, b.t2, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.t1, b.t1, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.t1, b.t0, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.t0, b.t1, c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.t0, b.t0, c, 0, 0, 0);
+}
+
+}  // namespace fneus

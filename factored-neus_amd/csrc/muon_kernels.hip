@@ -1,0 +1,447 @@
+// The Muon update of weight matrices: momentum, orthogonalisation by Newton-Schulz products, step -- every matrix of a model in the same
+// 2 + 3 * steps launches.  For each matrix u, as X [m][n] with m <= n (the transpose where rows > cols):
+//   X = u / max(|u|_F, eps);   steps times:  A = X X^T,  B = b A + c A A,  X <- a X + B X
+// All three products run on the tiled engine (mm_engine.h), whose operands lie along k: X and its transpose are both kept (the epilogue
+// writes the two), A and B are symmetric.
+//
+// Numbers: fp16 planes with fp32 sums.  Every entry of X, A and B is bounded (the polynomial keeps the singular values below about 1.2),
+// entries as small as 1 / n matter, and the fp16 matrix instruction takes subnormal operands as zero, so a plane holds its matrix times a
+// power of two that puts the bound just below fp16's largest value (2^14 for the usual coefficients).  prec 2: one plane, 11 bits -- the
+// error that 16-bit gradients bring along, an eighth of what bf16 operands would add.  prec 3: a second plane holds what the first one's
+// rounding left, times another 2^11, so that it is as normal as the first; products hi hi + hi lo + lo hi (22 bits: fp32's accuracy at
+// half the matrix work of three bf16 terms).
+#include <math.h>
+#include "mm_engine.h"
+#include "fneus_kernels.h"
+
+namespace fneus {
+
+constexpr int kMuonMaxJobs = 32;             // per launch (kernel-argument space); more take further rounds of launches
+constexpr int kMuonChunks = 256;             // partial sums of a matrix's norm
+constexpr float kLoScale = 2048.0f;          // the second plane's extra scale
+
+struct MuonJob {
+    void *grad, *momentum, *param, *out;
+    int rows, cols;
+    float adjust;
+    int first;                               // first tile of this launch
+    long off;                                // its scratch
+};
+
+struct MuonJobs {
+    MuonJob j[kMuonMaxJobs];
+    int n;
+    unsigned char* scratch;
+};
+
+struct MuonNum {
+    float a, b, c;                           // the polynomial
+    int ex, ea, eb;                          // planes hold X 2^ex, A 2^ea, B 2^eb
+    float eps, mu, omu, wd;
+    int nesterov, zero_grad, nesterov_step;
+    const float* lr;
+};
+
+// where a matrix's buffers lie in its scratch: norm partials, X / Xt twice (a step reads one pair and writes the other), A, B
+struct MuonLay {
+    int m, n;
+    bool trans;
+    unsigned ldx, ldt;                       // bytes of a plane's row: X and (Xt, A, B)
+    long px, pt, pa;                         // bytes of a plane
+    long x[2], t[2], a, b, total;
+};
+__host__ __device__ inline MuonLay muon_lay(int rows, int cols, int planes) {
+    MuonLay L;
+    L.trans = rows > cols;
+    L.m = L.trans ? cols : rows;
+    L.n = L.trans ? rows : cols;
+    L.ldx = (unsigned)((L.n + 63) / 64) * 128u;
+    L.ldt = (unsigned)((L.m + 63) / 64) * 128u;
+    L.px = (long)L.m * L.ldx;
+    L.pt = (long)L.n * L.ldt;
+    L.pa = (long)L.m * L.ldt;
+    long o = kMuonChunks * 8;
+    for (int k = 0; k < 2; ++k) {
+        L.x[k] = o, o += planes * L.px;
+        L.t[k] = o, o += planes * L.pt;
+    }
+    L.a = o, o += planes * L.pa;
+    L.b = o, o += planes * L.pa;
+    L.total = (o + 255) / 256 * 256;
+    return L;
+}
+
+FN_DEV int muon_find(const MuonJobs& js, int wg) {
+    int q = 0;
+    while (q + 1 < js.n && js.j[q + 1].first <= wg) ++q;
+    return q;
+}
+
+// u = (1 - mu) g + mu m', m' = mu m + (1 - mu) g as it is stored
+template <class T>
+FN_DEV float muon_u(float g, float m, const MuonNum& P) { return P.nesterov ? P.omu * g + P.mu * m : m; }
+
+// launch 1: the momentum, and the partial sums of |u|^2 (fp64: no overflow, no underflow), kMuonChunks workgroups a matrix
+template <class T, bool MOM>
+__global__ void __launch_bounds__(256) muon_norm_kernel(MuonJobs js, MuonNum P) {
+    const int q = blockIdx.x / kMuonChunks, c = blockIdx.x % kMuonChunks;
+    const MuonJob& J = js.j[q];
+    const long total = (long)J.rows * J.cols;
+    const T* g = (const T*)J.grad;
+    T* m = (T*)J.momentum;
+    constexpr int V = Chunk<T>::N;
+    double s = 0.0;
+    for (long at = ((long)c * 256 + threadIdx.x) * V; at < total; at += (long)kMuonChunks * 256 * V) {
+        const int valid = total - at < V ? (int)(total - at) : V;
+        float gv[V], mv[V];
+        load_chunk<T>(g + at, valid, gv);
+        if constexpr (MOM) {
+            load_chunk<T>(m + at, valid, mv);
+#pragma unroll
+            for (int k = 0; k < V; ++k) mv[k] = (float)(T)(P.mu * mv[k] + P.omu * gv[k]);
+            store_chunk<T>(m + at, valid, mv);
+#pragma unroll
+            for (int k = 0; k < V; ++k) gv[k] = muon_u<T>(gv[k], mv[k], P);
+        }
+#pragma unroll
+        for (int k = 0; k < V; ++k) s += (double)gv[k] * (double)gv[k];
+    }
+    __shared__ double red[4];
+#pragma unroll
+    for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d, 64);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) reinterpret_cast<double*>(js.scratch + J.off)[c] = red[0] + red[1] + red[2] + red[3];
+}
+
+// one value's planes: hi at p, lo behind it
+template <int NP>
+FN_DEV void muon_split(float v, _Float16& hi, _Float16& lo) {
+    hi = (_Float16)v;
+    if constexpr (NP == 2) lo = (_Float16)((v - (float)hi) * kLoScale);
+}
+
+// launch 2: X and Xt (with their zero padding) of 64 x 64 tiles of u
+template <class T, bool MOM, int NP>
+__global__ void __launch_bounds__(256) muon_init_kernel(MuonJobs js, MuonNum P) {
+    __shared__ float tile[64][65];
+    __shared__ double red[4];
+    const MuonJob& J = js.j[muon_find(js, blockIdx.x)];
+    const MuonLay L = muon_lay(J.rows, J.cols, NP);
+    unsigned char* S = js.scratch + J.off;
+    double s = reinterpret_cast<const double*>(S)[threadIdx.x];       // kMuonChunks == 256 partials
+#pragma unroll
+    for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d, 64);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    const int tiles_c = (J.cols + 63) / 64;
+    const int t = blockIdx.x - J.first, r0 = 64 * (t / tiles_c), c0 = 64 * (t % tiles_c);
+    const int lc = threadIdx.x & 63, lr = threadIdx.x >> 6;
+#pragma unroll 4
+    for (int r = lr; r < 64; r += 4) {
+        float u = 0.0f;
+        if (r0 + r < J.rows && c0 + lc < J.cols) {
+            const long at = (long)(r0 + r) * J.cols + c0 + lc;
+            u = (float)((const T*)J.grad)[at];
+            if constexpr (MOM) {
+                u = muon_u<T>(u, (float)((const T*)J.momentum)[at], P);
+                if (P.zero_grad) ((T*)J.grad)[at] = (T)0.0f;
+            }
+        }
+        tile[r][lc] = u;
+    }
+    __syncthreads();
+    const double norm = sqrt(red[0] + red[1] + red[2] + red[3]);
+    const float scale = (float)(ldexp(1.0, P.ex) / (norm > (double)P.eps || norm != norm ? norm : (double)P.eps));
+    // rows along the matrix's own rows: X, or Xt of the transpose; and the other one
+    _Float16* along = reinterpret_cast<_Float16*>(S + (L.trans ? L.t[0] : L.x[0]));
+    _Float16* across = reinterpret_cast<_Float16*>(S + (L.trans ? L.x[0] : L.t[0]));
+    const unsigned ld_al = (L.trans ? L.ldt : L.ldx) / 2, ld_ac = (L.trans ? L.ldx : L.ldt) / 2;
+    const long pl_al = (L.trans ? L.pt : L.px) / 2, pl_ac = (L.trans ? L.px : L.pt) / 2;
+#pragma unroll 4
+    for (int r = lr; r < 64; r += 4) {
+        _Float16 hi, lo;
+        if (r0 + r < J.rows) {
+            muon_split<NP>(tile[r][lc] * scale, hi, lo);
+            _Float16* o = along + (long)(r0 + r) * ld_al + c0 + lc;
+            o[0] = hi;
+            if constexpr (NP == 2) o[pl_al] = lo;
+        }
+        if (c0 + r < J.cols) {
+            muon_split<NP>(tile[lc][r] * scale, hi, lo);
+            _Float16* o = across + (long)(c0 + r) * ld_ac + r0 + lc;
+            o[0] = hi;
+            if constexpr (NP == 2) o[pl_ac] = lo;
+        }
+    }
+}
+
+template <int NP>
+FN_DEV MmOperand muon_op(const unsigned char* base, long plane, unsigned row_bytes) {
+    MmOperand o;
+    o.plane[0] = base;
+    o.plane[1] = NP == 2 ? base + plane : base;
+    o.plane[2] = base;
+    o.row_bytes = row_bytes;
+    return o;
+}
+
+// four consecutive values of a plane pair as fp32 (times 2^e of the plane)
+template <int NP>
+FN_DEV void muon_read4(const unsigned char* p, long plane, float (&v)[4]) {
+    const f16x4 hi = *reinterpret_cast<const f16x4*>(p);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = (float)hi[k];
+    if constexpr (NP == 2) {
+        const f16x4 lo = *reinterpret_cast<const f16x4*>(p + plane);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] += (float)lo[k] * (1.0f / kLoScale);
+    }
+}
+template <int NP>
+FN_DEV void muon_write4(unsigned char* p, long plane, const float (&v)[4], f16x4& hi, f16x4& lo) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        _Float16 a, b = (_Float16)0.0f;
+        muon_split<NP>(v[k], a, b);
+        hi[k] = a, lo[k] = b;
+    }
+    *reinterpret_cast<f16x4*>(p) = hi;
+    if constexpr (NP == 2) *reinterpret_cast<f16x4*>(p + plane) = lo;
+}
+
+enum { MU_GRAM = 0, MU_POLY = 1, MU_STEP = 2, MU_LAST = 3 };
+
+// GRAM: A = X X^T.  POLY: B = b A + c A A.  STEP: X' = a X + B X, both layouts.  LAST: the same into `out` or the parameter.
+template <class Cfg, int NP, int KIND, class T, bool MOM>
+__global__ void __launch_bounds__(Cfg::THREADS) muon_product_kernel(MuonJobs js, MuonNum P, int cur) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char mm_smem[];
+    const MuonJob& J = js.j[muon_find(js, blockIdx.x)];
+    const MuonLay L = muon_lay(J.rows, J.cols, NP);
+    unsigned char* S = js.scratch + J.off;
+    const int ni = L.m, nj = KIND <= MU_POLY ? L.m : L.n;
+    const int tiles_i = (ni + Cfg::BM - 1) / Cfg::BM, tiles_j = (nj + Cfg::BN - 1) / Cfg::BN;
+    int ti, tj;
+    mm_tile(blockIdx.x - J.first, (long)tiles_i * tiles_j, tiles_i, tiles_j, ti, tj);
+    const long i0 = (long)ti * Cfg::BM, j0 = (long)tj * Cfg::BN;
+    MmOperand A, B;
+    if constexpr (KIND == MU_GRAM) A = B = muon_op<NP>(S + L.x[cur], L.px, L.ldx);
+    else if constexpr (KIND == MU_POLY) A = B = muon_op<NP>(S + L.a, L.pa, L.ldt);
+    else A = muon_op<NP>(S + L.b, L.pa, L.ldt), B = muon_op<NP>(S + L.t[cur], L.pt, L.ldt);
+    const int k_tiles = (int)((KIND == MU_GRAM ? L.ldx : L.ldt) / 128);
+    f32x16 acc[Cfg::MI][Cfg::NJ];
+    mm_run<Cfg, _Float16, NP == 2>(mm_smem, A, B, i0, ni, j0, nj, k_tiles, NP == 2 ? kMmThree : kMmOne, 0, (NP == 2 ? 3 : 1) * k_tiles, kLoScale, acc);
+    const float lo = NP == 2 ? 1.0f / kLoScale : 1.0f;
+    // acc -> value: the product of the operands' scales (and the second plane's) is taken out, the result's put in
+    float f;
+    if constexpr (KIND == MU_GRAM) f = ldexpf(lo, P.ea - 2 * P.ex);
+    else if constexpr (KIND == MU_POLY) f = P.c * ldexpf(lo, P.eb - 2 * P.ea);
+    else f = ldexpf(lo, (KIND == MU_STEP ? P.ex : 0) - P.eb - P.ex);
+    const float lr = KIND == MU_LAST && MOM ? *P.lr : 0.0f;
+#pragma unroll
+    for (int m = 0; m < Cfg::MI; ++m) {
+        const long i = i0 + mm_row<Cfg>() + 32 * m;
+#pragma unroll
+        for (int n = 0; n < Cfg::NJ; ++n)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const long j = j0 + mm_col<Cfg>() + 32 * n + 8 * g;
+                float v[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = acc[m][n][4 * g + k] * f;
+                f16x4 hi, lo4;
+                if constexpr (KIND == MU_GRAM || KIND == MU_POLY) {
+                    if (i >= ni || j >= (long)L.ldt / 2) continue;
+                    if constexpr (KIND == MU_POLY) {
+                        float a[4];
+                        muon_read4<NP>(S + L.a + i * L.ldt + j * 2, L.pa, a);
+                        const float fb = ldexpf(P.b, P.eb - P.ea);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) v[k] += fb * a[k];
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) v[k] = j + k < nj ? v[k] : 0.0f;
+                    muon_write4<NP>(S + (KIND == MU_GRAM ? L.a : L.b) + i * L.ldt + j * 2, L.pa, v, hi, lo4);
+                } else {
+                    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    if (i < ni && j < (long)L.ldx / 2) muon_read4<NP>(S + L.x[cur] + i * L.ldx + j * 2, L.px, x);
+                    const float fa = KIND == MU_STEP ? P.a : ldexpf(P.a, -P.ex);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) v[k] = i < ni && j + k < nj ? v[k] + fa * x[k] : 0.0f;
+                    if constexpr (KIND == MU_STEP) {
+                        if (i < ni && j < (long)L.ldx / 2) muon_write4<NP>(S + L.x[cur ^ 1] + i * L.ldx + j * 2, L.px, v, hi, lo4);
+                        if (i < (long)L.ldt / 2) {
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                if (j + k < nj) {
+                                    _Float16 a, b = (_Float16)0.0f;
+                                    muon_split<NP>(v[k], a, b);
+                                    unsigned char* p = S + L.t[cur ^ 1] + (j + k) * L.ldt + i * 2;
+                                    *reinterpret_cast<_Float16*>(p) = a;
+                                    if constexpr (NP == 2) *reinterpret_cast<_Float16*>(p + L.pt) = b;
+                                }
+                        }
+                    } else if (i < ni) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (j + k < nj) {
+                                const long at = L.trans ? (j + k) * (long)J.cols + i : i * (long)J.cols + j + k;
+                                if constexpr (MOM) {
+                                    T* p = (T*)J.param + at;
+                                    *p = (T)((float)*p * (1.0f - lr * P.wd) - lr * J.adjust * v[k]);
+                                } else {
+                                    ((T*)J.out)[at] = (T)v[k];
+                                }
+                            }
+                    }
+                }
+            }
+    }
+}
+
+typedef MmCfg<64, 64, 2, 2, 3> MuonSmall;
+typedef MmCfg<128, 128, 2, 2, 2> MuonLarge;
+
+template <class Cfg, int NP, int KIND, class T, bool MOM>
+static void muon_product(MuonJobs& js, const MuonNum& P, int cur, hipStream_t stream) {
+    long tiles = 0;
+    for (int q = 0; q < js.n; ++q) {
+        MuonJob& J = js.j[q];
+        const long m = J.rows < J.cols ? J.rows : J.cols, n = J.rows < J.cols ? J.cols : J.rows;
+        J.first = (int)tiles;
+        tiles += ((m + Cfg::BM - 1) / Cfg::BM) * (((KIND <= MU_POLY ? m : n) + Cfg::BN - 1) / Cfg::BN);
+    }
+    auto kernel = muon_product_kernel<Cfg, NP, KIND, T, MOM>;
+    static const bool once = (allow_big_lds(kernel), true);
+    (void)once;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(Cfg::THREADS), Cfg::LDS, stream, js, P, cur);
+}
+
+template <class Cfg, int NP, class T, bool MOM>
+static void muon_steps(MuonJobs& js, const MuonNum& P, int steps, hipStream_t stream) {
+    for (int s = 0; s < steps; ++s) {
+        muon_product<Cfg, NP, MU_GRAM, T, MOM>(js, P, s & 1, stream);
+        muon_product<Cfg, NP, MU_POLY, T, MOM>(js, P, s & 1, stream);
+        if (s + 1 < steps) muon_product<Cfg, NP, MU_STEP, T, MOM>(js, P, s & 1, stream);
+        else muon_product<Cfg, NP, MU_LAST, T, MOM>(js, P, s & 1, stream);
+    }
+}
+
+template <class T, bool MOM, int NP>
+static int muon_run(const FneusMuonJob* jobs, int n_jobs, const MuonNum& P, int steps, unsigned char* scratch, hipStream_t stream) {
+    for (int first = 0; first < n_jobs; first += kMuonMaxJobs) {
+        MuonJobs js;
+        js.n = n_jobs - first < kMuonMaxJobs ? n_jobs - first : kMuonMaxJobs;
+        js.scratch = scratch;
+        long off = 0, tiles = 0, large = 0;
+        for (int q = 0; q < js.n; ++q) {
+            const FneusMuonJob& f = jobs[first + q];
+            MuonJob& J = js.j[q];
+            J.grad = f.grad, J.momentum = f.momentum, J.param = f.param, J.out = f.out;
+            J.rows = f.rows, J.cols = f.cols, J.adjust = f.adjust, J.off = off, J.first = (int)tiles;
+            off += muon_lay(f.rows, f.cols, NP).total;
+            tiles += (long)((f.rows + 63) / 64) * ((f.cols + 63) / 64);
+            const long m = f.rows < f.cols ? f.rows : f.cols;
+            large += ((m + 127) / 128) * ((m + 127) / 128);
+        }
+        hipLaunchKernelGGL((muon_norm_kernel<T, MOM>), dim3((unsigned)(js.n * kMuonChunks)), dim3(256), 0, stream, js, P);
+        hipLaunchKernelGGL((muon_init_kernel<T, MOM, NP>), dim3((unsigned)tiles), dim3(256), 0, stream, js, P);
+        if (large >= 128) muon_steps<MuonLarge, NP, T, MOM>(js, P, steps, stream);
+        else muon_steps<MuonSmall, NP, T, MOM>(js, P, steps, stream);
+    }
+    return launch_status();
+}
+
+static int muon_refuse(const char* msg) {
+    set_last_error(msg);
+    return -2;
+}
+
+// the largest power of two that keeps `bound` (with 2 % for rounding) within fp16, at most 2^14
+static int muon_exponent(double bound) {
+    int e = 14;
+    while (e > -14 && ldexp(bound * 1.02, e) > 65504.0) --e;
+    return e;
+}
+
+// bounds of the singular values over the steps (from [0, 1]: the Frobenius norm) give the planes' scales
+static bool muon_scales(double a, double b, double c, int steps, MuonNum& P) {
+    double top = 1.0, x = 1.0, poly = 0.0;
+    if (!isfinite(a) || !isfinite(b) || !isfinite(c)) return false;
+    for (int s = 0; s < steps; ++s) {
+        double next = 0.0;
+        for (int k = 0; k <= 512; ++k) {
+            const double v = top * k / 512.0, q = v * v;
+            const double p = fabs(b * q + c * q * q), w = fabs(a * v + b * v * q + c * v * q * q);
+            poly = p > poly ? p : poly;
+            next = w > next ? w : next;
+        }
+        x = top > x ? top : x;
+        top = next * 1.001 + 1e-6;
+        if (!(top <= 16.0)) return false;
+    }
+    // (the last step's result is not kept in planes)
+    P.ex = muon_exponent(x), P.ea = muon_exponent(x * x), P.eb = muon_exponent(poly > 1e-3 ? poly : 1e-3);
+    return true;
+}
+
+static int muon_check(const FneusMuonJob* jobs, int n_jobs, int steps, int prec, int dtype, void* scratch, long bytes, bool mom) {
+    if (n_jobs < 0 || (n_jobs > 0 && !jobs)) return muon_refuse("fneus_muon: jobs must be given");
+    if (steps < 1 || steps > 64) return muon_refuse("fneus_muon: 1 to 64 steps");
+    if ((prec != 2 && prec != 3) || dtype < 0 || dtype > 2) return muon_refuse("fneus_muon: prec 2 or 3, dtype 0..2");
+    for (int q = 0; q < n_jobs; ++q) {
+        const FneusMuonJob& f = jobs[q];
+        if (f.rows <= 0 || f.cols <= 0 || f.rows > 65536 || f.cols > 65536) return muon_refuse("fneus_muon: a matrix needs 1 to 65536 rows and columns");
+        if (!f.grad || (mom ? !f.momentum || !f.param : !f.out)) return muon_refuse("fneus_muon: grad, and momentum and param (or out), must be given");
+    }
+    if (n_jobs > 0 && (!scratch || bytes < fneus_muon_scratch_bytes(jobs, n_jobs, prec) || ((uintptr_t)scratch & 255)))
+        return muon_refuse("fneus_muon: scratch of fneus_muon_scratch_bytes bytes, 256-byte aligned, must be given");
+    return 0;
+}
+
+template <bool MOM>
+static int muon_dispatch(const FneusMuonJob* jobs, int n, const MuonNum& P, int steps, int prec, int dtype, void* scratch, hipStream_t s) {
+    unsigned char* w = (unsigned char*)scratch;
+    if (dtype == DT_F32) return prec == 3 ? muon_run<float, MOM, 2>(jobs, n, P, steps, w, s) : muon_run<float, MOM, 1>(jobs, n, P, steps, w, s);
+    if (dtype == DT_BF16) return prec == 3 ? muon_run<__bf16, MOM, 2>(jobs, n, P, steps, w, s) : muon_run<__bf16, MOM, 1>(jobs, n, P, steps, w, s);
+    return prec == 3 ? muon_run<_Float16, MOM, 2>(jobs, n, P, steps, w, s) : muon_run<_Float16, MOM, 1>(jobs, n, P, steps, w, s);
+}
+
+}  // namespace fneus
+
+using namespace fneus;
+
+extern "C" long fneus_muon_scratch_bytes(const FneusMuonJob* jobs, int n_jobs, int prec) {
+    long most = 0;
+    if (!jobs) return 0;
+    for (int first = 0; first < n_jobs; first += kMuonMaxJobs) {       // (a further round of launches uses the same memory: one stream)
+        long off = 0;
+        for (int q = first; q < n_jobs && q < first + kMuonMaxJobs; ++q)
+            if (jobs[q].rows > 0 && jobs[q].cols > 0) off += muon_lay(jobs[q].rows, jobs[q].cols, prec == 3 ? 2 : 1).total;
+        most = off > most ? off : most;
+    }
+    return most;
+}
+
+extern "C" int fneus_newton_schulz(const FneusMuonJob* jobs, int n_jobs, double a, double b, double c, int steps, double eps, int prec,
+                                   int dtype, void* scratch, long scratch_bytes, fneus_stream_t stream) {
+    fneus::clear_status();
+    if (int rc = muon_check(jobs, n_jobs, steps, prec, dtype, scratch, scratch_bytes, false)) return rc;
+    MuonNum P{};
+    P.a = (float)a, P.b = (float)b, P.c = (float)c, P.eps = (float)eps;
+    if (!(eps > 0.0) || !muon_scales(a, b, c, steps, P)) return muon_refuse("fneus_newton_schulz: eps > 0, a polynomial that keeps [0, 1] below 16 over the steps");
+    if (n_jobs == 0) return 0;
+    return muon_dispatch<false>(jobs, n_jobs, P, steps, prec, dtype, scratch, (hipStream_t)stream);
+}
+
+extern "C" int fneus_muon(const FneusMuonJob* jobs, int n_jobs, const float* lr, double mu, int nesterov, double weight_decay, double a,
+                          double b, double c, int steps, double eps, int prec, int dtype, int zero_grad, void* scratch,
+                          long scratch_bytes, fneus_stream_t stream) {
+    fneus::clear_status();
+    if (int rc = muon_check(jobs, n_jobs, steps, prec, dtype, scratch, scratch_bytes, true)) return rc;
+    MuonNum P{};
+    P.a = (float)a, P.b = (float)b, P.c = (float)c, P.eps = (float)eps;
+    if (!lr || !(eps > 0.0) || !muon_scales(a, b, c, steps, P)) return muon_refuse("fneus_muon: lr, eps > 0, a polynomial that keeps [0, 1] below 16 over the steps");
+    P.mu = (float)mu, P.omu = (float)(1.0 - mu), P.wd = (float)weight_decay, P.nesterov = nesterov, P.zero_grad = zero_grad, P.lr = lr;
+    if (n_jobs == 0) return 0;
+    return muon_dispatch<true>(jobs, n_jobs, P, steps, prec, dtype, scratch, (hipStream_t)stream);
+}

@@ -1,0 +1,435 @@
+// Layer norm over the last axis, forward and backward (fp32 / bf16 / fp16; statistics and sums in fp32).
+//   row x[n]:  mu = mean(x),  var = mean((x - mu)^2),  r = 1 / sqrt(var + eps),  xh = (x - mu) r,  y = xh w + b
+//   backward:  g = dy w,  dx = r (g - mean(g) - xh mean(g xh)),  dw = sum_rows dy xh,  db = sum_rows dy
+// Memory bound: the forward reads x and writes y, the backward reads dy and x and writes dx.  A TEAM of TPR threads owns a row and
+// holds it in registers (EPT values a thread, 16-byte chunks): one pass over memory, the variance from the centred values (two
+// passes over registers: a row with a large mean keeps its digits).  TPR = 16 (sums by DPP), 64, 256 or 1024 threads; wider rows
+// take the streaming kernels, which read a row from the caches again.
+// The weight gradients: a team keeps its columns' sums of dy xh and dy in registers over all the rows it takes, the teams of a
+// workgroup are added in LDS, every workgroup writes ONE partial row, and a second launch adds the partial rows in a fixed order: no
+// atomics, the same bits in every run.
+#include "fneus_types.h"
+#include "fneus_kernels.h"
+
+namespace fneus {
+
+constexpr int kNormMaxGrid = 1024;       // workgroups of the backward = partial rows of the weight gradients
+
+// sums of v over the team, in every thread of it.  `red`: LDS floats, 2 * TPR / 64 (TPR > 64); `flip` alternates the half used, so
+// one barrier a sum is enough
+template <int TPR>
+FN_DEV float team_sum(float v, float* red, int& flip) {
+    if constexpr (TPR == 16) return row16_sum(v);
+    v = wave_sum(v);
+    if constexpr (TPR > 64) {
+        constexpr int W = TPR / 64;
+        float* r = red + flip * W;
+        flip ^= 1;
+        if ((threadIdx.x & 63) == 0) r[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) v += r[w];
+    }
+    return v;
+}
+
+template <class T, class P>
+struct NormArgs {
+    const T *x, *dy;
+    const P *w, *b;
+    T *y, *dx;
+    float *mean, *rstd;
+    float* partial;          // [grid][2][n]
+    long ldx, ldy, lddy, lddx;
+    long rows;
+    int n;
+    float eps;
+};
+
+template <class T, class P, int TPR, int EPT>
+__global__ void __launch_bounds__(TPR > 256 ? TPR : 256) layer_norm_fwd_kernel(NormArgs<T, P> a) {
+    constexpr int V = Chunk<T>::N, NC = EPT / V, TEAMS = TPR > 256 ? 1 : 256 / TPR;
+    __shared__ float red[2 * (TPR > 64 ? TPR / 64 : 1)];
+    int flip = 0;
+    const int t = threadIdx.x % TPR;
+    const long row = (long)blockIdx.x * TEAMS + threadIdx.x / TPR;
+    if (TPR <= 64 && row >= a.rows) return;          // (a team of more than a wave is the whole workgroup: its row exists)
+    const T* __restrict__ x = a.x + row * a.ldx;
+    float v[NC][V];
+    float s = 0.0f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int col = (c * TPR + t) * V;
+        load_chunk<T>(x + col, a.n - col, v[c]);
+    }
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int k = 0; k < V; ++k) s += v[c][k];
+    const float len = (float)a.n;            // (divisions, not a reciprocal: the mean of equal values is that value)
+    const float mu = team_sum<TPR>(s, red, flip) / len;
+    float q = 0.0f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int left = a.n - (c * TPR + t) * V;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            v[c][k] -= mu;
+            q += k < left ? v[c][k] * v[c][k] : 0.0f;
+        }
+    }
+    const float r = 1.0f / sqrtf(team_sum<TPR>(q, red, flip) / len + a.eps);
+    T* __restrict__ y = a.y + row * a.ldy;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int col = (c * TPR + t) * V, left = a.n - col;
+        if (left <= 0) break;
+        float w[V], o[V];
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            w[k] = a.w ? (k < left ? (float)a.w[col + k] : 0.0f) : 1.0f;
+            o[k] = a.b ? (k < left ? (float)a.b[col + k] : 0.0f) : 0.0f;
+        }
+#pragma unroll
+        for (int k = 0; k < V; ++k) o[k] = v[c][k] * r * w[k] + o[k];
+        store_chunk<T>(y + col, left, o);
+    }
+    if (t == 0) {
+        a.mean[row] = mu;
+        a.rstd[row] = r;
+    }
+}
+
+// rows wider than a team's registers: a workgroup a row, three passes (the second and third from the caches)
+template <class T, class P>
+__global__ void __launch_bounds__(1024) layer_norm_fwd_stream_kernel(NormArgs<T, P> a) {
+    constexpr int V = Chunk<T>::N;
+    __shared__ float red[32];
+    int flip = 0;
+    const long row = blockIdx.x;
+    const T* x = a.x + row * a.ldx;
+    const float len = (float)a.n;
+    float s = 0.0f, v[V];
+    for (long col = (long)threadIdx.x * V; col < a.n; col += 1024 * V) {
+        load_chunk<T>(x + col, (int)(a.n - col), v);
+#pragma unroll
+        for (int k = 0; k < V; ++k) s += v[k];
+    }
+    const float mu = team_sum<1024>(s, red, flip) / len;
+    float q = 0.0f;
+    for (long col = (long)threadIdx.x * V; col < a.n; col += 1024 * V) {
+        const int left = (int)(a.n - col);
+        load_chunk<T>(x + col, left, v);
+#pragma unroll
+        for (int k = 0; k < V; ++k) q += k < left ? (v[k] - mu) * (v[k] - mu) : 0.0f;
+    }
+    const float r = 1.0f / sqrtf(team_sum<1024>(q, red, flip) / len + a.eps);
+    for (long col = (long)threadIdx.x * V; col < a.n; col += 1024 * V) {
+        const int left = (int)(a.n - col);
+        load_chunk<T>(x + col, left, v);
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+            if (k < left) v[k] = (v[k] - mu) * r * (a.w ? (float)a.w[col + k] : 1.0f) + (a.b ? (float)a.b[col + k] : 0.0f);
+        store_chunk<T>(a.y + row * a.ldy + col, left, v);
+    }
+    if (threadIdx.x == 0) {
+        a.mean[row] = mu;
+        a.rstd[row] = r;
+    }
+}
+
+// dx of the rows blockIdx, blockIdx + grid, ... and, PARAMS, this workgroup's partial row of (dw, db)
+template <class T, class P, int TPR, int EPT, bool PARAMS>
+__global__ void __launch_bounds__(TPR > 256 ? TPR : 256) layer_norm_bwd_kernel(NormArgs<T, P> a) {
+    constexpr int V = Chunk<T>::N, NC = EPT / V, TEAMS = TPR > 256 ? 1 : 256 / TPR;
+    __shared__ float red[2 * (TPR > 64 ? TPR / 64 : 1)];
+    __shared__ float fold[PARAMS && TEAMS > 1 ? TEAMS : 1][PARAMS && TEAMS > 1 ? TPR * EPT : 1];
+    int flip = 0;
+    const int t = threadIdx.x % TPR, team = threadIdx.x / TPR;
+    float w[NC][V], dw[NC][V], db[NC][V];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int col = (c * TPR + t) * V;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            w[c][k] = a.w ? (col + k < a.n ? (float)a.w[col + k] : 0.0f) : 1.0f;
+            dw[c][k] = 0.0f;
+            db[c][k] = 0.0f;
+        }
+    }
+    const float inv_n = 1.0f / (float)a.n;
+    for (long base = (long)blockIdx.x * TEAMS; base < a.rows; base += (long)gridDim.x * TEAMS) {
+        const long row = base + team;
+        const bool live = row < a.rows;               // (TPR > 64: one team, always live: every wave meets the barriers)
+        const T* __restrict__ x = a.x + row * a.ldx;
+        const T* __restrict__ dy = a.dy + row * a.lddy;
+        float xh[NC][V], d[NC][V];
+        const float mu = live ? a.mean[row] : 0.0f, r = live ? a.rstd[row] : 0.0f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int col = (c * TPR + t) * V, left = live ? a.n - col : 0;
+            load_chunk<T>(x + col, left, xh[c]);
+            load_chunk<T>(dy + col, left, d[c]);
+        }
+        float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int left = live ? a.n - (c * TPR + t) * V : 0;
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                const float h = k < left ? (xh[c][k] - mu) * r : 0.0f;
+                if constexpr (PARAMS) {
+                    dw[c][k] += d[c][k] * h;
+                    db[c][k] += d[c][k];
+                }
+                const float g = d[c][k] * w[c][k];
+                s1 += g;
+                s2 += g * h;
+                xh[c][k] = h;
+                d[c][k] = g;
+            }
+        }
+        s1 = team_sum<TPR>(s1, red, flip) * inv_n;
+        s2 = team_sum<TPR>(s2, red, flip) * inv_n;
+        T* __restrict__ dx = a.dx + row * a.lddx;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int col = (c * TPR + t) * V, left = live ? a.n - col : 0;
+            if (left <= 0) break;
+            float o[V];
+#pragma unroll
+            for (int k = 0; k < V; ++k) o[k] = r * (d[c][k] - s1 - xh[c][k] * s2);
+            store_chunk<T>(dx + col, left, o);
+        }
+    }
+    if constexpr (PARAMS) {
+        float* out = a.partial + (long)blockIdx.x * 2 * a.n;
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+            if constexpr (TEAMS > 1) {
+                __syncthreads();
+#pragma unroll
+                for (int c = 0; c < NC; ++c)
+#pragma unroll
+                    for (int k = 0; k < V; ++k) fold[team][(c * TPR + t) * V + k] = which ? db[c][k] : dw[c][k];
+                __syncthreads();
+                for (int col = threadIdx.x; col < a.n; col += 256) {
+                    float s = 0.0f;
+#pragma unroll
+                    for (int m = 0; m < TEAMS; ++m) s += fold[m][col];
+                    out[which * (long)a.n + col] = s;
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    const int col = (c * TPR + t) * V;
+#pragma unroll
+                    for (int k = 0; k < V; ++k)
+                        if (col + k < a.n) out[which * (long)a.n + col + k] = which ? db[c][k] : dw[c][k];
+                }
+            }
+        }
+    }
+}
+
+template <class T, class P>
+__global__ void __launch_bounds__(1024) layer_norm_bwd_stream_kernel(NormArgs<T, P> a) {
+    constexpr int V = Chunk<T>::N;
+    __shared__ float red[32];
+    int flip = 0;
+    const long row = blockIdx.x;
+    const T *x = a.x + row * a.ldx, *dy = a.dy + row * a.lddy;
+    const float mu = a.mean[row], r = a.rstd[row], inv_n = 1.0f / (float)a.n;
+    float s1 = 0.0f, s2 = 0.0f, v[V], d[V];
+    for (long col = (long)threadIdx.x * V; col < a.n; col += 1024 * V) {
+        const int left = (int)(a.n - col);
+        load_chunk<T>(x + col, left, v);
+        load_chunk<T>(dy + col, left, d);
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+            if (k < left) {
+                const float g = d[k] * (a.w ? (float)a.w[col + k] : 1.0f);
+                s1 += g;
+                s2 += g * (v[k] - mu) * r;
+            }
+    }
+    s1 = team_sum<1024>(s1, red, flip) * inv_n;
+    s2 = team_sum<1024>(s2, red, flip) * inv_n;
+    for (long col = (long)threadIdx.x * V; col < a.n; col += 1024 * V) {
+        const int left = (int)(a.n - col);
+        load_chunk<T>(x + col, left, v);
+        load_chunk<T>(dy + col, left, d);
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+            if (k < left) v[k] = r * (d[k] * (a.w ? (float)a.w[col + k] : 1.0f) - s1 - (v[k] - mu) * r * s2);
+        store_chunk<T>(a.dx + row * a.lddx + col, left, v);
+    }
+}
+
+// the streaming form's partial rows: a thread a column, the rows blockIdx.y, blockIdx.y + gridDim.y, ...
+template <class T, class P>
+__global__ void __launch_bounds__(256) layer_norm_params_kernel(NormArgs<T, P> a) {
+    const long col = (long)blockIdx.x * 256 + threadIdx.x;
+    if (col >= a.n) return;
+    float dw = 0.0f, db = 0.0f;
+    for (long row = blockIdx.y; row < a.rows; row += gridDim.y) {
+        const float d = (float)a.dy[row * a.lddy + col];
+        dw += d * (((float)a.x[row * a.ldx + col] - a.mean[row]) * a.rstd[row]);
+        db += d;
+    }
+    float* out = a.partial + (long)blockIdx.y * 2 * a.n;
+    out[col] = dw;
+    out[a.n + col] = db;
+}
+
+// dw, db = the sums of the partial rows in their order: 32 columns a workgroup, 32 threads a column
+template <class P>
+__global__ void __launch_bounds__(1024) layer_norm_fold_kernel(const float* __restrict__ partial, int parts, int n, P* __restrict__ dw,
+                                                               P* __restrict__ db) {
+    __shared__ float red[32][33];
+    const int lane = threadIdx.x & 31, group = threadIdx.x >> 5;
+    const long col = (long)blockIdx.x * 32 + lane;           // of the 2 n columns
+    float s = 0.0f;
+    if (col < 2L * n)
+        for (int p = group; p < parts; p += 32) s += partial[(long)p * 2 * n + col];
+    red[group][lane] = s;
+    __syncthreads();
+    if (threadIdx.x < 32 && col < 2L * n) {
+        s = 0.0f;
+#pragma unroll
+        for (int g = 0; g < 32; ++g) s += red[g][lane];
+        if (col < n) {
+            if (dw) dw[col] = (P)s;
+        } else if (db) {
+            db[col - n] = (P)s;
+        }
+    }
+}
+
+struct NormShape { int tpr, ept; };      // tpr 0: streaming
+
+// 16 values a thread are the most that four register arrays of them leave room for; the fewest threads that hold the row
+static NormShape norm_shape(int n) {
+    if (n <= 256) return {16, 16};
+    if (n <= 512) return {64, 8};
+    if (n <= 1024) return {64, 16};
+    if (n <= 2048) return {256, 8};
+    if (n <= 4096) return {256, 16};
+    if (n <= 8192) return {1024, 8};
+    if (n <= 16384) return {1024, 16};
+    return {0, 0};
+}
+
+static int norm_grid(long rows, int n) {
+    const NormShape s = norm_shape(n);
+    const int teams = s.tpr == 0 ? 1 : (s.tpr > 256 ? 1 : 256 / s.tpr);
+    const long need = (rows + teams - 1) / teams;
+    const long most = s.tpr == 0 ? 64 : (s.tpr >= 256 ? 512 : kNormMaxGrid);
+    return (int)(need < most ? need : most);
+}
+
+#define FN_NORM_SHAPES(CALL) \
+    switch (s.tpr * 100 + s.ept) { \
+        case 1616: CALL(16, 16); break; \
+        case 6408: CALL(64, 8); break; \
+        case 6416: CALL(64, 16); break; \
+        case 25608: CALL(256, 8); break; \
+        case 25616: CALL(256, 16); break; \
+        case 102408: CALL(1024, 8); break; \
+        default: CALL(1024, 16); break; \
+    }
+
+template <class T, class P>
+static void norm_fwd_launch(const NormArgs<T, P>& a, hipStream_t stream) {
+    const NormShape s = norm_shape(a.n);
+    if (s.tpr == 0) {
+        hipLaunchKernelGGL((layer_norm_fwd_stream_kernel<T, P>), dim3((unsigned)a.rows), dim3(1024), 0, stream, a);
+        return;
+    }
+    const int threads = s.tpr > 256 ? s.tpr : 256, teams = threads / s.tpr;
+    const dim3 grid((unsigned)((a.rows + teams - 1) / teams));
+#define CALL(TPR, EPT) hipLaunchKernelGGL((layer_norm_fwd_kernel<T, P, TPR, EPT>), grid, dim3(threads), 0, stream, a)
+    FN_NORM_SHAPES(CALL)
+#undef CALL
+}
+
+template <class T, class P>
+static void norm_bwd_launch(const NormArgs<T, P>& a, P* dw, P* db, hipStream_t stream) {
+    const NormShape s = norm_shape(a.n);
+    const int grid = norm_grid(a.rows, a.n);
+    const bool params = dw || db;
+    if (s.tpr == 0) {
+        hipLaunchKernelGGL((layer_norm_bwd_stream_kernel<T, P>), dim3((unsigned)a.rows), dim3(1024), 0, stream, a);
+        if (params) hipLaunchKernelGGL((layer_norm_params_kernel<T, P>), dim3((unsigned)((a.n + 255) / 256), (unsigned)grid), dim3(256), 0, stream, a);
+    } else {
+        const int threads = s.tpr > 256 ? s.tpr : 256, teams = threads / s.tpr;
+        const unsigned all = (unsigned)((a.rows + teams - 1) / teams);
+        if (params) {
+#define CALL(TPR, EPT) hipLaunchKernelGGL((layer_norm_bwd_kernel<T, P, TPR, EPT, true>), dim3((unsigned)grid), dim3(threads), 0, stream, a)
+            FN_NORM_SHAPES(CALL)
+#undef CALL
+        } else {
+#define CALL(TPR, EPT) hipLaunchKernelGGL((layer_norm_bwd_kernel<T, P, TPR, EPT, false>), dim3(all), dim3(threads), 0, stream, a)
+            FN_NORM_SHAPES(CALL)
+#undef CALL
+        }
+    }
+    if (params)
+        hipLaunchKernelGGL((layer_norm_fold_kernel<P>), dim3((unsigned)((2L * a.n + 31) / 32)), dim3(1024), 0, stream, a.partial, grid, a.n, dw, db);
+}
+
+static int norm_check(const char* what, const void* x, const void* out, const void* mean, const void* rstd, long rows, int n, int dtype,
+                      int wtype, long ld0, long ld1) {
+    if (rows < 0 || n <= 0 || rows > 0x7fffffffL) { set_last_error(what); return -2; }
+    if (dtype < 0 || dtype > 2 || (wtype != dtype && wtype != DT_F32) || ld0 < n || ld1 < n) { set_last_error(what); return -2; }
+    if (rows > 0 && (!x || !out || !mean || !rstd)) { set_last_error(what); return -2; }
+    return 0;
+}
+
+}  // namespace fneus
+
+using namespace fneus;
+
+#define FN_NORM_TYPES(CALL) \
+    if (dtype == DT_F32) CALL(float, float) \
+    else if (dtype == DT_BF16 && wtype == DT_BF16) CALL(__bf16, __bf16) \
+    else if (dtype == DT_BF16) CALL(__bf16, float) \
+    else if (wtype == DT_F16) CALL(_Float16, _Float16) \
+    else CALL(_Float16, float)
+
+extern "C" int fneus_layer_norm_fwd(const void* x, long ldx, const void* weight, const void* bias, void* y, long ldy, float* mean,
+                                    float* rstd, long rows, int n, float eps, int dtype, int wtype, fneus_stream_t stream_) {
+    hipStream_t stream = (hipStream_t)stream_;
+    fneus::clear_status();
+    if (int rc = norm_check("fneus_layer_norm_fwd: 0 <= rows < 2^31, n > 0, row strides >= n, dtype 0..2, weights of the same type or fp32, x, y, "
+                            "mean and rstd given", x, y, mean, rstd, rows, n, dtype, wtype, ldx, ldy)) return rc;
+    if (rows == 0) return 0;
+#define CALL(T, P) { NormArgs<T, P> a{}; a.x = (const T*)x; a.w = (const P*)weight; a.b = (const P*)bias; a.y = (T*)y; a.mean = mean; \
+        a.rstd = rstd; a.ldx = ldx; a.ldy = ldy; a.rows = rows; a.n = n; a.eps = eps; norm_fwd_launch<T, P>(a, stream); }
+    FN_NORM_TYPES(CALL)
+#undef CALL
+    return fneus::launch_status();
+}
+
+extern "C" long fneus_layer_norm_bwd_scratch_floats(long rows, int n) {
+    if (rows <= 0 || n <= 0) return 0;
+    return (long)norm_grid(rows, n) * 2 * n;
+}
+
+extern "C" int fneus_layer_norm_bwd(const void* dy, long lddy, const void* x, long ldx, const void* weight, const float* mean,
+                                    const float* rstd, void* dx, long lddx, void* dweight, void* dbias, float* scratch, long rows,
+                                    int n, int dtype, int wtype, fneus_stream_t stream_) {
+    hipStream_t stream = (hipStream_t)stream_;
+    fneus::clear_status();
+    const char* what = "fneus_layer_norm_bwd: 0 < rows < 2^31, n > 0, row strides >= n, dtype 0..2, weights of the same type or fp32, dy, x, mean, "
+                       "rstd, dx (and scratch for the weight gradients) given";
+    if (int rc = norm_check(what, x, dx, mean, rstd, rows, n, dtype, wtype, ldx, lddx)) return rc;
+    if (lddy < n || rows == 0 || !dy || ((dweight || dbias) && !scratch)) { fneus::set_last_error(what); return -2; }
+#define CALL(T, P) { NormArgs<T, P> a{}; a.x = (const T*)x; a.dy = (const T*)dy; a.w = (const P*)weight; a.dx = (T*)dx; \
+        a.mean = const_cast<float*>(mean); a.rstd = const_cast<float*>(rstd); a.partial = scratch; a.ldx = ldx; a.lddy = lddy; \
+        a.lddx = lddx; a.rows = rows; a.n = n; norm_bwd_launch<T, P>(a, (P*)dweight, (P*)dbias, stream); }
+    FN_NORM_TYPES(CALL)
+#undef CALL
+    return fneus::launch_status();
+}

@@ -65,6 +65,17 @@ class FneusMlpJob(C.Structure):
                [(n, C.c_int) for n in ("rows", "n_in", "n_out", "act", "act_in")]
 
 
+class FneusLinear(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("x", "weight", "bias", "residual", "y", "z", "dy", "dx", "dweight", "dbias", "scratch")] + \
+               [(n, C.c_long) for n in ("scratch_bytes", "rows", "ldx", "ld_residual", "lddy")] + \
+               [(n, C.c_int) for n in ("n_in", "n_out", "act", "dtype")]
+
+
+class FneusMuonJob(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("grad", "momentum", "param", "out")] + \
+               [("rows", C.c_int), ("cols", C.c_int), ("adjust", C.c_float), ("pad_", C.c_int)]
+
+
 class FneusGemmPPJob(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("a_hi", "a_lo", "b_hi", "b_lo", "a2_hi", "a2_lo", "b2_hi", "b2_lo")] + \
                [(n, C.c_uint32) for n in ("a_blk", "b_blk", "a2_blk", "b2_blk")] + \
@@ -159,6 +170,15 @@ def _load():
         "fneus_mlp_forward": (C.c_int, [C.POINTER(FneusMlpJob), ip, vp]),
         "fneus_mlp_backward_input": (C.c_int, [C.POINTER(FneusMlpJob), ip, vp]),
         "fneus_mlp_backward_params": (C.c_int, [C.POINTER(FneusMlpJob), ip, vp]),
+        "fneus_layer_norm_fwd": (C.c_int, [vp, l, vp, vp, vp, l, vp, vp, l, ip, f, ip, ip, vp]),
+        "fneus_layer_norm_bwd": (C.c_int, [vp, l, vp, l, vp, vp, vp, vp, l, vp, vp, vp, l, ip, ip, ip, vp]),
+        "fneus_layer_norm_bwd_scratch_floats": (C.c_long, [l, ip]),
+        "fneus_linear_scratch_bytes": (C.c_long, [C.POINTER(FneusLinear), ip]),
+        "fneus_linear_fwd": (C.c_int, [C.POINTER(FneusLinear), vp]),
+        "fneus_linear_bwd": (C.c_int, [C.POINTER(FneusLinear), vp]),
+        "fneus_muon_scratch_bytes": (C.c_long, [C.POINTER(FneusMuonJob), ip, ip]),
+        "fneus_newton_schulz": (C.c_int, [C.POINTER(FneusMuonJob), ip] + [C.c_double] * 3 + [ip, C.c_double, ip, ip, vp, l, vp]),
+        "fneus_muon": (C.c_int, [C.POINTER(FneusMuonJob), ip, vp, C.c_double, ip] + [C.c_double] * 4 + [ip, C.c_double, ip, ip, ip, vp, l, vp]),
         "fneus_lvis_visibility": (C.c_int, [vp, vp, vp, vp, vp, vp, ip, ip, ip, vp, ip, vp]),
         "fneus_lvis_blob_bytes": (C.c_size_t, []),
         "fneus_lvis_h16_pack": (C.c_int, [vp, vp, vp]),

@@ -1,6 +1,7 @@
 """Thin torch-tensor wrappers over the C ABI (device memory + stream plumbing only; no maths here)."""
 from __future__ import annotations
 
+import contextlib as _contextlib
 import ctypes as C
 from typing import Optional
 
@@ -1216,6 +1217,295 @@ def mlp_backward_input(jobs):
 def mlp_backward_params(jobs):
     """one launch: d_weight = (dy * act'(y))^T x and d_bias = its column sums for every job (both overwritten)"""
     _launch("fneus_mlp_backward_params", lib.fneus_mlp_backward_params, _mlp_jobs(jobs), len(jobs), _stream())
+
+
+# ---- layer norm, fp32 / bf16 / fp16 (csrc/norm_kernels.hip) ---------------------------------------------------------------------------
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _device_scope(t: torch.Tensor):
+    """the launches of an operator go to the device of its tensors, whichever is current"""
+    return _contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def _rows(t: torch.Tensor, name: str, like: Optional[torch.Tensor] = None, shape=None) -> torch.Tensor:
+    """a [rows, n] CUDA tensor of a supported type as the kernels read it: unit stride within a row, rows apart by at least n (another
+    layout -- a transposed or broadcast view -- is copied); `like`: the type and device it has to have"""
+    if t.dim() != 2 or t.dtype not in _DTYPES or not t.is_cuda:
+        raise ValueError(f"{name} must be a [rows, n] CUDA tensor of float32, bfloat16 or float16")
+    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+        raise ValueError(f"{name} must be of type {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must have the shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.is_contiguous():
+        return t
+    rows, n = t.shape
+    return t if (n <= 1 or t.stride(1) == 1) and (rows <= 1 or t.stride(0) >= n) else t.contiguous()
+
+
+def _ld(t: torch.Tensor) -> int:
+    return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
+
+
+def _vector(t: Optional[torch.Tensor], name: str, n: int, like: torch.Tensor, types) -> Optional[torch.Tensor]:
+    if t is None:
+        return None
+    if t.dim() != 1 or t.shape[0] != n or t.dtype not in types or t.device != like.device:
+        raise ValueError(f"{name} must be a [{n}] tensor of {' or '.join(str(d) for d in types)} on {like.device}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _norm_weights(weight, bias, x):
+    types = (x.dtype,) if x.dtype == torch.float32 else (x.dtype, torch.float32)
+    weight, bias = _vector(weight, "layer_norm: weight", x.shape[1], x, types), _vector(bias, "layer_norm: bias", x.shape[1], x, types)
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise ValueError("layer_norm: weight and bias must have one type")
+    t = weight if weight is not None else bias
+    return weight, bias, 0 if t is None else _DTYPES[t.dtype]
+
+
+def layer_norm_fwd(x, weight=None, bias=None, eps: float = 1e-5):
+    """x [rows, n] -> (y, mean [rows], rstd [rows]): y = (x - mean) rstd weight + bias over each row, rstd = 1 / sqrt(var + eps).
+    weight / bias [n]: x's type or float32, or None.  mean and rstd (float32) are what layer_norm_bwd takes."""
+    x = _rows(x, "layer_norm: x")
+    rows, n = x.shape
+    if n == 0:
+        raise ValueError("layer_norm: rows without values have no mean")
+    weight, bias, wtype = _norm_weights(weight, bias, x)
+    with _device_scope(x):
+        y = torch.empty_like(x, memory_format=torch.contiguous_format)
+        mean, rstd = torch.empty(2, rows, dtype=torch.float32, device=x.device).unbind(0)
+        _launch("fneus_layer_norm_fwd", lib.fneus_layer_norm_fwd, _ptr(x), _ld(x), _ptr(weight), _ptr(bias), _ptr(y), n, _ptr(mean), _ptr(rstd),
+                rows, n, eps, _DTYPES[x.dtype], wtype, _stream())
+    return y, mean, rstd
+
+
+def layer_norm_bwd(dy, x, weight, mean, rstd, need_params: bool = True):
+    """(dx, dweight, dbias) of layer_norm_fwd; dweight and dbias [n] in weight's type (float32 where there is no weight), summed over the
+    rows in a fixed order, or None without need_params"""
+    x = _rows(x, "layer_norm: x")
+    dy = _rows(dy, "layer_norm: dy", x, x.shape)
+    rows, n = x.shape
+    weight, _, wtype = _norm_weights(weight, None, x)
+    if weight is None and x.dtype != torch.float32:
+        wtype = 0
+    mean, rstd = _vector(mean, "layer_norm: mean", rows, x, (torch.float32,)), _vector(rstd, "layer_norm: rstd", rows, x, (torch.float32,))
+    ptype = torch.float32 if weight is None else weight.dtype
+    with _device_scope(x):
+        dx = torch.empty_like(x, memory_format=torch.contiguous_format)
+        dw = db = scratch = None
+        if need_params:
+            dw, db = torch.empty(2, n, dtype=ptype, device=x.device).unbind(0)
+            if rows == 0:
+                dw.zero_(), db.zero_()
+            else:
+                scratch = torch.empty(lib.fneus_layer_norm_bwd_scratch_floats(rows, n), dtype=torch.float32, device=x.device)
+        if rows:
+            _launch("fneus_layer_norm_bwd", lib.fneus_layer_norm_bwd, _ptr(dy), _ld(dy), _ptr(x), _ld(x), _ptr(weight), _ptr(mean), _ptr(rstd),
+                    _ptr(dx), n, _ptr(dw), _ptr(db), _ptr(scratch), rows, n, _DTYPES[x.dtype], wtype, _stream())
+    return dx, dw, db
+
+
+# ---- linear layer with bias, activation and residual in its epilogue (csrc/linear_kernels.hip) ------------------------------------------
+ACT_SOFTPLUS100, ACT_GELU, ACT_SILU = 4, 5, 6
+LINEAR_ACTS = {"none": ACT_NONE, "relu": ACT_RELU, "leaky": ACT_LEAKY02, "sigmoid": ACT_SIGMOID, "softplus": ACT_SOFTPLUS100,
+               "gelu": ACT_GELU, "silu": ACT_SILU}
+
+
+def _act_code(act) -> int:
+    code = LINEAR_ACTS.get(act, act) if isinstance(act, str) else act
+    if not isinstance(code, int) or not 0 <= code <= ACT_SILU:
+        raise ValueError(f"linear: act must be one of {sorted(LINEAR_ACTS)} (or its ACT_* code), got {act!r}")
+    return code
+
+
+def _linear_weight(weight, x):
+    if weight.dim() != 2 or weight.dtype != x.dtype or weight.device != x.device:
+        raise ValueError(f"linear: weight must be a [n_out, n_in] tensor of {x.dtype} on {x.device}")
+    if weight.shape[1] == 0 or weight.shape[0] == 0:
+        raise ValueError("linear: a weight without elements")
+    return weight if weight.is_contiguous() else weight.contiguous()
+
+
+def _linear_scratch(job, backward: int, device):
+    n = lib.fneus_linear_scratch_bytes(C.byref(job), backward)
+    if n <= 0:
+        return None
+    t = torch.empty(n, dtype=torch.uint8, device=device)
+    job.scratch, job.scratch_bytes = t.data_ptr(), n
+    return t
+
+
+def linear_fwd(x, weight, bias=None, act="none", residual=None, train: bool = False):
+    """(y, z): y = act(x weight^T + bias) + residual of x [rows, n_in], weight [n_out, n_in], bias [n_out], residual [rows, n_out], all of one
+    type (float32, bfloat16, float16); act: a key of LINEAR_ACTS or its code.  z: with train and an activation, the pre-activation
+    linear_bwd takes, else None."""
+    code = _act_code(act)
+    x = _rows(x, "linear: x")
+    weight = _linear_weight(weight, x)
+    rows, (n_out, n_in) = x.shape[0], weight.shape
+    if x.shape[1] != n_in:
+        raise ValueError(f"linear: x has {x.shape[1]} columns, weight takes {n_in}")
+    bias = _vector(bias, "linear: bias", n_out, x, (x.dtype,))
+    with _device_scope(x):
+        y = torch.empty(rows, n_out, dtype=x.dtype, device=x.device)
+        z = torch.empty_like(y) if train and code != ACT_NONE else None
+        job = _lib.FneusLinear(x=x.data_ptr(), weight=weight.data_ptr(), y=y.data_ptr(), rows=rows, ldx=_ld(x), n_in=n_in, n_out=n_out,
+                               act=code, dtype=_DTYPES[x.dtype])
+        if bias is not None:
+            job.bias = bias.data_ptr()
+        if residual is not None:
+            residual = _rows(residual, "linear: residual", x, (rows, n_out))
+            job.residual, job.ld_residual = residual.data_ptr(), _ld(residual)
+        if z is not None:
+            job.z = z.data_ptr()
+        if rows:
+            scratch = _linear_scratch(job, 0, x.device)      # noqa: F841  (kept until the launch is enqueued)
+            _launch("fneus_linear_fwd", lib.fneus_linear_fwd, C.byref(job), _stream())
+    return y, z
+
+
+def linear_bwd(dy, x, weight, z=None, act="none", need=(True, True, True)):
+    """(dx, dweight, dbias) of linear_fwd(..., train=True), each where `need` asks for it, else None; the residual's gradient is dy.
+    dbias [n_out] comes in the one type of the other arrays."""
+    code = _act_code(act)
+    x = _rows(x, "linear: x")
+    weight = _linear_weight(weight, x)
+    rows, (n_out, n_in) = x.shape[0], weight.shape
+    if x.shape[1] != n_in:
+        raise ValueError(f"linear: x has {x.shape[1]} columns, weight takes {n_in}")
+    dy = _rows(dy, "linear: dy", x, (rows, n_out))
+    if code != ACT_NONE:
+        if z is None:
+            raise ValueError("linear_bwd: an activation needs the z of linear_fwd(..., train=True)")
+        z = _rows(z, "linear: z", x, (rows, n_out)).contiguous()
+    with _device_scope(x):
+        dx = torch.empty(rows, n_in, dtype=x.dtype, device=x.device) if need[0] else None
+        dw = torch.empty(n_out, n_in, dtype=x.dtype, device=x.device) if need[1] else None
+        db = torch.empty(n_out, dtype=x.dtype, device=x.device) if need[2] else None
+        if rows == 0:
+            for t in (dw, db):
+                if t is not None:
+                    t.zero_()
+        elif any(need):
+            job = _lib.FneusLinear(x=x.data_ptr(), weight=weight.data_ptr(), dy=dy.data_ptr(), rows=rows, ldx=_ld(x), lddy=_ld(dy), n_in=n_in,
+                                   n_out=n_out, act=code, dtype=_DTYPES[x.dtype])
+            if code != ACT_NONE:
+                job.z = z.data_ptr()
+            if dx is not None:
+                job.dx = dx.data_ptr()
+            if dw is not None:
+                job.dweight = dw.data_ptr()
+            if db is not None:
+                job.dbias = db.data_ptr()
+            scratch = _linear_scratch(job, 1, x.device)      # noqa: F841
+            _launch("fneus_linear_bwd", lib.fneus_linear_bwd, C.byref(job), _stream())
+    return dx, dw, db
+
+
+# ---- Muon: momentum, orthogonalisation by Newton-Schulz products, step (csrc/muon_kernels.hip) -------------------------------------------
+NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+
+
+def _muon_prec(prec, dtype) -> int:
+    """fp32 matrices: PREC_PARITY (two fp16 terms, three products); 16-bit ones: PREC_H16 (one fp16 product)"""
+    if prec is None:
+        return PREC_PARITY if dtype == torch.float32 else PREC_H16
+    if prec not in (PREC_PARITY, PREC_H16):
+        raise ValueError("muon: prec must be PREC_PARITY or PREC_H16")
+    return prec
+
+
+def _muon_matrices(ts, name, like=None):
+    ts = list(ts)
+    for k, t in enumerate(ts):
+        ref = like[k] if like is not None else ts[0]
+        if not torch.is_tensor(t) or t.dim() != 2 or not t.is_cuda or t.dtype not in _DTYPES or t.dtype != ref.dtype or t.device != ref.device \
+                or not t.is_contiguous() or t.numel() == 0:
+            raise ValueError(f"muon: {name} must be contiguous, non-empty CUDA matrices of one supported type on one device")
+        if like is not None and t.shape != ref.shape:
+            raise ValueError(f"muon: {name}[{k}] is {tuple(t.shape)}, its parameter {tuple(ref.shape)}")
+    return ts
+
+
+def muon_adjust(adjust, rows: int, cols: int) -> float:
+    """the factor on the learning rate: "match_rms" 0.2 sqrt(max(rows, cols)) (an update of Adam's rms), "original" sqrt(max(1, rows / cols)),
+    or a number"""
+    if adjust == "match_rms":
+        return 0.2 * max(rows, cols) ** 0.5
+    if adjust == "original":
+        return max(1.0, rows / cols) ** 0.5
+    if isinstance(adjust, (int, float)) and not isinstance(adjust, bool):
+        return float(adjust)
+    raise ValueError('muon: adjust must be "match_rms", "original" or a number')
+
+
+def muon_jobs(params, grads, momenta, adjust="match_rms"):
+    """the table of muon_step for lists that stay: a caller that keeps it skips the checks of its tensors in every step"""
+    params = _muon_matrices(params, "params")
+    grads, momenta = _muon_matrices(grads, "grads", params), _muon_matrices(momenta, "momenta", params)
+    if not len(params) == len(grads) == len(momenta):
+        raise ValueError("muon: params, grads and momenta must be lists of one length")
+    if len({t.data_ptr() for t in params + grads + momenta}) != 3 * len(params):
+        raise ValueError("muon: a tensor appears twice among params, grads and momenta")
+    jobs = (_lib.FneusMuonJob * max(1, len(params)))()
+    for j, p, g, m in zip(jobs, params, grads, momenta):
+        j.grad, j.momentum, j.param = g.data_ptr(), m.data_ptr(), p.data_ptr()
+        j.rows, j.cols = p.shape
+        j.adjust = muon_adjust(adjust, *p.shape)
+    return jobs, len(params), (params[0] if params else None)
+
+
+def muon_launch(table, lr, momentum, nesterov, weight_decay, coefficients, steps, eps, prec, zero_grad):
+    jobs, n, like = table
+    if n == 0:
+        return
+    prec = _muon_prec(prec, like.dtype)
+    a, b, c = coefficients
+    with _device_scope(like):
+        scratch = torch.empty(lib.fneus_muon_scratch_bytes(jobs, n, prec), dtype=torch.uint8, device=like.device)
+        _launch("fneus_muon", lib.fneus_muon, jobs, n, _ptr(lr), momentum, int(nesterov), weight_decay, a, b, c, steps, eps, prec,
+                _DTYPES[like.dtype], int(zero_grad), _ptr(scratch), scratch.numel(), _stream())
+
+
+def muon_step(params, grads, momenta, lr, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0, adjust="match_rms",
+              coefficients=NS_COEFFICIENTS, steps: int = 5, eps: float = 1e-7, prec: Optional[int] = None, zero_grad: bool = False):
+    """One Muon update of every matrix, in place: m <- mu m + (1 - mu) g;  u = (1 - mu) g + mu m (nesterov) or m;
+    p <- p (1 - lr weight_decay) - lr adjust NS(u), NS as in newton_schulz.  params, grads, momenta: lists of contiguous matrices of one
+    type; lr: float32 device scalar (a captured step sees its changes) or a number; zero_grad clears the gradients after use."""
+    table = muon_jobs(params, grads, momenta, adjust)
+    if table[1] == 0:
+        return
+    like = table[2]
+    if not torch.is_tensor(lr):
+        lr = torch.full((), float(lr), dtype=torch.float32, device=like.device)
+    if lr.numel() != 1 or lr.dtype != torch.float32 or lr.device != like.device:
+        raise ValueError("muon: lr must be a float32 scalar on the parameters' device")
+    muon_launch(table, lr, momentum, nesterov, weight_decay, coefficients, steps, eps, prec, zero_grad)
+
+
+def newton_schulz(g, coefficients=NS_COEFFICIENTS, steps: int = 5, eps: float = 1e-7, prec: Optional[int] = None):
+    """The matrix g [rows, cols], or each of a stack [count, rows, cols], with its singular values taken towards 1: X = g / max(|g|_F, eps), then
+    `steps` times X <- a X + (b A + c A^2) X, A = X X^T (for rows > cols on the transpose).  -> a tensor of g's shape and type"""
+    if g.dim() not in (2, 3) or not g.is_cuda or g.dtype not in _DTYPES:
+        raise ValueError("newton_schulz: a CUDA matrix, or a stack of them, of float32, bfloat16 or float16")
+    prec = _muon_prec(prec, g.dtype)
+    g = g if g.is_contiguous() else g.contiguous()
+    with _device_scope(g):
+        out = torch.empty_like(g)
+        if g.numel() == 0:
+            return out
+        rows, cols = g.shape[-2:]
+        n, step = g.numel() // (rows * cols), rows * cols * g.element_size()
+        jobs = (_lib.FneusMuonJob * n)()
+        src, dst = g.data_ptr(), out.data_ptr()
+        for k, j in enumerate(jobs):
+            j.grad, j.out, j.rows, j.cols = src + k * step, dst + k * step, rows, cols
+        scratch = torch.empty(lib.fneus_muon_scratch_bytes(jobs, n, prec), dtype=torch.uint8, device=g.device)
+        a, b, c = coefficients
+        _launch("fneus_newton_schulz", lib.fneus_newton_schulz, jobs, n, a, b, c, steps, eps, prec, _DTYPES[g.dtype], _ptr(scratch),
+                scratch.numel(), _stream())
+    return out
 
 
 def outside_z(rays_o, rays_d, n_outside: int, n_samples: int, far=None, u=None):

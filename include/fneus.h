@@ -623,6 +623,43 @@ int fneus_composite_bwd(const float* rays_o, const float* rays_d, const float* m
                         float* d_bg_alpha /*[B][n+n_out] or NULL*/, float* d_bg_color /*or NULL*/,
                         const float* background_rgb /*as in the forward: a constant*/, int background_rows, fneus_stream_t stream);
 
+/* ---- layer norm over the last axis (beside the weight-norm fold: the normalisation of residual trunks) ------------------------------
+ * Not in the reference.  dtype: 0 fp32, 1 bf16, 2 fp16 (x, y, dy, dx); wtype: the type of weight / bias and of their gradients, dtype or 0.
+ * Rows of n values, row strides ld* >= n in elements, any alignment; weight / bias may be NULL (1 / 0).  Statistics and sums in fp32,
+ * outputs rounded once.  y = (x - mean) rstd w + b, rstd = 1 / sqrt(var + eps) (var: biased); mean, rstd [rows] are the backward's.
+ * rows == 0: nothing is done (forward), refused (backward).  NaN and infinities stay in their row (forward, dx). */
+int fneus_layer_norm_fwd(const void* x, long ldx, const void* weight, const void* bias, void* y, long ldy, float* mean, float* rstd,
+                         long rows, int n, float eps, int dtype, int wtype, fneus_stream_t stream);
+/* dx, and dweight / dbias [n] (either may be NULL; OVERWRITTEN) through `scratch` (fneus_layer_norm_bwd_scratch_floats(rows, n) floats):
+ * partial rows added in a fixed order, bit-reproducible. */
+int fneus_layer_norm_bwd(const void* dy, long lddy, const void* x, long ldx, const void* weight, const float* mean, const float* rstd,
+                         void* dx, long lddx, void* dweight, void* dbias, float* scratch, long rows, int n, int dtype, int wtype,
+                         fneus_stream_t stream);
+long fneus_layer_norm_bwd_scratch_floats(long rows, int n);
+
+/* ---- linear layer with bias, activation and residual in its epilogue (beside fneus_mlp_*: those take fp32 stacks of a few hundred rows) --
+ * Not in the reference.  y = act(x W^T + b) + residual for any row count, fp32, bf16 or fp16 (one type for every array), products on the
+ * matrix cores with fp32 sums (fp32 operands as three bf16 terms, six products: fp32's accuracy), rounded once.  Row-major; x, residual and dy
+ * have row strides in elements, any alignment; weight [n_out][n_in], y, z, dx, dweight are contiguous.
+ * act: 0 none, 1 ReLU, 2 LeakyReLU(0.2), 3 sigmoid, 4 softplus(beta 100), 5 GELU (erf), 6 SiLU.
+ * forward: x, weight, (bias), (residual) -> y and, where z is given, the pre-activation z [rows][n_out] (what the backward of act != 0 reads).
+ * backward: dy, x, weight, z -> dx [rows][n_in], dweight [n_out][n_in], dbias [n_out], each where given (OVERWRITTEN); the residual's gradient
+ * is dy.  Sums in a fixed order: bit-reproducible.  rows == 0: forward nothing, backward refused.  An fp32 infinity or NaN in an operand
+ * gives NaN wherever it takes part.  `scratch`: fneus_linear_scratch_bytes(job, backward) bytes, 16-byte aligned, not shared between calls in flight. */
+typedef struct FneusLinear {
+    const void *x, *weight, *bias, *residual;
+    void *y, *z;
+    const void* dy;
+    void *dx, *dweight, *dbias;
+    void* scratch;
+    long scratch_bytes;
+    long rows, ldx, ld_residual, lddy;
+    int n_in, n_out, act, dtype;   /* dtype: 0 fp32, 1 bf16, 2 fp16 */
+} FneusLinear;
+long fneus_linear_scratch_bytes(const FneusLinear* job /*host*/, int backward);
+int fneus_linear_fwd(const FneusLinear* job /*host*/, fneus_stream_t stream);
+int fneus_linear_bwd(const FneusLinear* job /*host*/, fneus_stream_t stream);
+
 /* ---- optimiser: torch.optim.Adam.step() over the whole model in one launch (exp_runner.py:108, 179-181) ---------- */
 /* segs: HOST array of contiguous parameter runs (32 per launch).  lr: device scalar.  step: device float[2] -- [0] the steps
  * taken so far (this update uses step[0] + 1 for the bias corrections and leaves it there), [1] scratch of the launch, zero
@@ -630,6 +667,27 @@ int fneus_composite_bwd(const float* rays_o, const float* rays_d, const float* m
  * gradient after use. */
 int fneus_adam(const FneusAdamSegment* segs, int n_segs, const float* lr, float* step, double beta1, double beta2,
                double eps, int zero_grad, fneus_stream_t stream);
+
+/* ---- optimiser of weight matrices: Muon (beside fneus_adam; not in the reference) ---------------------------------------------------------
+ * Newton-Schulz orthogonalisation of each matrix u [rows][cols]: X = u / max(|u|_F, eps), `steps` times  A = X X^T, X <- a X + (b A + c A^2) X
+ * (on the transpose where rows > cols).  prec 3: operands as two fp16 terms under power-of-two scales, three products (fp32's accuracy);
+ * prec 2: one fp16 product (11 bits; what a 16-bit matrix carries).  Sums in fp32, the norm in fp64.  A zero matrix gives zero.
+ * fneus_newton_schulz: out = NS(grad).  fneus_muon, in place:  momentum <- mu momentum + (1 - mu) grad;  u = (1 - mu) grad + mu momentum
+ * (nesterov) or momentum;  param <- param (1 - lr weight_decay) - lr adjust_j NS(u).  lr: device scalar.  dtype: of grad, momentum, param,
+ * out (0 fp32, 1 bf16, 2 fp16), all contiguous.  zero_grad != 0 clears each gradient after use.  jobs: HOST array, any number; no two may
+ * share memory.  `scratch`: fneus_muon_scratch_bytes bytes, 256-byte aligned, not shared between calls in flight. */
+typedef struct FneusMuonJob {
+    void *grad, *momentum, *param, *out;
+    int rows, cols;
+    float adjust;
+    int pad_;
+} FneusMuonJob;
+long fneus_muon_scratch_bytes(const FneusMuonJob* jobs /*host array*/, int n_jobs, int prec);
+int fneus_newton_schulz(const FneusMuonJob* jobs /*host array*/, int n_jobs, double a, double b, double c, int steps, double eps, int prec,
+                        int dtype, void* scratch, long scratch_bytes, fneus_stream_t stream);
+int fneus_muon(const FneusMuonJob* jobs /*host array*/, int n_jobs, const float* lr, double mu, int nesterov, double weight_decay, double a,
+               double b, double c, int steps, double eps, int prec, int dtype, int zero_grad, void* scratch, long scratch_bytes,
+               fneus_stream_t stream);
 
 /* ---- box calibration (bench.py `box`; not part of the reference's path) ------------------------------------------------------------
  * fneus_probe_mfma: 1024 x 4 waves issue iters x 16 v_mfma_f32_32x32x16_bf16 back to back on the 32 KiB of bf16 operands given (random

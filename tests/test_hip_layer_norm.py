@@ -1,0 +1,195 @@
+"""Layer norm (csrc/norm_kernels.hip) against the formula in float64, forward, backward and its refusals.
+
+Tolerances.  Outputs are rounded once to their type: at most eps(t) / 2 of the value.  Before that, fp32: a row's mean and centred sum of
+squares are sums of n terms (errors below (log-tree of <= 64 partial sums of <= 16 .. 64 terms) ~ 2^-24 x 64 of the sum of magnitudes); the
+normalised value inherits the mean's error divided by the spread.  With inputs of offset / spread <= 8 that is < 64 x 8 x 2^-24 = 3e-5 of a
+unit-variance value in the worst case; the bound used is 2e-5 of the largest magnitude plus the rounding of the output type."""
+import os
+import sys
+
+import pytest
+import torch
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+sys.path.insert(0, os.path.join(ROOT, "factored-neus_amd"))
+
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+# every team size and both ends of each, odd widths, single values, the streaming form
+WIDTHS = [1, 2, 7, 39, 255, 256, 257, 511, 513, 1024, 1031, 2049, 4096, 4099, 8193, 16384, 16411]
+
+
+def formula(x, w, b, eps, dy=None):
+    x, w, b = x.double(), w.double(), b.double()
+    mean = x.mean(1, keepdim=True)
+    r = 1.0 / torch.sqrt(((x - mean) ** 2).mean(1, keepdim=True) + eps)
+    xh = (x - mean) * r
+    y = xh * w + b
+    if dy is None:
+        return y, mean[:, 0], r[:, 0]
+    g = dy.double() * w
+    dx = r * (g - g.mean(1, keepdim=True) - xh * (g * xh).mean(1, keepdim=True))
+    return y, mean[:, 0], r[:, 0], dx, (dy.double() * xh).sum(0), dy.double().sum(0)
+
+
+def close(got, want, t, what, slack=2e-5):
+    scale = float(want.abs().max()) + 1e-30
+    lim = want.abs() * (torch.finfo(t).eps / 2) * 1.01 + slack * scale
+    err = (got.double().cpu() - want).abs()
+    assert bool((err <= lim).all()), (what, float((err - lim).max()), scale)
+
+
+def inputs(rows, n, t, seed=0, wt=None, device="cuda"):
+    g = torch.Generator().manual_seed(seed + 7 * n + rows)
+    x = (torch.randn(rows, n, generator=g) + torch.randn(rows, 1, generator=g) * 2).to(t)
+    w, b = (1 + 0.3 * torch.randn(n, generator=g)).to(wt or t), (0.3 * torch.randn(n, generator=g)).to(wt or t)
+    dy = torch.randn(rows, n, generator=g).to(t)
+    return [v.to(device) for v in (x, w, b, dy)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("n", WIDTHS)
+@pytest.mark.parametrize("rows", [1, 5, 67])
+def test_layer_norm_against_float64(t, n, rows):
+    from fneus import ops
+    x, w, b, dy = inputs(rows, n, t)
+    y, mean, rstd = ops.layer_norm_fwd(x, w, b, 1e-5)
+    dx, dw, db = ops.layer_norm_bwd(dy, x, w, mean, rstd)
+    assert y.dtype == dx.dtype == dw.dtype == db.dtype == t and mean.dtype == torch.float32
+    ref = formula(x.cpu(), w.cpu(), b.cpu(), 1e-5, dy.cpu())
+    for got, want, tt, what in zip((y, mean, rstd, dx, dw, db), ref, (t, torch.float32, torch.float32, t, t, t), ("y", "mean", "rstd", "dx", "dw", "db")):
+        if what == "dx" and n <= 2:
+            # (one or two values: the three terms of dx cancel to eps-size; the bound is of the terms that cancel, r |g|)
+            g = float((dy.double() * w.double()).abs().max()) * float(rstd.max())
+            assert float((got.double().cpu() - want).abs().max()) <= g * (2e-5 + torch.finfo(tt).eps / 2)
+            continue
+        close(got, want, tt, what)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", TYPES)
+def test_layer_norm_many_rows_and_strides(t):
+    """rows that the backward's workgroups take in several turns; row strides, an unaligned start, a transposed view, a broadcast cotangent"""
+    from fneus import ops
+    x, w, b, dy = inputs(20011, 96, t)
+    y, mean, rstd = ops.layer_norm_fwd(x, w, b)
+    dx, dw, db = ops.layer_norm_bwd(dy, x, w, mean, rstd)
+    for got, want, what in zip((y, dx, dw, db), [formula(x.cpu(), w.cpu(), b.cpu(), 1e-5, dy.cpu())[k] for k in (0, 3, 4, 5)], "y dx dw db".split()):
+        close(got, want, t, what)
+    # views: the same values, the same bits
+    wide = torch.zeros(20011, 131, dtype=t, device="cuda")
+    wide[:, 3:99] = x
+    assert torch.equal(ops.layer_norm_fwd(wide[:, 3:99], w, b)[0], y)
+    assert torch.equal(ops.layer_norm_fwd(x.t().contiguous().t(), w, b)[0], y)
+    wide_dy = torch.zeros(20011, 101, dtype=t, device="cuda")
+    wide_dy[:, 5:101] = dy
+    got = ops.layer_norm_bwd(wide_dy[:, 5:101], wide[:, 3:99], w, mean, rstd)
+    assert all(torch.equal(p, q) for p, q in zip(got, (dx, dw, db)))
+    one = dy[:1].expand(20011, 96)
+    assert all(torch.equal(p, q) for p, q in zip(ops.layer_norm_bwd(one, x, w, mean, rstd), ops.layer_norm_bwd(one.contiguous(), x, w, mean, rstd)))
+    again = ops.layer_norm_bwd(dy, x, w, mean, rstd)
+    assert all(torch.equal(p, q) for p, q in zip(again, (dx, dw, db)))          # fixed order of sums
+    assert ops.layer_norm_bwd(dy, x, w, mean, rstd, need_params=False)[1:] == (None, None)
+
+
+@pytest.mark.gpu
+def test_layer_norm_weight_types_and_none():
+    from fneus import ops
+    for t in (torch.bfloat16, torch.float16):
+        x, w, b, dy = inputs(33, 200, t, wt=torch.float32)
+        y, mean, rstd = ops.layer_norm_fwd(x, w, b)
+        dx, dw, db = ops.layer_norm_bwd(dy, x, w, mean, rstd)
+        ref = formula(x.cpu(), w.cpu(), b.cpu(), 1e-5, dy.cpu())
+        assert dw.dtype == db.dtype == torch.float32
+        close(y, ref[0], t, "y"), close(dx, ref[3], t, "dx"), close(dw, ref[4], torch.float32, "dw"), close(db, ref[5], torch.float32, "db")
+        y0, mean, rstd = ops.layer_norm_fwd(x)
+        one, zero = torch.ones(200), torch.zeros(200)
+        ref = formula(x.cpu(), one, zero, 1e-5, dy.cpu())
+        close(y0, ref[0], t, "y")
+        dx, dw, db = ops.layer_norm_bwd(dy, x, None, mean, rstd)
+        close(dx, ref[3], t, "dx"), close(dw, ref[4], torch.float32, "dw")
+        yb, _, _ = ops.layer_norm_fwd(x, None, b)
+        close(yb, ref[0] + b.double().cpu(), t, "y with a bias alone")
+
+
+@pytest.mark.gpu
+def test_layer_norm_extremes():
+    """NaN and infinities stay in their row; a constant row gives the bias; a large offset keeps its digits; no rows"""
+    from fneus import ops
+    x, w, b, dy = inputs(9, 300, torch.float32)
+    clean = ops.layer_norm_fwd(x, w, b)[0].clone()
+    bad = x.clone()
+    bad[2, 7], bad[5, 0] = float("nan"), float("inf")
+    y, mean, rstd = ops.layer_norm_fwd(bad, w, b)
+    keep = [r for r in range(9) if r not in (2, 5)]
+    assert torch.equal(y[keep], clean[keep]) and bool(torch.isnan(y[2]).all()) and bool(torch.isnan(y[5]).any())
+    dx = ops.layer_norm_bwd(dy, bad, w, mean, rstd)[0]
+    assert bool(torch.isfinite(dx[keep]).all()) and bool(torch.isnan(dx[2]).all())
+    y, mean, rstd = ops.layer_norm_fwd(torch.full((3, 300), 2.5, device="cuda"), w, b)
+    assert float((y - b).abs().max()) < 1e-6
+    far = torch.randn(4, 300, dtype=torch.float64) + 1.0e4                          # offset / spread 1e4: the input's own rounding is 1e-3 of it
+    xf = far.float()
+    close(ops.layer_norm_fwd(xf.cuda(), w, b)[0], formula(xf, w.cpu(), b.cpu(), 1e-5)[0], torch.float32, "offset", slack=1e-3)
+    y, mean, rstd = ops.layer_norm_fwd(x[:0], w, b)
+    assert y.shape == (0, 300) and mean.shape == (0,)
+    dx, dw, db = ops.layer_norm_bwd(dy[:0], x[:0], w, mean, rstd)
+    assert dx.shape == (0, 300) and float(dw.abs().max()) == 0.0 and float(db.abs().max()) == 0.0
+
+
+@pytest.mark.gpu
+def test_layer_norm_graph_and_streams():
+    from fneus import ops
+    x, w, b, dy = inputs(700, 256, torch.float32)
+    def run():
+        y, mean, rstd = ops.layer_norm_fwd(x, w, b)
+        return (y,) + ops.layer_norm_bwd(dy, x, w, mean, rstd)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for k in range(3):
+        x.copy_(torch.randn_like(x))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(out, run())), k
+
+
+def test_layer_norm_refusals_cpu():
+    from fneus import ops
+    x = torch.randn(4, 8)
+    with pytest.raises(ValueError):
+        ops.layer_norm_fwd(x)                                  # no CPU fallback
+
+
+def test_layer_norm_abi_refusals_cpu():
+    """the C entries check before they launch"""
+    import ctypes as C
+    from fneus._lib import lib
+    p = C.c_void_p(64)
+    f = lambda rows, n, ldx, ldy, dt, wt, x=p: lib.fneus_layer_norm_fwd(x, ldx, None, None, p, ldy, p, p, rows, n, 1e-5, dt, wt, None)  # noqa: E731
+    assert f(0, 8, 8, 8, 0, 0) == 0
+    for args in ((-1, 8, 8, 8, 0, 0), (4, 0, 8, 8, 0, 0), (4, 8, 7, 8, 0, 0), (4, 8, 8, 7, 0, 0), (4, 8, 8, 8, 3, 0), (4, 8, 8, 8, 0, 1),
+                 (4, 8, 8, 8, 1, 2), (1 << 31, 8, 8, 8, 0, 0)):
+        assert f(*args) == -2, args
+    assert f(4, 8, 8, 8, 0, 0, x=None) == -2
+    b = lambda rows, scratch, dy=p: lib.fneus_layer_norm_bwd(dy, 8, p, 8, None, p, p, p, 8, p, p, scratch, rows, 8, 0, 0, None)  # noqa: E731
+    assert b(0, p) == -2 and b(4, None) == -2 and b(4, p, dy=None) == -2
+    assert lib.fneus_layer_norm_bwd_scratch_floats(0, 8) == 0 and lib.fneus_layer_norm_bwd_scratch_floats(5, 8) == 16
+
+
+@pytest.mark.gpu
+def test_layer_norm_refusals():
+    from fneus import ops
+    x = torch.randn(4, 8, device="cuda")
+    w = torch.ones(8, device="cuda")
+    for bad in (lambda: ops.layer_norm_fwd(x[0]), lambda: ops.layer_norm_fwd(x.double()), lambda: ops.layer_norm_fwd(x, w[:7]),
+                lambda: ops.layer_norm_fwd(x, w.double()), lambda: ops.layer_norm_fwd(x, w.half()), lambda: ops.layer_norm_fwd(x, w.cpu()),
+                lambda: ops.layer_norm_fwd(x.half(), w.half(), w), lambda: ops.layer_norm_fwd(x[:, :0]),
+                lambda: ops.layer_norm_bwd(x[:3], x, w, w[:4], w[:4]), lambda: ops.layer_norm_bwd(x.half(), x, w, w[:4], w[:4]),
+                lambda: ops.layer_norm_bwd(x, x, w, w[:3], w[:4])):
+        with pytest.raises(ValueError):
+            bad()

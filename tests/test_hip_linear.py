@@ -1,0 +1,254 @@
+"""The linear layer with bias, activation and residual (csrc/linear_kernels.hip) against float64, forward, backward and its refusals.
+
+Tolerances, per element, with S = |x| |W|^T + |b| (or the product's own operands) in 64 bits:
+  rounding of the output          eps(t) / 2 |value|
+  fp32 sums of K terms            (4 + 2 sqrt(K)) 2^-23 S       (K roundings of at most 2^-24 of partial sums <= S, as a random walk, with margin 4;
+                                                                 the three-term form of fp32 drops 2^-24 of each product)
+  delta rounded to 16 bits        eps(t) / 2 of sum |delta| |W|  (a bf16 / fp16 operand of the backward's products: every term half a step)
+  the activation                  4 x 2^-23 |z| + its slope (<= 1.13) times the error of z
+The backward is compared with the formula at the z it is given."""
+import math
+import os
+import sys
+
+import pytest
+import torch
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+sys.path.insert(0, os.path.join(ROOT, "factored-neus_amd"))
+
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+ACTS = ["none", "relu", "leaky", "sigmoid", "softplus", "gelu", "silu"]
+# (rows, n_in, n_out): one row, the row kernel's last row and the first beyond it, one value, odd sizes, a tile's edges, the tiled kernel's
+# sizes on and off its borders, a long contraction of few columns (split) and few rows with a long contraction
+SIZES = [(1, 1, 1), (1, 512, 144), (1, 4099, 70), (3, 7, 5), (16, 256, 256), (17, 90, 256), (33, 63, 129), (100, 512, 512), (257, 31, 64),
+         (300, 65, 33), (640, 512, 384), (1000, 777, 1111), (2048, 256, 256), (1025, 520, 1032), (5000, 40, 24), (20000, 256, 128), (64, 4096, 96)]
+
+
+def act64(z, act):
+    return {"none": lambda: z, "relu": lambda: z.clamp(min=0), "leaky": lambda: torch.where(z > 0, z, 0.2 * z), "sigmoid": lambda: torch.sigmoid(z),
+            "softplus": lambda: torch.logaddexp(torch.zeros_like(z), 100 * z) / 100, "gelu": lambda: z * 0.5 * torch.special.erfc(-z * math.sqrt(0.5)),
+            "silu": lambda: z * torch.sigmoid(z)}[act]()
+
+
+def dact64(z, act):
+    s = torch.sigmoid(z)
+    return {"none": lambda: torch.ones_like(z), "relu": lambda: (z > 0).double(), "leaky": lambda: torch.where(z > 0, 1.0, 0.2).double(),
+            "sigmoid": lambda: s * (1 - s), "softplus": lambda: torch.sigmoid(100 * z),
+            "gelu": lambda: 0.5 * torch.special.erfc(-z * math.sqrt(0.5)) + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi),
+            "silu": lambda: s * (1 + z * (1 - s))}[act]()
+
+
+def inputs(rows, n_in, n_out, t, seed=0):
+    g = torch.Generator().manual_seed(seed + rows + 3 * n_in + 5 * n_out)
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    return [v.to(t).cuda() for v in (r(rows, n_in), r(n_out, n_in) / math.sqrt(n_in), 0.3 * r(n_out), r(rows, n_out), r(rows, n_out))]
+
+
+def check(got, want, lim, what):
+    err = (got.double() - want).abs()
+    bad = ~(err <= lim)
+    assert not bool(bad.any()), (what, float((err / lim.clamp(min=1e-300)).max()), int(bad.sum()), got.shape)
+
+
+def half(t):
+    return torch.finfo(t).eps / 2 * 1.01
+
+
+def sums(k):
+    return (4 + 2 * math.sqrt(k)) * 2.0 ** -23
+
+
+def forward_and_backward(rows, n_in, n_out, t, act, res, bias=True, need=(True, True, True)):
+    from fneus import ops
+    x, w, b, r, dy = inputs(rows, n_in, n_out, t)
+    b, r = (b if bias else None), (r if res else None)
+    y, z = ops.linear_fwd(x, w, b, act=act, residual=r, train=True)
+    assert (z is None) == (act == "none") and y.dtype == t
+    xd, wd = x.double(), w.double()
+    zd, S = xd @ wd.t(), xd.abs() @ wd.t().abs()
+    if bias:
+        zd, S = zd + b.double(), S + b.double().abs()
+    ez = sums(n_in) * S
+    want = act64(zd, act)
+    lim = 1.13 * ez + 4 * 2.0 ** -23 * (zd.abs() + want.abs())
+    if res:
+        want = want + r.double()
+        lim = lim + 2.0 ** -23 * want.abs()
+    check(y, want, lim + half(t) * (want.abs() + lim) + torch.finfo(t).smallest_normal, "y")
+    if z is not None:
+        check(z, zd, ez + half(t) * (zd.abs() + ez) + torch.finfo(t).smallest_normal, "z")
+    dx, dw, db = ops.linear_bwd(dy, x, w, z, act=act, need=need)
+    d = dy.double() * (dact64(z.double(), act) if z is not None else 1.0)
+    # the derivative in fp32: exp / erf to a few 2^-24, and softplus' argument 100 z
+    ed = dy.double().abs() * 8 * 2.0 ** -23 * (1 + (100 * z.double().abs()).clamp(max=20) * (act == "softplus") if z is not None else 1)
+    op = d.abs() * half(t) * (t != torch.float32) + ed
+    tiny = torch.finfo(t).smallest_normal
+    for got, want, lim, k, what in ((dx, d @ wd, (op @ wd.abs()), n_out, "dx"), (dw, d.t() @ xd, (op.t() @ xd.abs()), rows, "dw"),
+                                    (db, d.sum(0), ed.sum(0), rows, "db")):
+        if got is None:
+            continue
+        total = {"dx": d.abs() @ wd.abs(), "dw": d.abs().t() @ xd.abs(), "db": d.abs().sum(0)}[what]
+        lim = lim + sums(k) * total
+        flush = tiny * {"dx": wd.abs().sum(0)[None, :], "dw": xd.abs().sum(0)[None, :], "db": torch.zeros_like(want)}[what] * (t == torch.float16)
+        check(got, want, lim + half(t) * (want.abs() + lim) + tiny + flush, what)      # (fp16: operands below its normal range count as zero)
+    assert [g is not None for g in (dx, dw, db)] == list(need)
+    return y, z, dx, dw, db
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("size", SIZES, ids=str)
+def test_linear_sizes(t, size):
+    forward_and_backward(*size, t, "gelu", True)
+    forward_and_backward(*size, t, "none", False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("size", [(5, 70, 40), (200, 130, 77), (640, 512, 384)], ids=str)
+def test_linear_activations(t, act, size):
+    forward_and_backward(*size, t, act, False, bias=False)
+    forward_and_backward(*size, t, act, True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("size", [(9, 40, 24), (150, 66, 130), (4096, 256, 256)], ids=str)
+def test_linear_each_gradient_alone(t, size):
+    full = forward_and_backward(*size, t, "silu", False)[2:]
+    for k in range(3):
+        got = forward_and_backward(*size, t, "silu", False, need=tuple(i == k for i in range(3)))[2:]
+        assert torch.equal(got[k], full[k])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("size", [(7, 96, 40), (130, 96, 72), (3000, 256, 192)], ids=str)
+def test_linear_views_and_repeats(t, size):
+    """row strides, unaligned starts, transposed and broadcast views: the same values; the same bits in every run"""
+    from fneus import ops
+    rows, n_in, n_out = size
+    x, w, b, r, dy = inputs(*size, t)
+    y, z = ops.linear_fwd(x, w, b, act="silu", residual=r, train=True)
+    g = ops.linear_bwd(dy, x, w, z, act="silu")
+    wide = lambda v, pad: torch.cat([torch.full_like(v[:, :1], 7.0), v, v[:, :pad]], 1)[:, 1:1 + v.shape[1]]  # noqa: E731
+    xs, rs, ds = wide(x, 6), wide(r, 3), wide(dy, 5)
+    for xv, rv, dv in ((xs, rs, ds), (x.t().contiguous().t(), r.t().contiguous().t(), dy.t().contiguous().t())):
+        y2, z2 = ops.linear_fwd(xv, w, b, act="silu", residual=rv, train=True)
+        g2 = ops.linear_bwd(dv, xv, w, z2, act="silu")
+        for p, q in zip((y2, z2) + g2, (y, z) + g):
+            scale = float(q.double().abs().max())
+            assert float((p.double() - q.double()).abs().max()) <= scale * (2 * torch.finfo(t).eps + 2e-5)
+        assert torch.equal(ops.linear_fwd(xv, w, b, act="silu", residual=rv)[0], y2)
+    y3, _ = ops.linear_fwd(x, w, b, act="silu", residual=r)
+    assert torch.equal(y3, y)
+    assert all(torch.equal(p, q) for p, q in zip(ops.linear_bwd(dy, x, w, z, act="silu"), g))
+    one = dy[:1].expand(rows, n_out)
+    assert all(torch.equal(p, q) for p, q in zip(ops.linear_bwd(one, x, w, z, act="silu"), ops.linear_bwd(one.contiguous(), x, w, z, act="silu")))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [(6, 64, 48), (200, 96, 80), (2048, 512, 512)], ids=str)
+def test_linear_nan_stays_in_its_row(size):
+    from fneus import ops
+    x, w, b, r, _ = inputs(*size, torch.float32)
+    for t in TYPES:
+        xt, wt, bt, rt = (v.to(t) for v in (x, w, b, r))
+        clean = ops.linear_fwd(xt, wt, bt, act="relu", residual=rt)[0]
+        bad = xt.clone()
+        bad[3, 5], bad[1, 0] = float("nan"), float("inf")
+        y = ops.linear_fwd(bad, wt, bt, act="none", residual=rt)[0]
+        assert bool(torch.isnan(y[3]).all()) and not bool(torch.isfinite(y[1]).any())
+        yr = ops.linear_fwd(bad, wt, bt, act="relu", residual=rt)[0]
+        keep = [k for k in range(size[0]) if k not in (1, 3)]
+        assert torch.equal(yr[keep], clean[keep]) and bool(torch.isnan(yr[3]).all())
+
+
+@pytest.mark.gpu
+def test_linear_gradient_against_differences():
+    """<dL/dx, v> against (L(x + h v) - L(x - h v)) / 2h in 64 bits, through the kernel's own forward values in fp32"""
+    from fneus import ops
+    x, w, b, r, dy = inputs(40, 48, 56, torch.float32)
+    for act in ("sigmoid", "gelu", "silu", "softplus"):
+        y, z = ops.linear_fwd(x, w, b, act=act, residual=r, train=True)
+        dx, dw, db = ops.linear_bwd(dy, x, w, z, act=act)
+        loss = lambda xx, ww, bb: float((act64(xx @ ww.t() + bb, act) * dy.double()).sum())  # noqa: E731
+        h = 1e-6
+        for grad, which in ((dx, 0), (dw, 1), (db, 2)):
+            args = [x.double(), w.double(), b.double()]
+            v = torch.randn(grad.shape, generator=torch.Generator().manual_seed(5), dtype=torch.float64).cuda()
+            up, dn = list(args), list(args)
+            up[which], dn[which] = args[which] + h * v, args[which] - h * v
+            num = (loss(*up) - loss(*dn)) / (2 * h)
+            ref = float((grad.double() * v).sum())
+            scale = float((grad.double().abs() * v.abs()).sum())
+            assert abs(num - ref) <= 1e-5 * scale, (act, which, num, ref)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", TYPES)
+def test_linear_graph_and_no_rows(t):
+    from fneus import ops
+    for size in ((200, 130, 77), (2048, 512, 512)):
+        x, w, b, r, dy = inputs(*size, t)
+        def run():
+            y, z = ops.linear_fwd(x, w, b, act="gelu", residual=r, train=True)
+            return (y, z) + ops.linear_bwd(dy, x, w, z, act="gelu")
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            run()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = run()
+        for k in range(3):
+            x.copy_(torch.randn(x.shape, device="cuda"))
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(p, q) for p, q in zip(out, run())), k
+    y, z = ops.linear_fwd(x[:0], w, b, act="gelu", residual=r[:0], train=True)
+    assert y.shape == (0, 512)
+    dx, dw, db = ops.linear_bwd(dy[:0], x[:0], w, z, act="gelu")
+    assert dx.shape == (0, 512) and float(dw.abs().max()) == 0.0 and float(db.abs().max()) == 0.0
+
+
+def test_linear_abi_refusals_cpu():
+    import ctypes as C
+    from fneus._lib import lib, FneusLinear
+    ok = dict(x=64, weight=64, y=64, rows=0, ldx=8, n_in=8, n_out=8, act=0, dtype=0)
+    fwd = lambda **k: lib.fneus_linear_fwd(C.byref(FneusLinear(**dict(ok, **k))), None)  # noqa: E731
+    assert fwd() == 0                                                # no rows: nothing is launched
+    for k in (dict(rows=-1), dict(n_in=0), dict(n_out=0), dict(act=7), dict(act=-1), dict(dtype=3), dict(rows=4, x=None), dict(rows=4, weight=None),
+              dict(rows=4, y=None), dict(rows=4, ldx=7), dict(rows=4, residual=64, ld_residual=7), dict(rows=1 << 31), dict(n_in=1 << 23)):
+        assert fwd(**k) == -2, k
+    okb = dict(ok, rows=4, dy=64, lddy=8, dx=64, dweight=64, dbias=64)
+    bwd = lambda **k: lib.fneus_linear_bwd(C.byref(FneusLinear(**dict(okb, **k))), None)  # noqa: E731
+    for k in (dict(rows=0), dict(dy=None), dict(lddy=7), dict(act=1), dict(weight=None), dict(x=None), dict(ldx=7),
+              dict(dx=None, dweight=None, dbias=None)):
+        assert bwd(**k) == -2, k
+    assert lib.fneus_linear_fwd(None, None) == -2
+
+
+def test_linear_refusals_cpu():
+    from fneus import ops
+    x = torch.randn(4, 8)
+    with pytest.raises(ValueError):
+        ops.linear_fwd(x, torch.randn(3, 8))
+    with pytest.raises(ValueError):
+        ops.linear_fwd(x, torch.randn(3, 8), act="tanh")
+
+
+@pytest.mark.gpu
+def test_linear_refusals():
+    from fneus import ops
+    x, w, b, r, dy = inputs(4, 8, 6, torch.float32)
+    for bad in (lambda: ops.linear_fwd(x, w[:, :7]), lambda: ops.linear_fwd(x, w.half()), lambda: ops.linear_fwd(x, w, b.half()),
+                lambda: ops.linear_fwd(x, w, b[:5]), lambda: ops.linear_fwd(x, w, b, residual=r[:, :5]), lambda: ops.linear_fwd(x, w, b, act=7),
+                lambda: ops.linear_fwd(x[0], w), lambda: ops.linear_fwd(x.double(), w.double()), lambda: ops.linear_fwd(x, w.cpu()),
+                lambda: ops.linear_bwd(dy, x, w, None, act="gelu"), lambda: ops.linear_bwd(dy[:3], x, w), lambda: ops.linear_bwd(dy.half(), x, w),
+                lambda: ops.linear_fwd(x, w[:0])):
+        with pytest.raises(ValueError):
+            bad()

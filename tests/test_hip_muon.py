@@ -1,0 +1,214 @@
+"""Muon (csrc/muon_kernels.hip): the momentum, the Newton-Schulz orthogonalisation and the step against float64, and the refusals.
+
+Tolerances, of the orthogonalised matrix in the Frobenius norm.  prec 3 holds every operand to 22 bits (2^-23 relative, half a step), prec 2
+to 11 (2^-12).  A step rounds three operands; the relative error passes a step with at most |p'(s)| s / |p(s)| <= 1.6 once the singular values
+are in the polynomial's interval and <= 1 before it.  15 roundings x 2.5: 5e-6 and (2^-12 / sqrt 3 x 15 x 2.5) 5e-3; the bounds are 1e-5 and
+5e-3, plus the rounding of the output type (its half step)."""
+import math
+import os
+import sys
+
+import pytest
+import torch
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+sys.path.insert(0, os.path.join(ROOT, "factored-neus_amd"))
+
+C3 = (3.4445, -4.7750, 2.0315)
+SIZES = [(1, 1), (1, 300), (2, 3), (39, 256), (64, 64), (63, 65), (256, 256), (217, 256), (512, 63), (144, 512), (256, 1), (129, 1000), (700, 640)]
+
+
+def ns64(u, steps=5, eps=1e-7, coef=C3):
+    a, b, c = coef
+    x = u.double()
+    x = x / max(float(x.norm()), eps)
+    if x.shape[0] > x.shape[1]:
+        return ns64(u.t(), steps, eps, coef).t()
+    for _ in range(steps):
+        g = x @ x.t()
+        x = a * x + (b * g + c * (g @ g)) @ x
+    return x
+
+
+def matrix(rows, cols, seed=0, spread=0.7):
+    g = torch.Generator().manual_seed(seed + 1000 * rows + cols)
+    m = torch.randn(rows, cols, generator=g)
+    return m * torch.exp(spread * (torch.randn(rows, 1, generator=g) + torch.randn(1, cols, generator=g))) * 1e-3
+
+
+def bound(prec, t):
+    return (1e-5 if prec == 3 else 5e-3) + torch.finfo(t).eps / 2
+
+
+def off(got, want):
+    return float((got.double().cpu() - want).norm() / want.norm())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("size", SIZES, ids=str)
+def test_newton_schulz_against_float64(t, size):
+    from fneus import ops
+    g = (matrix(*size) * (100 if t == torch.float16 else 1)).to(t)
+    want = ns64(g)
+    for prec in (None, ops.PREC_PARITY, ops.PREC_H16):
+        got = ops.newton_schulz(g.cuda(), prec=prec)
+        assert got.dtype == t and got.shape == g.shape
+        p = prec or (3 if t == torch.float32 else 2)
+        assert off(got, want) <= bound(p, t), (prec, off(got, want))
+
+
+@pytest.mark.gpu
+def test_newton_schulz_large_and_stacked():
+    """the 128-wide tiles, more matrices than one round of launches takes, every matrix as on its own, the same bits in every run"""
+    from fneus import ops
+    g = matrix(1537, 1800).cuda()
+    want = ns64(g)
+    got = ops.newton_schulz(g)
+    assert off(got, want.cpu()) <= bound(3, torch.float32)
+    assert torch.equal(ops.newton_schulz(g), got)
+    got = ops.newton_schulz(g.t().contiguous())
+    assert off(got, want.t().cpu()) <= bound(3, torch.float32)
+    stack = torch.stack([matrix(40, 30, seed=k) for k in range(70)]).cuda()
+    out = ops.newton_schulz(stack)
+    for k in (0, 31, 32, 69):
+        assert torch.equal(out[k], ops.newton_schulz(stack[k]))
+        assert off(out[k], ns64(stack[k].cpu())) <= bound(3, torch.float32)
+
+
+@pytest.mark.gpu
+def test_newton_schulz_properties():
+    """singular values in the polynomial's interval, the singular vectors kept; scale-free; other polynomials and step counts; zero, tiny,
+    huge, rank-deficient and NaN matrices"""
+    from fneus import ops
+    g = matrix(96, 130).cuda()
+    o = ops.newton_schulz(g)
+    s = torch.linalg.svdvals(o.double())
+    assert 0.6 < float(s.min()) and float(s.max()) < 1.25
+    for f in (2.0 ** 40, 2.0 ** -40):
+        assert torch.equal(ops.newton_schulz(g * f, eps=1e-30), ops.newton_schulz(g, eps=1e-30))
+    assert off(ops.newton_schulz(g * 1e30), ns64(g.cpu())) <= 2e-5           # |g|^2 beyond fp32's range
+    for coef, steps in (((2.0, -1.5, 0.5), 1), ((1.875, -1.25, 0.375), 12), ((8.28, -23.6, 17.3), 1)):
+        assert off(ops.newton_schulz(g, coefficients=coef, steps=steps), ns64(g.cpu(), steps, coef=coef)) <= 1e-5
+    assert float(ops.newton_schulz(torch.zeros(20, 30, device="cuda")).abs().max()) == 0.0
+    tiny = torch.full((4, 4), 1e-12, device="cuda")                           # below eps: divided by eps, not by the norm
+    assert off(ops.newton_schulz(tiny), ns64(tiny.cpu())) <= 1e-5
+    # rank 3: what rounding adds in the directions without a singular value grows by a^5 = 485, a^4 = 141, a^3 = 41, ... from the step it
+    # enters at.  |X|_F is 1 at first and at most 1.2 sqrt 3 = 2.1 later, half a step of 22 bits is 2^-23 of it, |NS|_F >= 0.7 sqrt 3 = 1.2:
+    # 2^-23 (485 + 2.1 (141 + 41 + 12 + 3.4 + 1)) / 1.2 = 9e-5 (fp32 arithmetic: half of it)
+    low = (matrix(200, 3) @ matrix(3, 150)).cuda()
+    assert off(ops.newton_schulz(low), ns64(low.cpu())) <= 9e-5
+    bad = g.clone()
+    bad[3, 4] = float("nan")
+    assert bool(torch.isnan(ops.newton_schulz(bad)).all())
+    assert ops.newton_schulz(g[:0]).shape == (0, 130)
+    view = torch.randn(50, 40, device="cuda").t()
+    assert torch.equal(ops.newton_schulz(view), ops.newton_schulz(view.contiguous()))
+
+
+def step64(p, g, m, lr, mu, nesterov, wd, adj):
+    m = mu * m.double() + (1 - mu) * g.double()
+    u = (1 - mu) * g.double() + mu * m if nesterov else m
+    return p.double() * (1 - lr * wd) - lr * adj * ns64(u), m
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nesterov", [True, False])
+def test_muon_step_against_float64(nesterov):
+    from fneus import ops
+    sizes = [(256, 256), (512, 63), (144, 512), (512, 512), (3, 1), (256, 90)]
+    ps, gs, ms = ([matrix(*s, seed=k).cuda() for s in sizes] for k in (1, 2, 3))
+    want = []
+    for p, g, m in zip(ps, gs, ms):
+        adj = ops.muon_adjust("original", *p.shape)
+        want.append(step64(p.cpu(), g.cpu(), m.cpu(), 0.03, 0.9, nesterov, 0.1, adj))
+    lr = torch.full((), 0.03, device="cuda")
+    ops.muon_step(ps, gs, ms, lr, momentum=0.9, nesterov=nesterov, weight_decay=0.1, adjust="original", zero_grad=True)
+    for (wp, wm), p, m, g in zip(want, ps, ms, gs):
+        assert off(m, wm) <= 4 * 2.0 ** -24
+        assert off(p, wp) <= 1e-5 + 4 * 2.0 ** -24
+        assert float(g.abs().max()) == 0.0
+    assert abs(ops.muon_adjust("match_rms", 4, 100) - 2.0) < 1e-12 and ops.muon_adjust(0.5, 3, 3) == 0.5
+
+
+@pytest.mark.gpu
+def test_muon_step_sixteen_bits_and_frozen_gradients():
+    from fneus import ops
+    for t in (torch.bfloat16, torch.float16):
+        p, g, m = (matrix(120, 200, seed=k).mul(200).to(t).cuda() for k in (1, 2, 3))
+        keep = g.clone()
+        p0, m0 = p.cpu(), m.cpu()
+        ops.muon_step([p], [g], [m], 0.02, adjust=1.0)
+        assert torch.equal(g, keep)
+        wm = (0.95 * m0.double() + (1 - 0.95) * keep.cpu().double())
+        assert off(m, wm) <= torch.finfo(t).eps / 2 + 1e-6
+        wp = p0.double() - 0.02 * ns64((1 - 0.95) * keep.cpu().double() + 0.95 * m.cpu().double())
+        assert off(p, wp) <= 5e-3 + torch.finfo(t).eps / 2
+
+
+@pytest.mark.gpu
+def test_muon_step_in_a_graph():
+    """replayed with new gradients and a new learning rate between the replays, against the eager step"""
+    from fneus import ops
+    sizes = [(256, 256), (100, 60), (512, 144)]
+    ps, gs, ms = ([matrix(*s, seed=k).cuda() for s in sizes] for k in (1, 2, 3))
+    lr = torch.full((), 0.02, device="cuda")
+    pe, me = [p.clone() for p in ps], [m.clone() for m in ms]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ops.muon_step(ps, gs, ms, lr)
+    torch.cuda.current_stream().wait_stream(side)
+    ops.muon_step(pe, gs, me, lr)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.muon_step(ps, gs, ms, lr)
+    for k in range(3):
+        for g in gs:
+            g.copy_(torch.randn_like(g))
+        lr.fill_(0.01 / (k + 1))
+        graph.replay()
+        torch.cuda.synchronize()
+        ops.muon_step(pe, gs, me, lr)
+        assert all(torch.equal(a, b) for a, b in zip(ps + ms, pe + me)), k
+
+
+def test_muon_refusals_cpu():
+    import ctypes as C
+    from fneus import ops
+    from fneus._lib import lib, FneusMuonJob
+    with pytest.raises(ValueError):
+        ops.newton_schulz(torch.randn(3, 3))
+    with pytest.raises(ValueError):
+        ops.muon_step([torch.randn(3, 3)], [torch.randn(3, 3)], [torch.randn(3, 3)], 0.1)
+    ops.muon_step([], [], [], 0.1)
+    jobs = (FneusMuonJob * 1)()
+    jobs[0].grad, jobs[0].out, jobs[0].rows, jobs[0].cols = 256, 256, 4, 4
+    need = lib.fneus_muon_scratch_bytes(jobs, 1, 3)
+    assert need > 0 and need > lib.fneus_muon_scratch_bytes(jobs, 1, 2)
+    ns = lambda coef=C3, steps=5, eps=1e-7, prec=3, dtype=0, scratch=256, n=None, jobs=jobs: lib.fneus_newton_schulz(  # noqa: E731
+        jobs, 1, *coef, steps, eps, prec, dtype, C.c_void_p(scratch), need if n is None else n, None)
+    for k in (dict(steps=0), dict(steps=65), dict(eps=0.0), dict(prec=1), dict(dtype=3), dict(scratch=None), dict(scratch=264), dict(n=need - 1),
+              dict(coef=(9.0, 9.0, 9.0)), dict(coef=(float("nan"), 1.0, 1.0))):
+        assert ns(**k) == -2, k
+    for field, value in (("rows", 0), ("cols", -1), ("rows", 70000), ("grad", None), ("out", None)):
+        bad = (FneusMuonJob * 1)()
+        bad[0].grad, bad[0].out, bad[0].rows, bad[0].cols = 256, 256, 4, 4
+        setattr(bad[0], field, value)
+        assert ns(jobs=bad, n=1 << 40) == -2, field
+    assert lib.fneus_muon(jobs, 1, C.c_void_p(256), 0.9, 1, 0.0, *C3, 5, 1e-7, 3, 0, 0, C.c_void_p(256), need, None) == -2      # no momentum, no parameter
+
+
+@pytest.mark.gpu
+def test_muon_refusals():
+    from fneus import ops
+    p, g, m = (torch.randn(6, 5, device="cuda") for _ in range(3))
+    for bad in (lambda: ops.muon_step([p], [g[:5]], [m], 0.1), lambda: ops.muon_step([p], [g], [], 0.1), lambda: ops.muon_step([p], [p], [m], 0.1),
+                lambda: ops.muon_step([p[0]], [g[0]], [m[0]], 0.1), lambda: ops.muon_step([p], [g.half()], [m], 0.1),
+                lambda: ops.muon_step([p.t()], [g.t()], [m.t()], 0.1), lambda: ops.muon_step([p, p], [g, m], [m, g], 0.1),
+                lambda: ops.muon_step([p], [g], [m], torch.ones(2, device="cuda")), lambda: ops.muon_step([p], [g], [m], 0.1, adjust="other"),
+                lambda: ops.muon_step([p], [g], [m], 0.1, prec=1), lambda: ops.newton_schulz(p.double()), lambda: ops.newton_schulz(p[0])):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(RuntimeError):
+        ops.newton_schulz(p, steps=0)
