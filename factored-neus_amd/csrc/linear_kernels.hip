@@ -1,7 +1,8 @@
 // Linear layer with bias, activation and residual in its epilogue, forward and backward, fp32 / bf16 / fp16:
 //   z = x W^T + b,  y = act(z) + res;      delta = dy act'(z),  dx = delta W,  dW = delta^T x,  db = column sums of delta
 // The three products are one form, D(i, j) = sum_k A(i, k) B(j, k), with either operand stored along k or along its rows.
-#include "linear_act.h"
+#include <stdlib.h>
+#include "mm_engine.h"
 #include "fneus_kernels.h"
 
 namespace fneus {
@@ -189,6 +190,376 @@ __global__ void __launch_bounds__(512) linear_row_kernel(LinProduct P) {
     }
 }
 
+// ---- the tiled form ------------------------------------------------------------------------------------------------------------
+struct LinTiled {
+    MmOperand a, b;
+    const void *bias, *res;
+    void *d, *z;
+    float* partial;              // [splits][ni][nj]
+    long ni, ldres, ldd;
+    int nj, k_tiles, tail, act, splits, tiles_i, tiles_j, pad_;
+};
+
+enum { LIN_EPI_FWD = 0, LIN_EPI_STORE = 1, LIN_EPI_PART = 2 };
+
+template <class T> struct Quad;
+template <> struct Quad<float> { typedef float type __attribute__((ext_vector_type(4), aligned(4))); };
+template <> struct Quad<__bf16> { typedef __bf16 type __attribute__((ext_vector_type(4), aligned(2))); };
+template <> struct Quad<_Float16> { typedef _Float16 type __attribute__((ext_vector_type(4), aligned(2))); };
+
+template <class T>
+FN_DEV void quad_load(const T* p, int valid, float (&v)[4]) {
+    if (valid >= 4) {
+        const typename Quad<T>::type q = *reinterpret_cast<const typename Quad<T>::type*>(p);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = (float)q[k];
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = k < valid ? (float)p[k] : 0.0f;
+    }
+}
+template <class T>
+FN_DEV void quad_store(T* p, int valid, const float (&v)[4]) {
+    if (valid >= 4) {
+        typename Quad<T>::type q;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) q[k] = (T)v[k];
+        *reinterpret_cast<typename Quad<T>::type*>(p) = q;
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (k < valid) p[k] = (T)v[k];
+    }
+}
+
+// bias, pre-activation, activation, residual of four consecutive outputs of row i
+template <class T>
+FN_DEV void lin_finish(const T* bias, const T* res, T* d, T* z, int act, int valid, float (&v)[4]) {
+    float q[4];
+    if (bias) {
+        quad_load(bias, valid, q);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] += q[k];
+    }
+    if (z) quad_store(z, valid, v);
+    if (act) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = lin_act(v[k], act);
+    }
+    if (res) {
+        quad_load(res, valid, q);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] += q[k];
+    }
+    quad_store(d, valid, v);
+}
+
+// The epilogue goes through LDS, 32 rows of a wave at a time: the accumulators hold a column of 32 rows in a register, memory wants rows;
+// and the loop that finishes four outputs exists once, not once per register.
+template <class Cfg, class T, bool AKM, bool BKM, int EPI>
+__global__ void __launch_bounds__(Cfg::THREADS, 2) linear_tiled_kernel(LinTiled P) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char mm_smem[];
+    const long tiles = (long)P.tiles_i * P.tiles_j;
+    const long t = mm_spread(blockIdx.x, tiles * P.splits);
+    const int split = (int)(t / tiles);
+    int ti, tj;
+    mm_tile(t - split * tiles, P.tiles_i, P.tiles_j, ti, tj);
+    const long i0 = (long)ti * Cfg::BM, j0 = (long)tj * Cfg::BN;
+    const int it0 = (int)((long)P.k_tiles * split / P.splits), it1 = (int)((long)P.k_tiles * (split + 1) / P.splits);
+    f32x16 acc[Cfg::MI][Cfg::NJ];
+    mm_run<Cfg, T, AKM, BKM, false, true>(mm_smem, P.a, P.b, i0, P.ni, j0, P.nj, P.k_tiles, P.tail, kMmOne, it0, it1, split == P.splits - 1, 1.0f, acc);
+    constexpr int STRIDE = Cfg::WN + 4;
+    static_assert(Cfg::WAVES * 32 * STRIDE * 4 <= Cfg::LDS, "the epilogue's rows fit the ring");
+    float* rows = reinterpret_cast<float*>(mm_smem) + mm_wave() * 32 * STRIDE;
+    const int lane = threadIdx.x & 63;
+    __syncthreads();                                  // (everyone has read the last stage)
+#pragma unroll
+    for (int m = 0; m < Cfg::MI; ++m) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int n = 0; n < Cfg::NJ; ++n)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                f32x4 q;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) q[k] = acc[m][n][4 * g + k];
+                *reinterpret_cast<f32x4*>(rows + (lane & 31) * STRIDE + 32 * n + 8 * g + 4 * (lane >> 5)) = q;
+            }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        constexpr int QUADS = Cfg::WN / 4;
+#pragma unroll 2
+        for (int s = 0; s < 32 * QUADS / 64; ++s) {
+            const int at = s * 64 + lane, r = at / QUADS, c = 4 * (at % QUADS);
+            const long i = i0 + mm_wave_i<Cfg>() + 32 * m + r;
+            const long j = j0 + mm_wave_j<Cfg>() + c;
+            if (i >= P.ni || j >= P.nj) continue;
+            const int valid = (int)(P.nj - j);
+            const f32x4 q = *reinterpret_cast<const f32x4*>(rows + r * STRIDE + c);
+            float v[4] = {q[0], q[1], q[2], q[3]};
+            if constexpr (EPI == LIN_EPI_FWD)
+                lin_finish<T>(P.bias ? (const T*)P.bias + j : nullptr, P.res ? (const T*)P.res + i * P.ldres + j : nullptr, (T*)P.d + i * P.ldd + j,
+                              P.z ? (T*)P.z + i * P.ldd + j : nullptr, P.act, valid, v);
+            else if constexpr (EPI == LIN_EPI_STORE) quad_store<T>((T*)P.d + i * P.ldd + j, valid, v);
+            else quad_store<float>(P.partial + ((long)split * P.ni + i) * P.nj + j, valid, v);
+        }
+    }
+}
+
+// the partial products of a split contraction, added in their order, and the epilogue
+template <class T, bool FWD>
+__global__ void __launch_bounds__(256) linear_reduce_kernel(LinTiled P) {
+    const int quads = (P.nj + 3) / 4;
+    const long at = (long)blockIdx.x * 256 + threadIdx.x;
+    if (at >= P.ni * quads) return;
+    const long i = at / quads;
+    const int j = 4 * (int)(at - i * quads), valid = P.nj - j;
+    const float* p = P.partial + i * P.nj + j;
+    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+    for (int s = 0; s < P.splits; ++s) {
+        float q[4];
+        quad_load<float>(p + (long)s * P.ni * P.nj, valid, q);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] += q[k];
+    }
+    if constexpr (FWD)
+        lin_finish<T>(P.bias ? (const T*)P.bias + j : nullptr, P.res ? (const T*)P.res + i * P.ldres + j : nullptr, (T*)P.d + i * P.ldd + j,
+                      P.z ? (T*)P.z + i * P.ldd + j : nullptr, P.act, valid, v);
+    else quad_store<T>((T*)P.d + i * P.ldd + j, valid, v);
+}
+
+// a matrix whose rows the tiled kernel's 16-byte accesses do not fit, copied to rows that do (zeros behind)
+template <class T>
+__global__ void __launch_bounds__(256) linear_pad_kernel(const T* __restrict__ x, long ld, long rows, int n, T* __restrict__ out, int ldp) {
+    constexpr int V = Chunk<T>::N;
+    const int chunks = ldp / V;
+    for (long at = (long)blockIdx.x * 256 + threadIdx.x; at < rows * chunks; at += (long)gridDim.x * 256) {
+        const long r = at / chunks;
+        const int c = V * (int)(at - r * chunks);
+        float v[V];
+        load_chunk<T>(x + r * ld + c, n - c, v);
+        store_chunk<T>(out + r * ldp + c, V, v);
+    }
+}
+
+// delta = dy act'(z) (rounded to T for the products; rows of ldp, zeros behind) and the column sums of delta before that rounding: 32
+// chunks of columns a workgroup, 8 rows at a time, a partial row of sums per blockIdx.y
+template <class T>
+__global__ void __launch_bounds__(256) linear_delta_kernel(const T* __restrict__ dy, long lddy, const T* __restrict__ z, int act, long rows, int n,
+                                                           T* __restrict__ delta, int ldp, float* __restrict__ sums) {
+    constexpr int V = Chunk<T>::N;
+    __shared__ float red[8][32 * V];
+    const int c = threadIdx.x & 31, r = threadIdx.x >> 5;
+    const int col = (blockIdx.x * 32 + c) * V, left = n - col;
+    const long r0 = rows * blockIdx.y / gridDim.y, r1 = rows * (blockIdx.y + 1) / gridDim.y;
+    float s[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) s[k] = 0.0f;
+    for (long row = r0 + r; row < r1; row += 8) {
+        float v[V], q[V];
+        load_chunk<T>(dy + row * lddy + col, left, v);
+        if (act) {
+            load_chunk<T>(z + row * n + col, left, q);
+#pragma unroll
+            for (int k = 0; k < V; ++k) v[k] *= lin_dact(q[k], act);
+        }
+#pragma unroll
+        for (int k = 0; k < V; ++k) s[k] += v[k];
+        if (delta && col < ldp) store_chunk<T>(delta + row * ldp + col, V, v);
+    }
+    if (!sums) return;
+#pragma unroll
+    for (int k = 0; k < V; ++k) red[r][c * V + k] = s[k];
+    __syncthreads();
+    for (int at = threadIdx.x; at < 32 * V; at += 256) {
+        const int j = blockIdx.x * 32 * V + at;
+        float v = 0.0f;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v += red[q][at];
+        if (j < n) sums[(long)blockIdx.y * n + j] = v;
+    }
+}
+
+template <class T>
+__global__ void __launch_bounds__(1024) linear_fold_kernel(const float* __restrict__ sums, int parts, int n, T* __restrict__ out) {
+    __shared__ float red[32][33];
+    const int lane = threadIdx.x & 31, group = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
+    float s = 0.0f;
+    if (col < n)
+        for (int p = group; p < parts; p += 32) s += sums[(long)p * n + col];
+    red[group][lane] = s;
+    __syncthreads();
+    if (threadIdx.x < 32 && col < n) {
+        s = 0.0f;
+#pragma unroll
+        for (int g = 0; g < 32; ++g) s += red[g][lane];
+        out[col] = (T)s;
+    }
+}
+
+typedef MmCfg<128, 128, 2, 2, 2> LinMid;          // 4 waves, 64 KiB of LDS: two workgroups a CU
+typedef MmCfg<256, 256, 2, 4, 2> LinBig;          // 8 waves, 128 KiB: one
+
+// How a product runs: tile size and the parts of its contraction.
+struct LinShape { int big, splits; };
+static LinShape lin_shape(long ni, long nj, long nk, int kv) {
+    const long t256 = ((ni + 255) / 256) * ((nj + 255) / 256), t128 = ((ni + 127) / 128) * ((nj + 127) / 128);
+    const long k_tiles = nk / kv;
+    LinShape s{0, 1};
+    if (t256 >= 240) s.big = 1;
+    else if (t128 < 256) {                      // split until two workgroups a CU are there, at least 8 stages each, 32 x 128 MiB of partials at most
+        long want = (512 + t128 - 1) / t128, most = k_tiles / 8;
+        const long room = (1L << 28) / (ni * nj > 0 ? ni * nj : 1);
+        if (want > most) want = most;
+        if (want > room) want = room;
+        if (want > 1) s.splits = (int)want;
+    }
+    return s;
+}
+
+// Everything a call launches and where its scratch lies.
+struct LinPlan {
+    bool tiled;
+    bool pad_x, pad_w, delta;
+    int ldx, ldw, ldd, sum_parts;              // padded row lengths
+    LinShape fwd, dx, dw;
+    long off_x, off_w, off_delta, off_sums, off_part, total;
+};
+
+static long lin_up(long v, long to) { return (v + to - 1) / to * to; }
+
+template <class T>
+static bool lin_aligned(const void* p, long ld, long n, bool k_major) {
+    constexpr int V = 16 / (int)sizeof(T);
+    return ((uintptr_t)p & 15) == 0 && ld % V == 0 && (!k_major || n % V == 0);
+}
+
+// Which form: the tiled kernel from kLinTiledWork multiplications on (a direct tile is one launch and needs no scratch; the tiled kernel
+// shares its operands).
+static const long kLinTiledWork = getenv("FNEUS_LINEAR_TILED") ? atol(getenv("FNEUS_LINEAR_TILED")) : (1L << 27);
+
+template <class T>
+static LinPlan lin_plan(const FneusLinear& f, bool backward) {
+    constexpr int V = 16 / (int)sizeof(T), KV = 128 / (int)sizeof(T);
+    LinPlan p;
+    memset(&p, 0, sizeof p);
+    const double work = (double)f.rows * f.n_in * f.n_out;
+    p.tiled = f.rows > 16 && f.n_in >= V && f.n_out >= V && work >= (double)kLinTiledWork;
+    if (!p.tiled) return p;
+    long o = 0, part = 0;
+    auto take = [&](long bytes) { const long at = o; o += lin_up(bytes, 256); return at; };
+    auto partial = [&](const LinShape& s, long ni, long nj) { if (s.splits > 1) { const long b = (long)s.splits * ni * nj * 4; part = b > part ? b : part; } };
+    if (!backward) {
+        p.pad_x = !lin_aligned<T>(f.x, f.ldx, f.n_in, false);
+        p.pad_w = !lin_aligned<T>(f.weight, f.n_in, f.n_in, false);
+        p.fwd = lin_shape(f.rows, f.n_out, f.n_in, KV);
+        partial(p.fwd, f.rows, f.n_out);
+    } else {
+        p.pad_x = f.dweight && !lin_aligned<T>(f.x, f.ldx, f.n_in, true);
+        p.pad_w = f.dx && !lin_aligned<T>(f.weight, f.n_in, f.n_in, true);
+        p.delta = (f.dx || f.dweight) && (f.act != 0 || !lin_aligned<T>(f.dy, f.lddy, f.n_out, f.dweight != nullptr));
+        p.dx = lin_shape(f.rows, f.n_in, f.n_out, KV);
+        p.dw = lin_shape(f.n_out, f.n_in, f.rows, KV);
+        if (f.dx) partial(p.dx, f.rows, f.n_in);
+        if (f.dweight) partial(p.dw, f.n_out, f.n_in);
+        if (p.delta) p.ldd = (int)lin_up(f.n_out, V), p.off_delta = take(f.rows * p.ldd * (long)sizeof(T));
+        if (p.delta || f.dbias) {
+            const long strips = (f.n_out + 32 * V - 1) / (32 * V);
+            long parts = (1024 + strips - 1) / strips, most = (f.rows + 31) / 32;
+            p.sum_parts = (int)(parts < most ? parts : most);
+            if (f.dbias) p.off_sums = take((long)p.sum_parts * f.n_out * 4);
+        }
+    }
+    if (p.pad_x) p.ldx = (int)lin_up(f.n_in, V), p.off_x = take(f.rows * p.ldx * (long)sizeof(T));
+    if (p.pad_w) p.ldw = (int)lin_up(f.n_in, V), p.off_w = take((long)f.n_out * p.ldw * (long)sizeof(T));
+    p.off_part = o;
+    p.total = o + part;
+    return p;
+}
+
+static MmOperand lin_operand(const void* p, long ld, int e) {
+    MmOperand o;
+    o.plane[0] = o.plane[1] = o.plane[2] = (const unsigned char*)p;
+    o.row_bytes = ld * e;
+    return o;
+}
+
+template <class Cfg, class T, bool AKM, bool BKM, int EPI>
+static void lin_tiled_launch(const LinTiled& t, hipStream_t stream) {
+    auto kernel = linear_tiled_kernel<Cfg, T, AKM, BKM, EPI>;
+    allow_big_lds(kernel);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((long)t.tiles_i * t.tiles_j * t.splits)), dim3(Cfg::THREADS), Cfg::LDS, stream, t);
+}
+
+template <class T, bool AKM, bool BKM, bool FWD>
+static void lin_tiled_product(LinTiled t, const LinShape& s, long nk, float* partial, hipStream_t stream) {
+    constexpr int KV = 128 / (int)sizeof(T);
+    const int b = s.big ? 256 : 128;
+    t.k_tiles = (int)(nk / KV), t.tail = (int)(nk % KV), t.splits = s.splits, t.partial = partial;
+    t.tiles_i = (int)((t.ni + b - 1) / b), t.tiles_j = (t.nj + b - 1) / b;
+    if (s.splits > 1) {
+        lin_tiled_launch<LinMid, T, AKM, BKM, LIN_EPI_PART>(t, stream);
+        const long threads = t.ni * ((t.nj + 3) / 4);
+        hipLaunchKernelGGL((linear_reduce_kernel<T, FWD>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, stream, t);
+    } else if (s.big) {
+        lin_tiled_launch<LinBig, T, AKM, BKM, FWD ? LIN_EPI_FWD : LIN_EPI_STORE>(t, stream);
+    } else {
+        lin_tiled_launch<LinMid, T, AKM, BKM, FWD ? LIN_EPI_FWD : LIN_EPI_STORE>(t, stream);
+    }
+}
+
+template <class T>
+static const void* lin_pad(const void* x, long ld, long rows, int n, unsigned char* out, int ldp, hipStream_t stream) {
+    const long chunks = rows * (ldp / Chunk<T>::N), grid = (chunks + 255) / 256;
+    hipLaunchKernelGGL((linear_pad_kernel<T>), dim3((unsigned)(grid < 4096 ? grid : 4096)), dim3(256), 0, stream, (const T*)x, ld, rows, n, (T*)out, ldp);
+    return out;
+}
+
+template <class T>
+static void lin_tiled_fwd(const FneusLinear& f, const LinPlan& p, hipStream_t stream) {
+    unsigned char* S = (unsigned char*)f.scratch;
+    const void *x = f.x, *w = f.weight;
+    long ldx = f.ldx, ldw = f.n_in;
+    if (p.pad_x) x = lin_pad<T>(x, ldx, f.rows, f.n_in, S + p.off_x, p.ldx, stream), ldx = p.ldx;
+    if (p.pad_w) w = lin_pad<T>(w, ldw, f.n_out, f.n_in, S + p.off_w, p.ldw, stream), ldw = p.ldw;
+    LinTiled t{};
+    t.a = lin_operand(x, ldx, sizeof(T)), t.b = lin_operand(w, ldw, sizeof(T));
+    t.bias = f.bias, t.res = f.residual, t.ldres = f.ld_residual, t.d = f.y, t.z = f.z, t.ldd = f.n_out, t.ni = f.rows, t.nj = f.n_out, t.act = f.act;
+    lin_tiled_product<T, false, false, true>(t, p.fwd, f.n_in, (float*)(S + p.off_part), stream);
+}
+
+template <class T>
+static void lin_tiled_bwd(const FneusLinear& f, const LinPlan& p, hipStream_t stream) {
+    unsigned char* S = (unsigned char*)f.scratch;
+    const void *x = f.x, *w = f.weight, *d = f.dy;
+    long ldx = f.ldx, ldw = f.n_in, ldd = f.lddy;
+    float* part = (float*)(S + p.off_part);
+    if (p.delta || f.dbias) {
+        const unsigned strips = (unsigned)((f.n_out + 32 * Chunk<T>::N - 1) / (32 * Chunk<T>::N));
+        float* sums = f.dbias ? (float*)(S + p.off_sums) : nullptr;
+        hipLaunchKernelGGL((linear_delta_kernel<T>), dim3(strips, (unsigned)p.sum_parts), dim3(256), 0, stream, (const T*)f.dy, f.lddy, (const T*)f.z, f.act,
+                           f.rows, f.n_out, p.delta ? (T*)(S + p.off_delta) : nullptr, p.ldd, sums);
+        if (f.dbias) hipLaunchKernelGGL((linear_fold_kernel<T>), dim3((unsigned)((f.n_out + 31) / 32)), dim3(1024), 0, stream, sums, p.sum_parts, f.n_out, (T*)f.dbias);
+        if (p.delta) d = S + p.off_delta, ldd = p.ldd;
+    }
+    if (f.dx) {
+        if (p.pad_w) w = lin_pad<T>(w, ldw, f.n_out, f.n_in, S + p.off_w, p.ldw, stream), ldw = p.ldw;
+        LinTiled t{};
+        t.a = lin_operand(d, ldd, sizeof(T)), t.b = lin_operand(w, ldw, sizeof(T));
+        t.d = f.dx, t.ldd = f.n_in, t.ni = f.rows, t.nj = f.n_in;
+        lin_tiled_product<T, false, true, false>(t, p.dx, f.n_out, part, stream);
+    }
+    if (f.dweight) {
+        if (p.pad_x) x = lin_pad<T>(x, ldx, f.rows, f.n_in, S + p.off_x, p.ldx, stream), ldx = p.ldx;
+        LinTiled t{};
+        t.a = lin_operand(d, ldd, sizeof(T)), t.b = lin_operand(x, ldx, sizeof(T));
+        t.d = f.dweight, t.ldd = f.n_in, t.ni = f.n_out, t.nj = f.n_in;
+        lin_tiled_product<T, true, true, false>(t, p.dw, f.rows, part, stream);
+    }
+}
+
 static int lin_refuse(const char* msg) {
     set_last_error(msg);
     return -2;
@@ -211,8 +582,18 @@ static int lin_check(const FneusLinear* f, bool backward) {
     return 0;
 }
 
+static bool lin_scratch_ok(const FneusLinear& f, const LinPlan& p) {
+    return p.total == 0 || (f.scratch && f.scratch_bytes >= p.total && ((uintptr_t)f.scratch & 15) == 0);
+}
+
 template <class T>
 static int lin_fwd(const FneusLinear& f, hipStream_t stream) {
+    const LinPlan plan = lin_plan<T>(f, false);
+    if (plan.tiled) {
+        if (!lin_scratch_ok(f, plan)) return lin_refuse("fneus_linear_fwd: scratch of fneus_linear_scratch_bytes bytes, 16-byte aligned, must be given");
+        lin_tiled_fwd<T>(f, plan, stream);
+        return launch_status();
+    }
     LinProduct p{};
     p.a = f.x, p.lda = f.ldx, p.b = f.weight, p.ldb = f.n_in, p.bias = f.bias, p.res = f.residual, p.ldres = f.ld_residual;
     p.d = f.y, p.z = f.z, p.ldd = f.n_out, p.ni = f.rows, p.nj = f.n_out, p.nk = f.n_in, p.act = f.act;
@@ -229,6 +610,12 @@ static int lin_fwd(const FneusLinear& f, hipStream_t stream) {
 
 template <class T>
 static int lin_bwd(const FneusLinear& f, hipStream_t stream) {
+    const LinPlan plan = lin_plan<T>(f, true);
+    if (plan.tiled) {
+        if (!lin_scratch_ok(f, plan)) return lin_refuse("fneus_linear_bwd: scratch of fneus_linear_scratch_bytes bytes, 16-byte aligned, must be given");
+        lin_tiled_bwd<T>(f, plan, stream);
+        return launch_status();
+    }
     LinProduct dx{}, dw{};
     const void* z = f.act ? f.z : nullptr;
     dx.a = f.dy, dx.lda = f.lddy, dx.az = z, dx.ldz = f.n_out, dx.b = f.weight, dx.ldb = f.n_in, dx.d = f.dx, dx.ldd = f.n_in;
@@ -246,7 +633,12 @@ static int lin_bwd(const FneusLinear& f, hipStream_t stream) {
 
 using namespace fneus;
 
-extern "C" long fneus_linear_scratch_bytes(const FneusLinear* f, int backward) { return 0; }
+extern "C" long fneus_linear_scratch_bytes(const FneusLinear* f, int backward) {
+    if (!f || f->rows <= 0 || f->n_in <= 0 || f->n_out <= 0) return 0;
+    if (f->dtype == DT_F32) return lin_plan<float>(*f, backward != 0).total;
+    if (f->dtype == DT_BF16) return lin_plan<__bf16>(*f, backward != 0).total;
+    return lin_plan<_Float16>(*f, backward != 0).total;
+}
 
 extern "C" int fneus_linear_fwd(const FneusLinear* f, fneus_stream_t stream) {
     fneus::clear_status();

@@ -1,24 +1,30 @@
-// Tiled matrix product D(i, j) = sum_k A(i, k) B(j, k) over 16-bit PLANES (linear_kernels.hip, muon_kernels.hip).
+// Tiled matrix product D(i, j) = sum_k A(i, k) B(j, k) (linear_kernels.hip, muon_kernels.hip).
 //
-// A plane is a matrix of bf16 or fp16 values stored along k: row r at base + r * row_bytes, k padded with zeros to a multiple of 64 (so
-// a row is a whole number of 128-byte lines and no load needs a mask along k).  An operand of more bits is several planes (its terms),
-// and the contraction then runs over SEGMENTS, one per pair of terms: the pipeline does not drain between them.
+// Operands are bf16, fp16 or fp32 matrices in memory, stored along k ("rows": element (i, k) at i * row_bytes + k) or along i ("k-major":
+// (i, k) at k * row_bytes + i), 16-byte aligned.  An operand of more terms than one is several planes (muon_kernels.hip), and the
+// contraction then runs over SEGMENTS, one per pair of terms: the pipeline does not drain between them.  An fp32 operand is split into three
+// bf16 terms behind LDS (linear_act.h).
 //
-// A workgroup owns a BM x BN tile of D; 64 values of k of both operands are one stage of an LDS ring, filled by LDS-DMA (no staging
-// registers), read back as the 16-byte fragments of v_mfma_f32_32x32x16.  Rows of 128 bytes would put the 32 lanes of a fragment read on
-// the same banks: the 16-byte chunk c of row r lies at slot c ^ (r & 7), applied to the DMA's global addresses (its LDS side is linear),
-// and every group of 8 lanes reads 8 different slots.
-// Rows beyond an operand's last are loaded as its last row again: their products end in elements of D nobody stores.
+// A workgroup owns a BM x BN tile of D; one stage of an LDS ring holds 128 bytes of k of every row of both operands (64 values of 16 bits,
+// 32 of 32), filled by LDS-DMA (no staging registers).
+//   rows:    a row is 128 bytes; its 16-byte chunk c lies at slot c ^ (row & 7), applied to the DMA's global addresses (its LDS side is
+//            linear): the 8 lanes that read 16 bytes in one cycle hit 8 different slots.
+//   k-major, 16 bits: a line is one k, BM values; chunk c of line k at slot c ^ ((k & 7) << 1); ds_read_b64_tr_b16 hands every lane four
+//            consecutive k of its row (16 lanes read 4 lines x 32 bytes, which the swizzle puts on different banks).
+//   k-major, 32 bits: the same lines, 4-byte reads, 32 consecutive values a half wave.
+// Rows beyond an operand's last are loaded as its last row (k-major: its first chunk) again: their products end in elements of D nobody
+// stores.  The last values of k, where they do not fill a stage, are brought by ordinary loads with zeros behind them.
 #pragma once
-#include "fneus_types.h"
+#include "linear_act.h"
 
 namespace fneus {
 
 typedef __attribute__((address_space(3))) unsigned char mm_lds_t;
+typedef __attribute__((address_space(3))) bf16x4 mm_lds_bf16x4_t;
 
 struct MmOperand {
     const unsigned char* plane[3];
-    unsigned row_bytes;
+    long row_bytes;
 };
 
 template <int BM_, int BN_, int WGM, int WGN, int STAGES_>
@@ -47,67 +53,141 @@ FN_DEV const unsigned char* mm_uniform(const unsigned char* p) {
     return (const unsigned char*)(((unsigned long)hi << 32) | lo);
 }
 
-template <class T> struct MmVec;
-template <> struct MmVec<__bf16> {
-    typedef bf16x8 type;
-    static FN_DEV f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
-};
-template <> struct MmVec<_Float16> {
-    typedef fn_f16x8 type;
-    static FN_DEV f32x16 mfma(fn_f16x8 a, fn_f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
-};
-
 // Segment tables, 4 bits a segment: the terms of A (bits 0, 1) and B (bits 2, 3).
 constexpr unsigned kMmOne = 0x0u;                 // 1 segment
 constexpr unsigned kMmThree = 0x140u;             // 3: (0, 0), (0, 1), (1, 0): two-term operands
-constexpr unsigned kMmSix = 0x041528u;            // 6: (0, 2), (2, 0), (1, 1), (1, 0), (0, 1), (0, 0): three-term operands, smallest first
 
 // acc[mi][nj], element e of a lane: row i = mi * 32 + (lane & 31), column j = nj * 32 + 8 (e >> 2) + 4 (lane >> 5) + (e & 3) of the
-// wave's part of the tile (mm_i0, mm_j0): four consecutive columns in four consecutive registers.
-template <class Cfg>
+// wave's part of the tile: four consecutive columns in four consecutive registers.
 FN_DEV int mm_wave() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }
 template <class Cfg>
-FN_DEV int mm_row() { return (mm_wave<Cfg>() / Cfg::WAVES_N) * Cfg::WM + (int)(threadIdx.x & 31); }
+FN_DEV int mm_wave_i() { return (mm_wave() / Cfg::WAVES_N) * Cfg::WM; }
 template <class Cfg>
-FN_DEV int mm_col() { return (mm_wave<Cfg>() % Cfg::WAVES_N) * Cfg::WN + 4 * (int)((threadIdx.x >> 5) & 1); }
+FN_DEV int mm_wave_j() { return (mm_wave() % Cfg::WAVES_N) * Cfg::WN; }
 
-// it: steps of 64 along the concatenated segments, [it0, it1) of n_seg * k_tiles.  After segment 0 the sums are multiplied by `carry`
-// (RESCALE: the later segments' terms are held at a larger scale).
-template <class Cfg, class T, bool RESCALE>
-FN_DEV void mm_run(unsigned char* smem, const MmOperand& A, const MmOperand& B, long i0, long ni, long j0, long nj, int k_tiles,
-                   unsigned segs, int it0, int it1, float carry, f32x16 (&acc)[Cfg::MI][Cfg::NJ]) {
-    typedef typename MmVec<T>::type V8;
-    const int lane = threadIdx.x & 63, wave = mm_wave<Cfg>();
+// One operand's side of a stage: which bytes its DMA fetches, where a fragment lies.
+template <class T, bool KM, int B>
+struct MmSide {
+    static constexpr int E = sizeof(T), KV = 128 / E;            // values of k in a stage
+    static constexpr int LINE = KM ? B * E : 128, CHUNKS = LINE / 16, LINES = KM ? KV : B;      // LINES * LINE == B * 128
+    static FN_DEV int slot(int line, int c) {
+        if constexpr (KM) return E == 2 ? c ^ (((line & 7) << 1) & (CHUNKS - 1)) : c;
+        else return c ^ (line & 7);
+    }
+    // byte offset (from the tile's origin, at the stage's first k) of what DMA instruction q brings to this lane's 16 bytes of LDS
+    static FN_DEV unsigned dma_offset(int q, int lane, int valid_rows, long row_bytes) {
+        const int at = q * 64 + lane, line = at / CHUNKS, c = slot(line, at % CHUNKS);
+        if constexpr (KM) return (unsigned)line * (unsigned)row_bytes + (unsigned)(c * (16 / E) < valid_rows ? c : 0) * 16u;
+        else return (unsigned)(line < valid_rows ? line : valid_rows - 1) * (unsigned)row_bytes + (unsigned)c * 16u;
+    }
+    // a stage whose k ends after `left` values: ordinary loads, zeros behind
+    static FN_DEV void fill_tail(unsigned char* lds, const unsigned char* src, int valid_rows, long row_bytes, int left, int thread, int threads) {
+        for (int at = thread; at < B * 8; at += threads) {
+            const int line = at / CHUNKS, c = at % CHUNKS;
+            T v[16 / E];
+#pragma unroll
+            for (int e = 0; e < 16 / E; ++e) {
+                const int i = KM ? c * (16 / E) + e : line, k = KM ? line : c * (16 / E) + e;
+                v[e] = i < valid_rows && k < left ? reinterpret_cast<const T*>(src + (KM ? k : i) * row_bytes)[KM ? i : k] : (T)0.0f;
+            }
+            __builtin_memcpy(lds + line * LINE + slot(line, c) * 16, v, 16);
+        }
+    }
+};
+
+// Fragments of one wave's rows w0 .. of an operand; base: LDS address of the operand's part of a stage
+template <class T, bool KM, int B, int COUNT>
+struct MmReader {
+    typedef MmSide<T, KM, B> Side;
+    unsigned at[(KM && sizeof(T) == 2) ? 2 * COUNT : COUNT];
+    unsigned x7;
+    FN_DEV void init(int w0, int lane) {
+        const int r = lane & 31, h = lane >> 5;
+        x7 = (unsigned)(lane & 7);
+        if constexpr (!KM) {
+#pragma unroll
+            for (int m = 0; m < COUNT; ++m) at[m] = (unsigned)(w0 + 32 * m + r) * 128u;
+        } else if constexpr (sizeof(T) == 2) {
+            const int fh = (lane >> 4) & 1, q = (lane & 15) >> 2, p = lane & 3;
+#pragma unroll
+            for (int m = 0; m < COUNT; ++m)
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const int k = 8 * h + 4 * t + q, c = (w0 + 32 * m) / 8 + 2 * fh + (p >> 1);
+                    at[2 * m + t] = (unsigned)(k * Side::LINE + Side::slot(k, c) * 16 + (p & 1) * 8);
+                }
+        } else {
+#pragma unroll
+            for (int m = 0; m < COUNT; ++m) at[m] = (unsigned)(8 * h * Side::LINE + (w0 + 32 * m + r) * 4);
+        }
+    }
+    // k = 16 ks + 8 (lane >> 5) .. + 7
+    FN_DEV void read(const unsigned char* base, int m, int ks, int h, LinFrag<T>& f) const {
+        if constexpr (!KM && sizeof(T) == 2) {
+            f.t = *reinterpret_cast<const decltype(f.t)*>(base + at[m] + (((unsigned)(2 * ks + h) ^ x7) << 4));
+        } else if constexpr (!KM) {
+            float v[8];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const f32x4 q = *reinterpret_cast<const f32x4*>(base + at[m] + (((unsigned)(4 * ks + 2 * h + u) ^ x7) << 4));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[4 * u + e] = q[e];
+            }
+            lin_frag(v, f);
+        } else if constexpr (sizeof(T) == 2) {
+            bf16x8 v;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const bf16x4 q = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((mm_lds_bf16x4_t*)(base + at[2 * m + t] + ks * 16 * Side::LINE));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[4 * t + e] = q[e];
+            }
+            f.t = __builtin_bit_cast(decltype(f.t), v);
+        } else {
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = *reinterpret_cast<const float*>(base + at[m] + (16 * ks + e) * Side::LINE);
+            lin_frag(v, f);
+        }
+    }
+};
+
+// steps [it0, it1) of the concatenated segments, `k_tiles` full stages each; tail: values of k behind the last full stage (one segment
+// only), taken when TAIL and `with_tail`.  After segment 0 the sums are multiplied by `carry` (RESCALE: the later segments' terms are held
+// at a larger scale; it0 == 0).  ni - i0 and nj - j0 are positive.
+template <class Cfg, class T, bool AKM, bool BKM, bool RESCALE, bool TAIL>
+FN_DEV void mm_run(unsigned char* smem, const MmOperand& A, const MmOperand& B, long i0, long ni, long j0, long nj, int k_tiles, int tail,
+                   unsigned segs, int it0, int it1, bool with_tail, float carry, f32x16 (&acc)[Cfg::MI][Cfg::NJ]) {
+    typedef MmSide<T, AKM, Cfg::BM> SideA;
+    typedef MmSide<T, BKM, Cfg::BN> SideB;
+    const int lane = threadIdx.x & 63, wave = mm_wave(), h = lane >> 5;
 #pragma unroll
     for (int m = 0; m < Cfg::MI; ++m)
 #pragma unroll
         for (int n = 0; n < Cfg::NJ; ++n)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[m][n][e] = 0.0f;
-    // this wave's DMA: 8 rows an instruction, lane -> row lane >> 3, slot lane & 7 <- chunk slot ^ (row & 7)
+    const int va = (int)(ni - i0 < Cfg::BM ? ni - i0 : Cfg::BM), vb = (int)(nj - j0 < Cfg::BN ? nj - j0 : Cfg::BN);
+    // this wave's DMA
     const int q0 = wave * Cfg::DPW;
     const bool is_b = q0 >= Cfg::BM / 8;
-    const unsigned row_bytes = is_b ? B.row_bytes : A.row_bytes;
-    const unsigned char *pl0 = is_b ? B.plane[0] : A.plane[0], *pl1 = is_b ? B.plane[1] : A.plane[1], *pl2 = is_b ? B.plane[2] : A.plane[2];
-    const long first = is_b ? j0 : i0, count = is_b ? nj : ni;
-    const int valid = (int)(count - first < 256 ? count - first : 256);        // >= 1
-    const int row0 = (q0 - (is_b ? Cfg::BM / 8 : 0)) * 8 + (lane >> 3);
     unsigned off[Cfg::DPW];
 #pragma unroll
-    for (int d = 0; d < Cfg::DPW; ++d) {
-        const int row = row0 + 8 * d;
-        off[d] = (unsigned)(row < valid ? row : valid - 1) * row_bytes + ((unsigned)((lane & 7) ^ (lane >> 3)) << 4);
-    }
-    int is_seg = it0 / k_tiles, is_kt = it0 - is_seg * k_tiles;
+    for (int d = 0; d < Cfg::DPW; ++d)
+        off[d] = is_b ? SideB::dma_offset(q0 + d - Cfg::BM / 8, lane, vb, B.row_bytes) : SideA::dma_offset(q0 + d, lane, va, A.row_bytes);
+    const long origin = is_b ? (BKM ? j0 * (long)sizeof(T) : j0 * B.row_bytes) : (AKM ? i0 * (long)sizeof(T) : i0 * A.row_bytes);
+    const long step = is_b ? (BKM ? SideB::KV * B.row_bytes : 128) : (AKM ? SideA::KV * A.row_bytes : 128);
+    const unsigned char *pl0 = is_b ? B.plane[0] : A.plane[0], *pl1 = is_b ? B.plane[1] : A.plane[1];
+    int is_seg = it0 / (k_tiles > 0 ? k_tiles : 1), is_kt = it0 - is_seg * k_tiles;
     auto base_of = [&](int seg) {
         const unsigned c = (segs >> (4 * seg + (is_b ? 2 : 0))) & 3;
-        return mm_uniform((c == 0 ? pl0 : (c == 1 ? pl1 : pl2)) + first * (long)row_bytes);
+        return mm_uniform((c ? pl1 : pl0) + origin);
     };
     const unsigned char* base = base_of(is_seg);
     const unsigned lds_base = (unsigned)(uintptr_t)(mm_lds_t*)(smem + q0 * 1024);
     int is_stage = 0;
     auto issue = [&]() {
-        const unsigned char* src = base + (long)is_kt * 128;
+        const unsigned char* src = mm_uniform(base + (long)is_kt * step);
         const unsigned dst = lds_base + is_stage * Cfg::STAGE_BYTES;
 #pragma unroll
         for (int d = 0; d < Cfg::DPW; ++d) {
@@ -123,35 +203,38 @@ FN_DEV void mm_run(unsigned char* smem, const MmOperand& A, const MmOperand& B, 
         if (++is_kt == k_tiles) {
             is_kt = 0;
             ++is_seg;
-            base = base_of(is_seg < 6 ? is_seg : 0);
+            base = base_of(is_seg < 7 ? is_seg : 0);
         }
     };
     constexpr int P = Cfg::STAGES - 1;
     for (int s = 0; s < P; ++s)
         if (it0 + s < it1) issue();
-    const unsigned char* ra = smem + mm_row<Cfg>() * 128;
-    const unsigned char* rb = smem + Cfg::BM * 128 + ((wave % Cfg::WAVES_N) * Cfg::WN + (lane & 31)) * 128;
-    const int h = lane >> 5;
-    int stage = 0, left0 = RESCALE ? k_tiles - it0 : 0;
+    MmReader<T, AKM, Cfg::BM, Cfg::MI> ra;
+    MmReader<T, BKM, Cfg::BN, Cfg::NJ> rb;
+    ra.init(mm_wave_i<Cfg>(), lane);
+    rb.init(mm_wave_j<Cfg>(), lane);
+    auto compute = [&](const unsigned char* pa) {
+        const unsigned char* pb = pa + Cfg::BM * 128;
+#pragma unroll
+        for (int ks = 0; ks < SideA::KV / 16; ++ks) {
+            LinFrag<T> fa[Cfg::MI], fb[Cfg::NJ];
+#pragma unroll
+            for (int m = 0; m < Cfg::MI; ++m) ra.read(pa, m, ks, h, fa[m]);
+#pragma unroll
+            for (int n = 0; n < Cfg::NJ; ++n) rb.read(pb, n, ks, h, fb[n]);
+#pragma unroll
+            for (int m = 0; m < Cfg::MI; ++m)
+#pragma unroll
+                for (int n = 0; n < Cfg::NJ; ++n) acc[m][n] = lin_mfma32(fb[n], fa[m], acc[m][n]);
+        }
+    };
+    int stage = 0, left0 = RESCALE ? k_tiles : 0;
 #pragma unroll 1
     for (int it = it0; it < it1; ++it) {
         if (it1 - 1 - it >= P - 1) mm_wait_barrier<(P - 1) * Cfg::DPW>();
         else mm_wait_barrier<0>();
         if (it + P < it1) issue();
-        const unsigned char *pa = ra + stage * Cfg::STAGE_BYTES, *pb = rb + stage * Cfg::STAGE_BYTES;
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-            const unsigned x = (unsigned)((2 * ks + h) ^ (lane & 7)) << 4;
-            V8 fa[Cfg::MI], fb[Cfg::NJ];
-#pragma unroll
-            for (int m = 0; m < Cfg::MI; ++m) fa[m] = *reinterpret_cast<const V8*>(pa + m * 4096 + x);
-#pragma unroll
-            for (int n = 0; n < Cfg::NJ; ++n) fb[n] = *reinterpret_cast<const V8*>(pb + n * 4096 + x);
-#pragma unroll
-            for (int m = 0; m < Cfg::MI; ++m)
-#pragma unroll
-                for (int n = 0; n < Cfg::NJ; ++n) acc[m][n] = MmVec<T>::mfma(fb[n], fa[m], acc[m][n]);
-        }
+        compute(smem + stage * Cfg::STAGE_BYTES);
         stage = stage + 1 == Cfg::STAGES ? 0 : stage + 1;
         if constexpr (RESCALE) {
             if (--left0 == 0) {
@@ -164,13 +247,27 @@ FN_DEV void mm_run(unsigned char* smem, const MmOperand& A, const MmOperand& B, 
             }
         }
     }
+    if constexpr (TAIL) {
+        if (with_tail && tail > 0) {
+            mm_wait_barrier<0>();                        // (the ring is empty; everyone has read its last stage)
+            const unsigned char* sa = A.plane[0] + (AKM ? i0 * (long)sizeof(T) + (long)k_tiles * SideA::KV * A.row_bytes : i0 * A.row_bytes + k_tiles * 128L);
+            const unsigned char* sb = B.plane[0] + (BKM ? j0 * (long)sizeof(T) + (long)k_tiles * SideB::KV * B.row_bytes : j0 * B.row_bytes + k_tiles * 128L);
+            SideA::fill_tail(smem, sa, va, A.row_bytes, tail, threadIdx.x, Cfg::THREADS);
+            SideB::fill_tail(smem + Cfg::BM * 128, sb, vb, B.row_bytes, tail, threadIdx.x, Cfg::THREADS);
+            mm_wait_barrier<0>();
+            compute(smem);
+        }
+    }
 }
 
-// tile index -> (row, column) of tiles: workgroups of one XCD (launch index mod 8) take one contiguous stretch of the tiles, and a
-// stretch runs down 8 rows of tiles before it moves to the next column: the operand rows of a stretch stay in that XCD's L2
-FN_DEV void mm_tile(long wg, long tiles, int tiles_i, int tiles_j, int& ti, int& tj) {
-    const long q = tiles >> 3, r = tiles & 7, xcd = wg & 7;
-    const long t = xcd * q + (xcd < r ? xcd : r) + (wg >> 3);
+// Launch index -> work item: the workgroups of one XCD (launch index mod 8) take one contiguous stretch of the items, so that what
+// neighbours share stays in that XCD's L2.
+FN_DEV long mm_spread(long wg, long total) {
+    const long q = total >> 3, r = total & 7, xcd = wg & 7;
+    return xcd * q + (xcd < r ? xcd : r) + (wg >> 3);
+}
+// tile index -> (row, column) of tiles: down 8 rows of tiles, then the next column
+FN_DEV void mm_tile(long t, int tiles_i, int tiles_j, int& ti, int& tj) {
     const long band = 8L * tiles_j;
     const int b = (int)(t / band), in = (int)(t - b * band);
     const int rows = tiles_i - 8 * b < 8 ? tiles_i - 8 * b : 8;

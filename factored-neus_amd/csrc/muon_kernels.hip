@@ -1,8 +1,7 @@
 // The Muon update of weight matrices: momentum, orthogonalisation by Newton-Schulz products, step -- every matrix of a model in the same
 // 2 + 3 * steps launches.  For each matrix u, as X [m][n] with m <= n (the transpose where rows > cols):
 //   X = u / max(|u|_F, eps);   steps times:  A = X X^T,  B = b A + c A A,  X <- a X + B X
-// All three products run on the tiled engine (mm_engine.h), whose operands lie along k: X and its transpose are both kept (the epilogue
-// writes the two), A and B are symmetric.
+// All three products run on the tiled engine (mm_engine.h): X X^T and A A on operands stored along k, B X with X k-major.
 //
 // Numbers: fp16 planes with fp32 sums.  Every entry of X, A and B is bounded (the polynomial keeps the singular values below about 1.2),
 // entries as small as 1 / n matter, and the fp16 matrix instruction takes subnormal operands as zero, so a plane holds its matrix times a
@@ -42,29 +41,27 @@ struct MuonNum {
     const float* lr;
 };
 
-// where a matrix's buffers lie in its scratch: norm partials, X / Xt twice (a step reads one pair and writes the other), A, B
+// where a matrix's buffers lie in its scratch: norm partials, X twice (a step reads one and writes the other), A, B.  Rows of X and
+// columns of all are padded with zeros to multiples of 64: whole stages of the engine's ring
 struct MuonLay {
-    int m, n;
+    int m, n, mp;
     bool trans;
-    unsigned ldx, ldt;                       // bytes of a plane's row: X and (Xt, A, B)
-    long px, pt, pa;                         // bytes of a plane
-    long x[2], t[2], a, b, total;
+    unsigned ldx, lda;                       // bytes of a plane's row: X, and A and B
+    long px, pa;                             // bytes of a plane
+    long x[2], a, b, total;
 };
 __host__ __device__ inline MuonLay muon_lay(int rows, int cols, int planes) {
     MuonLay L;
     L.trans = rows > cols;
     L.m = L.trans ? cols : rows;
     L.n = L.trans ? rows : cols;
+    L.mp = (L.m + 63) / 64 * 64;
     L.ldx = (unsigned)((L.n + 63) / 64) * 128u;
-    L.ldt = (unsigned)((L.m + 63) / 64) * 128u;
-    L.px = (long)L.m * L.ldx;
-    L.pt = (long)L.n * L.ldt;
-    L.pa = (long)L.m * L.ldt;
+    L.lda = (unsigned)L.mp * 2u;
+    L.px = (long)L.mp * L.ldx;
+    L.pa = (long)L.m * L.lda;
     long o = kMuonChunks * 8;
-    for (int k = 0; k < 2; ++k) {
-        L.x[k] = o, o += planes * L.px;
-        L.t[k] = o, o += planes * L.pt;
-    }
+    for (int k = 0; k < 2; ++k) L.x[k] = o, o += planes * L.px;
     L.a = o, o += planes * L.pa;
     L.b = o, o += planes * L.pa;
     L.total = (o + 255) / 256 * 256;
@@ -121,7 +118,7 @@ FN_DEV void muon_split(float v, _Float16& hi, _Float16& lo) {
     if constexpr (NP == 2) lo = (_Float16)((v - (float)hi) * kLoScale);
 }
 
-// launch 2: X and Xt (with their zero padding) of 64 x 64 tiles of u
+// launch 2: X (with its zero padding) from 64 x 64 tiles of u
 template <class T, bool MOM, int NP>
 __global__ void __launch_bounds__(256) muon_init_kernel(MuonJobs js, MuonNum P) {
     __shared__ float tile[64][65];
@@ -152,31 +149,20 @@ __global__ void __launch_bounds__(256) muon_init_kernel(MuonJobs js, MuonNum P) 
     __syncthreads();
     const double norm = sqrt(red[0] + red[1] + red[2] + red[3]);
     const float scale = (float)(ldexp(1.0, P.ex) / (norm > (double)P.eps || norm != norm ? norm : (double)P.eps));
-    // rows along the matrix's own rows: X, or Xt of the transpose; and the other one
-    _Float16* along = reinterpret_cast<_Float16*>(S + (L.trans ? L.t[0] : L.x[0]));
-    _Float16* across = reinterpret_cast<_Float16*>(S + (L.trans ? L.x[0] : L.t[0]));
-    const unsigned ld_al = (L.trans ? L.ldt : L.ldx) / 2, ld_ac = (L.trans ? L.ldx : L.ldt) / 2;
-    const long pl_al = (L.trans ? L.pt : L.px) / 2, pl_ac = (L.trans ? L.px : L.pt) / 2;
+    _Float16* x = reinterpret_cast<_Float16*>(S + L.x[0]);
+    const unsigned ld = L.ldx / 2;
 #pragma unroll 4
-    for (int r = lr; r < 64; r += 4) {
+    for (int r = lr; r < 64; r += 4) {               // (r, lc): row and column of X within the tile
         _Float16 hi, lo;
-        if (r0 + r < J.rows) {
-            muon_split<NP>(tile[r][lc] * scale, hi, lo);
-            _Float16* o = along + (long)(r0 + r) * ld_al + c0 + lc;
-            o[0] = hi;
-            if constexpr (NP == 2) o[pl_al] = lo;
-        }
-        if (c0 + r < J.cols) {
-            muon_split<NP>(tile[lc][r] * scale, hi, lo);
-            _Float16* o = across + (long)(c0 + r) * ld_ac + r0 + lc;
-            o[0] = hi;
-            if constexpr (NP == 2) o[pl_ac] = lo;
-        }
+        muon_split<NP>((L.trans ? tile[lc][r] : tile[r][lc]) * scale, hi, lo);
+        _Float16* o = x + (long)((L.trans ? c0 : r0) + r) * ld + (L.trans ? r0 : c0) + lc;
+        o[0] = hi;
+        if constexpr (NP == 2) o[L.px / 2] = lo;
     }
 }
 
 template <int NP>
-FN_DEV MmOperand muon_op(const unsigned char* base, long plane, unsigned row_bytes) {
+FN_DEV MmOperand muon_op(const unsigned char* base, long plane, long row_bytes) {
     MmOperand o;
     o.plane[0] = base;
     o.plane[1] = NP == 2 ? base + plane : base;
@@ -211,9 +197,9 @@ FN_DEV void muon_write4(unsigned char* p, long plane, const float (&v)[4], f16x4
 
 enum { MU_GRAM = 0, MU_POLY = 1, MU_STEP = 2, MU_LAST = 3 };
 
-// GRAM: A = X X^T.  POLY: B = b A + c A A.  STEP: X' = a X + B X, both layouts.  LAST: the same into `out` or the parameter.
+// GRAM: A = X X^T.  POLY: B = b A + c A A.  STEP: X' = a X + B X.  LAST: the same into `out` or the parameter.
 template <class Cfg, int NP, int KIND, class T, bool MOM>
-__global__ void __launch_bounds__(Cfg::THREADS) muon_product_kernel(MuonJobs js, MuonNum P, int cur) {
+__global__ void __launch_bounds__(Cfg::THREADS, 2) muon_product_kernel(MuonJobs js, MuonNum P, int cur) {
     extern __shared__ __attribute__((aligned(16))) unsigned char mm_smem[];
     const MuonJob& J = js.j[muon_find(js, blockIdx.x)];
     const MuonLay L = muon_lay(J.rows, J.cols, NP);
@@ -221,15 +207,16 @@ __global__ void __launch_bounds__(Cfg::THREADS) muon_product_kernel(MuonJobs js,
     const int ni = L.m, nj = KIND <= MU_POLY ? L.m : L.n;
     const int tiles_i = (ni + Cfg::BM - 1) / Cfg::BM, tiles_j = (nj + Cfg::BN - 1) / Cfg::BN;
     int ti, tj;
-    mm_tile(blockIdx.x - J.first, (long)tiles_i * tiles_j, tiles_i, tiles_j, ti, tj);
+    mm_tile(mm_spread(blockIdx.x - J.first, (long)tiles_i * tiles_j), tiles_i, tiles_j, ti, tj);
     const long i0 = (long)ti * Cfg::BM, j0 = (long)tj * Cfg::BN;
     MmOperand A, B;
     if constexpr (KIND == MU_GRAM) A = B = muon_op<NP>(S + L.x[cur], L.px, L.ldx);
-    else if constexpr (KIND == MU_POLY) A = B = muon_op<NP>(S + L.a, L.pa, L.ldt);
-    else A = muon_op<NP>(S + L.b, L.pa, L.ldt), B = muon_op<NP>(S + L.t[cur], L.pt, L.ldt);
-    const int k_tiles = (int)((KIND == MU_GRAM ? L.ldx : L.ldt) / 128);
+    else if constexpr (KIND == MU_POLY) A = B = muon_op<NP>(S + L.a, L.pa, L.lda);
+    else A = muon_op<NP>(S + L.b, L.pa, L.lda), B = muon_op<NP>(S + L.x[cur], L.px, L.ldx);
+    const int k_tiles = (int)((KIND == MU_GRAM ? L.ldx : L.lda) / 128);
     f32x16 acc[Cfg::MI][Cfg::NJ];
-    mm_run<Cfg, _Float16, NP == 2>(mm_smem, A, B, i0, ni, j0, nj, k_tiles, NP == 2 ? kMmThree : kMmOne, 0, (NP == 2 ? 3 : 1) * k_tiles, kLoScale, acc);
+    mm_run<Cfg, _Float16, false, (KIND >= MU_STEP), NP == 2, false>(mm_smem, A, B, i0, ni, j0, nj, k_tiles, 0, NP == 2 ? kMmThree : kMmOne, 0,
+                                                                    (NP == 2 ? 3 : 1) * k_tiles, false, kLoScale, acc);
     const float lo = NP == 2 ? 1.0f / kLoScale : 1.0f;
     // acc -> value: the product of the operands' scales (and the second plane's) is taken out, the result's put in
     float f;
@@ -239,28 +226,28 @@ __global__ void __launch_bounds__(Cfg::THREADS) muon_product_kernel(MuonJobs js,
     const float lr = KIND == MU_LAST && MOM ? *P.lr : 0.0f;
 #pragma unroll
     for (int m = 0; m < Cfg::MI; ++m) {
-        const long i = i0 + mm_row<Cfg>() + 32 * m;
+        const long i = i0 + mm_wave_i<Cfg>() + 32 * m + (threadIdx.x & 31);
 #pragma unroll
         for (int n = 0; n < Cfg::NJ; ++n)
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const long j = j0 + mm_col<Cfg>() + 32 * n + 8 * g;
+                const long j = j0 + mm_wave_j<Cfg>() + 32 * n + 8 * g + 4 * ((threadIdx.x >> 5) & 1);
                 float v[4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) v[k] = acc[m][n][4 * g + k] * f;
                 f16x4 hi, lo4;
                 if constexpr (KIND == MU_GRAM || KIND == MU_POLY) {
-                    if (i >= ni || j >= (long)L.ldt / 2) continue;
+                    if (i >= ni || j >= (long)L.lda / 2) continue;
                     if constexpr (KIND == MU_POLY) {
                         float a[4];
-                        muon_read4<NP>(S + L.a + i * L.ldt + j * 2, L.pa, a);
+                        muon_read4<NP>(S + L.a + i * L.lda + j * 2, L.pa, a);
                         const float fb = ldexpf(P.b, P.eb - P.ea);
 #pragma unroll
                         for (int k = 0; k < 4; ++k) v[k] += fb * a[k];
                     }
 #pragma unroll
                     for (int k = 0; k < 4; ++k) v[k] = j + k < nj ? v[k] : 0.0f;
-                    muon_write4<NP>(S + (KIND == MU_GRAM ? L.a : L.b) + i * L.ldt + j * 2, L.pa, v, hi, lo4);
+                    muon_write4<NP>(S + (KIND == MU_GRAM ? L.a : L.b) + i * L.lda + j * 2, L.pa, v, hi, lo4);
                 } else {
                     float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                     if (i < ni && j < (long)L.ldx / 2) muon_read4<NP>(S + L.x[cur] + i * L.ldx + j * 2, L.px, x);
@@ -268,18 +255,7 @@ __global__ void __launch_bounds__(Cfg::THREADS) muon_product_kernel(MuonJobs js,
 #pragma unroll
                     for (int k = 0; k < 4; ++k) v[k] = i < ni && j + k < nj ? v[k] + fa * x[k] : 0.0f;
                     if constexpr (KIND == MU_STEP) {
-                        if (i < ni && j < (long)L.ldx / 2) muon_write4<NP>(S + L.x[cur ^ 1] + i * L.ldx + j * 2, L.px, v, hi, lo4);
-                        if (i < (long)L.ldt / 2) {
-#pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                if (j + k < nj) {
-                                    _Float16 a, b = (_Float16)0.0f;
-                                    muon_split<NP>(v[k], a, b);
-                                    unsigned char* p = S + L.t[cur ^ 1] + (j + k) * L.ldt + i * 2;
-                                    *reinterpret_cast<_Float16*>(p) = a;
-                                    if constexpr (NP == 2) *reinterpret_cast<_Float16*>(p + L.pt) = b;
-                                }
-                        }
+                        if (i < L.mp && j < (long)L.ldx / 2) muon_write4<NP>(S + L.x[cur ^ 1] + i * L.ldx + j * 2, L.px, v, hi, lo4);
                     } else if (i < ni) {
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
