@@ -47,6 +47,37 @@ FN_DEV void store_chunk(T* p, int valid, const float (&v)[Chunk<T>::N]) {
     }
 }
 
+// the same for a run of V values, V a multiple of the chunk
+template <class T, int V>
+FN_DEV void load_run(const T* p, int valid, float (&v)[V]) {
+    constexpr int N = Chunk<T>::N;
+#pragma unroll
+    for (int c = 0; c < V / N; ++c) {
+        float q[N];
+        load_chunk<T>(p + c * N, valid - c * N, q);
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[c * N + k] = q[k];
+    }
+}
+
+// Sums of `parts` rows of partial sums (row p at partial + p * stride) for the 8 columns col0 .. col0 + 7 by 1024 threads: 128 threads a
+// column, then a tree in LDS: a fixed order.  The result of column c is in the threads c < 8.
+FN_DEV float fold_rows8(const float* __restrict__ partial, int parts, long stride, long col0, long cols, float (&red)[128][9]) {
+    const int c = threadIdx.x & 7, g = threadIdx.x >> 3;
+    float s = 0.0f;
+    if (col0 + c < cols) {
+#pragma unroll 4
+        for (int p = g; p < parts; p += 128) s += partial[p * stride + col0 + c];
+    }
+    red[g][c] = s;
+#pragma unroll
+    for (int d = 64; d; d >>= 1) {
+        __syncthreads();
+        if (g < d) red[g][c] += red[g + d][c];
+    }
+    return red[0][c];                      // (g == 0 has written it itself)
+}
+
 // sum over the 16 lanes of a DPP row, in every lane (quad permutes, half mirror, mirror: no LDS traffic)
 FN_DEV float row16_sum(float v) {
     v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0xB1, 0xF, 0xF, true));

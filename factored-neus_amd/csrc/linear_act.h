@@ -7,15 +7,32 @@ namespace fneus {
 
 constexpr int kLinActs = 7;
 
-FN_DEV float lin_sigmoid(float z) { return 1.0f / (1.0f + expf(-z)); }
+// exp by the base-2 instruction, 1 / x by the reciprocal instruction (1 ulp each): sigmoid to 2e-8 absolute
+FN_DEV float lin_exp(float x) { return fast_exp2(x * kLog2e); }
+FN_DEV float lin_sigmoid(float z) { return fast_rcp(1.0f + lin_exp(-z)); }
+
+// Phi(z), the normal distribution's integral, and e = exp(-z^2 / 2): Abramowitz & Stegun 7.1.26 for erfc(|z| / sqrt 2) (1.5e-7 absolute;
+// the small tail is formed directly, the large side as its complement)
+FN_DEV float lin_phi(float z, float& e) {
+    const float x = fabsf(z) * 0.70710678118654752f;
+    e = lin_exp(-x * x);
+    const float t = fast_rcp(1.0f + 0.3275911f * x);
+    const float p = ((((1.061405429f * t - 1.453152027f) * t + 1.421413741f) * t - 0.284496736f) * t + 0.254829592f) * t;
+    const float tail = 0.5f * p * e;
+    return z < 0.0f ? tail : 1.0f - tail;
+}
 
 FN_DEV float lin_act(float z, int act) {
     switch (act) {
         case 1: return z > 0.0f ? z : (z != z ? z : 0.0f);
         case 2: return z > 0.0f ? z : 0.2f * z;
         case 3: return lin_sigmoid(z);
-        case 4: return fmaxf(z, 0.0f) + log1pf(expf(-100.0f * fabsf(z))) * 0.01f + (z != z ? z : 0.0f);
-        case 5: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+        case 4: {
+            const float e = lin_exp(-100.0f * fabsf(z));
+            const float l = e < 0.01f ? e * (1.0f - e * (0.5f - e * 0.33333333f)) : fast_log2(1.0f + e) * kLn2;
+            return (z > 0.0f ? z : (z != z ? z : 0.0f)) + l * 0.01f;
+        }
+        case 5: { float e; return z * lin_phi(z, e); }
         case 6: return z * lin_sigmoid(z);
         default: return z;
     }
@@ -28,7 +45,7 @@ FN_DEV float lin_dact(float z, int act) {
         case 2: return z > 0.0f ? 1.0f : 0.2f;
         case 3: { const float s = lin_sigmoid(z); return s * (1.0f - s); }
         case 4: return lin_sigmoid(100.0f * z);
-        case 5: return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * (0.39894228040143268f * expf(-0.5f * z * z));
+        case 5: { float e; const float p = lin_phi(z, e); return p + z * (0.39894228040143268f * e); }
         case 6: { const float s = lin_sigmoid(z); return s * (1.0f + z * (1.0f - s)); }
         default: return 1.0f;
     }

@@ -307,23 +307,39 @@ __global__ void __launch_bounds__(Cfg::THREADS, 2) linear_tiled_kernel(LinTiled 
     }
 }
 
-// the partial products of a split contraction, added in their order, and the epilogue
-template <class T, bool FWD>
+// the partial products of a split contraction and the epilogue: GROUPS threads share the parts of four outputs, each adds its own in order,
+// the groups are added in order
+template <class T, bool FWD, int GROUPS>
 __global__ void __launch_bounds__(256) linear_reduce_kernel(LinTiled P) {
+    __shared__ float red[GROUPS > 1 ? GROUPS : 1][GROUPS > 1 ? 256 / GROUPS : 1][4];
     const int quads = (P.nj + 3) / 4;
-    const long at = (long)blockIdx.x * 256 + threadIdx.x;
-    if (at >= P.ni * quads) return;
-    const long i = at / quads;
-    const int j = 4 * (int)(at - i * quads), valid = P.nj - j;
-    const float* p = P.partial + i * P.nj + j;
+    const int slot = threadIdx.x % (256 / GROUPS), group = threadIdx.x / (256 / GROUPS);
+    const long at = (long)blockIdx.x * (256 / GROUPS) + slot;
+    const bool live = at < P.ni * quads;
+    const long i = live ? at / quads : 0;
+    const int j = live ? 4 * (int)(at - i * quads) : 0, valid = P.nj - j;
     float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (live) {
+        const float* p = P.partial + i * P.nj + j;
 #pragma unroll 8
-    for (int s = 0; s < P.splits; ++s) {
-        float q[4];
-        quad_load<float>(p + (long)s * P.ni * P.nj, valid, q);
+        for (int s = group; s < P.splits; s += GROUPS) {
+            float q[4];
+            quad_load<float>(p + (long)s * P.ni * P.nj, valid, q);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] += q[k];
+            for (int k = 0; k < 4; ++k) v[k] += q[k];
+        }
     }
+    if constexpr (GROUPS > 1) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) red[group][slot][k] = v[k];
+        __syncthreads();
+        if (group) return;
+#pragma unroll
+        for (int g = 1; g < GROUPS; ++g)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] += red[g][slot][k];
+    }
+    if (!live) return;
     if constexpr (FWD)
         lin_finish<T>(P.bias ? (const T*)P.bias + j : nullptr, P.res ? (const T*)P.res + i * P.ldres + j : nullptr, (T*)P.d + i * P.ldd + j,
                       P.z ? (T*)P.z + i * P.ldd + j : nullptr, P.act, valid, v);
@@ -384,33 +400,30 @@ __global__ void __launch_bounds__(256) linear_delta_kernel(const T* __restrict__
 
 template <class T>
 __global__ void __launch_bounds__(1024) linear_fold_kernel(const float* __restrict__ sums, int parts, int n, T* __restrict__ out) {
-    __shared__ float red[32][33];
-    const int lane = threadIdx.x & 31, group = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
-    float s = 0.0f;
-    if (col < n)
-        for (int p = group; p < parts; p += 32) s += sums[(long)p * n + col];
-    red[group][lane] = s;
-    __syncthreads();
-    if (threadIdx.x < 32 && col < n) {
-        s = 0.0f;
-#pragma unroll
-        for (int g = 0; g < 32; ++g) s += red[g][lane];
-        out[col] = (T)s;
-    }
+    __shared__ float red[128][9];
+    const float s = fold_rows8(sums, parts, n, 8L * blockIdx.x, n, red);
+    if (threadIdx.x < 8 && 8 * blockIdx.x + threadIdx.x < (unsigned)n) out[8 * blockIdx.x + threadIdx.x] = (T)s;
 }
 
+typedef MmCfg<64, 64, 2, 2, 4> LinSmall;          // 4 waves, 64 KiB of LDS, three stages in flight
 typedef MmCfg<128, 128, 2, 2, 2> LinMid;          // 4 waves, 64 KiB of LDS: two workgroups a CU
 typedef MmCfg<256, 256, 2, 4, 2> LinBig;          // 8 waves, 128 KiB: one
 
 // How a product runs: tile size and the parts of its contraction.
-struct LinShape { int big, splits; };
+struct LinShape { int tile, splits; };            // tile: 64, 128, 256
 static LinShape lin_shape(long ni, long nj, long nk, int kv) {
     const long t256 = ((ni + 255) / 256) * ((nj + 255) / 256), t128 = ((ni + 127) / 128) * ((nj + 127) / 128);
     const long k_tiles = nk / kv;
-    LinShape s{0, 1};
-    if (t256 >= 240) s.big = 1;
-    else if (t128 < 256) {                      // split until two workgroups a CU are there, at least 8 stages each, 32 x 128 MiB of partials at most
-        long want = (512 + t128 - 1) / t128, most = k_tiles / 8;
+    const long t64 = ((ni + 63) / 64) * ((nj + 63) / 64);
+    LinShape s{128, 1};
+    static const int form = getenv("FNEUS_LINEAR_TILE") ? atoi(getenv("FNEUS_LINEAR_TILE")) : 0;
+    static const int split = getenv("FNEUS_LINEAR_SPLIT") ? atoi(getenv("FNEUS_LINEAR_SPLIT")) : 0;
+    if (form) s.tile = form;
+    else if (t256 >= 240) s.tile = 256;
+    else if (t128 < 256) s.tile = 64;
+    const long t = s.tile == 64 ? t64 : (s.tile == 128 ? t128 : t256);
+    if (t < 256 && s.tile != 256) {     // split until two workgroups a CU are there, at least 8 stages each, 2^28 partial sums at most
+        long want = split ? split : (512 + t - 1) / t, most = split ? k_tiles : k_tiles / 8;
         const long room = (1L << 28) / (ni * nj > 0 ? ni * nj : 1);
         if (want > most) want = most;
         if (want > room) want = room;
@@ -496,14 +509,18 @@ static void lin_tiled_launch(const LinTiled& t, hipStream_t stream) {
 template <class T, bool AKM, bool BKM, bool FWD>
 static void lin_tiled_product(LinTiled t, const LinShape& s, long nk, float* partial, hipStream_t stream) {
     constexpr int KV = 128 / (int)sizeof(T);
-    const int b = s.big ? 256 : 128;
+    const int b = s.tile;
     t.k_tiles = (int)(nk / KV), t.tail = (int)(nk % KV), t.splits = s.splits, t.partial = partial;
     t.tiles_i = (int)((t.ni + b - 1) / b), t.tiles_j = (t.nj + b - 1) / b;
     if (s.splits > 1) {
-        lin_tiled_launch<LinMid, T, AKM, BKM, LIN_EPI_PART>(t, stream);
-        const long threads = t.ni * ((t.nj + 3) / 4);
-        hipLaunchKernelGGL((linear_reduce_kernel<T, FWD>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, stream, t);
-    } else if (s.big) {
+        if (s.tile == 64) lin_tiled_launch<LinSmall, T, AKM, BKM, LIN_EPI_PART>(t, stream);
+        else lin_tiled_launch<LinMid, T, AKM, BKM, LIN_EPI_PART>(t, stream);
+        const long quads = t.ni * ((t.nj + 3) / 4);
+        if (s.splits >= 16) hipLaunchKernelGGL((linear_reduce_kernel<T, FWD, 8>), dim3((unsigned)((quads + 31) / 32)), dim3(256), 0, stream, t);
+        else hipLaunchKernelGGL((linear_reduce_kernel<T, FWD, 1>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, stream, t);
+    } else if (s.tile == 64) {
+        lin_tiled_launch<LinSmall, T, AKM, BKM, FWD ? LIN_EPI_FWD : LIN_EPI_STORE>(t, stream);
+    } else if (s.tile == 256) {
         lin_tiled_launch<LinBig, T, AKM, BKM, FWD ? LIN_EPI_FWD : LIN_EPI_STORE>(t, stream);
     } else {
         lin_tiled_launch<LinMid, T, AKM, BKM, FWD ? LIN_EPI_FWD : LIN_EPI_STORE>(t, stream);
@@ -541,7 +558,7 @@ static void lin_tiled_bwd(const FneusLinear& f, const LinPlan& p, hipStream_t st
         float* sums = f.dbias ? (float*)(S + p.off_sums) : nullptr;
         hipLaunchKernelGGL((linear_delta_kernel<T>), dim3(strips, (unsigned)p.sum_parts), dim3(256), 0, stream, (const T*)f.dy, f.lddy, (const T*)f.z, f.act,
                            f.rows, f.n_out, p.delta ? (T*)(S + p.off_delta) : nullptr, p.ldd, sums);
-        if (f.dbias) hipLaunchKernelGGL((linear_fold_kernel<T>), dim3((unsigned)((f.n_out + 31) / 32)), dim3(1024), 0, stream, sums, p.sum_parts, f.n_out, (T*)f.dbias);
+        if (f.dbias) hipLaunchKernelGGL((linear_fold_kernel<T>), dim3((unsigned)((f.n_out + 7) / 8)), dim3(1024), 0, stream, sums, p.sum_parts, f.n_out, (T*)f.dbias);
         if (p.delta) d = S + p.off_delta, ldd = p.ldd;
     }
     if (f.dx) {

@@ -3,7 +3,7 @@
 //   backward:  g = dy w,  dx = r (g - mean(g) - xh mean(g xh)),  dw = sum_rows dy xh,  db = sum_rows dy
 // Memory bound: the forward reads x and writes y, the backward reads dy and x and writes dx.  A TEAM of TPR threads owns a row and
 // holds it in registers (EPT values a thread, 16-byte chunks): one pass over memory, the variance from the centred values (two
-// passes over registers: a row with a large mean keeps its digits).  TPR = 16 (sums by DPP), 64, 256 or 1024 threads; wider rows
+// passes over registers: a row with a large mean keeps its digits).  TPR = 16 (sums by DPP), 64, 256 or 512 threads; wider rows
 // take the streaming kernels, which read a row from the caches again.
 // The weight gradients: a team keeps its columns' sums of dy xh and dy in registers over all the rows it takes, the teams of a
 // workgroup are added in LDS, every workgroup writes ONE partial row, and a second launch adds the partial rows in a fixed order: no
@@ -13,7 +13,8 @@
 
 namespace fneus {
 
-constexpr int kNormMaxGrid = 1024;       // workgroups of the backward = partial rows of the weight gradients
+constexpr int kNormMaxGrid = 1024;       // workgroups of the backward at most
+constexpr long kNormFwdGrid = 2048;      // of the forward: 8 a CU
 
 // sums of v over the team, in every thread of it.  `red`: LDS floats, 2 * TPR / 64 (TPR > 64); `flip` alternates the half used, so
 // one barrier a sum is enough
@@ -47,57 +48,68 @@ struct NormArgs {
     float eps;
 };
 
+// rows blockIdx, blockIdx + grid, ...: the weights stay in registers
 template <class T, class P, int TPR, int EPT>
 __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) layer_norm_fwd_kernel(NormArgs<T, P> a) {
     constexpr int V = Chunk<T>::N, NC = EPT / V, TEAMS = TPR > 256 ? 1 : 256 / TPR;
     __shared__ float red[2 * (TPR > 64 ? TPR / 64 : 1)];
     int flip = 0;
     const int t = threadIdx.x % TPR;
-    const long row = (long)blockIdx.x * TEAMS + threadIdx.x / TPR;
-    if (TPR <= 64 && row >= a.rows) return;          // (a team of more than a wave is the whole workgroup: its row exists)
-    const T* __restrict__ x = a.x + row * a.ldx;
-    float v[NC][V];
-    float s = 0.0f;
+    P w[NC][V], b[NC][V];                            // (in their own type: half the registers for 16 bits)
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
         const int col = (c * TPR + t) * V;
-        load_chunk<T>(x + col, a.n - col, v[c]);
+        float q[V];
+        if (a.w) load_run<P, V>(a.w + col, a.n - col, q);
+#pragma unroll
+        for (int k = 0; k < V; ++k) w[c][k] = a.w ? (P)q[k] : (P)1.0f;
+        if (a.b) load_run<P, V>(a.b + col, a.n - col, q);
+#pragma unroll
+        for (int k = 0; k < V; ++k) b[c][k] = a.b ? (P)q[k] : (P)0.0f;
     }
+    const float len = (float)a.n;                    // (divisions, not a reciprocal: the mean of equal values is that value)
+    for (long base = (long)blockIdx.x * TEAMS; base < a.rows; base += (long)gridDim.x * TEAMS) {
+        const long row = base + threadIdx.x / TPR;
+        const bool live = row < a.rows;              // (TPR > 64: one team, always live: every wave meets the barriers)
+        const T* __restrict__ x = a.x + row * a.ldx;
+        float v[NC][V];
+        float s = 0.0f;
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-        for (int k = 0; k < V; ++k) s += v[c][k];
-    const float len = (float)a.n;            // (divisions, not a reciprocal: the mean of equal values is that value)
-    const float mu = team_sum<TPR>(s, red, flip) / len;
-    float q = 0.0f;
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-        const int left = a.n - (c * TPR + t) * V;
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-            v[c][k] -= mu;
-            q += k < left ? v[c][k] * v[c][k] : 0.0f;
-        }
-    }
-    const float r = 1.0f / sqrtf(team_sum<TPR>(q, red, flip) / len + a.eps);
-    T* __restrict__ y = a.y + row * a.ldy;
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-        const int col = (c * TPR + t) * V, left = a.n - col;
-        if (left <= 0) break;
-        float w[V], o[V];
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-            w[k] = a.w ? (k < left ? (float)a.w[col + k] : 0.0f) : 1.0f;
-            o[k] = a.b ? (k < left ? (float)a.b[col + k] : 0.0f) : 0.0f;
+        for (int c = 0; c < NC; ++c) {
+            const int col = (c * TPR + t) * V;
+            load_chunk<T>(x + col, live ? a.n - col : 0, v[c]);
         }
 #pragma unroll
-        for (int k = 0; k < V; ++k) o[k] = v[c][k] * r * w[k] + o[k];
-        store_chunk<T>(y + col, left, o);
-    }
-    if (t == 0) {
-        a.mean[row] = mu;
-        a.rstd[row] = r;
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int k = 0; k < V; ++k) s += v[c][k];
+        const float mu = team_sum<TPR>(s, red, flip) / len;
+        float q = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int left = a.n - (c * TPR + t) * V;
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                v[c][k] -= mu;
+                q += k < left ? v[c][k] * v[c][k] : 0.0f;
+            }
+        }
+        const float r = 1.0f / sqrtf(team_sum<TPR>(q, red, flip) / len + a.eps);
+        if (!live) continue;
+        T* __restrict__ y = a.y + row * a.ldy;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int col = (c * TPR + t) * V, left = a.n - col;
+            if (left <= 0) break;
+            float o[V];
+#pragma unroll
+            for (int k = 0; k < V; ++k) o[k] = v[c][k] * r * (float)w[c][k] + (float)b[c][k];
+            store_chunk<T>(y + col, left, o);
+        }
+        if (t == 0) {
+            a.mean[row] = mu;
+            a.rstd[row] = r;
+        }
     }
 }
 
@@ -151,9 +163,10 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) layer_norm_bwd_kernel(N
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
         const int col = (c * TPR + t) * V;
+        if (a.w) load_run<P, V>(a.w + col, a.n - col, w[c]);
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-            w[c][k] = a.w ? (col + k < a.n ? (float)a.w[col + k] : 0.0f) : 1.0f;
+            if (!a.w) w[c][k] = 1.0f;
             dw[c][k] = 0.0f;
             db[c][k] = 0.0f;
         }
@@ -283,22 +296,14 @@ __global__ void __launch_bounds__(256) layer_norm_params_kernel(NormArgs<T, P> a
     out[a.n + col] = db;
 }
 
-// dw, db = the sums of the partial rows in their order: 32 columns a workgroup, 32 threads a column
+// dw, db = the sums of the partial rows
 template <class P>
 __global__ void __launch_bounds__(1024) layer_norm_fold_kernel(const float* __restrict__ partial, int parts, int n, P* __restrict__ dw,
                                                                P* __restrict__ db) {
-    __shared__ float red[32][33];
-    const int lane = threadIdx.x & 31, group = threadIdx.x >> 5;
-    const long col = (long)blockIdx.x * 32 + lane;           // of the 2 n columns
-    float s = 0.0f;
-    if (col < 2L * n)
-        for (int p = group; p < parts; p += 32) s += partial[(long)p * 2 * n + col];
-    red[group][lane] = s;
-    __syncthreads();
-    if (threadIdx.x < 32 && col < 2L * n) {
-        s = 0.0f;
-#pragma unroll
-        for (int g = 0; g < 32; ++g) s += red[g][lane];
+    __shared__ float red[128][9];
+    const long col0 = 8L * blockIdx.x, col = col0 + threadIdx.x;          // of the 2 n columns
+    const float s = fold_rows8(partial, parts, 2L * n, col0, 2L * n, red);
+    if (threadIdx.x < 8 && col < 2L * n) {
         if (col < n) {
             if (dw) dw[col] = (P)s;
         } else if (db) {
@@ -309,23 +314,23 @@ __global__ void __launch_bounds__(1024) layer_norm_fold_kernel(const float* __re
 
 struct NormShape { int tpr, ept; };      // tpr 0: streaming
 
-// 16 values a thread are the most that four register arrays of them leave room for; the fewest threads that hold the row
+// The narrowest team whose threads hold the row in at most 32 values each (the backward keeps five registers a value); 16 threads up to
+// 256 values (sums by DPP, four rows a wave), one wave up to 2048 (no barrier), four and eight waves up to 8192 and 16384
 static NormShape norm_shape(int n) {
     if (n <= 256) return {16, 16};
-    if (n <= 512) return {64, 8};
-    if (n <= 1024) return {64, 16};
-    if (n <= 2048) return {256, 8};
-    if (n <= 4096) return {256, 16};
-    if (n <= 8192) return {1024, 8};
-    if (n <= 16384) return {1024, 16};
+    if (n <= 2048) return {64, 8 * ((n + 511) / 512)};
+    if (n <= 8192) return {256, 8 * ((n + 2047) / 2048)};
+    if (n <= 16384) return {512, 8 * ((n + 4095) / 4096)};
     return {0, 0};
 }
 
+static int norm_teams(const NormShape& s) { return s.tpr == 0 || s.tpr > 256 ? 1 : 256 / s.tpr; }
+
+// workgroups of the backward = partial rows of the weight gradients
 static int norm_grid(long rows, int n) {
     const NormShape s = norm_shape(n);
-    const int teams = s.tpr == 0 ? 1 : (s.tpr > 256 ? 1 : 256 / s.tpr);
-    const long need = (rows + teams - 1) / teams;
-    const long most = s.tpr == 0 ? 64 : (s.tpr >= 256 ? 512 : kNormMaxGrid);
+    const long need = (rows + norm_teams(s) - 1) / norm_teams(s);
+    const long most = s.tpr == 0 ? 64 : (s.tpr >= 64 ? 512 : kNormMaxGrid);
     return (int)(need < most ? need : most);
 }
 
@@ -334,10 +339,13 @@ static int norm_grid(long rows, int n) {
         case 1616: CALL(16, 16); break; \
         case 6408: CALL(64, 8); break; \
         case 6416: CALL(64, 16); break; \
-        case 25608: CALL(256, 8); break; \
+        case 6424: CALL(64, 24); break; \
+        case 6432: CALL(64, 32); break; \
         case 25616: CALL(256, 16); break; \
-        case 102408: CALL(1024, 8); break; \
-        default: CALL(1024, 16); break; \
+        case 25624: CALL(256, 24); break; \
+        case 25632: CALL(256, 32); break; \
+        case 51224: CALL(512, 24); break; \
+        default: CALL(512, 32); break; \
     }
 
 template <class T, class P>
@@ -347,8 +355,9 @@ static void norm_fwd_launch(const NormArgs<T, P>& a, hipStream_t stream) {
         hipLaunchKernelGGL((layer_norm_fwd_stream_kernel<T, P>), dim3((unsigned)a.rows), dim3(1024), 0, stream, a);
         return;
     }
-    const int threads = s.tpr > 256 ? s.tpr : 256, teams = threads / s.tpr;
-    const dim3 grid((unsigned)((a.rows + teams - 1) / teams));
+    const int threads = s.tpr > 256 ? s.tpr : 256, teams = norm_teams(s);
+    const long need = (a.rows + teams - 1) / teams;
+    const dim3 grid((unsigned)(need < kNormFwdGrid ? need : kNormFwdGrid));
 #define CALL(TPR, EPT) hipLaunchKernelGGL((layer_norm_fwd_kernel<T, P, TPR, EPT>), grid, dim3(threads), 0, stream, a)
     FN_NORM_SHAPES(CALL)
 #undef CALL
@@ -376,7 +385,7 @@ static void norm_bwd_launch(const NormArgs<T, P>& a, P* dw, P* db, hipStream_t s
         }
     }
     if (params)
-        hipLaunchKernelGGL((layer_norm_fold_kernel<P>), dim3((unsigned)((2L * a.n + 31) / 32)), dim3(1024), 0, stream, a.partial, grid, a.n, dw, db);
+        hipLaunchKernelGGL((layer_norm_fold_kernel<P>), dim3((unsigned)((2L * a.n + 7) / 8)), dim3(1024), 0, stream, a.partial, grid, a.n, dw, db);
 }
 
 static int norm_check(const char* what, const void* x, const void* out, const void* mean, const void* rstd, long rows, int n, int dtype,
