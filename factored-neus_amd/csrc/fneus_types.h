@@ -47,6 +47,37 @@ FN_DEV void store_chunk(T* p, int valid, const float (&v)[Chunk<T>::N]) {
     }
 }
 
+// four consecutive values
+template <class T> struct Quad;
+template <> struct Quad<float> { typedef float type __attribute__((ext_vector_type(4), aligned(4))); };
+template <> struct Quad<__bf16> { typedef __bf16 type __attribute__((ext_vector_type(4), aligned(2))); };
+template <> struct Quad<_Float16> { typedef _Float16 type __attribute__((ext_vector_type(4), aligned(2))); };
+
+template <class T>
+FN_DEV void quad_load(const T* p, int valid, float (&v)[4]) {
+    if (valid >= 4) {
+        const typename Quad<T>::type q = *reinterpret_cast<const typename Quad<T>::type*>(p);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = (float)q[k];
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = k < valid ? (float)p[k] : 0.0f;
+    }
+}
+template <class T>
+FN_DEV void quad_store(T* p, int valid, const float (&v)[4]) {
+    if (valid >= 4) {
+        typename Quad<T>::type q;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) q[k] = (T)v[k];
+        *reinterpret_cast<typename Quad<T>::type*>(p) = q;
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (k < valid) p[k] = (T)v[k];
+    }
+}
+
 // the same for a run of V values, V a multiple of the chunk
 template <class T, int V>
 FN_DEV void load_run(const T* p, int valid, float (&v)[V]) {

@@ -2,6 +2,7 @@
 //   z = x W^T + b,  y = act(z) + res;      delta = dy act'(z),  dx = delta W,  dW = delta^T x,  db = column sums of delta
 // The three products are one form, D(i, j) = sum_k A(i, k) B(j, k), with either operand stored along k or along its rows.
 #include <stdlib.h>
+#include <type_traits>
 #include "mm_engine.h"
 #include "fneus_kernels.h"
 
@@ -24,29 +25,31 @@ struct LinProduct {
     long first_tile;
 };
 
-// 8 values of an operand for one lane, (i, k0 .. k0 + 7), zero beyond the matrix.  ROWS: stored along k (unaligned 16-byte loads),
-// else element (i, k) at p[k ld + i] (the 32 lanes of a half read consecutive values)
-template <class T, bool ROWS>
+// 8 values of an operand for one lane, (i, k0 .. k0 + 7).  ROWS: stored along k (unaligned 16-byte loads), else element (i, k) at
+// p[k ld + i] (the lanes of a half read consecutive values).  No branch around a load, whose result the compiler would wait for inside it:
+// a row beyond the last is the last one again (its products end in elements nobody stores); MASKED, the last values of k: addresses are
+// kept below kend and what lies beyond counts as zero.
+template <class T, bool ROWS, bool MASKED>
 FN_DEV void lin_load8(const T* __restrict__ p, long ld, long i, long ni, long k0, long kend, float (&v)[8]) {
-    const bool in = i < ni;
-    if constexpr (ROWS) {
+    i = i < ni ? i : ni - 1;
+    if constexpr (ROWS && !MASKED) {
         const T* q = p + i * ld + k0;
-        const long left = in ? kend - k0 : 0;
         constexpr int N = Chunk<T>::N;
-        if (left >= 8) {
 #pragma unroll
-            for (int c = 0; c < 8 / N; ++c) {
-                const typename Chunk<T>::type u = *reinterpret_cast<const typename Chunk<T>::type*>(q + c * N);
+        for (int c = 0; c < 8 / N; ++c) {
+            const typename Chunk<T>::type u = *reinterpret_cast<const typename Chunk<T>::type*>(q + c * N);
 #pragma unroll
-                for (int k = 0; k < N; ++k) v[c * N + k] = (float)u[k];
-            }
-        } else {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = k < left ? (float)q[k] : 0.0f;
+            for (int k = 0; k < N; ++k) v[c * N + k] = (float)u[k];
         }
     } else {
+        const T* q = ROWS ? p + i * ld : p + i;
+        const long step = ROWS ? 1 : ld;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = in && k0 + k < kend ? (float)p[(k0 + k) * ld + i] : 0.0f;
+        for (int k = 0; k < 8; ++k) v[k] = (float)q[(MASKED && k0 + k >= kend ? kend - 1 : k0 + k) * step];
+        if constexpr (MASKED) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = k0 + k < kend ? v[k] : 0.0f;
+        }
     }
 }
 
@@ -55,7 +58,7 @@ FN_DEV void lin_load8(const T* __restrict__ p, long ld, long i, long ni, long k0
 // chip, where a launch's latency is what counts: one launch forward, one backward.
 template <class T, int KIND>
 FN_DEV void lin_direct_tile(const LinProduct& P, long tile, float (*red)[16][65], float (*red_db)[32]) {
-    constexpr bool AROWS = KIND != LIN_DW, BROWS = KIND == LIN_FWD;
+    constexpr bool AROWS = KIND != LIN_DW, BROWS = KIND == LIN_FWD;      // (how a and b are stored)
     const long i0 = 32 * (tile / P.tiles_j);
     const int j0 = 32 * (int)(tile % P.tiles_j);
     const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
@@ -67,19 +70,21 @@ FN_DEV void lin_direct_tile(const LinProduct& P, long tile, float (*red)[16][65]
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[e] = 0.0f;
     float asum = 0.0f;
-    constexpr int U = 2;
-    for (long k = kb; k < ke; k += 16 * U) {
+    const bool scaled = KIND != LIN_FWD && az, multiply = KIND != LIN_DW || P.d;       // (no D: the bias gradient alone)
+    auto round = [&](auto masked, auto unroll, long k) {
+        constexpr bool M = decltype(masked)::value;
+        constexpr int U = decltype(unroll)::value;
         float av[U][8], bv[U][8], zv[U][8];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const long k0 = k + 16 * u + 8 * h;
-            lin_load8<T, AROWS>(a, P.lda, i0 + r, P.ni, k0, ke, av[u]);
-            lin_load8<T, BROWS>(b, P.ldb, j0 + r, P.d ? P.nj : 0, k0, ke, bv[u]);      // (no D: the bias gradient alone)
-            if (KIND != LIN_FWD && az) lin_load8<T, AROWS>(az, P.ldz, i0 + r, P.ni, k0, ke, zv[u]);
+            lin_load8<T, AROWS, M>(a, P.lda, i0 + r, P.ni, k0, ke, av[u]);
+            if (multiply) lin_load8<T, BROWS, M>(b, P.ldb, j0 + r, P.nj, k0, ke, bv[u]);
+            if (scaled) lin_load8<T, AROWS, M>(az, P.ldz, i0 + r, P.ni, k0, ke, zv[u]);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            if (KIND != LIN_FWD && az) {
+            if (scaled) {
 #pragma unroll
                 for (int s = 0; s < 8; ++s) av[u][s] *= lin_dact(zv[u][s], P.act);
             }
@@ -87,12 +92,18 @@ FN_DEV void lin_direct_tile(const LinProduct& P, long tile, float (*red)[16][65]
 #pragma unroll
                 for (int s = 0; s < 8; ++s) asum += av[u][s];
             }
-            LinFrag<T> fa, fb;
-            lin_frag(av[u], fa);
-            lin_frag(bv[u], fb);
-            acc = lin_mfma32(fb, fa, acc);           // accumulator rows = j, columns (lanes) = i
+            if (multiply) {
+                LinFrag<T> fa, fb;
+                lin_frag(av[u], fa);
+                lin_frag(bv[u], fb);
+                acc = lin_mfma32(fb, fa, acc);           // accumulator rows = j, columns (lanes) = i
+            }
         }
-    }
+    };
+    long k = kb;
+    for (; k + 64 <= ke; k += 64) round(std::false_type{}, std::integral_constant<int, 4>{}, k);
+    for (; k + 16 <= ke; k += 16) round(std::false_type{}, std::integral_constant<int, 1>{}, k);
+    if (k < ke) round(std::true_type{}, std::integral_constant<int, 1>{}, k);
 #pragma unroll
     for (int e = 0; e < 16; ++e) red[wave][e][lane] = acc[e];
     if constexpr (KIND == LIN_DW) {
@@ -156,13 +167,14 @@ __global__ void __launch_bounds__(512) linear_row_kernel(LinProduct P) {
     const long kb = wave * part, ke = kb + part < P.nk ? kb + part : P.nk;
     const T *a = (const T*)P.a, *b = (const T*)P.b;
     f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    constexpr int U = 4;
-    for (long k = kb; k < ke; k += 32 * U) {
+    auto round = [&](auto masked, auto unroll, long k) {
+        constexpr bool M = decltype(masked)::value;
+        constexpr int U = decltype(unroll)::value;
         float av[U][8], bv[U][8];
 #pragma unroll
-        for (int u = 0; u < U; ++u) lin_load8<T, true>(b, P.ldb, j0 + r, P.nj, k + 32 * u + 8 * g, ke, bv[u]);
+        for (int u = 0; u < U; ++u) lin_load8<T, true, M>(b, P.ldb, j0 + r, P.nj, k + 32 * u + 8 * g, ke, bv[u]);
 #pragma unroll
-        for (int u = 0; u < U; ++u) lin_load8<T, true>(a, P.lda, r, P.ni, k + 32 * u + 8 * g, ke, av[u]);
+        for (int u = 0; u < U; ++u) lin_load8<T, true, M>(a, P.lda, r, P.ni, k + 32 * u + 8 * g, ke, av[u]);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             LinFrag<T> fa, fb;
@@ -170,7 +182,12 @@ __global__ void __launch_bounds__(512) linear_row_kernel(LinProduct P) {
             lin_frag(bv[u], fb);
             acc = lin_mfma16(fb, fa, acc);
         }
-    }
+    };
+    long k = kb;
+    constexpr int DEEP = sizeof(T) == 2 ? 8 : 4;             // loads of W in flight a wave
+    for (; k + 32 * DEEP <= ke; k += 32 * DEEP) round(std::false_type{}, std::integral_constant<int, DEEP>{}, k);
+    for (; k + 32 <= ke; k += 32) round(std::false_type{}, std::integral_constant<int, 1>{}, k);
+    if (k < ke) round(std::true_type{}, std::integral_constant<int, 1>{}, k);
 #pragma unroll
     for (int e = 0; e < 4; ++e) red[wave][4 * g + e][r] = acc[e];        // row j = 4 g + e, column i = r
     __syncthreads();
@@ -201,36 +218,6 @@ struct LinTiled {
 };
 
 enum { LIN_EPI_FWD = 0, LIN_EPI_STORE = 1, LIN_EPI_PART = 2 };
-
-template <class T> struct Quad;
-template <> struct Quad<float> { typedef float type __attribute__((ext_vector_type(4), aligned(4))); };
-template <> struct Quad<__bf16> { typedef __bf16 type __attribute__((ext_vector_type(4), aligned(2))); };
-template <> struct Quad<_Float16> { typedef _Float16 type __attribute__((ext_vector_type(4), aligned(2))); };
-
-template <class T>
-FN_DEV void quad_load(const T* p, int valid, float (&v)[4]) {
-    if (valid >= 4) {
-        const typename Quad<T>::type q = *reinterpret_cast<const typename Quad<T>::type*>(p);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = (float)q[k];
-    } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = k < valid ? (float)p[k] : 0.0f;
-    }
-}
-template <class T>
-FN_DEV void quad_store(T* p, int valid, const float (&v)[4]) {
-    if (valid >= 4) {
-        typename Quad<T>::type q;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) q[k] = (T)v[k];
-        *reinterpret_cast<typename Quad<T>::type*>(p) = q;
-    } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (k < valid) p[k] = (T)v[k];
-    }
-}
 
 // bias, pre-activation, activation, residual of four consecutive outputs of row i
 template <class T>

@@ -10,6 +10,7 @@
 // rounding left, times another 2^11, so that it is as normal as the first; products hi hi + hi lo + lo hi (22 bits: fp32's accuracy at
 // half the matrix work of three bf16 terms).
 #include <math.h>
+#include <stdlib.h>
 #include "mm_engine.h"
 #include "fneus_kernels.h"
 
@@ -197,17 +198,31 @@ FN_DEV void muon_write4(unsigned char* p, long plane, const float (&v)[4], f16x4
 
 enum { MU_GRAM = 0, MU_POLY = 1, MU_STEP = 2, MU_LAST = 3 };
 
+// The tiles on and above the diagonal of a symmetric product, numbered by columns
+FN_DEV void muon_upper(int t, int& ti, int& tj) {
+    tj = (int)((sqrtf(8.0f * (float)t + 1.0f) - 1.0f) * 0.5f);
+    while ((tj + 1) * (tj + 2) / 2 <= t) ++tj;
+    while (tj * (tj + 1) / 2 > t) --tj;
+    ti = t - tj * (tj + 1) / 2;
+}
+
 // GRAM: A = X X^T.  POLY: B = b A + c A A.  STEP: X' = a X + B X.  LAST: the same into `out` or the parameter.
+// A and B are symmetric: the tiles below the diagonal are the mirror images the tiles above it write.  The epilogue goes through LDS, 32
+// rows of a wave at a time, so that either orientation writes runs of a line.
 template <class Cfg, int NP, int KIND, class T, bool MOM>
 __global__ void __launch_bounds__(Cfg::THREADS, 2) muon_product_kernel(MuonJobs js, MuonNum P, int cur) {
     extern __shared__ __attribute__((aligned(16))) unsigned char mm_smem[];
     const MuonJob& J = js.j[muon_find(js, blockIdx.x)];
     const MuonLay L = muon_lay(J.rows, J.cols, NP);
     unsigned char* S = js.scratch + J.off;
-    const int ni = L.m, nj = KIND <= MU_POLY ? L.m : L.n;
+    constexpr bool SYM = KIND <= MU_POLY;
+    const int ni = L.m, nj = SYM ? L.m : L.n;
     const int tiles_i = (ni + Cfg::BM - 1) / Cfg::BM, tiles_j = (nj + Cfg::BN - 1) / Cfg::BN;
+    const long tiles = SYM ? (long)tiles_i * (tiles_i + 1) / 2 : (long)tiles_i * tiles_j;
     int ti, tj;
-    mm_tile(mm_spread(blockIdx.x - J.first, (long)tiles_i * tiles_j), tiles_i, tiles_j, ti, tj);
+    const long t = mm_spread(blockIdx.x - J.first, tiles);
+    if constexpr (SYM) muon_upper((int)t, ti, tj);
+    else mm_tile(t, tiles_i, tiles_j, ti, tj);
     const long i0 = (long)ti * Cfg::BM, j0 = (long)tj * Cfg::BN;
     MmOperand A, B;
     if constexpr (KIND == MU_GRAM) A = B = muon_op<NP>(S + L.x[cur], L.px, L.ldx);
@@ -223,82 +238,151 @@ __global__ void __launch_bounds__(Cfg::THREADS, 2) muon_product_kernel(MuonJobs 
     if constexpr (KIND == MU_GRAM) f = ldexpf(lo, P.ea - 2 * P.ex);
     else if constexpr (KIND == MU_POLY) f = P.c * ldexpf(lo, P.eb - 2 * P.ea);
     else f = ldexpf(lo, (KIND == MU_STEP ? P.ex : 0) - P.eb - P.ex);
+    const float fb = KIND == MU_POLY ? ldexpf(P.b, P.eb - P.ea) : 0.0f;
+    const float fa = KIND == MU_STEP ? P.a : ldexpf(P.a, -P.ex);
     const float lr = KIND == MU_LAST && MOM ? *P.lr : 0.0f;
+    const float keep = 1.0f - lr * P.wd, step = lr * J.adjust;
+    const bool turn = SYM ? ti != tj : (KIND == MU_LAST && L.trans);          // the second orientation is written too (SYM) or alone
+    constexpr int STRIDE = Cfg::WN + 4;
+    static_assert(Cfg::WAVES * 32 * STRIDE * 4 <= Cfg::LDS, "the epilogue's rows fit the ring");
+    float* rows = reinterpret_cast<float*>(mm_smem) + mm_wave() * 32 * STRIDE;
+    const int lane = threadIdx.x & 63;
+    __syncthreads();                                  // (everyone has read the last stage)
 #pragma unroll
     for (int m = 0; m < Cfg::MI; ++m) {
-        const long i = i0 + mm_wave_i<Cfg>() + 32 * m + (threadIdx.x & 31);
+        const long ib = i0 + mm_wave_i<Cfg>() + 32 * m, jb = j0 + mm_wave_j<Cfg>();
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int n = 0; n < Cfg::NJ; ++n)
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const long j = j0 + mm_wave_j<Cfg>() + 32 * n + 8 * g + 4 * ((threadIdx.x >> 5) & 1);
-                float v[4];
+                f32x4 q;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) v[k] = acc[m][n][4 * g + k] * f;
-                f16x4 hi, lo4;
-                if constexpr (KIND == MU_GRAM || KIND == MU_POLY) {
-                    if (i >= ni || j >= (long)L.lda / 2) continue;
-                    if constexpr (KIND == MU_POLY) {
-                        float a[4];
-                        muon_read4<NP>(S + L.a + i * L.lda + j * 2, L.pa, a);
-                        const float fb = ldexpf(P.b, P.eb - P.ea);
+                for (int k = 0; k < 4; ++k) q[k] = acc[m][n][4 * g + k] * f;
+                *reinterpret_cast<f32x4*>(rows + (lane & 31) * STRIDE + 32 * n + 8 * g + 4 * (lane >> 5)) = q;
+            }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        constexpr int QUADS = Cfg::WN / 4;
+#pragma unroll 2
+        for (int s = 0; s < 32 * QUADS / 64; ++s) {
+            const int at = s * 64 + lane, r = at / QUADS, c = 4 * (at % QUADS);
+            const long i = ib + r, j = jb + c;
+            float* cell = rows + r * STRIDE + c;
+            const f32x4 q = *reinterpret_cast<const f32x4*>(cell);
+            float v[4] = {q[0], q[1], q[2], q[3]};
+            f16x4 hi, lo4;
+            if constexpr (SYM) {
+                if (i >= ni || j >= L.mp) continue;
+                if constexpr (KIND == MU_POLY) {
+                    float a[4];
+                    muon_read4<NP>(S + L.a + i * L.lda + j * 2, L.pa, a);
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) v[k] += fb * a[k];
+                    for (int k = 0; k < 4; ++k) v[k] += fb * a[k];
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = j + k < nj ? v[k] : 0.0f;
+                muon_write4<NP>(S + (KIND == MU_GRAM ? L.a : L.b) + i * L.lda + j * 2, L.pa, v, hi, lo4);
+            } else {
+                if (j >= (long)L.ldx / 2 || i >= L.mp) continue;
+                float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                if (i < ni) muon_read4<NP>(S + L.x[cur] + i * L.ldx + j * 2, L.px, x);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = i < ni && j + k < nj ? v[k] + fa * x[k] : 0.0f;
+                if constexpr (KIND == MU_STEP) {
+                    muon_write4<NP>(S + L.x[cur ^ 1] + i * L.ldx + j * 2, L.px, v, hi, lo4);
+                } else if (!L.trans && i < ni) {
+                    T* p = (T*)(MOM ? J.param : J.out) + i * (long)J.cols + j;
+                    const int valid = (int)(nj - j);
+                    if constexpr (MOM) {
+                        float w[4];
+                        quad_load(p, valid, w);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) v[k] = w[k] * keep - step * v[k];
                     }
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) v[k] = j + k < nj ? v[k] : 0.0f;
-                    muon_write4<NP>(S + (KIND == MU_GRAM ? L.a : L.b) + i * L.lda + j * 2, L.pa, v, hi, lo4);
-                } else {
-                    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    if (i < ni && j < (long)L.ldx / 2) muon_read4<NP>(S + L.x[cur] + i * L.ldx + j * 2, L.px, x);
-                    const float fa = KIND == MU_STEP ? P.a : ldexpf(P.a, -P.ex);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) v[k] = i < ni && j + k < nj ? v[k] + fa * x[k] : 0.0f;
-                    if constexpr (KIND == MU_STEP) {
-                        if (i < L.mp && j < (long)L.ldx / 2) muon_write4<NP>(S + L.x[cur ^ 1] + i * L.ldx + j * 2, L.px, v, hi, lo4);
-                    } else if (i < ni) {
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            if (j + k < nj) {
-                                const long at = L.trans ? (j + k) * (long)J.cols + i : i * (long)J.cols + j + k;
-                                if constexpr (MOM) {
-                                    T* p = (T*)J.param + at;
-                                    *p = (T)((float)*p * (1.0f - lr * P.wd) - lr * J.adjust * v[k]);
-                                } else {
-                                    ((T*)J.out)[at] = (T)v[k];
-                                }
-                            }
-                    }
+                    quad_store(p, valid, v);
                 }
             }
+            if (turn && (KIND == MU_POLY || KIND == MU_LAST)) *reinterpret_cast<f32x4*>(cell) = f32x4{v[0], v[1], v[2], v[3]};
+        }
+        if constexpr (KIND == MU_STEP) continue;
+        if (!turn) continue;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll 2
+        for (int s = 0; s < Cfg::WN * 8 / 64; ++s) {
+            const int at = s * 64 + lane, c = at / 8, r = 4 * (at % 8);
+            const long i = ib + r, j = jb + c;
+            if (j >= nj || i >= ni) continue;
+            float v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = rows[(r + k) * STRIDE + c];
+            if constexpr (SYM) {
+                // (i + k >= ni: the padding of row j, zero as the tile on the other side of the diagonal leaves it)
+                f16x4 hi, lo4;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = i + k < ni ? v[k] : 0.0f;
+                muon_write4<NP>(S + (KIND == MU_GRAM ? L.a : L.b) + j * L.lda + i * 2, L.pa, v, hi, lo4);
+            } else {
+                T* p = (T*)(MOM ? J.param : J.out) + j * (long)J.cols + i;
+                const int valid = (int)(ni - i);
+                if constexpr (MOM) {
+                    float w[4];
+                    quad_load(p, valid, w);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) v[k] = w[k] * keep - step * v[k];
+                }
+                quad_store(p, valid, v);
+            }
+        }
     }
 }
 
-typedef MmCfg<64, 64, 2, 2, 3> MuonSmall;
-typedef MmCfg<128, 128, 2, 2, 2> MuonLarge;
+typedef MmCfg<64, 64, 2, 2, 5> MuonSmall;          // 80 KiB: four stages in flight, two workgroups a CU
+typedef MmCfg<128, 128, 2, 2, 2> MuonMid;          // 64 KiB, two
+typedef MmCfg<256, 256, 2, 4, 2> MuonBig;          // 128 KiB, one
+
+static long muon_tiles(long m, long n, bool sym, int b) {
+    const long ti = (m + b - 1) / b, tj = (n + b - 1) / b;
+    return sym ? ti * (ti + 1) / 2 : ti * tj;
+}
 
 template <class Cfg, int NP, int KIND, class T, bool MOM>
-static void muon_product(MuonJobs& js, const MuonNum& P, int cur, hipStream_t stream) {
+static void muon_product_launch(MuonJobs& js, const MuonNum& P, int cur, hipStream_t stream) {
     long tiles = 0;
     for (int q = 0; q < js.n; ++q) {
         MuonJob& J = js.j[q];
-        const long m = J.rows < J.cols ? J.rows : J.cols, n = J.rows < J.cols ? J.cols : J.rows;
         J.first = (int)tiles;
-        tiles += ((m + Cfg::BM - 1) / Cfg::BM) * (((KIND <= MU_POLY ? m : n) + Cfg::BN - 1) / Cfg::BN);
+        tiles += muon_tiles(J.rows < J.cols ? J.rows : J.cols, J.rows < J.cols ? J.cols : J.rows, KIND <= MU_POLY, Cfg::BM);
     }
     auto kernel = muon_product_kernel<Cfg, NP, KIND, T, MOM>;
-    static const bool once = (allow_big_lds(kernel), true);
-    (void)once;
+    allow_big_lds(kernel);
     hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(Cfg::THREADS), Cfg::LDS, stream, js, P, cur);
 }
 
-template <class Cfg, int NP, class T, bool MOM>
+// the largest tile that leaves no more than a quarter of the CUs without one
+template <int NP, int KIND, class T, bool MOM>
+static void muon_product(MuonJobs& js, const MuonNum& P, int cur, hipStream_t stream) {
+    long big = 0, mid = 0;
+    for (int q = 0; q < js.n; ++q) {
+        const MuonJob& J = js.j[q];
+        const long m = J.rows < J.cols ? J.rows : J.cols, n = J.rows < J.cols ? J.cols : J.rows;
+        big += muon_tiles(m, n, KIND <= MU_POLY, 256), mid += muon_tiles(m, n, KIND <= MU_POLY, 128);
+    }
+    static const int form = getenv("FNEUS_MUON_TILE") ? atoi(getenv("FNEUS_MUON_TILE")) : 0;
+    if (form ? form == 256 : big >= 192) muon_product_launch<MuonBig, NP, KIND, T, MOM>(js, P, cur, stream);
+    else if (form ? form == 128 : mid >= 192) muon_product_launch<MuonMid, NP, KIND, T, MOM>(js, P, cur, stream);
+    else muon_product_launch<MuonSmall, NP, KIND, T, MOM>(js, P, cur, stream);
+}
+
+template <int NP, class T, bool MOM>
 static void muon_steps(MuonJobs& js, const MuonNum& P, int steps, hipStream_t stream) {
     for (int s = 0; s < steps; ++s) {
-        muon_product<Cfg, NP, MU_GRAM, T, MOM>(js, P, s & 1, stream);
-        muon_product<Cfg, NP, MU_POLY, T, MOM>(js, P, s & 1, stream);
-        if (s + 1 < steps) muon_product<Cfg, NP, MU_STEP, T, MOM>(js, P, s & 1, stream);
-        else muon_product<Cfg, NP, MU_LAST, T, MOM>(js, P, s & 1, stream);
+        muon_product<NP, MU_GRAM, T, MOM>(js, P, s & 1, stream);
+        muon_product<NP, MU_POLY, T, MOM>(js, P, s & 1, stream);
+        if (s + 1 < steps) muon_product<NP, MU_STEP, T, MOM>(js, P, s & 1, stream);
+        else muon_product<NP, MU_LAST, T, MOM>(js, P, s & 1, stream);
     }
 }
 
@@ -308,7 +392,7 @@ static int muon_run(const FneusMuonJob* jobs, int n_jobs, const MuonNum& P, int 
         MuonJobs js;
         js.n = n_jobs - first < kMuonMaxJobs ? n_jobs - first : kMuonMaxJobs;
         js.scratch = scratch;
-        long off = 0, tiles = 0, large = 0;
+        long off = 0, tiles = 0;
         for (int q = 0; q < js.n; ++q) {
             const FneusMuonJob& f = jobs[first + q];
             MuonJob& J = js.j[q];
@@ -316,13 +400,10 @@ static int muon_run(const FneusMuonJob* jobs, int n_jobs, const MuonNum& P, int 
             J.rows = f.rows, J.cols = f.cols, J.adjust = f.adjust, J.off = off, J.first = (int)tiles;
             off += muon_lay(f.rows, f.cols, NP).total;
             tiles += (long)((f.rows + 63) / 64) * ((f.cols + 63) / 64);
-            const long m = f.rows < f.cols ? f.rows : f.cols;
-            large += ((m + 127) / 128) * ((m + 127) / 128);
         }
         hipLaunchKernelGGL((muon_norm_kernel<T, MOM>), dim3((unsigned)(js.n * kMuonChunks)), dim3(256), 0, stream, js, P);
         hipLaunchKernelGGL((muon_init_kernel<T, MOM, NP>), dim3((unsigned)tiles), dim3(256), 0, stream, js, P);
-        if (large >= 128) muon_steps<MuonLarge, NP, T, MOM>(js, P, steps, stream);
-        else muon_steps<MuonSmall, NP, T, MOM>(js, P, steps, stream);
+        muon_steps<NP, T, MOM>(js, P, steps, stream);
     }
     return launch_status();
 }

@@ -1,7 +1,6 @@
 """Thin torch-tensor wrappers over the C ABI (device memory + stream plumbing only; no maths here)."""
 from __future__ import annotations
 
-import contextlib as _contextlib
 import ctypes as C
 from typing import Optional
 
@@ -1221,11 +1220,14 @@ def mlp_backward_params(jobs):
 
 # ---- layer norm, fp32 / bf16 / fp16 (csrc/norm_kernels.hip) ---------------------------------------------------------------------------
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_FLOAT = (torch.float32,)
 
 
-def _device_scope(t: torch.Tensor):
-    """the launches of an operator go to the device of its tensors, whichever is current"""
-    return _contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
+def _at(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
 
 
 def _rows(t: torch.Tensor, name: str, like: Optional[torch.Tensor] = None, shape=None) -> torch.Tensor:
@@ -1244,19 +1246,20 @@ def _rows(t: torch.Tensor, name: str, like: Optional[torch.Tensor] = None, shape
 
 
 def _ld(t: torch.Tensor) -> int:
-    return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
+    rows, n = t.shape
+    return t.stride(0) if rows > 1 and n > 0 else n
 
 
 def _vector(t: Optional[torch.Tensor], name: str, n: int, like: torch.Tensor, types) -> Optional[torch.Tensor]:
     if t is None:
         return None
-    if t.dim() != 1 or t.shape[0] != n or t.dtype not in types or t.device != like.device:
+    if t.shape != (n,) or t.dtype not in types or t.device != like.device:
         raise ValueError(f"{name} must be a [{n}] tensor of {' or '.join(str(d) for d in types)} on {like.device}")
     return t if t.is_contiguous() else t.contiguous()
 
 
 def _norm_weights(weight, bias, x):
-    types = (x.dtype,) if x.dtype == torch.float32 else (x.dtype, torch.float32)
+    types = (x.dtype, torch.float32)
     weight, bias = _vector(weight, "layer_norm: weight", x.shape[1], x, types), _vector(bias, "layer_norm: bias", x.shape[1], x, types)
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise ValueError("layer_norm: weight and bias must have one type")
@@ -1268,15 +1271,18 @@ def layer_norm_fwd(x, weight=None, bias=None, eps: float = 1e-5):
     """x [rows, n] -> (y, mean [rows], rstd [rows]): y = (x - mean) rstd weight + bias over each row, rstd = 1 / sqrt(var + eps).
     weight / bias [n]: x's type or float32, or None.  mean and rstd (float32) are what layer_norm_bwd takes."""
     x = _rows(x, "layer_norm: x")
+    device = x.device.index
+    if device != _current_device():              # the launches go to the device of the tensors, whichever is current
+        with torch.cuda.device(device):
+            return layer_norm_fwd(x, weight, bias, eps)
     rows, n = x.shape
     if n == 0:
         raise ValueError("layer_norm: rows without values have no mean")
     weight, bias, wtype = _norm_weights(weight, bias, x)
-    with _device_scope(x):
-        y = torch.empty_like(x, memory_format=torch.contiguous_format)
-        mean, rstd = torch.empty(2, rows, dtype=torch.float32, device=x.device).unbind(0)
-        _launch("fneus_layer_norm_fwd", lib.fneus_layer_norm_fwd, _ptr(x), _ld(x), _ptr(weight), _ptr(bias), _ptr(y), n, _ptr(mean), _ptr(rstd),
-                rows, n, eps, _DTYPES[x.dtype], wtype, _stream())
+    y = x.new_empty((rows, n))
+    mean, rstd = x.new_empty((rows,), dtype=torch.float32), x.new_empty((rows,), dtype=torch.float32)
+    _launch("fneus_layer_norm_fwd", lib.fneus_layer_norm_fwd, x.data_ptr(), _ld(x), _at(weight), _at(bias), y.data_ptr(), n, mean.data_ptr(),
+            rstd.data_ptr(), rows, n, eps, _DTYPES[x.dtype], wtype, _raw_stream(device))
     return y, mean, rstd
 
 
@@ -1284,25 +1290,26 @@ def layer_norm_bwd(dy, x, weight, mean, rstd, need_params: bool = True):
     """(dx, dweight, dbias) of layer_norm_fwd; dweight and dbias [n] in weight's type (float32 where there is no weight), summed over the
     rows in a fixed order, or None without need_params"""
     x = _rows(x, "layer_norm: x")
+    device = x.device.index
+    if device != _current_device():
+        with torch.cuda.device(device):
+            return layer_norm_bwd(dy, x, weight, mean, rstd, need_params)
     dy = _rows(dy, "layer_norm: dy", x, x.shape)
     rows, n = x.shape
     weight, _, wtype = _norm_weights(weight, None, x)
-    if weight is None and x.dtype != torch.float32:
-        wtype = 0
-    mean, rstd = _vector(mean, "layer_norm: mean", rows, x, (torch.float32,)), _vector(rstd, "layer_norm: rstd", rows, x, (torch.float32,))
-    ptype = torch.float32 if weight is None else weight.dtype
-    with _device_scope(x):
-        dx = torch.empty_like(x, memory_format=torch.contiguous_format)
-        dw = db = scratch = None
-        if need_params:
-            dw, db = torch.empty(2, n, dtype=ptype, device=x.device).unbind(0)
-            if rows == 0:
-                dw.zero_(), db.zero_()
-            else:
-                scratch = torch.empty(lib.fneus_layer_norm_bwd_scratch_floats(rows, n), dtype=torch.float32, device=x.device)
-        if rows:
-            _launch("fneus_layer_norm_bwd", lib.fneus_layer_norm_bwd, _ptr(dy), _ld(dy), _ptr(x), _ld(x), _ptr(weight), _ptr(mean), _ptr(rstd),
-                    _ptr(dx), n, _ptr(dw), _ptr(db), _ptr(scratch), rows, n, _DTYPES[x.dtype], wtype, _stream())
+    mean, rstd = _vector(mean, "layer_norm: mean", rows, x, _FLOAT), _vector(rstd, "layer_norm: rstd", rows, x, _FLOAT)
+    dx = x.new_empty((rows, n))
+    dw = db = scratch = None
+    if need_params:
+        ptype = torch.float32 if weight is None else weight.dtype
+        dw, db = x.new_empty((n,), dtype=ptype), x.new_empty((n,), dtype=ptype)
+        if rows == 0:
+            dw.zero_(), db.zero_()
+        else:
+            scratch = x.new_empty((lib.fneus_layer_norm_bwd_scratch_floats(rows, n),), dtype=torch.float32)
+    if rows:
+        _launch("fneus_layer_norm_bwd", lib.fneus_layer_norm_bwd, dy.data_ptr(), _ld(dy), x.data_ptr(), _ld(x), _at(weight), mean.data_ptr(),
+                rstd.data_ptr(), dx.data_ptr(), n, _at(dw), _at(db), _at(scratch), rows, n, _DTYPES[x.dtype], wtype, _raw_stream(device))
     return dx, dw, db
 
 
@@ -1327,11 +1334,11 @@ def _linear_weight(weight, x):
     return weight if weight.is_contiguous() else weight.contiguous()
 
 
-def _linear_scratch(job, backward: int, device):
-    n = lib.fneus_linear_scratch_bytes(C.byref(job), backward)
+def _linear_scratch(job, backward: int, x):
+    n = lib.fneus_linear_scratch_bytes(job, backward)
     if n <= 0:
         return None
-    t = torch.empty(n, dtype=torch.uint8, device=device)
+    t = x.new_empty((n,), dtype=torch.uint8)
     job.scratch, job.scratch_bytes = t.data_ptr(), n
     return t
 
@@ -1342,26 +1349,25 @@ def linear_fwd(x, weight, bias=None, act="none", residual=None, train: bool = Fa
     linear_bwd takes, else None."""
     code = _act_code(act)
     x = _rows(x, "linear: x")
+    device = x.device.index
+    if device != _current_device():
+        with torch.cuda.device(device):
+            return linear_fwd(x, weight, bias, act, residual, train)
     weight = _linear_weight(weight, x)
     rows, (n_out, n_in) = x.shape[0], weight.shape
     if x.shape[1] != n_in:
         raise ValueError(f"linear: x has {x.shape[1]} columns, weight takes {n_in}")
     bias = _vector(bias, "linear: bias", n_out, x, (x.dtype,))
-    with _device_scope(x):
-        y = torch.empty(rows, n_out, dtype=x.dtype, device=x.device)
-        z = torch.empty_like(y) if train and code != ACT_NONE else None
-        job = _lib.FneusLinear(x=x.data_ptr(), weight=weight.data_ptr(), y=y.data_ptr(), rows=rows, ldx=_ld(x), n_in=n_in, n_out=n_out,
-                               act=code, dtype=_DTYPES[x.dtype])
-        if bias is not None:
-            job.bias = bias.data_ptr()
-        if residual is not None:
-            residual = _rows(residual, "linear: residual", x, (rows, n_out))
-            job.residual, job.ld_residual = residual.data_ptr(), _ld(residual)
-        if z is not None:
-            job.z = z.data_ptr()
-        if rows:
-            scratch = _linear_scratch(job, 0, x.device)      # noqa: F841  (kept until the launch is enqueued)
-            _launch("fneus_linear_fwd", lib.fneus_linear_fwd, C.byref(job), _stream())
+    if residual is not None:
+        residual = _rows(residual, "linear: residual", x, (rows, n_out))
+    y = x.new_empty((rows, n_out))
+    z = x.new_empty((rows, n_out)) if train and code != ACT_NONE else None
+    if rows:
+        # x weight bias residual y z | dy dx dweight dbias | scratch scratch_bytes | rows ldx ld_residual lddy | n_in n_out act dtype
+        job = _lib.FneusLinear(x.data_ptr(), weight.data_ptr(), _at(bias), _at(residual), y.data_ptr(), _at(z), None, None, None, None, None, 0,
+                               rows, _ld(x), n_out if residual is None else _ld(residual), n_out, n_in, n_out, code, _DTYPES[x.dtype])
+        scratch = _linear_scratch(job, 0, x)      # noqa: F841  (kept until the launch is enqueued)
+        _launch("fneus_linear_fwd", lib.fneus_linear_fwd, job, _raw_stream(device))
     return y, z
 
 
@@ -1370,6 +1376,10 @@ def linear_bwd(dy, x, weight, z=None, act="none", need=(True, True, True)):
     dbias [n_out] comes in the one type of the other arrays."""
     code = _act_code(act)
     x = _rows(x, "linear: x")
+    device = x.device.index
+    if device != _current_device():
+        with torch.cuda.device(device):
+            return linear_bwd(dy, x, weight, z, act, need)
     weight = _linear_weight(weight, x)
     rows, (n_out, n_in) = x.shape[0], weight.shape
     if x.shape[1] != n_in:
@@ -1379,27 +1389,20 @@ def linear_bwd(dy, x, weight, z=None, act="none", need=(True, True, True)):
         if z is None:
             raise ValueError("linear_bwd: an activation needs the z of linear_fwd(..., train=True)")
         z = _rows(z, "linear: z", x, (rows, n_out)).contiguous()
-    with _device_scope(x):
-        dx = torch.empty(rows, n_in, dtype=x.dtype, device=x.device) if need[0] else None
-        dw = torch.empty(n_out, n_in, dtype=x.dtype, device=x.device) if need[1] else None
-        db = torch.empty(n_out, dtype=x.dtype, device=x.device) if need[2] else None
-        if rows == 0:
-            for t in (dw, db):
-                if t is not None:
-                    t.zero_()
-        elif any(need):
-            job = _lib.FneusLinear(x=x.data_ptr(), weight=weight.data_ptr(), dy=dy.data_ptr(), rows=rows, ldx=_ld(x), lddy=_ld(dy), n_in=n_in,
-                                   n_out=n_out, act=code, dtype=_DTYPES[x.dtype])
-            if code != ACT_NONE:
-                job.z = z.data_ptr()
-            if dx is not None:
-                job.dx = dx.data_ptr()
-            if dw is not None:
-                job.dweight = dw.data_ptr()
-            if db is not None:
-                job.dbias = db.data_ptr()
-            scratch = _linear_scratch(job, 1, x.device)      # noqa: F841
-            _launch("fneus_linear_bwd", lib.fneus_linear_bwd, C.byref(job), _stream())
+    else:
+        z = None
+    dx = x.new_empty((rows, n_in)) if need[0] else None
+    dw = x.new_empty((n_out, n_in)) if need[1] else None
+    db = x.new_empty((n_out,)) if need[2] else None
+    if rows == 0:
+        for t in (dw, db):
+            if t is not None:
+                t.zero_()
+    elif any(need):
+        job = _lib.FneusLinear(x.data_ptr(), weight.data_ptr(), None, None, None, _at(z), dy.data_ptr(), _at(dx), _at(dw), _at(db), None, 0, rows,
+                               _ld(x), n_out, _ld(dy), n_in, n_out, code, _DTYPES[x.dtype])
+        scratch = _linear_scratch(job, 1, x)      # noqa: F841
+        _launch("fneus_linear_bwd", lib.fneus_linear_bwd, job, _raw_stream(device))
     return dx, dw, db
 
 
@@ -1460,12 +1463,15 @@ def muon_launch(table, lr, momentum, nesterov, weight_decay, coefficients, steps
     jobs, n, like = table
     if n == 0:
         return
+    device = like.device.index
+    if device != _current_device():
+        with torch.cuda.device(device):
+            return muon_launch(table, lr, momentum, nesterov, weight_decay, coefficients, steps, eps, prec, zero_grad)
     prec = _muon_prec(prec, like.dtype)
     a, b, c = coefficients
-    with _device_scope(like):
-        scratch = torch.empty(lib.fneus_muon_scratch_bytes(jobs, n, prec), dtype=torch.uint8, device=like.device)
-        _launch("fneus_muon", lib.fneus_muon, jobs, n, _ptr(lr), momentum, int(nesterov), weight_decay, a, b, c, steps, eps, prec,
-                _DTYPES[like.dtype], int(zero_grad), _ptr(scratch), scratch.numel(), _stream())
+    scratch = like.new_empty((lib.fneus_muon_scratch_bytes(jobs, n, prec),), dtype=torch.uint8)
+    _launch("fneus_muon", lib.fneus_muon, jobs, n, lr.data_ptr(), momentum, int(nesterov), weight_decay, a, b, c, steps, eps, prec,
+            _DTYPES[like.dtype], int(zero_grad), scratch.data_ptr(), scratch.numel(), _raw_stream(device))
 
 
 def muon_step(params, grads, momenta, lr, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0, adjust="match_rms",
@@ -1489,22 +1495,25 @@ def newton_schulz(g, coefficients=NS_COEFFICIENTS, steps: int = 5, eps: float = 
     `steps` times X <- a X + (b A + c A^2) X, A = X X^T (for rows > cols on the transpose).  -> a tensor of g's shape and type"""
     if g.dim() not in (2, 3) or not g.is_cuda or g.dtype not in _DTYPES:
         raise ValueError("newton_schulz: a CUDA matrix, or a stack of them, of float32, bfloat16 or float16")
+    device = g.device.index
+    if device != _current_device():
+        with torch.cuda.device(device):
+            return newton_schulz(g, coefficients, steps, eps, prec)
     prec = _muon_prec(prec, g.dtype)
     g = g if g.is_contiguous() else g.contiguous()
-    with _device_scope(g):
-        out = torch.empty_like(g)
-        if g.numel() == 0:
-            return out
-        rows, cols = g.shape[-2:]
-        n, step = g.numel() // (rows * cols), rows * cols * g.element_size()
-        jobs = (_lib.FneusMuonJob * n)()
-        src, dst = g.data_ptr(), out.data_ptr()
-        for k, j in enumerate(jobs):
-            j.grad, j.out, j.rows, j.cols = src + k * step, dst + k * step, rows, cols
-        scratch = torch.empty(lib.fneus_muon_scratch_bytes(jobs, n, prec), dtype=torch.uint8, device=g.device)
-        a, b, c = coefficients
-        _launch("fneus_newton_schulz", lib.fneus_newton_schulz, jobs, n, a, b, c, steps, eps, prec, _DTYPES[g.dtype], _ptr(scratch),
-                scratch.numel(), _stream())
+    out = torch.empty_like(g)
+    if g.numel() == 0:
+        return out
+    rows, cols = g.shape[-2:]
+    n, step = g.numel() // (rows * cols), rows * cols * g.element_size()
+    jobs = (_lib.FneusMuonJob * n)()
+    src, dst = g.data_ptr(), out.data_ptr()
+    for k, j in enumerate(jobs):
+        j.grad, j.out, j.rows, j.cols = src + k * step, dst + k * step, rows, cols
+    scratch = g.new_empty((lib.fneus_muon_scratch_bytes(jobs, n, prec),), dtype=torch.uint8)
+    a, b, c = coefficients
+    _launch("fneus_newton_schulz", lib.fneus_newton_schulz, jobs, n, a, b, c, steps, eps, prec, _DTYPES[g.dtype], scratch.data_ptr(),
+            scratch.numel(), _raw_stream(device))
     return out
 
 
