@@ -38,6 +38,16 @@ FN_DEV float lin_act(float z, int act) {
     }
 }
 
+// the same by CLASS of codes, for a kernel that holds one class's instructions only: 0 the piecewise linear ones (none, ReLU, leaky: `slope`
+// of the negative side), 3 sigmoid and SiLU (`times`: times z), 4 softplus, 5 GELU
+__host__ __device__ constexpr int lin_class(int act) { return act <= 2 ? 0 : (act == 6 ? 3 : act); }
+template <int CLASS>
+FN_DEV float lin_act_of(float z, float slope, bool times) {
+    if constexpr (CLASS == 0) return z > 0.0f || z != z ? z : (slope == 0.0f ? 0.0f : slope * z);
+    else if constexpr (CLASS == 3) { const float s = lin_sigmoid(z); return times ? z * s : s; }
+    else return lin_act(z, CLASS);
+}
+
 // act'(z); at 0 the ReLUs take the slope of the negative side
 FN_DEV float lin_dact(float z, int act) {
     switch (act) {

@@ -241,9 +241,8 @@ FN_DEV void lin_finish(const T* bias, const T* res, T* d, T* z, int act, int val
     quad_store(d, valid, v);
 }
 
-// The epilogue goes through LDS, 32 rows of a wave at a time: the accumulators hold a column of 32 rows in a register, memory wants rows;
-// and the loop that finishes four outputs exists once, not once per register.
-template <class Cfg, class T, bool AKM, bool BKM, int EPI>
+// CLASS: the activation's (LIN_EPI_FWD)
+template <class Cfg, class T, bool AKM, bool BKM, int EPI, int CLASS>
 __global__ void __launch_bounds__(Cfg::THREADS, 2) linear_tiled_kernel(LinTiled P) {
     extern __shared__ __attribute__((aligned(16))) unsigned char mm_smem[];
     const long tiles = (long)P.tiles_i * P.tiles_j;
@@ -255,42 +254,43 @@ __global__ void __launch_bounds__(Cfg::THREADS, 2) linear_tiled_kernel(LinTiled 
     const int it0 = (int)((long)P.k_tiles * split / P.splits), it1 = (int)((long)P.k_tiles * (split + 1) / P.splits);
     f32x16 acc[Cfg::MI][Cfg::NJ];
     mm_run<Cfg, T, AKM, BKM, false, true>(mm_smem, P.a, P.b, i0, P.ni, j0, P.nj, P.k_tiles, P.tail, kMmOne, it0, it1, split == P.splits - 1, 1.0f, acc);
-    constexpr int STRIDE = Cfg::WN + 4;
-    static_assert(Cfg::WAVES * 32 * STRIDE * 4 <= Cfg::LDS, "the epilogue's rows fit the ring");
-    float* rows = reinterpret_cast<float*>(mm_smem) + mm_wave() * 32 * STRIDE;
-    const int lane = threadIdx.x & 63;
-    __syncthreads();                                  // (everyone has read the last stage)
-#pragma unroll
-    for (int m = 0; m < Cfg::MI; ++m) {
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int n = 0; n < Cfg::NJ; ++n)
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                f32x4 q;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) q[k] = acc[m][n][4 * g + k];
-                *reinterpret_cast<f32x4*>(rows + (lane & 31) * STRIDE + 32 * n + 8 * g + 4 * (lane >> 5)) = q;
-            }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        constexpr int QUADS = Cfg::WN / 4;
-#pragma unroll 2
-        for (int s = 0; s < 32 * QUADS / 64; ++s) {
-            const int at = s * 64 + lane, r = at / QUADS, c = 4 * (at % QUADS);
-            const long i = i0 + mm_wave_i<Cfg>() + 32 * m + r;
-            const long j = j0 + mm_wave_j<Cfg>() + c;
-            if (i >= P.ni || j >= P.nj) continue;
-            const int valid = (int)(P.nj - j);
-            const f32x4 q = *reinterpret_cast<const f32x4*>(rows + r * STRIDE + c);
-            float v[4] = {q[0], q[1], q[2], q[3]};
-            if constexpr (EPI == LIN_EPI_FWD)
-                lin_finish<T>(P.bias ? (const T*)P.bias + j : nullptr, P.res ? (const T*)P.res + i * P.ldres + j : nullptr, (T*)P.d + i * P.ldd + j,
-                              P.z ? (T*)P.z + i * P.ldd + j : nullptr, P.act, valid, v);
-            else if constexpr (EPI == LIN_EPI_STORE) quad_store<T>((T*)P.d + i * P.ldd + j, valid, v);
-            else quad_store<float>(P.partial + ((long)split * P.ni + i) * P.nj + j, valid, v);
+    if constexpr (EPI == LIN_EPI_FWD) {
+        constexpr int SLOTS = Cfg::WN / 8;
+        float bias[4] = {0.0f, 0.0f, 0.0f, 0.0f}, res[SLOTS][4];
+        {
+            const long j = j0 + mm_wave_j<Cfg>() + 4 * ((threadIdx.x & 63) % (Cfg::WN / 4));
+            if (P.bias && j < P.nj) quad_load((const T*)P.bias + j, (int)(P.nj - j), bias);
         }
+        const float slope = P.act == 0 ? 1.0f : (P.act == 2 ? 0.2f : 0.0f);
+        const bool times = P.act == 6;
+        mm_epilogue<Cfg>(mm_smem, i0, j0, 1.0f, acc,
+            [&](long i, long j, int s) {
+                if (P.res && i < P.ni && j < P.nj) quad_load((const T*)P.res + i * P.ldres + j, (int)(P.nj - j), res[s]);
+            },
+            [&](long i, long j, int s, float (&v)[4], float*) {
+                if (i >= P.ni || j >= P.nj) return;
+                const int valid = (int)(P.nj - j);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] += bias[k];
+                if (P.z) quad_store((T*)P.z + i * P.ldd + j, valid, v);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = lin_act_of<CLASS>(v[k], slope, times);
+                if (P.res) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) v[k] += res[s][k];
+                }
+                quad_store((T*)P.d + i * P.ldd + j, valid, v);
+            },
+            [](long, long, float*) {});
+    } else {
+        mm_epilogue<Cfg>(mm_smem, i0, j0, 1.0f, acc, [](long, long, int) {},
+            [&](long i, long j, int, float (&v)[4], float*) {
+                if (i >= P.ni || j >= P.nj) return;
+                const int valid = (int)(P.nj - j);
+                if constexpr (EPI == LIN_EPI_STORE) quad_store<T>((T*)P.d + i * P.ldd + j, valid, v);
+                else quad_store<float>(P.partial + ((long)split * P.ni + i) * P.nj + j, valid, v);
+            },
+            [](long, long, float*) {});
     }
 }
 
@@ -486,11 +486,25 @@ static MmOperand lin_operand(const void* p, long ld, int e) {
     return o;
 }
 
-template <class Cfg, class T, bool AKM, bool BKM, int EPI>
+template <class Cfg, class T, bool AKM, bool BKM, int EPI, int CLASS>
 static void lin_tiled_launch(const LinTiled& t, hipStream_t stream) {
-    auto kernel = linear_tiled_kernel<Cfg, T, AKM, BKM, EPI>;
+    auto kernel = linear_tiled_kernel<Cfg, T, AKM, BKM, EPI, CLASS>;
     allow_big_lds(kernel);
     hipLaunchKernelGGL(kernel, dim3((unsigned)((long)t.tiles_i * t.tiles_j * t.splits)), dim3(Cfg::THREADS), Cfg::LDS, stream, t);
+}
+
+template <class Cfg, class T, bool AKM, bool BKM, bool FWD>
+static void lin_tiled_whole(const LinTiled& t, hipStream_t stream) {
+    if constexpr (!FWD) {
+        lin_tiled_launch<Cfg, T, AKM, BKM, LIN_EPI_STORE, 0>(t, stream);
+    } else {
+        switch (lin_class(t.act)) {
+            case 0: lin_tiled_launch<Cfg, T, AKM, BKM, LIN_EPI_FWD, 0>(t, stream); break;
+            case 3: lin_tiled_launch<Cfg, T, AKM, BKM, LIN_EPI_FWD, 3>(t, stream); break;
+            case 4: lin_tiled_launch<Cfg, T, AKM, BKM, LIN_EPI_FWD, 4>(t, stream); break;
+            default: lin_tiled_launch<Cfg, T, AKM, BKM, LIN_EPI_FWD, 5>(t, stream); break;
+        }
+    }
 }
 
 template <class T, bool AKM, bool BKM, bool FWD>
@@ -500,17 +514,17 @@ static void lin_tiled_product(LinTiled t, const LinShape& s, long nk, float* par
     t.k_tiles = (int)(nk / KV), t.tail = (int)(nk % KV), t.splits = s.splits, t.partial = partial;
     t.tiles_i = (int)((t.ni + b - 1) / b), t.tiles_j = (t.nj + b - 1) / b;
     if (s.splits > 1) {
-        if (s.tile == 64) lin_tiled_launch<LinSmall, T, AKM, BKM, LIN_EPI_PART>(t, stream);
-        else lin_tiled_launch<LinMid, T, AKM, BKM, LIN_EPI_PART>(t, stream);
+        if (s.tile == 64) lin_tiled_launch<LinSmall, T, AKM, BKM, LIN_EPI_PART, 0>(t, stream);
+        else lin_tiled_launch<LinMid, T, AKM, BKM, LIN_EPI_PART, 0>(t, stream);
         const long quads = t.ni * ((t.nj + 3) / 4);
         if (s.splits >= 16) hipLaunchKernelGGL((linear_reduce_kernel<T, FWD, 8>), dim3((unsigned)((quads + 31) / 32)), dim3(256), 0, stream, t);
         else hipLaunchKernelGGL((linear_reduce_kernel<T, FWD, 1>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, stream, t);
     } else if (s.tile == 64) {
-        lin_tiled_launch<LinSmall, T, AKM, BKM, FWD ? LIN_EPI_FWD : LIN_EPI_STORE>(t, stream);
+        lin_tiled_whole<LinSmall, T, AKM, BKM, FWD>(t, stream);
     } else if (s.tile == 256) {
-        lin_tiled_launch<LinBig, T, AKM, BKM, FWD ? LIN_EPI_FWD : LIN_EPI_STORE>(t, stream);
+        lin_tiled_whole<LinBig, T, AKM, BKM, FWD>(t, stream);
     } else {
-        lin_tiled_launch<LinMid, T, AKM, BKM, FWD ? LIN_EPI_FWD : LIN_EPI_STORE>(t, stream);
+        lin_tiled_whole<LinMid, T, AKM, BKM, FWD>(t, stream);
     }
 }
 

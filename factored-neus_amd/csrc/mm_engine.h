@@ -260,6 +260,48 @@ FN_DEV void mm_run(unsigned char* smem, const MmOperand& A, const MmOperand& B, 
     }
 }
 
+// The epilogue: the accumulators hold a column of 32 rows in a register, memory wants rows, so a wave's 32 rows at a time go through its
+// part of LDS.  `load(i, j, slot)` fetches what the four outputs (i, j .. j + 3) need from memory -- all of a block's loads are in flight before
+// the first is used -- and `finish(i, j, slot, v, cell)` ends them; slot numbers the quads of a block, j is the same in all of a lane's.
+// `turn(ib, jb, rows)` runs once a block behind that.
+template <class Cfg, class Load, class Finish, class Turn>
+FN_DEV void mm_epilogue(unsigned char* smem, long i0, long j0, float scale, f32x16 (&acc)[Cfg::MI][Cfg::NJ], Load load, Finish finish, Turn turn) {
+    constexpr int STRIDE = Cfg::WN + 4, QUADS = Cfg::WN / 4, SLOTS = 32 * QUADS / 64;
+    static_assert(Cfg::WAVES * 32 * STRIDE * 4 <= Cfg::LDS, "the epilogue's rows fit the ring");
+    float* rows = reinterpret_cast<float*>(smem) + mm_wave() * 32 * STRIDE;
+    const int lane = threadIdx.x & 63, c = 4 * (lane % QUADS);
+    const long jb = j0 + mm_wave_j<Cfg>();
+    __syncthreads();                                  // (everyone has read the last stage)
+#pragma unroll
+    for (int m = 0; m < Cfg::MI; ++m) {
+        const long ib = i0 + mm_wave_i<Cfg>() + 32 * m;
+#pragma unroll
+        for (int s = 0; s < SLOTS; ++s) load(ib + (s * 64 + lane) / QUADS, jb + c, s);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int n = 0; n < Cfg::NJ; ++n)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                f32x4 q;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) q[k] = acc[m][n][4 * g + k] * scale;
+                *reinterpret_cast<f32x4*>(rows + (lane & 31) * STRIDE + 32 * n + 8 * g + 4 * (lane >> 5)) = q;
+            }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int s = 0; s < SLOTS; ++s) {
+            const int r = (s * 64 + lane) / QUADS;
+            float* cell = rows + r * STRIDE + c;
+            const f32x4 q = *reinterpret_cast<const f32x4*>(cell);
+            float v[4] = {q[0], q[1], q[2], q[3]};
+            finish(ib + r, jb + c, s, v, cell);
+        }
+        turn(ib, jb, rows);
+    }
+}
+
 // Launch index -> work item: the workgroups of one XCD (launch index mod 8) take one contiguous stretch of the items, so that what
 // neighbours share stays in that XCD's L2.
 FN_DEV long mm_spread(long wg, long total) {

@@ -24,14 +24,17 @@ struct MuonJob {
     void *grad, *momentum, *param, *out;
     int rows, cols;
     float adjust;
-    int first;                               // first tile of this launch
+    int pad_;
     long off;                                // its scratch
 };
 
+// `first`: the launch's first workgroup of each job (beyond the last: none).  The arguments lie in host memory, a line of them is a
+// microsecond away: the search reads the two lines of `first` at once, then one job.
 struct MuonJobs {
-    MuonJob j[kMuonMaxJobs];
-    int n;
+    int first[kMuonMaxJobs];
     unsigned char* scratch;
+    long n;
+    MuonJob j[kMuonMaxJobs];
 };
 
 struct MuonNum {
@@ -71,7 +74,8 @@ __host__ __device__ inline MuonLay muon_lay(int rows, int cols, int planes) {
 
 FN_DEV int muon_find(const MuonJobs& js, int wg) {
     int q = 0;
-    while (q + 1 < js.n && js.j[q + 1].first <= wg) ++q;
+#pragma unroll
+    for (int k = 1; k < kMuonMaxJobs; ++k) q += js.first[k] <= wg ? 1 : 0;
     return q;
 }
 
@@ -124,7 +128,8 @@ template <class T, bool MOM, int NP>
 __global__ void __launch_bounds__(256) muon_init_kernel(MuonJobs js, MuonNum P) {
     __shared__ float tile[64][65];
     __shared__ double red[4];
-    const MuonJob& J = js.j[muon_find(js, blockIdx.x)];
+    const int q = muon_find(js, blockIdx.x);
+    const MuonJob& J = js.j[q];
     const MuonLay L = muon_lay(J.rows, J.cols, NP);
     unsigned char* S = js.scratch + J.off;
     double s = reinterpret_cast<const double*>(S)[threadIdx.x];       // kMuonChunks == 256 partials
@@ -132,7 +137,7 @@ __global__ void __launch_bounds__(256) muon_init_kernel(MuonJobs js, MuonNum P) 
     for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d, 64);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
     const int tiles_c = (J.cols + 63) / 64;
-    const int t = blockIdx.x - J.first, r0 = 64 * (t / tiles_c), c0 = 64 * (t % tiles_c);
+    const int t = blockIdx.x - js.first[q], r0 = 64 * (t / tiles_c), c0 = 64 * (t % tiles_c);
     const int lc = threadIdx.x & 63, lr = threadIdx.x >> 6;
 #pragma unroll 4
     for (int r = lr; r < 64; r += 4) {
@@ -172,18 +177,6 @@ FN_DEV MmOperand muon_op(const unsigned char* base, long plane, long row_bytes) 
     return o;
 }
 
-// four consecutive values of a plane pair as fp32 (times 2^e of the plane)
-template <int NP>
-FN_DEV void muon_read4(const unsigned char* p, long plane, float (&v)[4]) {
-    const f16x4 hi = *reinterpret_cast<const f16x4*>(p);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = (float)hi[k];
-    if constexpr (NP == 2) {
-        const f16x4 lo = *reinterpret_cast<const f16x4*>(p + plane);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] += (float)lo[k] * (1.0f / kLoScale);
-    }
-}
 template <int NP>
 FN_DEV void muon_write4(unsigned char* p, long plane, const float (&v)[4], f16x4& hi, f16x4& lo) {
 #pragma unroll
@@ -212,7 +205,8 @@ FN_DEV void muon_upper(int t, int& ti, int& tj) {
 template <class Cfg, int NP, int KIND, class T, bool MOM>
 __global__ void __launch_bounds__(Cfg::THREADS, 2) muon_product_kernel(MuonJobs js, MuonNum P, int cur) {
     extern __shared__ __attribute__((aligned(16))) unsigned char mm_smem[];
-    const MuonJob& J = js.j[muon_find(js, blockIdx.x)];
+    const int q = muon_find(js, blockIdx.x);
+    const MuonJob& J = js.j[q];
     const MuonLay L = muon_lay(J.rows, J.cols, NP);
     unsigned char* S = js.scratch + J.off;
     constexpr bool SYM = KIND <= MU_POLY;
@@ -220,7 +214,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, 2) muon_product_kernel(MuonJobs 
     const int tiles_i = (ni + Cfg::BM - 1) / Cfg::BM, tiles_j = (nj + Cfg::BN - 1) / Cfg::BN;
     const long tiles = SYM ? (long)tiles_i * (tiles_i + 1) / 2 : (long)tiles_i * tiles_j;
     int ti, tj;
-    const long t = mm_spread(blockIdx.x - J.first, tiles);
+    const long t = mm_spread(blockIdx.x - js.first[q], tiles);
     if constexpr (SYM) muon_upper((int)t, ti, tj);
     else mm_tile(t, tiles_i, tiles_j, ti, tj);
     const long i0 = (long)ti * Cfg::BM, j0 = (long)tj * Cfg::BN;
@@ -243,100 +237,79 @@ __global__ void __launch_bounds__(Cfg::THREADS, 2) muon_product_kernel(MuonJobs 
     const float lr = KIND == MU_LAST && MOM ? *P.lr : 0.0f;
     const float keep = 1.0f - lr * P.wd, step = lr * J.adjust;
     const bool turn = SYM ? ti != tj : (KIND == MU_LAST && L.trans);          // the second orientation is written too (SYM) or alone
-    constexpr int STRIDE = Cfg::WN + 4;
-    static_assert(Cfg::WAVES * 32 * STRIDE * 4 <= Cfg::LDS, "the epilogue's rows fit the ring");
-    float* rows = reinterpret_cast<float*>(mm_smem) + mm_wave() * 32 * STRIDE;
-    const int lane = threadIdx.x & 63;
-    __syncthreads();                                  // (everyone has read the last stage)
-#pragma unroll
-    for (int m = 0; m < Cfg::MI; ++m) {
-        const long ib = i0 + mm_wave_i<Cfg>() + 32 * m, jb = j0 + mm_wave_j<Cfg>();
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int n = 0; n < Cfg::NJ; ++n)
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                f32x4 q;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) q[k] = acc[m][n][4 * g + k] * f;
-                *reinterpret_cast<f32x4*>(rows + (lane & 31) * STRIDE + 32 * n + 8 * g + 4 * (lane >> 5)) = q;
+    constexpr int STRIDE = Cfg::WN + 4, SLOTS = Cfg::WN / 8;
+    // what the quads of a block add: b A (POLY), a X (STEP, LAST), and the parameters they end in
+    f16x4 old_hi[SLOTS], old_lo[SLOTS];
+    float par[SLOTS][4];
+    const unsigned char* old = S + (KIND == MU_POLY ? L.a : L.x[cur]);
+    const long ld_old = KIND == MU_POLY ? L.lda : L.ldx, pl_old = KIND == MU_POLY ? L.pa : L.px, width = ld_old / 2;
+    mm_epilogue<Cfg>(mm_smem, i0, j0, f, acc,
+        [&](long i, long j, int s) {
+            if constexpr (KIND != MU_GRAM) {
+                old_hi[s] = old_lo[s] = f16x4{0, 0, 0, 0};
+                if (i < ni && j < width) {
+                    old_hi[s] = *reinterpret_cast<const f16x4*>(old + i * ld_old + j * 2);
+                    if constexpr (NP == 2) old_lo[s] = *reinterpret_cast<const f16x4*>(old + pl_old + i * ld_old + j * 2);
+                }
             }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        constexpr int QUADS = Cfg::WN / 4;
-#pragma unroll 2
-        for (int s = 0; s < 32 * QUADS / 64; ++s) {
-            const int at = s * 64 + lane, r = at / QUADS, c = 4 * (at % QUADS);
-            const long i = ib + r, j = jb + c;
-            float* cell = rows + r * STRIDE + c;
-            const f32x4 q = *reinterpret_cast<const f32x4*>(cell);
-            float v[4] = {q[0], q[1], q[2], q[3]};
+            if constexpr (KIND == MU_LAST && MOM)
+                if (!L.trans && i < ni && j < nj) quad_load((const T*)J.param + i * (long)J.cols + j, (int)(nj - j), par[s]);
+        },
+        [&](long i, long j, int s, float (&v)[4], float* cell) {
             f16x4 hi, lo4;
-            if constexpr (SYM) {
-                if (i >= ni || j >= L.mp) continue;
-                if constexpr (KIND == MU_POLY) {
-                    float a[4];
-                    muon_read4<NP>(S + L.a + i * L.lda + j * 2, L.pa, a);
+            if constexpr (KIND != MU_GRAM) {
+                const float w = KIND == MU_POLY ? fb : fa;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) v[k] += fb * a[k];
-                }
-#pragma unroll
-                for (int k = 0; k < 4; ++k) v[k] = j + k < nj ? v[k] : 0.0f;
-                muon_write4<NP>(S + (KIND == MU_GRAM ? L.a : L.b) + i * L.lda + j * 2, L.pa, v, hi, lo4);
-            } else {
-                if (j >= (long)L.ldx / 2 || i >= L.mp) continue;
-                float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                if (i < ni) muon_read4<NP>(S + L.x[cur] + i * L.ldx + j * 2, L.px, x);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) v[k] = i < ni && j + k < nj ? v[k] + fa * x[k] : 0.0f;
-                if constexpr (KIND == MU_STEP) {
-                    muon_write4<NP>(S + L.x[cur ^ 1] + i * L.ldx + j * 2, L.px, v, hi, lo4);
-                } else if (!L.trans && i < ni) {
-                    T* p = (T*)(MOM ? J.param : J.out) + i * (long)J.cols + j;
-                    const int valid = (int)(nj - j);
-                    if constexpr (MOM) {
-                        float w[4];
-                        quad_load(p, valid, w);
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) v[k] = w[k] * keep - step * v[k];
-                    }
-                    quad_store(p, valid, v);
-                }
+                for (int k = 0; k < 4; ++k) v[k] += w * ((float)old_hi[s][k] + (NP == 2 ? (float)old_lo[s][k] * (1.0f / kLoScale) : 0.0f));
             }
-            if (turn && (KIND == MU_POLY || KIND == MU_LAST)) *reinterpret_cast<f32x4*>(cell) = f32x4{v[0], v[1], v[2], v[3]};
-        }
-        if constexpr (KIND == MU_STEP) continue;
-        if (!turn) continue;
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll 2
-        for (int s = 0; s < Cfg::WN * 8 / 64; ++s) {
-            const int at = s * 64 + lane, c = at / 8, r = 4 * (at % 8);
-            const long i = ib + r, j = jb + c;
-            if (j >= nj || i >= ni) continue;
-            float v[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) v[k] = rows[(r + k) * STRIDE + c];
+            for (int k = 0; k < 4; ++k) v[k] = i < ni && j + k < nj ? v[k] : 0.0f;
+            if (turn) *reinterpret_cast<f32x4*>(cell) = f32x4{v[0], v[1], v[2], v[3]};
             if constexpr (SYM) {
-                // (i + k >= ni: the padding of row j, zero as the tile on the other side of the diagonal leaves it)
-                f16x4 hi, lo4;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) v[k] = i + k < ni ? v[k] : 0.0f;
-                muon_write4<NP>(S + (KIND == MU_GRAM ? L.a : L.b) + j * L.lda + i * 2, L.pa, v, hi, lo4);
-            } else {
-                T* p = (T*)(MOM ? J.param : J.out) + j * (long)J.cols + i;
-                const int valid = (int)(ni - i);
+                if (i < ni && j < L.mp) muon_write4<NP>(S + (KIND == MU_GRAM ? L.a : L.b) + i * L.lda + j * 2, L.pa, v, hi, lo4);
+            } else if constexpr (KIND == MU_STEP) {
+                if (i < L.mp && j < width) muon_write4<NP>(S + L.x[cur ^ 1] + i * L.ldx + j * 2, L.px, v, hi, lo4);
+            } else if (!L.trans && i < ni && j < nj) {
                 if constexpr (MOM) {
-                    float w[4];
-                    quad_load(p, valid, w);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) v[k] = w[k] * keep - step * v[k];
+                    for (int k = 0; k < 4; ++k) v[k] = par[s][k] * keep - step * v[k];
                 }
-                quad_store(p, valid, v);
+                quad_store((T*)(MOM ? J.param : J.out) + i * (long)J.cols + j, (int)(nj - j), v);
             }
-        }
-    }
+        },
+        [&](long ib, long jb, float* rows) {
+            if constexpr (KIND == MU_STEP) return;
+            if (!turn) return;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            const int lane = threadIdx.x & 63;
+            if constexpr (KIND == MU_LAST && MOM) {
+#pragma unroll
+                for (int s = 0; s < SLOTS; ++s) {
+                    const long j = jb + s * 8 + lane / 8, i = ib + 4 * (lane % 8);
+                    if (j < nj && i < ni) quad_load((const T*)J.param + j * (long)J.cols + i, (int)(ni - i), par[s]);
+                }
+            }
+#pragma unroll
+            for (int s = 0; s < SLOTS; ++s) {
+                const int c = s * 8 + lane / 8, r = 4 * (lane % 8);
+                const long i = ib + r, j = jb + c;
+                if (j >= nj || i >= ni) continue;
+                float v[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = rows[(r + k) * STRIDE + c];
+                if constexpr (SYM) {          // (beyond row ni - 1 the rows hold zeros: the padding of row j)
+                    f16x4 hi, lo4;
+                    muon_write4<NP>(S + (KIND == MU_GRAM ? L.a : L.b) + j * L.lda + i * 2, L.pa, v, hi, lo4);
+                } else {
+                    if constexpr (MOM) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) v[k] = par[s][k] * keep - step * v[k];
+                    }
+                    quad_store((T*)(MOM ? J.param : J.out) + j * (long)J.cols + i, (int)(ni - i), v);
+                }
+            }
+        });
 }
 
 typedef MmCfg<64, 64, 2, 2, 5> MuonSmall;          // 80 KiB: four stages in flight, two workgroups a CU
@@ -352,8 +325,8 @@ template <class Cfg, int NP, int KIND, class T, bool MOM>
 static void muon_product_launch(MuonJobs& js, const MuonNum& P, int cur, hipStream_t stream) {
     long tiles = 0;
     for (int q = 0; q < js.n; ++q) {
-        MuonJob& J = js.j[q];
-        J.first = (int)tiles;
+        const MuonJob& J = js.j[q];
+        js.first[q] = (int)tiles;
         tiles += muon_tiles(J.rows < J.cols ? J.rows : J.cols, J.rows < J.cols ? J.cols : J.rows, KIND <= MU_POLY, Cfg::BM);
     }
     auto kernel = muon_product_kernel<Cfg, NP, KIND, T, MOM>;
@@ -390,14 +363,15 @@ template <class T, bool MOM, int NP>
 static int muon_run(const FneusMuonJob* jobs, int n_jobs, const MuonNum& P, int steps, unsigned char* scratch, hipStream_t stream) {
     for (int first = 0; first < n_jobs; first += kMuonMaxJobs) {
         MuonJobs js;
-        js.n = n_jobs - first < kMuonMaxJobs ? n_jobs - first : kMuonMaxJobs;
+        js.n = n_jobs - first < kMuonMaxJobs ? n_jobs - first : kMuonMaxJobs;       // (a local: filled anew for every round)
         js.scratch = scratch;
+        for (int q = 0; q < kMuonMaxJobs; ++q) js.first[q] = 0x7fffffff;
         long off = 0, tiles = 0;
         for (int q = 0; q < js.n; ++q) {
             const FneusMuonJob& f = jobs[first + q];
             MuonJob& J = js.j[q];
             J.grad = f.grad, J.momentum = f.momentum, J.param = f.param, J.out = f.out;
-            J.rows = f.rows, J.cols = f.cols, J.adjust = f.adjust, J.off = off, J.first = (int)tiles;
+            J.rows = f.rows, J.cols = f.cols, J.adjust = f.adjust, J.off = off, js.first[q] = (int)tiles;
             off += muon_lay(f.rows, f.cols, NP).total;
             tiles += (long)((f.rows + 63) / 64) * ((f.cols + 63) / 64);
         }
