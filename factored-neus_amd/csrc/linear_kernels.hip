@@ -1,7 +1,6 @@
 // Linear layer with bias, activation and residual in its epilogue, forward and backward, fp32 / bf16 / fp16:
 //   z = x W^T + b,  y = act(z) + res;      delta = dy act'(z),  dx = delta W,  dW = delta^T x,  db = column sums of delta
 // The three products are one form, D(i, j) = sum_k A(i, k) B(j, k), with either operand stored along k or along its rows.
-#include <stdlib.h>
 #include <type_traits>
 #include "mm_engine.h"
 #include "fneus_kernels.h"
@@ -333,55 +332,79 @@ __global__ void __launch_bounds__(256) linear_reduce_kernel(LinTiled P) {
     else quad_store<T>((T*)P.d + i * P.ldd + j, valid, v);
 }
 
-// a matrix whose rows the tiled kernel's 16-byte accesses do not fit, copied to rows that do (zeros behind)
+// What a product needs ready, in one launch: matrices whose rows its 16-byte accesses do not fit, copied to rows that do (zeros behind), and
+// delta = dy act'(z) (rounded to T for the products; rows of ldp, zeros behind) with the column sums of delta before that rounding, a
+// partial row of sums for every `sum_parts`-th of the rows.
 template <class T>
-__global__ void __launch_bounds__(256) linear_pad_kernel(const T* __restrict__ x, long ld, long rows, int n, T* __restrict__ out, int ldp) {
+struct LinPad {
+    const T* x;
+    T* out;
+    long ld, rows;
+    int n, ldp, blocks, pad_;
+};
+template <class T>
+struct LinDelta {
+    const T *dy, *z;
+    T* delta;
+    float* sums;
+    long lddy, rows;
+    int n, ldp, act, strips, sum_parts, pad_;
+};
+
+template <class T>
+FN_DEV void lin_pad_block(const LinPad<T>& p, int block) {
     constexpr int V = Chunk<T>::N;
-    const int chunks = ldp / V;
-    for (long at = (long)blockIdx.x * 256 + threadIdx.x; at < rows * chunks; at += (long)gridDim.x * 256) {
+    const int chunks = p.ldp / V;
+    for (long at = (long)block * 256 + threadIdx.x; at < p.rows * chunks; at += (long)p.blocks * 256) {
         const long r = at / chunks;
         const int c = V * (int)(at - r * chunks);
         float v[V];
-        load_chunk<T>(x + r * ld + c, n - c, v);
-        store_chunk<T>(out + r * ldp + c, V, v);
+        load_chunk<T>(p.x + r * p.ld + c, p.n - c, v);
+        store_chunk<T>(p.out + r * p.ldp + c, V, v);
     }
 }
 
-// delta = dy act'(z) (rounded to T for the products; rows of ldp, zeros behind) and the column sums of delta before that rounding: 32
-// chunks of columns a workgroup, 8 rows at a time, a partial row of sums per blockIdx.y
 template <class T>
-__global__ void __launch_bounds__(256) linear_delta_kernel(const T* __restrict__ dy, long lddy, const T* __restrict__ z, int act, long rows, int n,
-                                                           T* __restrict__ delta, int ldp, float* __restrict__ sums) {
+__global__ void __launch_bounds__(256) linear_prepare_kernel(LinDelta<T> d, LinPad<T> px, LinPad<T> pw) {
     constexpr int V = Chunk<T>::N;
     __shared__ float red[8][32 * V];
+    const int first = d.strips * d.sum_parts;
+    if ((int)blockIdx.x >= first) {
+        const int at = (int)blockIdx.x - first;
+        if (at < px.blocks) lin_pad_block(px, at);
+        else lin_pad_block(pw, at - px.blocks);
+        return;
+    }
+    // 32 chunks of columns, 8 rows at a time
+    const int strip = blockIdx.x % d.strips, part = blockIdx.x / d.strips;
     const int c = threadIdx.x & 31, r = threadIdx.x >> 5;
-    const int col = (blockIdx.x * 32 + c) * V, left = n - col;
-    const long r0 = rows * blockIdx.y / gridDim.y, r1 = rows * (blockIdx.y + 1) / gridDim.y;
+    const int col = (strip * 32 + c) * V, left = d.n - col;
+    const long r0 = d.rows * part / d.sum_parts, r1 = d.rows * (part + 1) / d.sum_parts;
     float s[V];
 #pragma unroll
     for (int k = 0; k < V; ++k) s[k] = 0.0f;
     for (long row = r0 + r; row < r1; row += 8) {
         float v[V], q[V];
-        load_chunk<T>(dy + row * lddy + col, left, v);
-        if (act) {
-            load_chunk<T>(z + row * n + col, left, q);
+        load_chunk<T>(d.dy + row * d.lddy + col, left, v);
+        if (d.act) {
+            load_chunk<T>(d.z + row * d.n + col, left, q);
 #pragma unroll
-            for (int k = 0; k < V; ++k) v[k] *= lin_dact(q[k], act);
+            for (int k = 0; k < V; ++k) v[k] *= lin_dact(q[k], d.act);
         }
 #pragma unroll
         for (int k = 0; k < V; ++k) s[k] += v[k];
-        if (delta && col < ldp) store_chunk<T>(delta + row * ldp + col, V, v);
+        if (d.delta && col < d.ldp) store_chunk<T>(d.delta + row * d.ldp + col, V, v);
     }
-    if (!sums) return;
+    if (!d.sums) return;
 #pragma unroll
     for (int k = 0; k < V; ++k) red[r][c * V + k] = s[k];
     __syncthreads();
     for (int at = threadIdx.x; at < 32 * V; at += 256) {
-        const int j = blockIdx.x * 32 * V + at;
+        const int j = strip * 32 * V + at;
         float v = 0.0f;
 #pragma unroll
         for (int q = 0; q < 8; ++q) v += red[q][at];
-        if (j < n) sums[(long)blockIdx.y * n + j] = v;
+        if (j < d.n) d.sums[(long)part * d.n + j] = v;
     }
 }
 
@@ -396,24 +419,24 @@ typedef MmCfg<64, 64, 2, 2, 4> LinSmall;          // 4 waves, 64 KiB of LDS, thr
 typedef MmCfg<128, 128, 2, 2, 2> LinMid;          // 4 waves, 64 KiB of LDS: two workgroups a CU
 typedef MmCfg<256, 256, 2, 4, 2> LinBig;          // 8 waves, 128 KiB: one
 
-// How a product runs: tile size and the parts of its contraction.
+// How a product runs: tile size and the parts of its contraction.  256-wide tiles where they occupy the chip; below, MEASURED (us a launch
+// by the tile's width, 64 / 128): fp32 512^3 15 / 24, 4096 x 256 x 256 14 / 25, 2000 x 776 -> 1112 58 / 50, 256 x 4096 x 4096 105 / 65, 8192 x
+// 512 x 512 48 / 41; bf16 1024^3 11 / 18, 2000 x 776 -> 1112 21 / 20, 2048^3 33 / 31, 65536 x 256 x 256 38 / 27: a narrow tile where the
+// wide ones are few, but not where the contraction of fp32 (whose terms cost a narrow tile as much as its products) is long.
 struct LinShape { int tile, splits; };            // tile: 64, 128, 256
-static LinShape lin_shape(long ni, long nj, long nk, int kv) {
+template <class T>
+static LinShape lin_shape(long ni, long nj, long nk) {
     const long t256 = ((ni + 255) / 256) * ((nj + 255) / 256), t128 = ((ni + 127) / 128) * ((nj + 127) / 128);
-    const long k_tiles = nk / kv;
-    const long t64 = ((ni + 63) / 64) * ((nj + 63) / 64);
+    const long t64 = ((ni + 63) / 64) * ((nj + 63) / 64), k_tiles = nk / (128 / (long)sizeof(T));
     LinShape s{128, 1};
-    static const int form = getenv("FNEUS_LINEAR_TILE") ? atoi(getenv("FNEUS_LINEAR_TILE")) : 0;
-    static const int split = getenv("FNEUS_LINEAR_SPLIT") ? atoi(getenv("FNEUS_LINEAR_SPLIT")) : 0;
-    if (form) s.tile = form;
-    else if (t256 >= 240) s.tile = 256;
-    else if (t128 < 256) s.tile = 64;
+    if (t256 >= 240 && ni > 64 && nj > 64) s.tile = 256;
+    else if (ni <= 64 || nj <= 64) s.tile = 64;
+    else if (sizeof(T) == 2 ? t128 < 144 : t128 <= 64 && nk <= 1024) s.tile = 64;
     const long t = s.tile == 64 ? t64 : (s.tile == 128 ? t128 : t256);
     if (t < 256 && s.tile != 256) {     // split until two workgroups a CU are there, at least 8 stages each, 2^28 partial sums at most
-        long want = split ? split : (512 + t - 1) / t, most = split ? k_tiles : k_tiles / 8;
-        const long room = (1L << 28) / (ni * nj > 0 ? ni * nj : 1);
+        long want = (512 + t - 1) / t;
+        const long room = (1L << 28) / (ni * nj), most = k_tiles / 8 < room ? k_tiles / 8 : room;
         if (want > most) want = most;
-        if (want > room) want = room;
         if (want > 1) s.splits = (int)want;
     }
     return s;
@@ -436,17 +459,26 @@ static bool lin_aligned(const void* p, long ld, long n, bool k_major) {
     return ((uintptr_t)p & 15) == 0 && ld % V == 0 && (!k_major || n % V == 0);
 }
 
-// Which form: the tiled kernel from kLinTiledWork multiplications on (a direct tile is one launch and needs no scratch; the tiled kernel
-// shares its operands).
-static const long kLinTiledWork = getenv("FNEUS_LINEAR_TILED") ? atol(getenv("FNEUS_LINEAR_TILED")) : (1L << 27);
+// Which form: a direct tile is one launch for a direction and needs no scratch, the tiled kernel shares its operands.  MEASURED (us, forward /
+// backward, direct against tiled): fp32 512^3 9 / 26 against 15 / 35, 2048 x 512 x 512 23 / 88 against 20 / 48, 4096 x 256 x 256 15 / 114 against
+// 14 / 35; bf16 512^3 6 / 19 against 8 / 20, 4096 x 256 x 256 10 / 72 against 7 / 25: up to 2^27 multiplications (forward, fp32: 2^28), and for
+// the weight gradient, which the direct form does not split, up to 1024 rows.  The weight gradient of a few rows is its output: a direct
+// tile's eight waves have nothing to split (16 x 8192 -> 8192 fp32 683 us), so large ones are tiled from the first row on.
+template <class T>
+static bool lin_direct(const FneusLinear& f, bool backward) {
+    constexpr int V = 16 / (int)sizeof(T);
+    if (f.n_in < V || f.n_out < V || (!backward && f.rows <= 16)) return true;
+    const double work = (double)f.rows * f.n_in * f.n_out;
+    if (backward) return f.rows <= 1024 && work <= (double)(1L << 27) && (f.rows > 16 || (long)f.n_in * f.n_out <= 1L << 20);
+    return work <= (double)(sizeof(T) == 4 ? 1L << 28 : 1L << 27);
+}
 
 template <class T>
 static LinPlan lin_plan(const FneusLinear& f, bool backward) {
-    constexpr int V = 16 / (int)sizeof(T), KV = 128 / (int)sizeof(T);
+    constexpr int V = 16 / (int)sizeof(T);
     LinPlan p;
     memset(&p, 0, sizeof p);
-    const double work = (double)f.rows * f.n_in * f.n_out;
-    p.tiled = f.rows > 16 && f.n_in >= V && f.n_out >= V && work >= (double)kLinTiledWork;
+    p.tiled = !lin_direct<T>(f, backward);
     if (!p.tiled) return p;
     long o = 0, part = 0;
     auto take = [&](long bytes) { const long at = o; o += lin_up(bytes, 256); return at; };
@@ -454,14 +486,14 @@ static LinPlan lin_plan(const FneusLinear& f, bool backward) {
     if (!backward) {
         p.pad_x = !lin_aligned<T>(f.x, f.ldx, f.n_in, false);
         p.pad_w = !lin_aligned<T>(f.weight, f.n_in, f.n_in, false);
-        p.fwd = lin_shape(f.rows, f.n_out, f.n_in, KV);
+        p.fwd = lin_shape<T>(f.rows, f.n_out, f.n_in);
         partial(p.fwd, f.rows, f.n_out);
     } else {
         p.pad_x = f.dweight && !lin_aligned<T>(f.x, f.ldx, f.n_in, true);
         p.pad_w = f.dx && !lin_aligned<T>(f.weight, f.n_in, f.n_in, true);
         p.delta = (f.dx || f.dweight) && (f.act != 0 || !lin_aligned<T>(f.dy, f.lddy, f.n_out, f.dweight != nullptr));
-        p.dx = lin_shape(f.rows, f.n_in, f.n_out, KV);
-        p.dw = lin_shape(f.n_out, f.n_in, f.rows, KV);
+        p.dx = lin_shape<T>(f.rows, f.n_in, f.n_out);
+        p.dw = lin_shape<T>(f.n_out, f.n_in, f.rows);
         if (f.dx) partial(p.dx, f.rows, f.n_in);
         if (f.dweight) partial(p.dw, f.n_out, f.n_in);
         if (p.delta) p.ldd = (int)lin_up(f.n_out, V), p.off_delta = take(f.rows * p.ldd * (long)sizeof(T));
@@ -529,21 +561,30 @@ static void lin_tiled_product(LinTiled t, const LinShape& s, long nk, float* par
 }
 
 template <class T>
-static const void* lin_pad(const void* x, long ld, long rows, int n, unsigned char* out, int ldp, hipStream_t stream) {
-    const long chunks = rows * (ldp / Chunk<T>::N), grid = (chunks + 255) / 256;
-    hipLaunchKernelGGL((linear_pad_kernel<T>), dim3((unsigned)(grid < 4096 ? grid : 4096)), dim3(256), 0, stream, (const T*)x, ld, rows, n, (T*)out, ldp);
-    return out;
+static LinPad<T> lin_pad(const void* x, long ld, long rows, int n, unsigned char* out, int ldp) {
+    LinPad<T> p{};
+    const long blocks = (rows * (ldp / Chunk<T>::N) + 255) / 256;
+    p.x = (const T*)x, p.out = (T*)out, p.ld = ld, p.rows = rows, p.n = n, p.ldp = ldp, p.blocks = (int)(blocks < 2048 ? blocks : 2048);
+    return p;
+}
+
+template <class T>
+static void lin_prepare(const FneusLinear& f, const LinPlan& p, const LinDelta<T>& d, hipStream_t stream) {
+    unsigned char* S = (unsigned char*)f.scratch;
+    LinPad<T> px{}, pw{};
+    if (p.pad_x) px = lin_pad<T>(f.x, f.ldx, f.rows, f.n_in, S + p.off_x, p.ldx);
+    if (p.pad_w) pw = lin_pad<T>(f.weight, f.n_in, f.n_out, f.n_in, S + p.off_w, p.ldw);
+    const unsigned blocks = (unsigned)(d.strips * d.sum_parts + px.blocks + pw.blocks);
+    if (blocks) hipLaunchKernelGGL((linear_prepare_kernel<T>), dim3(blocks), dim3(256), 0, stream, d, px, pw);
 }
 
 template <class T>
 static void lin_tiled_fwd(const FneusLinear& f, const LinPlan& p, hipStream_t stream) {
     unsigned char* S = (unsigned char*)f.scratch;
-    const void *x = f.x, *w = f.weight;
-    long ldx = f.ldx, ldw = f.n_in;
-    if (p.pad_x) x = lin_pad<T>(x, ldx, f.rows, f.n_in, S + p.off_x, p.ldx, stream), ldx = p.ldx;
-    if (p.pad_w) w = lin_pad<T>(w, ldw, f.n_out, f.n_in, S + p.off_w, p.ldw, stream), ldw = p.ldw;
+    lin_prepare<T>(f, p, LinDelta<T>{}, stream);
     LinTiled t{};
-    t.a = lin_operand(x, ldx, sizeof(T)), t.b = lin_operand(w, ldw, sizeof(T));
+    t.a = p.pad_x ? lin_operand(S + p.off_x, p.ldx, sizeof(T)) : lin_operand(f.x, f.ldx, sizeof(T));
+    t.b = p.pad_w ? lin_operand(S + p.off_w, p.ldw, sizeof(T)) : lin_operand(f.weight, f.n_in, sizeof(T));
     t.bias = f.bias, t.res = f.residual, t.ldres = f.ld_residual, t.d = f.y, t.z = f.z, t.ldd = f.n_out, t.ni = f.rows, t.nj = f.n_out, t.act = f.act;
     lin_tiled_product<T, false, false, true>(t, p.fwd, f.n_in, (float*)(S + p.off_part), stream);
 }
@@ -551,28 +592,26 @@ static void lin_tiled_fwd(const FneusLinear& f, const LinPlan& p, hipStream_t st
 template <class T>
 static void lin_tiled_bwd(const FneusLinear& f, const LinPlan& p, hipStream_t stream) {
     unsigned char* S = (unsigned char*)f.scratch;
-    const void *x = f.x, *w = f.weight, *d = f.dy;
-    long ldx = f.ldx, ldw = f.n_in, ldd = f.lddy;
     float* part = (float*)(S + p.off_part);
+    LinDelta<T> d{};
     if (p.delta || f.dbias) {
-        const unsigned strips = (unsigned)((f.n_out + 32 * Chunk<T>::N - 1) / (32 * Chunk<T>::N));
-        float* sums = f.dbias ? (float*)(S + p.off_sums) : nullptr;
-        hipLaunchKernelGGL((linear_delta_kernel<T>), dim3(strips, (unsigned)p.sum_parts), dim3(256), 0, stream, (const T*)f.dy, f.lddy, (const T*)f.z, f.act,
-                           f.rows, f.n_out, p.delta ? (T*)(S + p.off_delta) : nullptr, p.ldd, sums);
-        if (f.dbias) hipLaunchKernelGGL((linear_fold_kernel<T>), dim3((unsigned)((f.n_out + 7) / 8)), dim3(1024), 0, stream, sums, p.sum_parts, f.n_out, (T*)f.dbias);
-        if (p.delta) d = S + p.off_delta, ldd = p.ldd;
+        d.dy = (const T*)f.dy, d.z = (const T*)f.z, d.delta = p.delta ? (T*)(S + p.off_delta) : nullptr, d.sums = f.dbias ? (float*)(S + p.off_sums) : nullptr;
+        d.lddy = f.lddy, d.rows = f.rows, d.n = f.n_out, d.ldp = p.ldd, d.act = f.act, d.sum_parts = p.sum_parts;
+        d.strips = (f.n_out + 32 * Chunk<T>::N - 1) / (32 * Chunk<T>::N);
     }
+    lin_prepare<T>(f, p, d, stream);
+    if (f.dbias)
+        hipLaunchKernelGGL((linear_fold_kernel<T>), dim3((unsigned)((f.n_out + 7) / 8)), dim3(1024), 0, stream, d.sums, p.sum_parts, f.n_out, (T*)f.dbias);
+    const MmOperand delta = p.delta ? lin_operand(S + p.off_delta, p.ldd, sizeof(T)) : lin_operand(f.dy, f.lddy, sizeof(T));
     if (f.dx) {
-        if (p.pad_w) w = lin_pad<T>(w, ldw, f.n_out, f.n_in, S + p.off_w, p.ldw, stream), ldw = p.ldw;
         LinTiled t{};
-        t.a = lin_operand(d, ldd, sizeof(T)), t.b = lin_operand(w, ldw, sizeof(T));
+        t.a = delta, t.b = p.pad_w ? lin_operand(S + p.off_w, p.ldw, sizeof(T)) : lin_operand(f.weight, f.n_in, sizeof(T));
         t.d = f.dx, t.ldd = f.n_in, t.ni = f.rows, t.nj = f.n_in;
         lin_tiled_product<T, false, true, false>(t, p.dx, f.n_out, part, stream);
     }
     if (f.dweight) {
-        if (p.pad_x) x = lin_pad<T>(x, ldx, f.rows, f.n_in, S + p.off_x, p.ldx, stream), ldx = p.ldx;
         LinTiled t{};
-        t.a = lin_operand(d, ldd, sizeof(T)), t.b = lin_operand(x, ldx, sizeof(T));
+        t.a = delta, t.b = p.pad_x ? lin_operand(S + p.off_x, p.ldx, sizeof(T)) : lin_operand(f.x, f.ldx, sizeof(T));
         t.d = f.dweight, t.ldd = f.n_in, t.ni = f.n_out, t.nj = f.n_in;
         lin_tiled_product<T, true, true, false>(t, p.dw, f.rows, part, stream);
     }
