@@ -213,29 +213,30 @@ FN_DEV void mm_run(unsigned char* smem, const MmOperand& A, const MmOperand& B, 
     MmReader<T, BKM, Cfg::BN, Cfg::NJ> rb;
     ra.init(mm_wave_i<Cfg>(), lane);
     rb.init(mm_wave_j<Cfg>(), lane);
-    auto compute = [&](const unsigned char* pa) {
+    constexpr int KS = SideA::KV / 16;
+    auto fetch = [&](const unsigned char* pa, int ks, LinFrag<T> (&fa)[Cfg::MI], LinFrag<T> (&fb)[Cfg::NJ]) {
         const unsigned char* pb = pa + Cfg::BM * 128;
 #pragma unroll
-        for (int ks = 0; ks < SideA::KV / 16; ++ks) {
+        for (int m = 0; m < Cfg::MI; ++m) ra.read(pa, m, ks, h, fa[m]);
+#pragma unroll
+        for (int n = 0; n < Cfg::NJ; ++n) rb.read(pb, n, ks, h, fb[n]);
+    };
+    auto multiply = [&](const LinFrag<T> (&fa)[Cfg::MI], const LinFrag<T> (&fb)[Cfg::NJ]) {
+#pragma unroll
+        for (int m = 0; m < Cfg::MI; ++m)
+#pragma unroll
+            for (int n = 0; n < Cfg::NJ; ++n) acc[m][n] = lin_mfma32(fb[n], fa[m], acc[m][n]);
+    };
+    auto compute = [&](const unsigned char* pa) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
             LinFrag<T> fa[Cfg::MI], fb[Cfg::NJ];
-#pragma unroll
-            for (int m = 0; m < Cfg::MI; ++m) ra.read(pa, m, ks, h, fa[m]);
-#pragma unroll
-            for (int n = 0; n < Cfg::NJ; ++n) rb.read(pb, n, ks, h, fb[n]);
-#pragma unroll
-            for (int m = 0; m < Cfg::MI; ++m)
-#pragma unroll
-                for (int n = 0; n < Cfg::NJ; ++n) acc[m][n] = lin_mfma32(fb[n], fa[m], acc[m][n]);
+            fetch(pa, ks, fa, fb);
+            multiply(fa, fb);
         }
     };
-    int stage = 0, left0 = RESCALE ? k_tiles : 0;
-#pragma unroll 1
-    for (int it = it0; it < it1; ++it) {
-        if (it1 - 1 - it >= P - 1) mm_wait_barrier<(P - 1) * Cfg::DPW>();
-        else mm_wait_barrier<0>();
-        if (it + P < it1) issue();
-        compute(smem + stage * Cfg::STAGE_BYTES);
-        stage = stage + 1 == Cfg::STAGES ? 0 : stage + 1;
+    int left0 = RESCALE ? k_tiles : 0;
+    auto rescale = [&]() {
         if constexpr (RESCALE) {
             if (--left0 == 0) {
 #pragma unroll
@@ -245,6 +246,50 @@ FN_DEV void mm_run(unsigned char* smem, const MmOperand& A, const MmOperand& B, 
 #pragma unroll
                         for (int e = 0; e < 16; ++e) acc[m][n][e] *= carry;
             }
+        }
+    };
+    int stage = 0;
+    auto wait = [&](int it) {               // stage `it` has landed, for everyone
+        if (it1 - 1 - it >= P - 1) mm_wait_barrier<(P - 1) * Cfg::DPW>();
+        else mm_wait_barrier<0>();
+    };
+    if constexpr (sizeof(T) == 2) {
+        // The fragments of the next 16 k are on their way from LDS while this one's are multiplied, across the stages too: the barrier that
+        // frees a stage's buffer comes when its last fragments are in registers, in front of their products.
+        if (it0 < it1) {
+            LinFrag<T> fa[2][Cfg::MI], fb[2][Cfg::NJ];
+            wait(it0);
+            if (it0 + P < it1) issue();
+            fetch(smem, 0, fa[0], fb[0]);
+#pragma unroll 1
+            for (int it = it0; it < it1; ++it) {
+                const unsigned char* pa = smem + stage * Cfg::STAGE_BYTES;
+                stage = stage + 1 == Cfg::STAGES ? 0 : stage + 1;
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    if (ks + 1 < KS) {
+                        fetch(pa, ks + 1, fa[(ks + 1) & 1], fb[(ks + 1) & 1]);
+                    } else if (it + 1 < it1) {
+                        wait(it + 1);
+                        if (it + 1 + P < it1) issue();
+                        fetch(smem + stage * Cfg::STAGE_BYTES, 0, fa[0], fb[0]);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                    multiply(fa[ks & 1], fb[ks & 1]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                rescale();
+            }
+        }
+        static_assert(KS % 2 == 0, "the two sets alternate");
+    } else {
+#pragma unroll 1
+        for (int it = it0; it < it1; ++it) {
+            wait(it);
+            if (it + P < it1) issue();
+            compute(smem + stage * Cfg::STAGE_BYTES);
+            stage = stage + 1 == Cfg::STAGES ? 0 : stage + 1;
+            rescale();
         }
     }
     if constexpr (TAIL) {
