@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, 2) linear_tiled_kernel(LinTiled 
         constexpr int SLOTS = Cfg::WN / 8;
         float bias[4] = {0.0f, 0.0f, 0.0f, 0.0f}, res[SLOTS][4];
         {
-            const long j = j0 + mm_wave_j<Cfg>() + 4 * ((threadIdx.x & 63) % (Cfg::WN / 4));
+            const long j = mm_quad_j<Cfg>(j0);
             if (P.bias && j < P.nj) quad_load((const T*)P.bias + j, (int)(P.nj - j), bias);
         }
         const float slope = P.act == 0 ? 1.0f : (P.act == 2 ? 0.2f : 0.0f);
@@ -541,9 +541,8 @@ static void lin_tiled_whole(const LinTiled& t, hipStream_t stream) {
 
 template <class T, bool AKM, bool BKM, bool FWD>
 static void lin_tiled_product(LinTiled t, const LinShape& s, long nk, float* partial, hipStream_t stream) {
-    constexpr int KV = 128 / (int)sizeof(T);
-    const int b = s.tile;
-    t.k_tiles = (int)(nk / KV), t.tail = (int)(nk % KV), t.splits = s.splits, t.partial = partial;
+    const int b = s.tile, kv = s.tile == 256 ? LinBig::template kv<T>() : (s.tile == 128 ? LinMid::template kv<T>() : LinSmall::template kv<T>());
+    t.k_tiles = (int)(nk / kv), t.tail = (int)(nk % kv), t.splits = s.splits, t.partial = partial;
     t.tiles_i = (int)((t.ni + b - 1) / b), t.tiles_j = (t.nj + b - 1) / b;
     if (s.splits > 1) {
         if (s.tile == 64) lin_tiled_launch<LinSmall, T, AKM, BKM, LIN_EPI_PART, 0>(t, stream);

@@ -27,12 +27,16 @@ struct MmOperand {
     long row_bytes;
 };
 
-template <int BM_, int BN_, int WGM, int WGN, int STAGES_>
+// GROUPS > 1: that many groups of waves share the k of every stage and their sums are added behind the last (a tile that is alone on its CU
+// is done that much sooner)
+template <int BM_, int BN_, int WGM, int WGN, int STAGES_, int GROUPS_ = 1>
 struct MmCfg {
-    static constexpr int BM = BM_, BN = BN_, WAVES = WGM * WGN, THREADS = 64 * WAVES, STAGES = STAGES_;
+    static constexpr int BM = BM_, BN = BN_, GROUPS = GROUPS_, GROUP_WAVES = WGM * WGN, WAVES = GROUPS * GROUP_WAVES, THREADS = 64 * WAVES;
+    static constexpr int STAGES = STAGES_, ROW = 128 * GROUPS;             // bytes of k of a row in a stage
+    template <class T> static constexpr int kv() { return ROW / (int)sizeof(T); }        // values of k in a stage
     static constexpr int WM = BM / WGM, WN = BN / WGN, MI = WM / 32, NJ = WN / 32, WAVES_N = WGN;
-    static constexpr int STAGE_BYTES = (BM + BN) * 128, DPW = (BM + BN) / 8 / WAVES, LDS = STAGES * STAGE_BYTES;
-    static_assert((BM / 8) % DPW == 0 && (BN / 8) % DPW == 0, "a wave fills rows of one operand");
+    static constexpr int STAGE_BYTES = (BM + BN) * ROW, DPW = STAGE_BYTES / 1024 / WAVES, LDS = STAGES * STAGE_BYTES;
+    static_assert((BM * ROW / 1024) % DPW == 0 && (BN * ROW / 1024) % DPW == 0, "a wave fills rows of one operand");
 };
 
 template <int N>
@@ -61,15 +65,21 @@ constexpr unsigned kMmThree = 0x140u;             // 3: (0, 0), (0, 1), (1, 0): 
 // wave's part of the tile: four consecutive columns in four consecutive registers.
 FN_DEV int mm_wave() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }
 template <class Cfg>
-FN_DEV int mm_wave_i() { return (mm_wave() / Cfg::WAVES_N) * Cfg::WM; }
+FN_DEV int mm_wave_i() { return (mm_wave() % Cfg::GROUP_WAVES / Cfg::WAVES_N) * Cfg::WM; }
 template <class Cfg>
 FN_DEV int mm_wave_j() { return (mm_wave() % Cfg::WAVES_N) * Cfg::WN; }
 
+// the places `load` and `finish` of mm_epilogue are called for, slot s of block 0
+template <class Cfg>
+FN_DEV long mm_quad_i(long i0, int s) { return i0 + mm_wave_i<Cfg>() + (s * 64 + (int)(threadIdx.x & 63)) / (Cfg::WN / 4); }
+template <class Cfg>
+FN_DEV long mm_quad_j(long j0) { return j0 + mm_wave_j<Cfg>() + 4 * ((int)(threadIdx.x & 63) % (Cfg::WN / 4)); }
+
 // One operand's side of a stage: which bytes its DMA fetches, where a fragment lies.
-template <class T, bool KM, int B>
+template <class T, bool KM, int B, int ROW>
 struct MmSide {
-    static constexpr int E = sizeof(T), KV = 128 / E;            // values of k in a stage
-    static constexpr int LINE = KM ? B * E : 128, CHUNKS = LINE / 16, LINES = KM ? KV : B;      // LINES * LINE == B * 128
+    static constexpr int E = sizeof(T), KV = ROW / E;            // values of k in a stage
+    static constexpr int LINE = KM ? B * E : ROW, CHUNKS = LINE / 16, LINES = KM ? KV : B;      // LINES * LINE == B * ROW
     static FN_DEV int slot(int line, int c) {
         if constexpr (KM) return E == 2 ? c ^ (((line & 7) << 1) & (CHUNKS - 1)) : c;
         else return c ^ (line & 7);
@@ -82,7 +92,7 @@ struct MmSide {
     }
     // a stage whose k ends after `left` values: ordinary loads, zeros behind
     static FN_DEV void fill_tail(unsigned char* lds, const unsigned char* src, int valid_rows, long row_bytes, int left, int thread, int threads) {
-        for (int at = thread; at < B * 8; at += threads) {
+        for (int at = thread; at < B * ROW / 16; at += threads) {
             const int line = at / CHUNKS, c = at % CHUNKS;
             T v[16 / E];
 #pragma unroll
@@ -96,9 +106,9 @@ struct MmSide {
 };
 
 // Fragments of one wave's rows w0 .. of an operand; base: LDS address of the operand's part of a stage
-template <class T, bool KM, int B, int COUNT>
+template <class T, bool KM, int B, int ROW, int COUNT>
 struct MmReader {
-    typedef MmSide<T, KM, B> Side;
+    typedef MmSide<T, KM, B, ROW> Side;
     unsigned at[(KM && sizeof(T) == 2) ? 2 * COUNT : COUNT];
     unsigned x7;
     FN_DEV void init(int w0, int lane) {
@@ -106,7 +116,7 @@ struct MmReader {
         x7 = (unsigned)(lane & 7);
         if constexpr (!KM) {
 #pragma unroll
-            for (int m = 0; m < COUNT; ++m) at[m] = (unsigned)(w0 + 32 * m + r) * 128u;
+            for (int m = 0; m < COUNT; ++m) at[m] = (unsigned)(w0 + 32 * m + r) * (unsigned)ROW;
         } else if constexpr (sizeof(T) == 2) {
             const int fh = (lane >> 4) & 1, q = (lane & 15) >> 2, p = lane & 3;
 #pragma unroll
@@ -158,8 +168,9 @@ struct MmReader {
 template <class Cfg, class T, bool AKM, bool BKM, bool RESCALE, bool TAIL>
 FN_DEV void mm_run(unsigned char* smem, const MmOperand& A, const MmOperand& B, long i0, long ni, long j0, long nj, int k_tiles, int tail,
                    unsigned segs, int it0, int it1, bool with_tail, float carry, f32x16 (&acc)[Cfg::MI][Cfg::NJ]) {
-    typedef MmSide<T, AKM, Cfg::BM> SideA;
-    typedef MmSide<T, BKM, Cfg::BN> SideB;
+    typedef MmSide<T, AKM, Cfg::BM, Cfg::ROW> SideA;
+    typedef MmSide<T, BKM, Cfg::BN, Cfg::ROW> SideB;
+    constexpr int QA = Cfg::BM * Cfg::ROW / 1024;        // DMA instructions of A's part of a stage
     const int lane = threadIdx.x & 63, wave = mm_wave(), h = lane >> 5;
 #pragma unroll
     for (int m = 0; m < Cfg::MI; ++m)
@@ -170,13 +181,13 @@ FN_DEV void mm_run(unsigned char* smem, const MmOperand& A, const MmOperand& B, 
     const int va = (int)(ni - i0 < Cfg::BM ? ni - i0 : Cfg::BM), vb = (int)(nj - j0 < Cfg::BN ? nj - j0 : Cfg::BN);
     // this wave's DMA
     const int q0 = wave * Cfg::DPW;
-    const bool is_b = q0 >= Cfg::BM / 8;
+    const bool is_b = q0 >= QA;
     unsigned off[Cfg::DPW];
 #pragma unroll
     for (int d = 0; d < Cfg::DPW; ++d)
-        off[d] = is_b ? SideB::dma_offset(q0 + d - Cfg::BM / 8, lane, vb, B.row_bytes) : SideA::dma_offset(q0 + d, lane, va, A.row_bytes);
+        off[d] = is_b ? SideB::dma_offset(q0 + d - QA, lane, vb, B.row_bytes) : SideA::dma_offset(q0 + d, lane, va, A.row_bytes);
     const long origin = is_b ? (BKM ? j0 * (long)sizeof(T) : j0 * B.row_bytes) : (AKM ? i0 * (long)sizeof(T) : i0 * A.row_bytes);
-    const long step = is_b ? (BKM ? SideB::KV * B.row_bytes : 128) : (AKM ? SideA::KV * A.row_bytes : 128);
+    const long step = is_b ? (BKM ? SideB::KV * B.row_bytes : Cfg::ROW) : (AKM ? SideA::KV * A.row_bytes : Cfg::ROW);
     const unsigned char *pl0 = is_b ? B.plane[0] : A.plane[0], *pl1 = is_b ? B.plane[1] : A.plane[1];
     int is_seg = it0 / (k_tiles > 0 ? k_tiles : 1), is_kt = it0 - is_seg * k_tiles;
     auto base_of = [&](int seg) {
@@ -209,17 +220,18 @@ FN_DEV void mm_run(unsigned char* smem, const MmOperand& A, const MmOperand& B, 
     constexpr int P = Cfg::STAGES - 1;
     for (int s = 0; s < P; ++s)
         if (it0 + s < it1) issue();
-    MmReader<T, AKM, Cfg::BM, Cfg::MI> ra;
-    MmReader<T, BKM, Cfg::BN, Cfg::NJ> rb;
+    MmReader<T, AKM, Cfg::BM, Cfg::ROW, Cfg::MI> ra;
+    MmReader<T, BKM, Cfg::BN, Cfg::ROW, Cfg::NJ> rb;
     ra.init(mm_wave_i<Cfg>(), lane);
     rb.init(mm_wave_j<Cfg>(), lane);
-    constexpr int KS = SideA::KV / 16;
+    constexpr int KS = SideA::KV / 16 / Cfg::GROUPS;         // of this group
+    const int ks0 = Cfg::GROUPS > 1 ? mm_wave() / Cfg::GROUP_WAVES * KS : 0;
     auto fetch = [&](const unsigned char* pa, int ks, LinFrag<T> (&fa)[Cfg::MI], LinFrag<T> (&fb)[Cfg::NJ]) {
-        const unsigned char* pb = pa + Cfg::BM * 128;
+        const unsigned char* pb = pa + Cfg::BM * Cfg::ROW;
 #pragma unroll
-        for (int m = 0; m < Cfg::MI; ++m) ra.read(pa, m, ks, h, fa[m]);
+        for (int m = 0; m < Cfg::MI; ++m) ra.read(pa, m, ks0 + ks, h, fa[m]);
 #pragma unroll
-        for (int n = 0; n < Cfg::NJ; ++n) rb.read(pb, n, ks, h, fb[n]);
+        for (int n = 0; n < Cfg::NJ; ++n) rb.read(pb, n, ks0 + ks, h, fb[n]);
     };
     auto multiply = [&](const LinFrag<T> (&fa)[Cfg::MI], const LinFrag<T> (&fb)[Cfg::NJ]) {
 #pragma unroll
@@ -295,13 +307,37 @@ FN_DEV void mm_run(unsigned char* smem, const MmOperand& A, const MmOperand& B, 
     if constexpr (TAIL) {
         if (with_tail && tail > 0) {
             mm_wait_barrier<0>();                        // (the ring is empty; everyone has read its last stage)
-            const unsigned char* sa = A.plane[0] + (AKM ? i0 * (long)sizeof(T) + (long)k_tiles * SideA::KV * A.row_bytes : i0 * A.row_bytes + k_tiles * 128L);
-            const unsigned char* sb = B.plane[0] + (BKM ? j0 * (long)sizeof(T) + (long)k_tiles * SideB::KV * B.row_bytes : j0 * B.row_bytes + k_tiles * 128L);
+            const unsigned char* sa = A.plane[0] + (AKM ? i0 * (long)sizeof(T) + (long)k_tiles * SideA::KV * A.row_bytes : i0 * A.row_bytes + k_tiles * (long)Cfg::ROW);
+            const unsigned char* sb = B.plane[0] + (BKM ? j0 * (long)sizeof(T) + (long)k_tiles * SideB::KV * B.row_bytes : j0 * B.row_bytes + k_tiles * (long)Cfg::ROW);
             SideA::fill_tail(smem, sa, va, A.row_bytes, tail, threadIdx.x, Cfg::THREADS);
-            SideB::fill_tail(smem + Cfg::BM * 128, sb, vb, B.row_bytes, tail, threadIdx.x, Cfg::THREADS);
+            SideB::fill_tail(smem + Cfg::BM * Cfg::ROW, sb, vb, B.row_bytes, tail, threadIdx.x, Cfg::THREADS);
             mm_wait_barrier<0>();
             compute(smem);
         }
+    }
+    if constexpr (Cfg::GROUPS > 1) {          // the groups' sums, added in their order by the first
+        constexpr int PART = Cfg::MI * Cfg::NJ * 16 * 64;
+        static_assert((Cfg::GROUPS - 1) * Cfg::GROUP_WAVES * PART * 4 <= Cfg::LDS, "the sums fit the ring");
+        float* sums = reinterpret_cast<float*>(smem) + (wave % Cfg::GROUP_WAVES) * PART + lane;
+        const int group = wave / Cfg::GROUP_WAVES;
+        __syncthreads();
+#pragma unroll
+        for (int m = 0; m < Cfg::MI; ++m)
+#pragma unroll
+            for (int n = 0; n < Cfg::NJ; ++n)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (group) sums[(group - 1) * Cfg::GROUP_WAVES * PART + ((m * Cfg::NJ + n) * 16 + e) * 64] = acc[m][n][e];
+        __syncthreads();
+        if (group) return;
+#pragma unroll
+        for (int g = 1; g < Cfg::GROUPS; ++g)
+#pragma unroll
+            for (int m = 0; m < Cfg::MI; ++m)
+#pragma unroll
+                for (int n = 0; n < Cfg::NJ; ++n)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) acc[m][n][e] += sums[(g - 1) * Cfg::GROUP_WAVES * PART + ((m * Cfg::NJ + n) * 16 + e) * 64];
     }
 }
 
@@ -309,19 +345,24 @@ FN_DEV void mm_run(unsigned char* smem, const MmOperand& A, const MmOperand& B, 
 // part of LDS.  `load(i, j, slot)` fetches what the four outputs (i, j .. j + 3) need from memory -- all of a block's loads are in flight before
 // the first is used -- and `finish(i, j, slot, v, cell)` ends them; slot numbers the quads of a block, j is the same in all of a lane's.
 // `turn(ib, jb, rows)` runs once a block behind that.
-template <class Cfg, class Load, class Finish, class Turn>
+// EARLY: the caller has made the loads in front of the product (one block a wave).  The first group's waves alone go in (mm_wave() <
+// GROUP_WAVES), the others only meet the barrier.
+template <class Cfg, bool EARLY = false, class Load, class Finish, class Turn>
 FN_DEV void mm_epilogue(unsigned char* smem, long i0, long j0, float scale, f32x16 (&acc)[Cfg::MI][Cfg::NJ], Load load, Finish finish, Turn turn) {
     constexpr int STRIDE = Cfg::WN + 4, QUADS = Cfg::WN / 4, SLOTS = 32 * QUADS / 64;
-    static_assert(Cfg::WAVES * 32 * STRIDE * 4 <= Cfg::LDS, "the epilogue's rows fit the ring");
+    static_assert(Cfg::GROUP_WAVES * 32 * STRIDE * 4 <= Cfg::LDS, "the epilogue's rows fit the ring");
+    static_assert(!EARLY || Cfg::MI == 1, "the early loads are the one block's");
     float* rows = reinterpret_cast<float*>(smem) + mm_wave() * 32 * STRIDE;
     const int lane = threadIdx.x & 63, c = 4 * (lane % QUADS);
     const long jb = j0 + mm_wave_j<Cfg>();
     __syncthreads();                                  // (everyone has read the last stage)
+    if (Cfg::GROUPS > 1 && mm_wave() >= Cfg::GROUP_WAVES) return;
 #pragma unroll
     for (int m = 0; m < Cfg::MI; ++m) {
         const long ib = i0 + mm_wave_i<Cfg>() + 32 * m;
 #pragma unroll
-        for (int s = 0; s < SLOTS; ++s) load(ib + (s * 64 + lane) / QUADS, jb + c, s);
+        for (int s = 0; s < SLOTS; ++s)
+            if constexpr (!EARLY) load(ib + (s * 64 + lane) / QUADS, jb + c, s);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
 #pragma unroll

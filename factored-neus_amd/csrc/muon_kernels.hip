@@ -28,25 +28,33 @@ struct MuonJob {
     long off;                                // its scratch
 };
 
-// `first`: the launch's first workgroup of each job (beyond the last: none).  The arguments lie in host memory, a line of them is a
-// microsecond away: the search reads the two lines of `first` at once, then one job.
 struct MuonJobs {
-    int first[kMuonMaxJobs];
+    MuonJob j[kMuonMaxJobs];
     unsigned char* scratch;
     long n;
-    MuonJob j[kMuonMaxJobs];
 };
 
 struct MuonNum {
     float a, b, c;                           // the polynomial
     int ex, ea, eb;                          // planes hold X 2^ex, A 2^ea, B 2^eb
     float eps, mu, omu, wd;
-    int nesterov, zero_grad, nesterov_step;
+    int nesterov, zero_grad;
     const float* lr;
 };
 
+// Arguments of the launches behind the first.  Arguments lie in host memory: their first lines arrive with the launch, each later line costs
+// a microsecond.  So the table of jobs travels once: the first launch leaves it at the start of the scratch.  `first`: the launch's first
+// workgroup of each job (beyond the last job: none).
+struct MuonArgs {
+    MuonNum P;
+    int cur;
+    unsigned char* scratch;
+    int first[kMuonMaxJobs];
+};
+constexpr long kMuonTable = kMuonMaxJobs * sizeof(MuonJob);
+
 // where a matrix's buffers lie in its scratch: norm partials, X twice (a step reads one and writes the other), A, B.  Rows of X and
-// columns of all are padded with zeros to multiples of 64: whole stages of the engine's ring
+// columns of all are padded with zeros to multiples of 128: whole stages of the engine's ring
 struct MuonLay {
     int m, n, mp;
     bool trans;
@@ -59,8 +67,8 @@ __host__ __device__ inline MuonLay muon_lay(int rows, int cols, int planes) {
     L.trans = rows > cols;
     L.m = L.trans ? cols : rows;
     L.n = L.trans ? rows : cols;
-    L.mp = (L.m + 63) / 64 * 64;
-    L.ldx = (unsigned)((L.n + 63) / 64) * 128u;
+    L.mp = (L.m + 127) / 128 * 128;
+    L.ldx = (unsigned)((L.n + 127) / 128) * 256u;
     L.lda = (unsigned)L.mp * 2u;
     L.px = (long)L.mp * L.ldx;
     L.pa = (long)L.m * L.lda;
@@ -72,11 +80,18 @@ __host__ __device__ inline MuonLay muon_lay(int rows, int cols, int planes) {
     return L;
 }
 
-FN_DEV int muon_find(const MuonJobs& js, int wg) {
+FN_DEV int muon_find(const MuonArgs& a, int wg) {
     int q = 0;
 #pragma unroll
-    for (int k = 1; k < kMuonMaxJobs; ++k) q += js.first[k] <= wg ? 1 : 0;
+    for (int k = 1; k < kMuonMaxJobs; ++k) q += a.first[k] <= wg ? 1 : 0;
     return q;
+}
+FN_DEV MuonJob muon_job(const MuonArgs& a, int q) {
+    MuonJob J = reinterpret_cast<const MuonJob*>(a.scratch)[q];
+    // (addresses read from memory are of no known space to the compiler: global, not flat, accesses)
+    J.grad = (void*)(FN_GLOBAL char*)J.grad, J.momentum = (void*)(FN_GLOBAL char*)J.momentum;
+    J.param = (void*)(FN_GLOBAL char*)J.param, J.out = (void*)(FN_GLOBAL char*)J.out;
+    return J;
 }
 
 // u = (1 - mu) g + mu m', m' = mu m + (1 - mu) g as it is stored
@@ -88,6 +103,7 @@ template <class T, bool MOM>
 __global__ void __launch_bounds__(256) muon_norm_kernel(MuonJobs js, MuonNum P) {
     const int q = blockIdx.x / kMuonChunks, c = blockIdx.x % kMuonChunks;
     const MuonJob& J = js.j[q];
+    if (c == 0 && threadIdx.x == 0) reinterpret_cast<MuonJob*>(js.scratch)[q] = J;
     const long total = (long)J.rows * J.cols;
     const T* g = (const T*)J.grad;
     T* m = (T*)J.momentum;
@@ -125,19 +141,20 @@ FN_DEV void muon_split(float v, _Float16& hi, _Float16& lo) {
 
 // launch 2: X (with its zero padding) from 64 x 64 tiles of u
 template <class T, bool MOM, int NP>
-__global__ void __launch_bounds__(256) muon_init_kernel(MuonJobs js, MuonNum P) {
+__global__ void __launch_bounds__(256) muon_init_kernel(MuonArgs args) {
     __shared__ float tile[64][65];
     __shared__ double red[4];
-    const int q = muon_find(js, blockIdx.x);
-    const MuonJob& J = js.j[q];
+    const MuonNum& P = args.P;
+    const int q = muon_find(args, blockIdx.x);
+    const MuonJob J = muon_job(args, q);
     const MuonLay L = muon_lay(J.rows, J.cols, NP);
-    unsigned char* S = js.scratch + J.off;
+    unsigned char* S = args.scratch + J.off;
     double s = reinterpret_cast<const double*>(S)[threadIdx.x];       // kMuonChunks == 256 partials
 #pragma unroll
     for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d, 64);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
-    const int tiles_c = (J.cols + 63) / 64;
-    const int t = blockIdx.x - js.first[q], r0 = 64 * (t / tiles_c), c0 = 64 * (t % tiles_c);
+    const int tiles_c = (J.cols + 127) / 128 * 2;
+    const int t = blockIdx.x - args.first[q], r0 = 64 * (t / tiles_c), c0 = 64 * (t % tiles_c);
     const int lc = threadIdx.x & 63, lr = threadIdx.x >> 6;
 #pragma unroll 4
     for (int r = lr; r < 64; r += 4) {
@@ -164,7 +181,20 @@ __global__ void __launch_bounds__(256) muon_init_kernel(MuonJobs js, MuonNum P) 
         _Float16* o = x + (long)((L.trans ? c0 : r0) + r) * ld + (L.trans ? r0 : c0) + lc;
         o[0] = hi;
         if constexpr (NP == 2) o[L.px / 2] = lo;
+        const int row = (L.trans ? c0 : r0) + r, col = (L.trans ? r0 : c0) + lc;
+        if (row >= L.m || col >= L.n) {              // the padding of the other X: the steps write the matrix alone
+            o += (L.x[1] - L.x[0]) / 2;
+            o[0] = (_Float16)0.0f;
+            if constexpr (NP == 2) o[L.px / 2] = (_Float16)0.0f;
+        }
     }
+    // the padding of A and B: columns m .. mp of row t, t + tiles, ...
+    const int tiles = tiles_c * ((J.rows + 127) / 128 * 2);
+    for (int row = t; row < L.m; row += tiles)
+        for (int at = threadIdx.x; at < 2 * NP * (L.mp - L.m); at += 256) {
+            const int which = at / (L.mp - L.m), col = L.m + at % (L.mp - L.m);
+            *reinterpret_cast<_Float16*>(S + (which & 1 ? L.b : L.a) + (which >> 1) * L.pa + (long)row * L.lda + col * 2) = (_Float16)0.0f;
+        }
 }
 
 template <int NP>
@@ -203,18 +233,20 @@ FN_DEV void muon_upper(int t, int& ti, int& tj) {
 // A and B are symmetric: the tiles below the diagonal are the mirror images the tiles above it write.  The epilogue goes through LDS, 32
 // rows of a wave at a time, so that either orientation writes runs of a line.
 template <class Cfg, int NP, int KIND, class T, bool MOM>
-__global__ void __launch_bounds__(Cfg::THREADS, 2) muon_product_kernel(MuonJobs js, MuonNum P, int cur) {
+__global__ void __launch_bounds__(Cfg::THREADS, 2) muon_product_kernel(MuonArgs args) {
     extern __shared__ __attribute__((aligned(16))) unsigned char mm_smem[];
-    const int q = muon_find(js, blockIdx.x);
-    const MuonJob& J = js.j[q];
+    const MuonNum& P = args.P;
+    const int cur = args.cur;
+    const int q = muon_find(args, blockIdx.x);
+    const MuonJob J = muon_job(args, q);
     const MuonLay L = muon_lay(J.rows, J.cols, NP);
-    unsigned char* S = js.scratch + J.off;
+    unsigned char* S = args.scratch + J.off;
     constexpr bool SYM = KIND <= MU_POLY;
     const int ni = L.m, nj = SYM ? L.m : L.n;
     const int tiles_i = (ni + Cfg::BM - 1) / Cfg::BM, tiles_j = (nj + Cfg::BN - 1) / Cfg::BN;
     const long tiles = SYM ? (long)tiles_i * (tiles_i + 1) / 2 : (long)tiles_i * tiles_j;
     int ti, tj;
-    const long t = mm_spread(blockIdx.x - js.first[q], tiles);
+    const long t = mm_spread(blockIdx.x - args.first[q], tiles);
     if constexpr (SYM) muon_upper((int)t, ti, tj);
     else mm_tile(t, tiles_i, tiles_j, ti, tj);
     const long i0 = (long)ti * Cfg::BM, j0 = (long)tj * Cfg::BN;
@@ -222,7 +254,29 @@ __global__ void __launch_bounds__(Cfg::THREADS, 2) muon_product_kernel(MuonJobs 
     if constexpr (KIND == MU_GRAM) A = B = muon_op<NP>(S + L.x[cur], L.px, L.ldx);
     else if constexpr (KIND == MU_POLY) A = B = muon_op<NP>(S + L.a, L.pa, L.lda);
     else A = muon_op<NP>(S + L.b, L.pa, L.lda), B = muon_op<NP>(S + L.x[cur], L.px, L.ldx);
-    const int k_tiles = (int)((KIND == MU_GRAM ? L.ldx : L.lda) / 128);
+    constexpr int STRIDE = Cfg::WN + 4, SLOTS = Cfg::WN / 8;
+    // what the quads of a block add: b A (POLY), a X (STEP, LAST), and the parameters they end in
+    f16x4 old_hi[SLOTS], old_lo[SLOTS];
+    float par[SLOTS][4];
+    const unsigned char* old = S + (KIND == MU_POLY ? L.a : L.x[cur]);
+    const long ld_old = KIND == MU_POLY ? L.lda : L.ldx, pl_old = KIND == MU_POLY ? L.pa : L.px, width = ld_old / 2;
+    constexpr bool EARLY = Cfg::MI == 1;
+    auto load = [&](long i, long j, int s) {
+            if constexpr (KIND != MU_GRAM) {
+                old_hi[s] = old_lo[s] = f16x4{0, 0, 0, 0};
+                if (i < ni && j < width) {
+                    old_hi[s] = *reinterpret_cast<const f16x4*>(old + i * ld_old + j * 2);
+                    if constexpr (NP == 2) old_lo[s] = *reinterpret_cast<const f16x4*>(old + pl_old + i * ld_old + j * 2);
+                }
+            }
+            if constexpr (KIND == MU_LAST && MOM)
+                if (!L.trans && i < ni && j < nj) quad_load((const T*)J.param + i * (long)J.cols + j, (int)(nj - j), par[s]);
+        };
+    if constexpr (EARLY) {
+#pragma unroll
+        for (int s = 0; s < SLOTS; ++s) load(mm_quad_i<Cfg>(i0, s), mm_quad_j<Cfg>(j0), s);
+    }
+    const int k_tiles = (int)((KIND == MU_GRAM ? L.ldx : L.lda) / Cfg::ROW);
     f32x16 acc[Cfg::MI][Cfg::NJ];
     mm_run<Cfg, _Float16, false, (KIND >= MU_STEP), NP == 2, false>(mm_smem, A, B, i0, ni, j0, nj, k_tiles, 0, NP == 2 ? kMmThree : kMmOne, 0,
                                                                     (NP == 2 ? 3 : 1) * k_tiles, false, kLoScale, acc);
@@ -237,24 +291,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, 2) muon_product_kernel(MuonJobs 
     const float lr = KIND == MU_LAST && MOM ? *P.lr : 0.0f;
     const float keep = 1.0f - lr * P.wd, step = lr * J.adjust;
     const bool turn = SYM ? ti != tj : (KIND == MU_LAST && L.trans);          // the second orientation is written too (SYM) or alone
-    constexpr int STRIDE = Cfg::WN + 4, SLOTS = Cfg::WN / 8;
-    // what the quads of a block add: b A (POLY), a X (STEP, LAST), and the parameters they end in
-    f16x4 old_hi[SLOTS], old_lo[SLOTS];
-    float par[SLOTS][4];
-    const unsigned char* old = S + (KIND == MU_POLY ? L.a : L.x[cur]);
-    const long ld_old = KIND == MU_POLY ? L.lda : L.ldx, pl_old = KIND == MU_POLY ? L.pa : L.px, width = ld_old / 2;
-    mm_epilogue<Cfg>(mm_smem, i0, j0, f, acc,
-        [&](long i, long j, int s) {
-            if constexpr (KIND != MU_GRAM) {
-                old_hi[s] = old_lo[s] = f16x4{0, 0, 0, 0};
-                if (i < ni && j < width) {
-                    old_hi[s] = *reinterpret_cast<const f16x4*>(old + i * ld_old + j * 2);
-                    if constexpr (NP == 2) old_lo[s] = *reinterpret_cast<const f16x4*>(old + pl_old + i * ld_old + j * 2);
-                }
-            }
-            if constexpr (KIND == MU_LAST && MOM)
-                if (!L.trans && i < ni && j < nj) quad_load((const T*)J.param + i * (long)J.cols + j, (int)(nj - j), par[s]);
-        },
+    mm_epilogue<Cfg, EARLY>(mm_smem, i0, j0, f, acc, load,
         [&](long i, long j, int s, float (&v)[4], float* cell) {
             f16x4 hi, lo4;
             if constexpr (KIND != MU_GRAM) {
@@ -312,7 +349,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, 2) muon_product_kernel(MuonJobs 
         });
 }
 
-typedef MmCfg<64, 64, 2, 2, 5> MuonSmall;          // 80 KiB: four stages in flight, two workgroups a CU
+typedef MmCfg<64, 64, 2, 2, 4, 2> MuonSmall;       // 8 waves, two sharing each stage's 128 k; 128 KiB: three stages in flight
 typedef MmCfg<128, 128, 2, 2, 2> MuonMid;          // 64 KiB, two
 typedef MmCfg<256, 256, 2, 4, 2> MuonBig;          // 128 KiB, one
 
@@ -322,21 +359,21 @@ static long muon_tiles(long m, long n, bool sym, int b) {
 }
 
 template <class Cfg, int NP, int KIND, class T, bool MOM>
-static void muon_product_launch(MuonJobs& js, const MuonNum& P, int cur, hipStream_t stream) {
+static void muon_product_launch(const MuonJobs& js, MuonArgs& args, hipStream_t stream) {
     long tiles = 0;
     for (int q = 0; q < js.n; ++q) {
         const MuonJob& J = js.j[q];
-        js.first[q] = (int)tiles;
+        args.first[q] = (int)tiles;
         tiles += muon_tiles(J.rows < J.cols ? J.rows : J.cols, J.rows < J.cols ? J.cols : J.rows, KIND <= MU_POLY, Cfg::BM);
     }
     auto kernel = muon_product_kernel<Cfg, NP, KIND, T, MOM>;
     allow_big_lds(kernel);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(Cfg::THREADS), Cfg::LDS, stream, js, P, cur);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(Cfg::THREADS), Cfg::LDS, stream, args);
 }
 
 // the largest tile that leaves no more than a quarter of the CUs without one
 template <int NP, int KIND, class T, bool MOM>
-static void muon_product(MuonJobs& js, const MuonNum& P, int cur, hipStream_t stream) {
+static void muon_product(const MuonJobs& js, MuonArgs& args, hipStream_t stream) {
     long big = 0, mid = 0;
     for (int q = 0; q < js.n; ++q) {
         const MuonJob& J = js.j[q];
@@ -344,18 +381,19 @@ static void muon_product(MuonJobs& js, const MuonNum& P, int cur, hipStream_t st
         big += muon_tiles(m, n, KIND <= MU_POLY, 256), mid += muon_tiles(m, n, KIND <= MU_POLY, 128);
     }
     static const int form = getenv("FNEUS_MUON_TILE") ? atoi(getenv("FNEUS_MUON_TILE")) : 0;
-    if (form ? form == 256 : big >= 192) muon_product_launch<MuonBig, NP, KIND, T, MOM>(js, P, cur, stream);
-    else if (form ? form == 128 : mid >= 192) muon_product_launch<MuonMid, NP, KIND, T, MOM>(js, P, cur, stream);
-    else muon_product_launch<MuonSmall, NP, KIND, T, MOM>(js, P, cur, stream);
+    if (form ? form == 256 : big >= 192) muon_product_launch<MuonBig, NP, KIND, T, MOM>(js, args, stream);
+    else if (form ? form == 128 : mid >= 192) muon_product_launch<MuonMid, NP, KIND, T, MOM>(js, args, stream);
+    else muon_product_launch<MuonSmall, NP, KIND, T, MOM>(js, args, stream);
 }
 
 template <int NP, class T, bool MOM>
-static void muon_steps(MuonJobs& js, const MuonNum& P, int steps, hipStream_t stream) {
+static void muon_steps(const MuonJobs& js, MuonArgs& args, int steps, hipStream_t stream) {
     for (int s = 0; s < steps; ++s) {
-        muon_product<NP, MU_GRAM, T, MOM>(js, P, s & 1, stream);
-        muon_product<NP, MU_POLY, T, MOM>(js, P, s & 1, stream);
-        if (s + 1 < steps) muon_product<NP, MU_STEP, T, MOM>(js, P, s & 1, stream);
-        else muon_product<NP, MU_LAST, T, MOM>(js, P, s & 1, stream);
+        args.cur = s & 1;
+        muon_product<NP, MU_GRAM, T, MOM>(js, args, stream);
+        muon_product<NP, MU_POLY, T, MOM>(js, args, stream);
+        if (s + 1 < steps) muon_product<NP, MU_STEP, T, MOM>(js, args, stream);
+        else muon_product<NP, MU_LAST, T, MOM>(js, args, stream);
     }
 }
 
@@ -365,19 +403,21 @@ static int muon_run(const FneusMuonJob* jobs, int n_jobs, const MuonNum& P, int 
         MuonJobs js;
         js.n = n_jobs - first < kMuonMaxJobs ? n_jobs - first : kMuonMaxJobs;       // (a local: filled anew for every round)
         js.scratch = scratch;
-        for (int q = 0; q < kMuonMaxJobs; ++q) js.first[q] = 0x7fffffff;
-        long off = 0, tiles = 0;
+        MuonArgs args;
+        args.P = P, args.cur = 0, args.scratch = scratch;
+        for (int q = 0; q < kMuonMaxJobs; ++q) args.first[q] = 0x7fffffff;
+        long off = kMuonTable, tiles = 0;
         for (int q = 0; q < js.n; ++q) {
             const FneusMuonJob& f = jobs[first + q];
             MuonJob& J = js.j[q];
             J.grad = f.grad, J.momentum = f.momentum, J.param = f.param, J.out = f.out;
-            J.rows = f.rows, J.cols = f.cols, J.adjust = f.adjust, J.off = off, js.first[q] = (int)tiles;
+            J.rows = f.rows, J.cols = f.cols, J.adjust = f.adjust, J.off = off, args.first[q] = (int)tiles;
             off += muon_lay(f.rows, f.cols, NP).total;
-            tiles += (long)((f.rows + 63) / 64) * ((f.cols + 63) / 64);
+            tiles += (long)((f.rows + 127) / 128) * ((f.cols + 127) / 128) * 4;
         }
         hipLaunchKernelGGL((muon_norm_kernel<T, MOM>), dim3((unsigned)(js.n * kMuonChunks)), dim3(256), 0, stream, js, P);
-        hipLaunchKernelGGL((muon_init_kernel<T, MOM, NP>), dim3((unsigned)tiles), dim3(256), 0, stream, js, P);
-        muon_steps<NP, T, MOM>(js, P, steps, stream);
+        hipLaunchKernelGGL((muon_init_kernel<T, MOM, NP>), dim3((unsigned)tiles), dim3(256), 0, stream, args);
+        muon_steps<NP, T, MOM>(js, args, steps, stream);
     }
     return launch_status();
 }
@@ -445,7 +485,7 @@ extern "C" long fneus_muon_scratch_bytes(const FneusMuonJob* jobs, int n_jobs, i
     long most = 0;
     if (!jobs) return 0;
     for (int first = 0; first < n_jobs; first += kMuonMaxJobs) {       // (a further round of launches uses the same memory: one stream)
-        long off = 0;
+        long off = kMuonTable;
         for (int q = first; q < n_jobs && q < first + kMuonMaxJobs; ++q)
             if (jobs[q].rows > 0 && jobs[q].cols > 0) off += muon_lay(jobs[q].rows, jobs[q].cols, prec == 3 ? 2 : 1).total;
         most = off > most ? off : most;
