@@ -415,8 +415,10 @@ __global__ void __launch_bounds__(1024) linear_fold_kernel(const float* __restri
     if (threadIdx.x < 8 && 8 * blockIdx.x + threadIdx.x < (unsigned)n) out[8 * blockIdx.x + threadIdx.x] = (T)s;
 }
 
-typedef MmCfg<64, 64, 2, 2, 4> LinSmall;          // 4 waves, 64 KiB of LDS, three stages in flight
-typedef MmCfg<128, 128, 2, 2, 2> LinMid;          // 4 waves, 64 KiB of LDS: two workgroups a CU
+typedef MmCfg<64, 64, 2, 2, 4> LinSmall;          // 4 waves, 64 KiB of LDS, three stages in flight: two workgroups a CU
+typedef MmCfg<64, 64, 2, 2, 4, 2> LinSmall8;      // 8 waves on each stage's k, 128 KiB: for a launch of no more than a workgroup a CU
+typedef MmCfg<128, 128, 2, 2, 2> LinMid;          // 4 waves, 64 KiB: two workgroups a CU
+typedef MmCfg<128, 128, 2, 2, 2, 2> LinMid8;      // 8 waves, 128 KiB: one
 typedef MmCfg<256, 256, 2, 4, 2> LinBig;          // 8 waves, 128 KiB: one
 
 // How a product runs: tile size and the parts of its contraction.  256-wide tiles where they occupy the chip; below, MEASURED (us a launch
@@ -433,8 +435,8 @@ static LinShape lin_shape(long ni, long nj, long nk) {
     else if (ni <= 64 || nj <= 64) s.tile = 64;
     else if (sizeof(T) == 2 ? t128 < 144 : t128 <= 64 && nk <= 1024) s.tile = 64;
     const long t = s.tile == 64 ? t64 : (s.tile == 128 ? t128 : t256);
-    if (t < 256 && s.tile != 256) {     // split until two workgroups a CU are there, at least 8 stages each, 2^28 partial sums at most
-        long want = (512 + t - 1) / t;
+    if (t <= 128 && s.tile != 256) {    // split to a workgroup a CU, at least 8 stages of 64 (32) k each, 2^28 partial sums at most
+        long want = 256 / t;
         const long room = (1L << 28) / (ni * nj), most = k_tiles / 8 < room ? k_tiles / 8 : room;
         if (want > most) want = most;
         if (want > 1) s.splits = (int)want;
@@ -539,23 +541,29 @@ static void lin_tiled_whole(const LinTiled& t, hipStream_t stream) {
     }
 }
 
+template <class Cfg, class T, bool AKM, bool BKM, bool FWD>
+static void lin_tiled_with(LinTiled t, long nk, hipStream_t stream) {
+    constexpr int kv = Cfg::template kv<T>();
+    t.k_tiles = (int)(nk / kv), t.tail = (int)(nk % kv);
+    if (t.splits > 1) lin_tiled_launch<Cfg, T, AKM, BKM, LIN_EPI_PART, 0>(t, stream);
+    else lin_tiled_whole<Cfg, T, AKM, BKM, FWD>(t, stream);
+}
+
 template <class T, bool AKM, bool BKM, bool FWD>
 static void lin_tiled_product(LinTiled t, const LinShape& s, long nk, float* partial, hipStream_t stream) {
-    const int b = s.tile, kv = s.tile == 256 ? LinBig::template kv<T>() : (s.tile == 128 ? LinMid::template kv<T>() : LinSmall::template kv<T>());
-    t.k_tiles = (int)(nk / kv), t.tail = (int)(nk % kv), t.splits = s.splits, t.partial = partial;
+    const int b = s.tile;
+    t.splits = s.splits, t.partial = partial;
     t.tiles_i = (int)((t.ni + b - 1) / b), t.tiles_j = (t.nj + b - 1) / b;
+    const bool few = (long)t.tiles_i * t.tiles_j * t.splits <= 256;
+    if (s.tile == 256) lin_tiled_with<LinBig, T, AKM, BKM, FWD>(t, nk, stream);
+    else if (s.tile == 128 && !few) lin_tiled_with<LinMid, T, AKM, BKM, FWD>(t, nk, stream);
+    else if (s.tile == 128) lin_tiled_with<LinMid8, T, AKM, BKM, FWD>(t, nk, stream);
+    else if (!few) lin_tiled_with<LinSmall, T, AKM, BKM, FWD>(t, nk, stream);
+    else lin_tiled_with<LinSmall8, T, AKM, BKM, FWD>(t, nk, stream);
     if (s.splits > 1) {
-        if (s.tile == 64) lin_tiled_launch<LinSmall, T, AKM, BKM, LIN_EPI_PART, 0>(t, stream);
-        else lin_tiled_launch<LinMid, T, AKM, BKM, LIN_EPI_PART, 0>(t, stream);
         const long quads = t.ni * ((t.nj + 3) / 4);
         if (s.splits >= 16) hipLaunchKernelGGL((linear_reduce_kernel<T, FWD, 8>), dim3((unsigned)((quads + 31) / 32)), dim3(256), 0, stream, t);
         else hipLaunchKernelGGL((linear_reduce_kernel<T, FWD, 1>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, stream, t);
-    } else if (s.tile == 64) {
-        lin_tiled_whole<LinSmall, T, AKM, BKM, FWD>(t, stream);
-    } else if (s.tile == 256) {
-        lin_tiled_whole<LinBig, T, AKM, BKM, FWD>(t, stream);
-    } else {
-        lin_tiled_whole<LinMid, T, AKM, BKM, FWD>(t, stream);
     }
 }
 

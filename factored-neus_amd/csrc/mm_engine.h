@@ -15,6 +15,7 @@
 // Rows beyond an operand's last are loaded as its last row (k-major: its first chunk) again: their products end in elements of D nobody
 // stores.  The last values of k, where they do not fill a stage, are brought by ordinary loads with zeros behind them.
 #pragma once
+#include <type_traits>
 #include "linear_act.h"
 
 namespace fneus {
@@ -265,7 +266,39 @@ FN_DEV void mm_run(unsigned char* smem, const MmOperand& A, const MmOperand& B, 
         if (it1 - 1 - it >= P - 1) mm_wait_barrier<(P - 1) * Cfg::DPW>();
         else mm_wait_barrier<0>();
     };
-    if constexpr (sizeof(T) == 2) {
+    if constexpr (sizeof(T) == 2 && Cfg::MI * Cfg::NJ == 1) {
+        // One accumulator a wave: its products are few and the reads' latency is what a stage takes, so a whole stage's fragments are on
+        // their way under the products of the one before.
+        LinFrag<T> fa[2][KS][Cfg::MI], fb[2][KS][Cfg::NJ];
+        auto fetch_stage = [&](int set, const unsigned char* pa) {
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) fetch(pa, ks, fa[set][ks], fb[set][ks]);
+        };
+        auto step = [&](int it, auto set_) {
+            constexpr int set = decltype(set_)::value;
+            stage = stage + 1 == Cfg::STAGES ? 0 : stage + 1;
+            if (it + 1 < it1) {
+                wait(it + 1);
+                fetch_stage(set ^ 1, smem + stage * Cfg::STAGE_BYTES);
+                if (it + 1 + P < it1) issue();
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) multiply(fa[set][ks], fb[set][ks]);
+            __builtin_amdgcn_sched_barrier(0);
+            rescale();
+        };
+        if (it0 < it1) {
+            wait(it0);
+            if (it0 + P < it1) issue();
+            fetch_stage(0, smem);
+#pragma unroll 1
+            for (int it = it0; it < it1; it += 2) {
+                step(it, std::integral_constant<int, 0>{});
+                if (it + 1 < it1) step(it + 1, std::integral_constant<int, 1>{});
+            }
+        }
+    } else if constexpr (sizeof(T) == 2) {
         // The fragments of the next 16 k are on their way from LDS while this one's are multiplied, across the stages too: the barrier that
         // frees a stage's buffer comes when its last fragments are in registers, in front of their products.
         if (it0 < it1) {

@@ -10,7 +10,6 @@
 // rounding left, times another 2^11, so that it is as normal as the first; products hi hi + hi lo + lo hi (22 bits: fp32's accuracy at
 // half the matrix work of three bf16 terms).
 #include <math.h>
-#include <stdlib.h>
 #include "mm_engine.h"
 #include "fneus_kernels.h"
 
@@ -47,7 +46,7 @@ struct MuonNum {
 // workgroup of each job (beyond the last job: none).
 struct MuonArgs {
     MuonNum P;
-    int cur;
+    int cur, total;                          // total: workgroups
     unsigned char* scratch;
     int first[kMuonMaxJobs];
 };
@@ -237,17 +236,17 @@ __global__ void __launch_bounds__(Cfg::THREADS, 2) muon_product_kernel(MuonArgs 
     extern __shared__ __attribute__((aligned(16))) unsigned char mm_smem[];
     const MuonNum& P = args.P;
     const int cur = args.cur;
-    const int q = muon_find(args, blockIdx.x);
+    const int wg = (int)mm_spread(blockIdx.x, args.total);      // (over all the matrices: a small one stays on one XCD)
+    const int q = muon_find(args, wg);
     const MuonJob J = muon_job(args, q);
     const MuonLay L = muon_lay(J.rows, J.cols, NP);
     unsigned char* S = args.scratch + J.off;
     constexpr bool SYM = KIND <= MU_POLY;
     const int ni = L.m, nj = SYM ? L.m : L.n;
     const int tiles_i = (ni + Cfg::BM - 1) / Cfg::BM, tiles_j = (nj + Cfg::BN - 1) / Cfg::BN;
-    const long tiles = SYM ? (long)tiles_i * (tiles_i + 1) / 2 : (long)tiles_i * tiles_j;
     int ti, tj;
-    const long t = mm_spread(blockIdx.x - args.first[q], tiles);
-    if constexpr (SYM) muon_upper((int)t, ti, tj);
+    const int t = wg - args.first[q];
+    if constexpr (SYM) muon_upper(t, ti, tj);
     else mm_tile(t, tiles_i, tiles_j, ti, tj);
     const long i0 = (long)ti * Cfg::BM, j0 = (long)tj * Cfg::BN;
     MmOperand A, B;
@@ -351,6 +350,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, 2) muon_product_kernel(MuonArgs 
 
 typedef MmCfg<64, 64, 2, 2, 4, 2> MuonSmall;       // 8 waves, two sharing each stage's 128 k; 128 KiB: three stages in flight
 typedef MmCfg<128, 128, 2, 2, 2> MuonMid;          // 64 KiB, two
+typedef MmCfg<128, 128, 2, 2, 2, 2> MuonMid8;      // 8 waves, 128 KiB: for no more than a workgroup a CU
 typedef MmCfg<256, 256, 2, 4, 2> MuonBig;          // 128 KiB, one
 
 static long muon_tiles(long m, long n, bool sym, int b) {
@@ -366,12 +366,13 @@ static void muon_product_launch(const MuonJobs& js, MuonArgs& args, hipStream_t 
         args.first[q] = (int)tiles;
         tiles += muon_tiles(J.rows < J.cols ? J.rows : J.cols, J.rows < J.cols ? J.cols : J.rows, KIND <= MU_POLY, Cfg::BM);
     }
+    args.total = (int)tiles;
     auto kernel = muon_product_kernel<Cfg, NP, KIND, T, MOM>;
     allow_big_lds(kernel);
     hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(Cfg::THREADS), Cfg::LDS, stream, args);
 }
 
-// the largest tile that leaves no more than a quarter of the CUs without one
+// the largest tile that still occupies the chip (256: three quarters of the CUs, 128: half of them)
 template <int NP, int KIND, class T, bool MOM>
 static void muon_product(const MuonJobs& js, MuonArgs& args, hipStream_t stream) {
     long big = 0, mid = 0;
@@ -380,9 +381,9 @@ static void muon_product(const MuonJobs& js, MuonArgs& args, hipStream_t stream)
         const long m = J.rows < J.cols ? J.rows : J.cols, n = J.rows < J.cols ? J.cols : J.rows;
         big += muon_tiles(m, n, KIND <= MU_POLY, 256), mid += muon_tiles(m, n, KIND <= MU_POLY, 128);
     }
-    static const int form = getenv("FNEUS_MUON_TILE") ? atoi(getenv("FNEUS_MUON_TILE")) : 0;
-    if (form ? form == 256 : big >= 192) muon_product_launch<MuonBig, NP, KIND, T, MOM>(js, args, stream);
-    else if (form ? form == 128 : mid >= 192) muon_product_launch<MuonMid, NP, KIND, T, MOM>(js, args, stream);
+    if (big >= 192) muon_product_launch<MuonBig, NP, KIND, T, MOM>(js, args, stream);
+    else if (mid > 256) muon_product_launch<MuonMid, NP, KIND, T, MOM>(js, args, stream);
+    else if (mid >= 128) muon_product_launch<MuonMid8, NP, KIND, T, MOM>(js, args, stream);
     else muon_product_launch<MuonSmall, NP, KIND, T, MOM>(js, args, stream);
 }
 
