@@ -18,6 +18,17 @@ template <> struct Chunk<float> { typedef f32x4_u type; static constexpr int N =
 template <> struct Chunk<__bf16> { typedef bf16x8_u type; static constexpr int N = 8; };
 template <> struct Chunk<_Float16> { typedef f16x8_u type; static constexpr int N = 8; };
 
+// N values at p of which the first `valid` (1 .. N - 1) exist: every load is made, the last value's again beyond it, so that all are in flight
+// at once (a load under a condition of its own is waited for inside it)
+template <class T, int N>
+FN_DEV void load_part(const T* p, int valid, float (&v)[N]) {
+    T q[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) q[k] = p[k < valid ? k : valid - 1];
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] = k < valid ? (float)q[k] : 0.0f;
+}
+
 // N values at p, of which the first `valid` exist (the others: 0)
 template <class T>
 FN_DEV void load_chunk(const T* p, int valid, float (&v)[Chunk<T>::N]) {
@@ -26,9 +37,11 @@ FN_DEV void load_chunk(const T* p, int valid, float (&v)[Chunk<T>::N]) {
         const typename Chunk<T>::type c = *reinterpret_cast<const typename Chunk<T>::type*>(p);
 #pragma unroll
         for (int k = 0; k < N; ++k) v[k] = (float)c[k];
+    } else if (valid > 0) {
+        load_part<T, N>(p, valid, v);
     } else {
 #pragma unroll
-        for (int k = 0; k < N; ++k) v[k] = k < valid ? (float)p[k] : 0.0f;
+        for (int k = 0; k < N; ++k) v[k] = 0.0f;
     }
 }
 
@@ -47,7 +60,7 @@ FN_DEV void store_chunk(T* p, int valid, const float (&v)[Chunk<T>::N]) {
     }
 }
 
-// four consecutive values
+// four consecutive values, valid >= 1
 template <class T> struct Quad;
 template <> struct Quad<float> { typedef float type __attribute__((ext_vector_type(4), aligned(4))); };
 template <> struct Quad<__bf16> { typedef __bf16 type __attribute__((ext_vector_type(4), aligned(2))); };
@@ -60,8 +73,7 @@ FN_DEV void quad_load(const T* p, int valid, float (&v)[4]) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) v[k] = (float)q[k];
     } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = k < valid ? (float)p[k] : 0.0f;
+        load_part<T, 4>(p, valid, v);
     }
 }
 template <class T>
