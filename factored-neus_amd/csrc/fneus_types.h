@@ -90,14 +90,32 @@ FN_DEV void quad_store(T* p, int valid, const float (&v)[4]) {
     }
 }
 
-// the same for a run of V values, V a multiple of the chunk
+// N values of a row of n >= N at column `col`, zeros beyond it, WITHOUT a branch (so that a thread's loads are all in flight at once): the 16
+// bytes that end with the row at the latest, shifted down to `col`
+template <class T>
+FN_DEV void load_row(const T* row, int col, int n, float (&v)[Chunk<T>::N]) {
+    constexpr int N = Chunk<T>::N;
+    const int start = col < n - N ? col : n - N, by = (col - start) * (int)sizeof(T) * 8;        // bits; >= 128: nothing of it exists
+    typename Chunk<T>::type c = *reinterpret_cast<const typename Chunk<T>::type*>(row + start);
+    if (n % N) {                                    // (the same for every thread)
+        u32x4 w;
+        __builtin_memcpy(&w, &c, 16);
+        const unsigned long lo = ((unsigned long)w[1] << 32) | w[0], hi = ((unsigned long)w[3] << 32) | w[2];
+        const unsigned long up = by < 64 ? hi >> (by & 63) : 0;
+        const unsigned long dn = by < 64 ? (lo >> (by & 63)) | ((hi << 1) << (63 - (by & 63))) : (by < 128 ? hi >> (by & 63) : 0);
+        w = u32x4{(unsigned)dn, (unsigned)(dn >> 32), (unsigned)up, (unsigned)(up >> 32)};
+        __builtin_memcpy(&c, &w, 16);
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] = n % N || by == 0 ? (float)c[k] : 0.0f;
+}
 template <class T, int V>
-FN_DEV void load_run(const T* p, int valid, float (&v)[V]) {
+FN_DEV void load_row_run(const T* row, int col, int n, float (&v)[V]) {
     constexpr int N = Chunk<T>::N;
 #pragma unroll
     for (int c = 0; c < V / N; ++c) {
         float q[N];
-        load_chunk<T>(p + c * N, valid - c * N, q);
+        load_row<T>(row, col + c * N, n, q);
 #pragma unroll
         for (int k = 0; k < N; ++k) v[c * N + k] = q[k];
     }

@@ -60,10 +60,10 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) layer_norm_fwd_kernel(N
     for (int c = 0; c < NC; ++c) {
         const int col = (c * TPR + t) * V;
         float q[V];
-        if (a.w) load_run<P, V>(a.w + col, a.n - col, q);
+        if (a.w) load_row_run<P, V>(a.w, col, a.n, q);
 #pragma unroll
         for (int k = 0; k < V; ++k) w[c][k] = a.w ? (P)q[k] : (P)1.0f;
-        if (a.b) load_run<P, V>(a.b + col, a.n - col, q);
+        if (a.b) load_row_run<P, V>(a.b, col, a.n, q);
 #pragma unroll
         for (int k = 0; k < V; ++k) b[c][k] = a.b ? (P)q[k] : (P)0.0f;
     }
@@ -71,13 +71,12 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) layer_norm_fwd_kernel(N
     for (long base = (long)blockIdx.x * TEAMS; base < a.rows; base += (long)gridDim.x * TEAMS) {
         const long row = base + threadIdx.x / TPR;
         const bool live = row < a.rows;              // (TPR > 64: one team, always live: every wave meets the barriers)
-        const T* __restrict__ x = a.x + row * a.ldx;
+        const T* __restrict__ x = a.x + (live ? row : 0) * a.ldx;
         float v[NC][V];
         float s = 0.0f;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            const int col = (c * TPR + t) * V;
-            load_chunk<T>(x + col, live ? a.n - col : 0, v[c]);
+            load_row<T>(x, (c * TPR + t) * V, a.n, v[c]);
         }
 #pragma unroll
         for (int c = 0; c < NC; ++c)
@@ -163,7 +162,7 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) layer_norm_bwd_kernel(N
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
         const int col = (c * TPR + t) * V;
-        if (a.w) load_run<P, V>(a.w + col, a.n - col, w[c]);
+        if (a.w) load_row_run<P, V>(a.w, col, a.n, w[c]);
 #pragma unroll
         for (int k = 0; k < V; ++k) {
             if (!a.w) w[c][k] = 1.0f;
@@ -175,15 +174,15 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) layer_norm_bwd_kernel(N
     for (long base = (long)blockIdx.x * TEAMS; base < a.rows; base += (long)gridDim.x * TEAMS) {
         const long row = base + team;
         const bool live = row < a.rows;               // (TPR > 64: one team, always live: every wave meets the barriers)
-        const T* __restrict__ x = a.x + row * a.ldx;
-        const T* __restrict__ dy = a.dy + row * a.lddy;
+        const long at = live ? row : 0;
+        const T* __restrict__ x = a.x + at * a.ldx;
+        const T* __restrict__ dy = a.dy + at * a.lddy;
         float xh[NC][V], d[NC][V];
-        const float mu = live ? a.mean[row] : 0.0f, r = live ? a.rstd[row] : 0.0f;
+        const float mu = a.mean[at], r = live ? a.rstd[at] : 0.0f;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            const int col = (c * TPR + t) * V, left = live ? a.n - col : 0;
-            load_chunk<T>(x + col, left, xh[c]);
-            load_chunk<T>(dy + col, left, d[c]);
+            load_row<T>(x, (c * TPR + t) * V, a.n, xh[c]);
+            load_row<T>(dy, (c * TPR + t) * V, a.n, d[c]);
         }
         float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
@@ -192,11 +191,12 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) layer_norm_bwd_kernel(N
 #pragma unroll
             for (int k = 0; k < V; ++k) {
                 const float h = k < left ? (xh[c][k] - mu) * r : 0.0f;
+                const float dk = k < left ? d[c][k] : 0.0f;
                 if constexpr (PARAMS) {
-                    dw[c][k] += d[c][k] * h;
-                    db[c][k] += d[c][k];
+                    dw[c][k] += dk * h;
+                    db[c][k] += dk;
                 }
-                const float g = d[c][k] * w[c][k];
+                const float g = dk * w[c][k];
                 s1 += g;
                 s2 += g * h;
                 xh[c][k] = h;
@@ -317,6 +317,7 @@ struct NormShape { int tpr, ept; };      // tpr 0: streaming
 // The narrowest team whose threads hold the row in at most 32 values each (the backward keeps five registers a value); 16 threads up to
 // 256 values (sums by DPP, four rows a wave), one wave up to 2048 (no barrier), four and eight waves up to 8192 and 16384
 static NormShape norm_shape(int n) {
+    if (n < 8) return {0, 0};             // (a chunk does not fit the row: the streaming form)
     if (n <= 256) return {16, 16};
     if (n <= 2048) return {64, 8 * ((n + 511) / 512)};
     if (n <= 8192) return {256, 8 * ((n + 2047) / 2048)};
