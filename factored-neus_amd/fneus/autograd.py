@@ -707,3 +707,60 @@ class Stage1LossFn(torch.autograd.Function):
             return tuple(ctx.saved_tensors) + (None,) * 9
         grads = torch._foreach_mul(list(ctx.saved_tensors), g)
         return tuple(grads) + (None,) * 9
+
+
+# ---- layer norm and the linear layer with a fused epilogue: any leading shape, float32 / bfloat16 / float16 ----------------------------
+class LayerNormFn(torch.autograd.Function):
+    """fneus_layer_norm_fwd / _bwd over the last axis"""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps: float):
+        x2 = x.reshape(-1, x.shape[-1])
+        y, mean, rstd = ops.layer_norm_fwd(x2, weight, bias, eps)
+        ctx.save_for_backward(x2, weight, mean, rstd)
+        ctx.shape, ctx.bias_type = x.shape, None if bias is None else bias.dtype
+        return y.reshape(x.shape)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x2, weight, mean, rstd = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx, dw, db = ops.layer_norm_bwd(dy.reshape(x2.shape), x2, weight, mean, rstd, need_params=need[1] or need[2])
+        return (dx.reshape(ctx.shape) if need[0] else None), (dw if need[1] else None), (db.to(ctx.bias_type) if need[2] else None), None
+
+
+def layer_norm(x, weight=None, bias=None, eps: float = 1e-5):
+    """(x - mean) / sqrt(var + eps) * weight + bias over the last axis of x [..., n] (ops.layer_norm_fwd / _bwd)"""
+    return LayerNormFn.apply(x, weight, bias, eps)
+
+
+class LinearFn(torch.autograd.Function):
+    """fneus_linear_fwd / _bwd: the pre-activation is kept where a gradient needs it"""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act):
+        x2, shape = x.reshape(-1, x.shape[-1]), x.shape[:-1] + weight.shape[:1]
+        if residual is not None and residual.shape != shape:
+            raise ValueError(f"linear: residual must have the output's shape {tuple(shape)}, got {tuple(residual.shape)}")
+        y, z = ops.linear_fwd(x2, weight, bias, act=act, residual=None if residual is None else residual.reshape(-1, shape[-1]),
+                              train=any(ctx.needs_input_grad[:3]))
+        ctx.save_for_backward(x2, weight, z)
+        ctx.act, ctx.x_shape = act, x.shape
+        return y.reshape(shape)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x2, weight, z = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx = dw = db = None
+        if any(need[:3]):
+            dx, dw, db = ops.linear_bwd(dy.reshape(-1, weight.shape[0]), x2, weight, z, act=ctx.act, need=need[:3])
+        return (None if dx is None else dx.reshape(ctx.x_shape)), dw, db, (dy if need[3] else None), None
+
+
+def linear(x, weight, bias=None, act="none", residual=None):
+    """act(x weight^T + bias) + residual for x [..., n_in], weight [n_out, n_in], residual of the output's shape; act: a key of
+    ops.LINEAR_ACTS (ops.linear_fwd / _bwd)"""
+    return LinearFn.apply(x, weight, bias, residual, act)

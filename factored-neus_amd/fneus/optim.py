@@ -153,3 +153,115 @@ class FlatAdam(torch.optim.Adam):
     @property
     def n_segments(self):
         return 0 if self._segs is None else len(self._segs)
+
+
+class FlatMuon(torch.optim.Optimizer):
+    """Muon for a model's weight matrices, FlatAdam for everything else, one learning rate for both (adjust="match_rms" gives a matrix's
+    update Adam's rms).  Every matrix of the model takes part in the same launches of fneus_muon (momentum, Newton-Schulz
+    orthogonalisation, step); learning rate and step count are device scalars, gradients are cleared by the kernels: capturable in a
+    hipGraph like FlatAdam, with its methods (set_lr, state_dict / load_state_dict).
+
+    params: parameters; the 2-D ones with no side shorter than `min_side` are Muon's (a layer with a handful of outputs has no spectrum to
+    level), the others Adam's.  State: `momentum_buffer` a matrix, torch.optim.Adam's of the others.  A parameter without a gradient is
+    skipped."""
+
+    def __init__(self, params, lr=1e-3, momentum=0.95, nesterov=True, weight_decay=0.0, adjust="match_rms", coefficients=None, steps=5,
+                 eps=1e-7, prec=None, betas=(0.9, 0.999), adam_eps=1e-8, min_side=32):
+        from . import ops
+        if not 0.0 <= momentum < 1.0 or steps < 1 or eps <= 0.0 or weight_decay < 0.0:
+            raise ValueError("FlatMuon: 0 <= momentum < 1, steps >= 1, eps > 0, weight_decay >= 0")
+        ops.muon_adjust(adjust, 1, 1)
+        super().__init__(params, dict(lr=float(lr), momentum=float(momentum), nesterov=bool(nesterov), weight_decay=float(weight_decay),
+                                      adjust=adjust, coefficients=tuple(coefficients or ops.NS_COEFFICIENTS), steps=int(steps), eps=float(eps)))
+        if len(self.param_groups) != 1:
+            raise NotImplementedError("FlatMuon supports a single parameter group")
+        ps = self.param_groups[0]["params"]
+        self.prec = prec
+        self.matrices = [p for p in ps if p.dim() == 2 and min(p.shape) >= min_side]
+        rest = [p for p in ps if not (p.dim() == 2 and min(p.shape) >= min_side)]
+        self.adam = FlatAdam(rest, lr=lr, betas=betas, eps=adam_eps) if rest else None
+        self._table = self._keys = self._lr_dev = self._lr_host = None
+
+    def set_lr(self, lr: float):
+        self.param_groups[0]["lr"] = float(lr)
+        if self.adam is not None:
+            self.adam.set_lr(lr)
+        if self._lr_dev is not None:
+            self._lr_dev.fill_(float(lr))
+            self._lr_host = float(lr)
+
+    def _live(self):
+        return [p for p in self.matrices if p.requires_grad and p.grad is not None]
+
+    def _build(self, ps):
+        from . import ops
+        for p in ps:
+            st = self.state[p]
+            if "momentum_buffer" not in st:
+                st["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
+        self._table = ops.muon_jobs([p.detach() for p in ps], [p.grad for p in ps], [self.state[p]["momentum_buffer"] for p in ps],
+                                    self.param_groups[0]["adjust"])
+        self._keys = [(p.data_ptr(), p.grad.data_ptr(), self.state[p]["momentum_buffer"].data_ptr()) for p in ps]
+        if self._lr_dev is None or self._lr_dev.device != ps[0].device:
+            self._lr_host = float(self.param_groups[0]["lr"])
+            self._lr_dev = torch.full((), self._lr_host, dtype=torch.float32, device=ps[0].device)
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        if closure is not None:
+            raise NotImplementedError("FlatMuon.step() takes no closure")
+        from . import ops
+        g = self.param_groups[0]
+        ps = self._live()
+        if self.adam is not None:
+            if self.adam.param_groups[0]["lr"] != g["lr"]:       # someone assigned param_groups[0]["lr"] directly
+                self.adam.set_lr(g["lr"])
+            if self.adam._params():
+                self.adam.step()
+        if not ps:
+            return
+        if self._keys != [(p.data_ptr(), p.grad.data_ptr(), self.state[p]["momentum_buffer"].data_ptr() if "momentum_buffer" in self.state[p] else 0)
+                          for p in ps]:
+            self._build(ps)
+        if float(g["lr"]) != self._lr_host:
+            self._lr_dev.fill_(float(g["lr"]))
+            self._lr_host = float(g["lr"])
+        ops.muon_launch(self._table, self._lr_dev, g["momentum"], g["nesterov"], g["weight_decay"], g["coefficients"], g["steps"], g["eps"],
+                        self.prec, True)
+
+    def state_dict(self):
+        if self.adam is not None:
+            for p in self.adam.param_groups[0]["params"]:
+                if p in self.adam.state:
+                    self.state[p] = dict(self.adam.state[p])
+        sd = super().state_dict()
+        for st in sd["state"].values():
+            if torch.is_tensor(st.get("step")):
+                st["step"] = st["step"].detach().clone().cpu()
+        return sd
+
+    def load_state_dict(self, state_dict):
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        ps = self.param_groups[0]["params"]
+        if len(ids) != len(ps):
+            raise ValueError(f"optimizer state_dict holds {len(ids)} parameters, this optimiser {len(ps)}")
+        muon = set(map(id, self.matrices))
+        for i, p in zip(ids, ps):
+            st = state_dict["state"].get(i)
+            key = "momentum_buffer" if id(p) in muon else "exp_avg"
+            if st is not None and (not torch.is_tensor(st.get(key)) or tuple(st[key].shape) != tuple(p.shape)):
+                raise ValueError(f"optimizer state of parameter {i} holds no {key} of shape {tuple(p.shape)}: another optimiser's, or another order")
+        super().load_state_dict(state_dict)
+        for p in ps:
+            st = self.state.get(p)
+            if st:
+                for k, v in st.items():
+                    if torch.is_tensor(v):
+                        st[k] = v.clone()              # (torch shares tensors with the dict it is given)
+        if self.adam is not None:
+            for p in self.adam.param_groups[0]["params"]:
+                if p in self.state:
+                    self.adam.state[p] = dict(self.state[p])
+            self.adam._segs = None
+        self._table = self._keys = None
+        self.set_lr(float(self.param_groups[0]["lr"]))

@@ -43,7 +43,8 @@ def stage2_loss(out: dict, reduce=None):
 class Stage2Trainer:
     def __init__(self, device, model_conf: Optional[dict] = None, prec: int = ops.PREC_PARITY, lr: float = 5e-4, seed: int = 0,
                  synthetic_init: bool = True, sdf_kwargs: Optional[dict] = None, use_graph: bool = False,
-                 distributed: bool = False):
+                 distributed: bool = False, optimizer: str = "adam"):
+        """optimizer: "adam" (the reference's) or "muon" (fneus/optim.py FlatMuon); model_conf["indirect_light"]: IndirectLight's arguments"""
         from models.fields import SDFNetwork, RenderingNetwork, SingleVarianceNetwork, RefColor, Lvis, IndirectLight
         from models.renderer import NeuSRenderer
         conf = model_conf or dict(WMASK_MODEL, lvis_renderer=LVIS_RENDERER)
@@ -52,14 +53,15 @@ class Stage2Trainer:
         self.color_network = RenderingNetwork(**conf["rendering_network"])
         self.deviation_network = SingleVarianceNetwork(**conf["variance_network"])
         self.refColor_network = RefColor()
-        self.lvis_network, self.indiLgt_network = Lvis(), IndirectLight()
+        self.lvis_network, self.indiLgt_network = Lvis(), IndirectLight(**conf.get("indirect_light", {}))
         if synthetic_init:
             T = lambda sd: {k: torch.from_numpy(v) for k, v in sd.items()}
             self.sdf_network.load_state_dict(T(synth.sdf_state_dict(seed, **(sdf_kwargs or {}))))
             self.color_network.load_state_dict(T(synth.color_state_dict(seed + 1)))
             self.refColor_network.load_state_dict(T(synth.refcolor_state_dict(seed + 2)))
             self.lvis_network.load_state_dict(T(synth.lvis_state_dict(seed + 4)))
-            self.indiLgt_network.load_state_dict(T(synth.indilgt_state_dict(seed + 5)))
+            if not conf.get("indirect_light", {}).get("residual", False):
+                self.indiLgt_network.load_state_dict(T(synth.indilgt_state_dict(seed + 5)))
         self.frozen = [self.sdf_network, self.deviation_network, self.color_network, self.refColor_network]
         for m in self.frozen + [self.lvis_network, self.indiLgt_network]:
             m.to(device)
@@ -70,7 +72,7 @@ class Stage2Trainer:
         self.color_network.set_precision(prec)
         # lvis.py:89-92
         self.params = list(self.lvis_network.parameters()) + list(self.indiLgt_network.parameters())
-        self._init_step_mode(use_graph, lr, distributed)
+        self._init_step_mode(use_graph, lr, distributed, optimizer)
         self.renderer = NeuSRenderer(**conf.get("lvis_renderer", LVIS_RENDERER), sdf_network=self.sdf_network,
                                      deviation_network=self.deviation_network, color_network=self.color_network,
                                      lvis_network=self.lvis_network, indiLgt_network=self.indiLgt_network)
@@ -87,7 +89,7 @@ class Stage2Trainer:
     # chain of hipGraphs cut at the collectives) with two exchanges -- the loss normalisers (hit count; stage 3: mask sum and the latent-sparsity statistics) summed over
     # the ranks BEFORE the loss, so that R ranks x B rays equal one R*B-ray batch, and ONE in-place all-reduce of the flat
     # gradient buffer all trained parameters' .grad are views of.  Every rank runs both every step (no data-dependent skip).
-    def _init_step_mode(self, use_graph: bool, lr: float, distributed: bool = False):
+    def _init_step_mode(self, use_graph: bool, lr: float, distributed: bool = False, optimizer: str = "adam"):
         import os
         from fneus.seggraph import SegmentedStep
         # (the distilled MLPs of stages 2 / 3 run on the fneus_mlp_* kernels since round 5 -- models/fields.py seq_group: there is no
@@ -122,7 +124,15 @@ class Stage2Trainer:
         # step counter and learning rate (graph-capturable), gradients cleared by the kernel.  MEASURED: torch's own step costs
         # 0.73 ms of GPU time per eager stage-2 step (20 tensors x its element-wise kernels), 0.5 ms inside the replayed graph.
         # FNEUS_STAGE_ADAM=torch keeps torch.optim.Adam.
-        if self.flat_adam:
+        # optimizer "muon": FlatMuon (the same file), the layers' matrices orthogonalised, the rest on FlatAdam; the same contract
+        if optimizer not in ("adam", "muon"):
+            raise ValueError(f"optimizer must be 'adam' or 'muon', got {optimizer!r}")
+        if optimizer == "muon":
+            if not self.flat_adam:
+                raise RuntimeError("optimizer 'muon' needs a GPU and the flat gradient buffers (FNEUS_STAGE_ADAM=flat)")
+            from fneus.optim import FlatMuon
+            self.optimizer = FlatMuon(self.params, lr=lr)
+        elif self.flat_adam:
             from fneus.optim import FlatAdam
             self.optimizer = FlatAdam(self.params, lr=lr)
         elif self.use_graph:      # a device-scalar learning rate: schedule updates reach the replayed optimiser step

@@ -37,7 +37,8 @@ def stage3_loss(out: dict, true_rgb, mask, reduce=None):
 
 class Stage3Trainer:
     def __init__(self, device, model_conf: Optional[dict] = None, prec: int = ops.PREC_PARITY, lr: float = 5e-4, seed: int = 0,
-                 synthetic_init: bool = True, mask_weight: float = 0.1, use_graph: bool = False, distributed: bool = False):
+                 synthetic_init: bool = True, mask_weight: float = 0.1, use_graph: bool = False, distributed: bool = False,
+                 optimizer: str = "adam"):
         from models.fields import SDFNetwork, SingleVarianceNetwork, RefColor, Lvis, IndirectLight
         from models.inverRender import EnvmapMaterialNetwork
         from models.renderer import NeuSRenderer
@@ -46,7 +47,7 @@ class Stage3Trainer:
         self.sdf_network = SDFNetwork(**conf["sdf_network"])
         self.deviation_network = SingleVarianceNetwork(**conf["variance_network"])
         self.refColor_network = RefColor()
-        self.lvis_network, self.indiLgt_network = Lvis(), IndirectLight()
+        self.lvis_network, self.indiLgt_network = Lvis(), IndirectLight(**conf.get("indirect_light", {}))
         torch.manual_seed(seed)
         self.mateIllu_network = EnvmapMaterialNetwork()
         if synthetic_init:
@@ -54,7 +55,8 @@ class Stage3Trainer:
             self.sdf_network.load_state_dict(T(synth.sdf_state_dict(seed)))
             self.refColor_network.load_state_dict(T(synth.refcolor_state_dict(seed + 2)))
             self.lvis_network.load_state_dict(T(synth.lvis_state_dict(seed + 4)))
-            self.indiLgt_network.load_state_dict(T(synth.indilgt_state_dict(seed + 5)))
+            if not conf.get("indirect_light", {}).get("residual", False):
+                self.indiLgt_network.load_state_dict(T(synth.indilgt_state_dict(seed + 5)))
             self.mateIllu_network.load_state_dict(T(synth.mateillu_state_dict(seed + 6)))
         self.frozen = [self.sdf_network, self.deviation_network, self.refColor_network, self.lvis_network, self.indiLgt_network]
         for m in self.frozen + [self.mateIllu_network]:
@@ -65,7 +67,7 @@ class Stage3Trainer:
         self.sdf_network.set_precision(prec)
         self.refColor_network.set_precision(prec)
         self.params = list(self.mateIllu_network.parameters())          # mateIllu.py:91-95
-        self._init_step_mode(use_graph, lr, distributed)
+        self._init_step_mode(use_graph, lr, distributed, optimizer)
         import os
         if self.grads is not None and os.environ.get("FNEUS_DIRECT_GRADS", "1") != "0":
             self._direct_modules = [self.mateIllu_network]      # its three MLPs: dW / db straight into the gradient arena

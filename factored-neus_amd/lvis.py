@@ -57,8 +57,11 @@ class Runner:
         self.learning_rate, self.learning_rate_alpha = tc.get_float("learning_rate"), tc.get_float("learning_rate_alpha")
         model_conf = {k: dict(self.conf["model"][k]) for k in ("sdf_network", "variance_network", "rendering_network",
                                                                 "lvis_renderer")}
+        if "indirect_light" in self.conf["model"]:           # { residual = True }: IndirectLight on residual layers
+            model_conf["indirect_light"] = dict(self.conf["model"]["indirect_light"])
         self.trainer = Stage2Trainer(self.device, model_conf=model_conf, prec=prec, lr=self.learning_rate, synthetic_init=False,
-                                     use_graph=use_graph, distributed=distributed)
+                                     use_graph=use_graph, distributed=distributed,
+                                     optimizer=tc.get_string("optimizer", "adam"))          # adam | muon
         self.rank = rank
         self.iter_step = 0
         geo = _latest(os.path.join(self.base_exp_dir_geometry, "checkpoints"), tc.get_int("end_iter"))

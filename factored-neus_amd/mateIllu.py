@@ -57,8 +57,11 @@ class Runner:
         self.warm_up_end = tc.get_float("warm_up_end", 0.0)
         self.mask_weight = tc.get_float("mask_weight")
         model_conf = {k: dict(self.conf["model"][k]) for k in ("sdf_network", "variance_network", "neus_renderer")}
+        if "indirect_light" in self.conf["model"]:           # as stage 2 trained it
+            model_conf["indirect_light"] = dict(self.conf["model"]["indirect_light"])
         self.trainer = Stage3Trainer(self.device, model_conf=model_conf, prec=prec, lr=self.learning_rate, synthetic_init=False,
-                                     mask_weight=self.mask_weight, use_graph=use_graph, distributed=distributed)
+                                     mask_weight=self.mask_weight, use_graph=use_graph, distributed=distributed,
+                                     optimizer=tc.get_string("optimizer", "adam"))          # adam | muon
         self.rank = rank
         self.iter_step = 0
         prev = _latest(os.path.join(self.base_exp_dir_lvis, "checkpoints"), tc.get_int("lvis.end_iter"))

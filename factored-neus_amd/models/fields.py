@@ -821,6 +821,44 @@ class Lvis(nn.Module):
         return out
 
 
+class ActLinear(nn.Module):
+    """act(x W^T + b) in one launch each way (fneus_linear_fwd / _bwd); nn.Linear's parameters, names and initialisation"""
+
+    def __init__(self, n_in: int, n_out: int, act: str = "none"):
+        super().__init__()
+        lin = nn.Linear(n_in, n_out)
+        self.weight, self.bias, self.act = lin.weight, lin.bias, act
+
+    def forward(self, x):
+        if not x.is_cuda:
+            return _LINEAR_ACTS[self.act](nn.functional.linear(x, self.weight, self.bias))
+        from fneus import autograd
+        return autograd.linear(x, self.weight, self.bias, act=self.act)
+
+
+_LINEAR_ACTS = {"none": lambda z: z, "relu": torch.relu, "leaky": lambda z: nn.functional.leaky_relu(z, 0.2), "sigmoid": torch.sigmoid,
+                "softplus": lambda z: nn.functional.softplus(z, beta=100), "gelu": nn.functional.gelu, "silu": nn.functional.silu}
+
+
+class ResidualLayer(nn.Module):
+    """x + act(LayerNorm(x) W^T + b): two launches forward (fneus_layer_norm_fwd, fneus_linear_fwd with the residual in its epilogue), their
+    backward passes backward"""
+
+    def __init__(self, width: int, act: str = "relu", eps: float = 1e-5):
+        super().__init__()
+        lin = nn.Linear(width, width)
+        self.weight, self.bias, self.act, self.eps = lin.weight, lin.bias, act, eps
+        self.norm_weight, self.norm_bias = nn.Parameter(torch.ones(width)), nn.Parameter(torch.zeros(width))
+
+    def forward(self, x):
+        if not x.is_cuda:
+            h = nn.functional.layer_norm(x, x.shape[-1:], self.norm_weight, self.norm_bias, self.eps)
+            return x + _LINEAR_ACTS[self.act](nn.functional.linear(h, self.weight, self.bias))
+        from fneus import autograd
+        h = autograd.layer_norm(x, self.norm_weight, self.norm_bias, self.eps)
+        return autograd.linear(h, self.weight, self.bias, act=self.act, residual=x)
+
+
 class DeferredIndirectLight:
     """IndirectLight(pts) that has not run yet (IndirectLight.deferred)"""
 
@@ -834,15 +872,19 @@ class DeferredIndirectLight:
 
 class IndirectLight(nn.Module):
     """Stage-2 indirect light as 24 spherical Gaussians per point (fields.py:372-413): 63 -> 512 x 4 -> 144 -> [n, 24, 7] =
-    (lobe axis from two sigmoid angles, sharpness 30 sigmoid + 0.1, relu amplitude x 3).  state_dict keys `indi.{0,..,8}`."""
+    (lobe axis from two sigmoid angles, sharpness 30 sigmoid + 0.1, relu amplitude x 3).  state_dict keys `indi.{0,..,8}`.
+    residual (conf model.indirect_light; not in the reference): the three hidden 512 -> 512 layers as ResidualLayer -- a trunk whose
+    gradient reaches the first layer unattenuated; state_dict keys `indi.{0,..,4}`."""
 
-    def __init__(self, num_lgt_sgs=24):
+    def __init__(self, num_lgt_sgs=24, residual: bool = False):
         super().__init__()
         self.num_lgt_sgs = num_lgt_sgs
         self.embedview_fn_view, _ = get_embedder(4)
         self.embedview_fn_pts, ch_pts = get_embedder(10)
         self.indi = nn.Sequential(nn.Linear(ch_pts, 512), nn.ReLU(), nn.Linear(512, 512), nn.ReLU(), nn.Linear(512, 512),
                                   nn.ReLU(), nn.Linear(512, 512), nn.ReLU(), nn.Linear(512, num_lgt_sgs * 6))
+        if residual:
+            self.indi = nn.Sequential(ActLinear(ch_pts, 512, "relu"), *(ResidualLayer(512) for _ in range(3)), ActLinear(512, num_lgt_sgs * 6))
 
     def radiance(self, pts, sample_dirs):
         """query_indir_illum(self(pts), sample_dirs) (calLvis.py:323-336) [n, S, 3] without materialising the lobes: the output

@@ -1,0 +1,286 @@
+"""Layer norm, the linear layer and Muon together, as a model and its trainer use them: models.fields.ResidualLayer / IndirectLight(residual=True)
+and fneus.optim.FlatMuon against the same network and the same optimiser in float64, the stage-2 / 3 trainers with optimizer="muon".
+
+Tolerances.  Gradients of the five-layer trunk in fp32: each layer adds about sqrt(512) 2^-24 = 1.3e-6 of its scale, ten products deep: 1e-4 of a
+tensor's largest value is the bound (a ReLU whose pre-activation lies within that of 0 would break it: the inputs are smooth activations).
+A Muon step in the float64 reference starts from the kernels' own gradients, so that the optimiser alone is compared: 1e-5 of the update
+(test_hip_muon.py), Adam 1e-5."""
+import os
+import sys
+
+import pytest
+import torch
+import torch.nn as nn
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+sys.path.insert(0, os.path.join(ROOT, "factored-neus_amd"))
+sys.path.insert(0, os.path.join(ROOT, "tests"))
+
+
+def trunk(width=64, n_in=39, n_out=36, act="silu", seed=0):
+    from models.fields import ActLinear, ResidualLayer
+    torch.manual_seed(seed)
+    net = nn.Sequential(ActLinear(n_in, width, act), *(ResidualLayer(width, act) for _ in range(3)), ActLinear(width, n_out))
+    with torch.no_grad():
+        for m in net:
+            if hasattr(m, "norm_weight"):
+                m.norm_weight.add_(0.2 * torch.randn(width))
+                m.norm_bias.add_(0.2 * torch.randn(width))
+    return net
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("width,rows", [(64, 5), (64, 300), (512, 512), (256, 4096)])
+def test_trunk_against_float64(width, rows):
+    net = trunk(width)
+    ref = trunk(width).double()                       # (on the CPU the modules run torch's own operators)
+    g = torch.Generator().manual_seed(3)
+    x, cot = torch.randn(rows, 39, generator=g), torch.randn(rows, 36, generator=g)
+    xr = x.double().requires_grad_(True)
+    yr = ref(xr)
+    (yr * cot.double()).sum().backward()
+    net = net.cuda()
+    xg = x.cuda().requires_grad_(True)
+    y = net(xg)
+    (y * cot.cuda()).sum().backward()
+    for got, want, name in [(y, yr, "y"), (xg.grad, xr.grad, "dx")] + [(p.grad, q.grad, n) for (n, p), q in zip(net.named_parameters(), ref.parameters())]:
+        err = float((got.detach().double().cpu() - want.detach()).abs().max()) / float(want.detach().abs().max())
+        assert err <= 1e-4, (name, err)
+
+
+@pytest.mark.gpu
+def test_trunk_shapes_frozen_and_partial_gradients():
+    from fneus import autograd
+    net = trunk().cuda()
+    x = torch.randn(4, 3, 39, device="cuda")
+    y = net(x)
+    assert y.shape == (4, 3, 36) and torch.equal(y.reshape(12, 36), net(x.reshape(12, 39)))
+    assert net(x[:0]).shape == (0, 3, 36)
+    net(x[:0]).sum().backward()
+    assert all(float(p.grad.abs().max()) == 0.0 for n, p in net.named_parameters() if "norm" not in n)
+    for p in net.parameters():
+        p.requires_grad_(False)
+        p.grad = None
+    assert not net(x).requires_grad
+    xg = x.clone().requires_grad_(True)
+    net(xg).sum().backward()
+    full = xg.grad.clone()
+    assert all(p.grad is None for p in net.parameters())
+    net[2].weight.requires_grad_(True)
+    xg.grad = None
+    net(xg).sum().backward()
+    assert torch.equal(xg.grad, full) and net[2].weight.grad is not None and net[2].bias.grad is None
+    with pytest.raises(ValueError):
+        autograd.linear(x, torch.randn(5, 39, device="cuda"), residual=torch.randn(5, device="cuda"))
+    w, b = torch.ones(39, device="cuda"), torch.zeros(39, device="cuda", requires_grad=True)
+    for args in ((None, None), (w, None), (None, b), (w.requires_grad_(True), b)):
+        xg = x.clone().requires_grad_(True)
+        autograd.layer_norm(xg, *args).square().sum().backward()
+        xr = x.detach().clone().requires_grad_(True)
+        nn.functional.layer_norm(xr, (39,), *[None if a is None else a.detach() for a in args]).square().sum().backward()
+        assert float((xg.grad - xr.grad).abs().max()) <= 2e-5
+    # gradients of gradients are refused, not wrong
+    xg = x.clone().requires_grad_(True)
+    (gx,) = torch.autograd.grad(autograd.layer_norm(xg, w).sum(), xg, create_graph=True)
+    with pytest.raises(RuntimeError):
+        gx.sum().backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [torch.bfloat16, torch.float16])
+def test_trunk_sixteen_bits(t):
+    """16-bit modules: forward and gradients within a few roundings (a half step each, 12 in a row, doubled) of float64 at the same weights"""
+    net = trunk(128).to(t)
+    ref = trunk(128).to(t).double()
+    x, cot = torch.randn(200, 39).to(t), torch.randn(200, 36).to(t)
+    yr = ref(x.double())
+    (yr * cot.double()).sum().backward()
+    net = net.cuda()
+    y = net(x.cuda())
+    (y * cot.cuda()).sum().backward()
+    lim = 24 * torch.finfo(t).eps / 2
+    for got, want, name in [(y, yr, "y")] + [(p.grad, q.grad, n) for (n, p), q in zip(net.named_parameters(), ref.parameters())]:
+        err = float((got.detach().double().cpu() - want.detach()).norm() / want.detach().norm())
+        assert err <= lim, (name, err)
+
+
+def muon64(p, g, m, lr, mu=0.95):
+    from test_hip_muon import ns64
+    m = mu * m + (1 - mu) * g
+    return p - lr * 0.2 * max(p.shape) ** 0.5 * ns64((1 - mu) * g + mu * m), m
+
+
+@pytest.mark.gpu
+def test_flat_muon_steps_against_float64():
+    from fneus.optim import FlatMuon
+    net = trunk().cuda()
+    opt = FlatMuon(net.parameters(), lr=3e-3)
+    names = {p: n for n, p in net.named_parameters()}
+    assert [names[p] for p in opt.matrices] == ["0.weight", "1.weight", "2.weight", "3.weight", "4.weight"]
+    for p in net.parameters():
+        p.grad = torch.zeros_like(p)
+    x, cot = torch.randn(80, 39, device="cuda"), torch.randn(80, 36, device="cuda")
+    mom = {p: torch.zeros_like(p, dtype=torch.float64) for p in opt.matrices}
+    adam = {p: (torch.zeros_like(p, dtype=torch.float64), torch.zeros_like(p, dtype=torch.float64)) for p in net.parameters() if p not in mom}
+    for step in range(1, 4):
+        lr = 3e-3 / step
+        opt.set_lr(lr)
+        (net(x) * cot).sum().backward()
+        before = {p: (p.detach().double().clone(), p.grad.double().clone()) for p in net.parameters()}
+        opt.step()
+        for p, (old, g) in before.items():
+            assert float(p.grad.abs().max()) == 0.0                          # cleared by the kernels
+            if p in mom:
+                want, m = muon64(old.cpu(), g.cpu(), mom[p].cpu(), lr)
+                mom[p] = m.cuda()
+                want = want.cuda()
+            else:
+                m, v = adam[p]
+                m, v = 0.9 * m + 0.1 * g, 0.999 * v + 0.001 * g * g
+                adam[p] = (m, v)
+                want = old - lr * (m / (1 - 0.9 ** step)) / ((v / (1 - 0.999 ** step)).sqrt() + 1e-8)
+            moved, err = float((want - old).norm()), float((p.detach().double() - want).norm())
+            assert err <= 2e-5 * moved + 2.0 ** -23 * float(want.norm()), (names[p], step, err, moved)
+
+
+@pytest.mark.gpu
+def test_flat_muon_state_dict_and_graph():
+    """a run that is saved, loaded into a fresh optimiser and continued equals the run that went on; a captured step equals the eager one"""
+    import io
+    from fneus.optim import FlatMuon
+    x, cot = torch.randn(80, 39, device="cuda"), torch.randn(80, 36, device="cuda")
+
+    def make():
+        net = trunk().cuda()
+        for p in net.parameters():
+            p.grad = torch.zeros_like(p)
+        return net, FlatMuon(net.parameters(), lr=2e-3)
+
+    def step(net, opt):
+        (net(x) * cot).sum().backward()
+        opt.step()
+
+    a, oa = make()
+    for _ in range(2):
+        step(a, oa)
+    buf = io.BytesIO()
+    torch.save({"net": a.state_dict(), "opt": oa.state_dict()}, buf)
+    buf.seek(0)
+    ck = torch.load(buf, map_location="cuda")
+    b, ob = make()
+    b.load_state_dict(ck["net"])
+    ob.load_state_dict(ck["opt"])
+    for _ in range(2):
+        step(a, oa), step(b, ob)
+    assert all(torch.equal(p, q) for p, q in zip(a.parameters(), b.parameters()))
+    with pytest.raises(ValueError):
+        ob.load_state_dict({"state": {0: {"exp_avg": torch.zeros(64, 39)}}, "param_groups": ck["opt"]["param_groups"]})
+    # capture on b, eager on a
+    import gc
+    gc.collect()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(b, ob)
+    torch.cuda.current_stream().wait_stream(side)
+    step(a, oa)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(b, ob)
+    for k in range(3):
+        oa.set_lr(1e-3 / (k + 1)), ob.set_lr(1e-3 / (k + 1))
+        x.copy_(torch.randn_like(x))
+        graph.replay()
+        torch.cuda.synchronize()
+        step(a, oa)
+        assert all(torch.equal(p, q) for p, q in zip(a.parameters(), b.parameters())), k
+
+
+@pytest.mark.gpu
+def test_flat_muon_skips_and_follows():
+    """a parameter without a gradient is left alone; re-attached gradients and an assigned learning rate are followed"""
+    from fneus.optim import FlatMuon
+    p, q, r = (nn.Parameter(torch.randn(40, 50, device="cuda")) for _ in range(3))
+    opt = FlatMuon([p, q, r], lr=1e-2)
+    opt.step()                                                        # no gradient at all: nothing to do
+    p.grad, q.grad = torch.randn_like(p), torch.randn_like(q)
+    keep = r.detach().clone()
+    old = p.detach().clone()
+    opt.step()
+    assert torch.equal(r, keep) and not torch.equal(p, old)
+    opt.param_groups[0]["lr"] = 0.0
+    p.grad = torch.randn_like(p)                                      # another buffer
+    old = p.detach().clone()
+    opt.step()
+    assert torch.equal(p, old) and float(p.grad.abs().max()) == 0.0
+
+
+def test_flat_muon_refusals_cpu():
+    from fneus.optim import FlatMuon
+    p = nn.Parameter(torch.randn(40, 50))
+    for bad in (dict(momentum=1.0), dict(steps=0), dict(eps=0.0), dict(adjust="other"), dict(weight_decay=-1.0)):
+        with pytest.raises(ValueError):
+            FlatMuon([p], **bad)
+    with pytest.raises(NotImplementedError):
+        FlatMuon([{"params": [p]}, {"params": [nn.Parameter(torch.randn(3))]}])
+    opt = FlatMuon([p, nn.Parameter(torch.randn(3)), nn.Parameter(torch.randn(50, 4))])
+    assert opt.matrices == [p] and len(opt.adam.param_groups[0]["params"]) == 2
+    p.grad = torch.randn_like(p)
+    with pytest.raises(ValueError):
+        opt.step()                                                    # no CPU fallback
+    with pytest.raises(NotImplementedError):
+        opt.step(lambda: None)
+
+
+def test_indirect_light_residual_cpu():
+    from models.fields import IndirectLight, _mlp_spec
+    net = IndirectLight(residual=True)
+    assert _mlp_spec(net.indi) is None and _mlp_spec(IndirectLight().indi) is not None
+    out = net(torch.randn(6, 3))
+    assert out.shape == (6, 24, 7)
+    out.sum().backward()
+    assert all(p.grad is not None for p in net.parameters())
+    assert sorted({k.rsplit(".", 1)[0] for k in net.state_dict()}) == ["indi.0", "indi.1", "indi.2", "indi.3", "indi.4"]
+
+
+def test_conf_selects_muon_and_residual():
+    from fneus import hocon
+    text = open(os.path.join(ROOT, "factored-neus_amd", "confs", "wmask.conf")).read()
+    conf = hocon.parse_string(text.replace("train {", "train {\n    optimizer = muon", 1).replace("model {", "model {\n    indirect_light { residual = True }", 1))
+    assert conf["train"].get_string("optimizer", "adam") == "muon" and dict(conf["model"]["indirect_light"]) == {"residual": True}
+    conf = hocon.parse_string(text)
+    assert conf["train"].get_string("optimizer", "adam") == "adam" and "indirect_light" not in conf["model"]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("use_graph", [False, True])
+@pytest.mark.parametrize("stage", [2, 3])
+def test_stage_trainers_with_muon_and_residual_trunk(stage, use_graph):
+    from fneus import synth
+    from fneus.trainer import WMASK_MODEL
+    from fneus.trainer2 import LVIS_RENDERER, Stage2Trainer
+    from fneus.trainer3 import Stage3Trainer
+    dev = torch.device("cuda:0")
+    conf = dict(WMASK_MODEL, indirect_light=dict(residual=True))
+    small = dict(n_samples=16, n_importance=16, n_outside=0, up_sample_steps=4, perturb=1.0)
+    if stage == 2:
+        tr = Stage2Trainer(dev, model_conf=dict(conf, lvis_renderer=dict(LVIS_RENDERER, **small)), seed=5, use_graph=use_graph, optimizer="muon")
+    else:
+        tr = Stage3Trainer(dev, model_conf=dict(conf, neus_renderer=small), seed=5, use_graph=use_graph, optimizer="muon")
+    data = torch.from_numpy(synth.ray_batch(32, seed=5, n_miss=2)).to(dev)
+    before = [p.detach().clone() for p in tr.params]
+    for _ in range(5):
+        out = tr.train_step(data)
+        assert out is not None and bool(torch.isfinite(out["loss"]))
+    assert tr.graph_error is None
+    moved = [not torch.equal(p, q) for p, q in zip(tr.params, before)]
+    assert len(tr.optimizer.matrices) > 0 and sum(moved) >= 0.9 * len(moved)
+    assert all(bool(torch.isfinite(p).all()) for p in tr.params)
+    sd = tr.optimizer_state_dict()
+    tr.load_optimizer_state_dict(sd)
+    tr.set_lr(1e-4)
+    assert tr.get_lr() == 1e-4
+    assert tr.train_step(data) is not None
+    with pytest.raises(ValueError):
+        (Stage2Trainer if stage == 2 else Stage3Trainer)(dev, optimizer="sgd")
