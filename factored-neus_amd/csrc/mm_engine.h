@@ -164,8 +164,8 @@ struct MmReader {
 };
 
 // steps [it0, it1) of the concatenated segments, `k_tiles` full stages each; tail: values of k behind the last full stage (one segment
-// only), taken when TAIL and `with_tail`.  After segment 0 the sums are multiplied by `carry` (RESCALE: the later segments' terms are held
-// at a larger scale; it0 == 0).  ni - i0 and nj - j0 are positive.
+// only), taken when TAIL and `with_tail`.  Segment 0's sums are multiplied by `carry` (RESCALE: the later segments' terms are held at a
+// larger scale).  ni - i0 and nj - j0 are positive.
 template <class Cfg, class T, bool AKM, bool BKM, bool RESCALE, bool TAIL>
 FN_DEV void mm_run(unsigned char* smem, const MmOperand& A, const MmOperand& B, long i0, long ni, long j0, long nj, int k_tiles, int tail,
                    unsigned segs, int it0, int it1, bool with_tail, float carry, f32x16 (&acc)[Cfg::MI][Cfg::NJ]) {
@@ -248,7 +248,7 @@ FN_DEV void mm_run(unsigned char* smem, const MmOperand& A, const MmOperand& B, 
             multiply(fa, fb);
         }
     };
-    int left0 = RESCALE ? k_tiles : 0;
+    int left0 = RESCALE ? k_tiles - it0 : 0;              // stages up to the end of segment 0 (<= 0: it lies behind)
     auto rescale = [&]() {
         if constexpr (RESCALE) {
             if (--left0 == 0) {
@@ -335,6 +335,16 @@ FN_DEV void mm_run(unsigned char* smem, const MmOperand& A, const MmOperand& B, 
             compute(smem + stage * Cfg::STAGE_BYTES);
             stage = stage + 1 == Cfg::STAGES ? 0 : stage + 1;
             rescale();
+        }
+    }
+    if constexpr (RESCALE) {
+        if (it1 < k_tiles) {                 // a part of segment 0 alone
+#pragma unroll
+            for (int m = 0; m < Cfg::MI; ++m)
+#pragma unroll
+                for (int n = 0; n < Cfg::NJ; ++n)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) acc[m][n][e] *= carry;
         }
     }
     if constexpr (TAIL) {

@@ -49,6 +49,9 @@ struct MuonArgs {
     int cur, total;                          // total: workgroups
     unsigned char* scratch;
     int first[kMuonMaxJobs];
+    // a symmetric product whose contractions are shared out evenly: `stages` a tile, parts of tiles at `parts`
+    int stages, pad_;
+    float* parts;
 };
 constexpr long kMuonTable = kMuonMaxJobs * sizeof(MuonJob);
 
@@ -228,10 +231,83 @@ FN_DEV void muon_upper(int t, int& ti, int& tj) {
     ti = t - tj * (tj + 1) / 2;
 }
 
+// A symmetric product of few wide tiles (4096: 136 of 256 x 256 for 256 CUs, 528 of 128 x 128 for twice as many places) leaves half the chip
+// idle in its last round.  There the stages of ALL its tiles, end to end, are shared out evenly to kMuonParts workgroups; each leaves the sums
+// of its part of a tile (two at most) and the product kernel's JOIN form adds a tile's parts in their order.
+constexpr int kMuonParts = 256;
+template <class Cfg>
+FN_DEV float* muon_part(const MuonArgs& a, int wg, int which) { return a.parts + ((long)wg * 2 + which) * (Cfg::BM * Cfg::BN) + threadIdx.x * 4; }
+FN_DEV long muon_part_begin(const MuonArgs& a, long wg) { return wg * a.total * a.stages / kMuonParts; }
+
+template <class Cfg>
+FN_DEV void muon_join(const MuonArgs& a, int tile, f32x16 (&acc)[Cfg::MI][Cfg::NJ]) {
+#pragma unroll
+    for (int m = 0; m < Cfg::MI; ++m)
+#pragma unroll
+        for (int n = 0; n < Cfg::NJ; ++n)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[m][n][e] = 0.0f;
+    const long lo = (long)tile * a.stages, hi = lo + a.stages, all = (long)a.total * a.stages;
+    int w = (int)(lo * kMuonParts / all);
+    while (w > 0 && muon_part_begin(a, w) > lo) --w;
+    while (muon_part_begin(a, w + 1) <= lo) ++w;              // the part that holds the tile's first stage
+    for (; w < kMuonParts && muon_part_begin(a, w) < hi; ++w) {
+        const float* p = muon_part<Cfg>(a, w, muon_part_begin(a, w) < lo ? 1 : 0);
+#pragma unroll
+        for (int m = 0; m < Cfg::MI; ++m)
+#pragma unroll
+            for (int n = 0; n < Cfg::NJ; ++n)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const f32x4 q = *reinterpret_cast<const f32x4*>(p + ((m * Cfg::NJ + n) * 4 + g) * (Cfg::THREADS * 4));
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) acc[m][n][4 * g + k] += q[k];
+                }
+    }
+}
+
+template <class Cfg, int NP, int KIND>
+__global__ void __launch_bounds__(Cfg::THREADS, 2) muon_part_kernel(MuonArgs args) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char mm_smem[];
+    const int wg = (int)mm_spread(blockIdx.x, kMuonParts);
+    long at = muon_part_begin(args, wg);
+    const long end = muon_part_begin(args, wg + 1);
+#pragma unroll 1
+    for (int which = 0; at < end; ++which) {
+        const int tile = (int)(at / args.stages), it0 = (int)(at - (long)tile * args.stages);
+        const int it1 = end - at < args.stages - it0 ? it0 + (int)(end - at) : args.stages;
+        const int q = muon_find(args, tile);
+        const MuonJob J = muon_job(args, q);
+        const MuonLay L = muon_lay(J.rows, J.cols, NP);
+        const unsigned char* S = args.scratch + J.off;
+        int ti, tj;
+        muon_upper(tile - args.first[q], ti, tj);
+        const MmOperand A = KIND == MU_GRAM ? muon_op<NP>(S + L.x[args.cur], L.px, L.ldx) : muon_op<NP>(S + L.a, L.pa, L.lda);
+        f32x16 acc[Cfg::MI][Cfg::NJ];
+        __syncthreads();                                  // (everyone has read the last part's last stage)
+        mm_run<Cfg, _Float16, false, false, NP == 2, false>(mm_smem, A, A, (long)ti * Cfg::BM, L.m, (long)tj * Cfg::BN, L.m,
+                                                            args.stages / (NP == 2 ? 3 : 1), 0, NP == 2 ? kMmThree : kMmOne, it0, it1, false, kLoScale, acc);
+        float* p = muon_part<Cfg>(args, wg, which);
+#pragma unroll
+        for (int m = 0; m < Cfg::MI; ++m)
+#pragma unroll
+            for (int n = 0; n < Cfg::NJ; ++n)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    f32x4 v;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) v[k] = acc[m][n][4 * g + k];
+                    *reinterpret_cast<f32x4*>(p + ((m * Cfg::NJ + n) * 4 + g) * (Cfg::THREADS * 4)) = v;
+                }
+        at += it1 - it0;
+    }
+}
+
 // GRAM: A = X X^T.  POLY: B = b A + c A A.  STEP: X' = a X + B X.  LAST: the same into `out` or the parameter.
 // A and B are symmetric: the tiles below the diagonal are the mirror images the tiles above it write.  The epilogue goes through LDS, 32
 // rows of a wave at a time, so that either orientation writes runs of a line.
-template <class Cfg, int NP, int KIND, class T, bool MOM>
+// JOIN: the tile's sums come from the parts of muon_part_kernel.
+template <class Cfg, int NP, int KIND, class T, bool MOM, bool JOIN>
 __global__ void __launch_bounds__(Cfg::THREADS, 2) muon_product_kernel(MuonArgs args) {
     extern __shared__ __attribute__((aligned(16))) unsigned char mm_smem[];
     const MuonNum& P = args.P;
@@ -277,8 +353,10 @@ __global__ void __launch_bounds__(Cfg::THREADS, 2) muon_product_kernel(MuonArgs 
     }
     const int k_tiles = (int)((KIND == MU_GRAM ? L.ldx : L.lda) / Cfg::ROW);
     f32x16 acc[Cfg::MI][Cfg::NJ];
-    mm_run<Cfg, _Float16, false, (KIND >= MU_STEP), NP == 2, false>(mm_smem, A, B, i0, ni, j0, nj, k_tiles, 0, NP == 2 ? kMmThree : kMmOne, 0,
-                                                                    (NP == 2 ? 3 : 1) * k_tiles, false, kLoScale, acc);
+    if constexpr (JOIN) muon_join<Cfg>(args, wg, acc);
+    else
+        mm_run<Cfg, _Float16, false, (KIND >= MU_STEP), NP == 2, false>(mm_smem, A, B, i0, ni, j0, nj, k_tiles, 0, NP == 2 ? kMmThree : kMmOne, 0,
+                                                                        (NP == 2 ? 3 : 1) * k_tiles, false, kLoScale, acc);
     const float lo = NP == 2 ? 1.0f / kLoScale : 1.0f;
     // acc -> value: the product of the operands' scales (and the second plane's) is taken out, the result's put in
     float f;
@@ -358,7 +436,21 @@ static long muon_tiles(long m, long n, bool sym, int b) {
     return sym ? ti * (ti + 1) / 2 : ti * tj;
 }
 
-template <class Cfg, int NP, int KIND, class T, bool MOM>
+// whether a symmetric product is shared out evenly: one shape (every tile as long), enough 256-wide tiles and stages that the parts are worth
+// their way through memory, and no more tiles than parts (a part then ends at most one tile).  MEASURED at 4096^2 (us a product): 528 tiles of
+// 128 x 128 310, shared out kShared
+static bool muon_shared(int rows, int cols, int n_jobs, int planes) {
+    const long m = rows < cols ? rows : cols, tiles = muon_tiles(m, m, true, 256) * n_jobs;
+    return tiles >= 96 && tiles <= kMuonParts && m >= 1024 * (3 - planes);
+}
+static bool muon_one_shape(const FneusMuonJob* jobs, int n) {
+    for (int q = 1; q < n; ++q)
+        if (jobs[q].rows != jobs[0].rows || jobs[q].cols != jobs[0].cols) return false;
+    return n > 0;
+}
+constexpr long kMuonPartBytes = (long)kMuonParts * 2 * MuonBig::BM * MuonBig::BN * 4;
+
+template <class Cfg, int NP, int KIND, class T, bool MOM, bool JOIN = false>
 static void muon_product_launch(const MuonJobs& js, MuonArgs& args, hipStream_t stream) {
     long tiles = 0;
     for (int q = 0; q < js.n; ++q) {
@@ -367,7 +459,14 @@ static void muon_product_launch(const MuonJobs& js, MuonArgs& args, hipStream_t 
         tiles += muon_tiles(J.rows < J.cols ? J.rows : J.cols, J.rows < J.cols ? J.cols : J.rows, KIND <= MU_POLY, Cfg::BM);
     }
     args.total = (int)tiles;
-    auto kernel = muon_product_kernel<Cfg, NP, KIND, T, MOM>;
+    if constexpr (JOIN) {
+        const MuonLay L = muon_lay(js.j[0].rows, js.j[0].cols, NP);
+        args.stages = (NP == 2 ? 3 : 1) * (int)((KIND == MU_GRAM ? L.ldx : L.lda) / Cfg::ROW);
+        auto part = muon_part_kernel<Cfg, NP, KIND>;
+        allow_big_lds(part);
+        hipLaunchKernelGGL(part, dim3(kMuonParts), dim3(Cfg::THREADS), Cfg::LDS, stream, args);
+    }
+    auto kernel = muon_product_kernel<Cfg, NP, KIND, T, MOM, JOIN>;
     allow_big_lds(kernel);
     hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(Cfg::THREADS), Cfg::LDS, stream, args);
 }
@@ -380,6 +479,12 @@ static void muon_product(const MuonJobs& js, MuonArgs& args, hipStream_t stream)
         const MuonJob& J = js.j[q];
         const long m = J.rows < J.cols ? J.rows : J.cols, n = J.rows < J.cols ? J.cols : J.rows;
         big += muon_tiles(m, n, KIND <= MU_POLY, 256), mid += muon_tiles(m, n, KIND <= MU_POLY, 128);
+    }
+    if constexpr (KIND <= MU_POLY) {
+        if (args.parts) {
+            muon_product_launch<MuonBig, NP, KIND, T, MOM, true>(js, args, stream);
+            return;
+        }
     }
     if (big >= 192) muon_product_launch<MuonBig, NP, KIND, T, MOM>(js, args, stream);
     else if (mid > 256) muon_product_launch<MuonMid, NP, KIND, T, MOM>(js, args, stream);
@@ -416,6 +521,8 @@ static int muon_run(const FneusMuonJob* jobs, int n_jobs, const MuonNum& P, int 
             off += muon_lay(f.rows, f.cols, NP).total;
             tiles += (long)((f.rows + 127) / 128) * ((f.cols + 127) / 128) * 4;
         }
+        args.stages = 0, args.parts = nullptr;
+        if (muon_one_shape(jobs + first, js.n) && muon_shared(js.j[0].rows, js.j[0].cols, js.n, NP)) args.parts = reinterpret_cast<float*>(scratch + off);
         hipLaunchKernelGGL((muon_norm_kernel<T, MOM>), dim3((unsigned)(js.n * kMuonChunks)), dim3(256), 0, stream, js, P);
         hipLaunchKernelGGL((muon_init_kernel<T, MOM, NP>), dim3((unsigned)tiles), dim3(256), 0, stream, args);
         muon_steps<NP, T, MOM>(js, args, steps, stream);
@@ -489,6 +596,8 @@ extern "C" long fneus_muon_scratch_bytes(const FneusMuonJob* jobs, int n_jobs, i
         long off = kMuonTable;
         for (int q = first; q < n_jobs && q < first + kMuonMaxJobs; ++q)
             if (jobs[q].rows > 0 && jobs[q].cols > 0) off += muon_lay(jobs[q].rows, jobs[q].cols, prec == 3 ? 2 : 1).total;
+        const int n = n_jobs - first < kMuonMaxJobs ? n_jobs - first : kMuonMaxJobs;
+        if (muon_one_shape(jobs + first, n) && muon_shared(jobs[first].rows, jobs[first].cols, n, prec == 3 ? 2 : 1)) off += kMuonPartBytes;
         most = off > most ? off : most;
     }
     return most;

@@ -1279,8 +1279,8 @@ def layer_norm_fwd(x, weight=None, bias=None, eps: float = 1e-5):
     if n == 0:
         raise ValueError("layer_norm: rows without values have no mean")
     weight, bias, wtype = _norm_weights(weight, bias, x)
-    y = x.new_empty((rows, n))
-    mean, rstd = x.new_empty((rows,), dtype=torch.float32), x.new_empty((rows,), dtype=torch.float32)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    mean, rstd = x.new_empty((2, rows), dtype=torch.float32).unbind(0)
     _launch("fneus_layer_norm_fwd", lib.fneus_layer_norm_fwd, x.data_ptr(), _ld(x), _at(weight), _at(bias), y.data_ptr(), n, mean.data_ptr(),
             rstd.data_ptr(), rows, n, eps, _DTYPES[x.dtype], wtype, _raw_stream(device))
     return y, mean, rstd
@@ -1298,11 +1298,10 @@ def layer_norm_bwd(dy, x, weight, mean, rstd, need_params: bool = True):
     rows, n = x.shape
     weight, _, wtype = _norm_weights(weight, None, x)
     mean, rstd = _vector(mean, "layer_norm: mean", rows, x, _FLOAT), _vector(rstd, "layer_norm: rstd", rows, x, _FLOAT)
-    dx = x.new_empty((rows, n))
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format)
     dw = db = scratch = None
     if need_params:
-        ptype = torch.float32 if weight is None else weight.dtype
-        dw, db = x.new_empty((n,), dtype=ptype), x.new_empty((n,), dtype=ptype)
+        dw, db = x.new_empty((2, n), dtype=torch.float32 if weight is None else weight.dtype).unbind(0)
         if rows == 0:
             dw.zero_(), db.zero_()
         else:
