@@ -9,6 +9,10 @@
 // error that 16-bit gradients bring along, an eighth of what bf16 operands would add.  prec 3: a second plane holds what the first one's
 // rounding left, times another 2^11, so that it is as normal as the first; products hi hi + hi lo + lo hi (22 bits: fp32's accuracy at
 // half the matrix work of three bf16 terms).
+//
+// What bounds it (MI355X, us): one fp32 4096^2 matrix 4600, of which matrix products 4470 at 1.0 - 1.1 PFLOP/s of fp16 MFMAs (a bare stream
+// of them: 1.6), the momentum and norm 56 (5 x 64 MiB: 6 TB/s); four bf16 4096 x 1024 531 (X X^T 41, A A 18, B X 48 a step); eight fp32
+// 256^2 145 = 17 launches of 8 .. 10: 1.3 until the job is read, 2.7 until the first stage has arrived from the other XCDs' writes, 0.4 a stage.
 #include <math.h>
 #include "mm_engine.h"
 #include "fneus_kernels.h"
@@ -437,8 +441,8 @@ static long muon_tiles(long m, long n, bool sym, int b) {
 }
 
 // whether a symmetric product is shared out evenly: one shape (every tile as long), enough 256-wide tiles and stages that the parts are worth
-// their way through memory, and no more tiles than parts (a part then ends at most one tile).  MEASURED at 4096^2 (us a product): 528 tiles of
-// 128 x 128 310, shared out kShared
+// their way through memory, and no more tiles than parts (a part then ends at most one tile).  MEASURED at 4096^2, prec 3 (us a product): 528
+// tiles of 128 x 128 310, shared out 206 and 38 .. 72 to join
 static bool muon_shared(int rows, int cols, int n_jobs, int planes) {
     const long m = rows < cols ? rows : cols, tiles = muon_tiles(m, m, true, 256) * n_jobs;
     return tiles >= 96 && tiles <= kMuonParts && m >= 1024 * (3 - planes);

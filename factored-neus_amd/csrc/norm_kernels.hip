@@ -8,6 +8,9 @@
 // The weight gradients: a team keeps its columns' sums of dy xh and dy in registers over all the rows it takes, the teams of a
 // workgroup are added in LDS, every workgroup writes ONE partial row, and a second launch adds the partial rows in a fixed order: no
 // atomics, the same bits in every run.
+// MEASURED (MI355X, us): forward 8192 x 8192 bf16 46 (5.8 TB/s with the caches' help; a copy of 1 GiB: 5.1), 65536 x 256 fp32 23 (5.8); backward
+// of the latter 33 (5.8) + 4.6 for the fold; 4099 x 1031 fp16 11 / 15 / 5: latency, unaligned rows; one row of 4096 3.4.  A workgroup of 1024
+// threads a row took 140 at 8192 x 8192: two rows a CU in flight, two barriers each.
 #include "fneus_types.h"
 #include "fneus_kernels.h"
 

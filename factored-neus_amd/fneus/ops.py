@@ -1448,8 +1448,9 @@ def muon_jobs(params, grads, momenta, adjust="match_rms"):
     grads, momenta = _muon_matrices(grads, "grads", params), _muon_matrices(momenta, "momenta", params)
     if not len(params) == len(grads) == len(momenta):
         raise ValueError("muon: params, grads and momenta must be lists of one length")
-    if len({t.data_ptr() for t in params + grads + momenta}) != 3 * len(params):
-        raise ValueError("muon: a tensor appears twice among params, grads and momenta")
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in params + grads + momenta)
+    if any(b[0] < a[1] for a, b in zip(spans, spans[1:])):
+        raise ValueError("muon: two of params, grads and momenta share memory")
     jobs = (_lib.FneusMuonJob * max(1, len(params)))()
     for j, p, g, m in zip(jobs, params, grads, momenta):
         j.grad, j.momentum, j.param = g.data_ptr(), m.data_ptr(), p.data_ptr()

@@ -211,6 +211,8 @@ class FlatMuon(torch.optim.Optimizer):
         if closure is not None:
             raise NotImplementedError("FlatMuon.step() takes no closure")
         from . import ops
+        if len(self.param_groups) != 1:
+            raise NotImplementedError("FlatMuon supports a single parameter group")
         g = self.param_groups[0]
         ps = self._live()
         if self.adam is not None:

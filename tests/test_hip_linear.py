@@ -150,6 +150,38 @@ def test_linear_views_and_repeats(t, size):
 
 
 @pytest.mark.gpu
+def test_linear_and_layer_norm_beyond_32_bits():
+    """rows 16 MiB apart (the tiled kernel's loads have 32-bit offsets within a tile: such rows are copied), and arrays of more than 2^32 bytes"""
+    from fneus import ops
+    w = torch.randn(256, 256, device="cuda").bfloat16()
+    far = torch.zeros(300 * ((1 << 23) + 8), dtype=torch.bfloat16, device="cuda").as_strided((300, 256), ((1 << 23) + 8, 1))
+    far.copy_(torch.randn(300, 256, device="cuda"))
+    near = far.contiguous()
+    wide = torch.cat([w] * 16)                                      # (large enough for the tiled form)
+    assert torch.equal(ops.linear_fwd(far, wide)[0], ops.linear_fwd(near, wide)[0])
+    dy = torch.randn(300, 4096, device="cuda").bfloat16()
+    assert all(torch.equal(a, b) for a, b in zip(ops.linear_bwd(dy, far, wide), ops.linear_bwd(dy, near, wide)))
+    assert torch.equal(ops.layer_norm_fwd(far)[0], ops.layer_norm_fwd(near)[0])
+    del far
+    rows = (1 << 24) + 300                                          # x 256 x 2 bytes = 8 GiB
+    x = torch.empty(rows, 256, dtype=torch.bfloat16, device="cuda")
+    x[-300:] = near
+    x[:-300] = 0
+    y, z = ops.linear_fwd(x, w, act="silu", train=True)
+    ref = ops.linear_fwd(near, w, act="silu", train=True)
+    lim = 2 * torch.finfo(torch.bfloat16).eps * float(ref[0].abs().max())
+    assert float((y[-300:].float() - ref[0].float()).abs().max()) <= lim and float(y[:-300].abs().max()) == 0.0
+    n, mean, rstd = ops.layer_norm_fwd(x)
+    assert torch.equal(n[-300:], ops.layer_norm_fwd(near)[0])
+    dx, dw, db = ops.linear_bwd(y, x, w, z, act="silu")
+    small = ops.linear_bwd(ref[0], near, w, ref[1], act="silu")
+    for a, b in ((dx[-300:], small[0]), (dw, small[1]), (db, small[2])):
+        assert float((a.float() - b.float()).abs().max()) <= 4 * torch.finfo(torch.bfloat16).eps * float(b.float().abs().max())
+    dl = ops.layer_norm_bwd(x, x, None, mean, rstd)[0]
+    assert float((dl[-300:].float() - ops.layer_norm_bwd(near, near, None, mean[-300:], rstd[-300:])[0].float()).abs().max()) == 0.0
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("size", [(6, 64, 48), (200, 96, 80), (2048, 512, 512)], ids=str)
 def test_linear_nan_stays_in_its_row(size):
     from fneus import ops

@@ -77,6 +77,41 @@ def test_newton_schulz_large_and_stacked():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("shape,t", [((3400, 3456), torch.float32), ((3456, 3400), torch.bfloat16), ((10, 1100, 1028), torch.float32)], ids=str)
+def test_newton_schulz_shared_out(shape, t):
+    """sizes whose symmetric products are shared out evenly and joined (105 tiles of one matrix; 150 of ten)"""
+    from fneus import ops
+    g = torch.randn(*shape, generator=torch.Generator().manual_seed(1)).to(t).cuda()
+    got = ops.newton_schulz(g)
+    prec = 3 if t == torch.float32 else 2
+    for k, (a, b) in enumerate([(got, g)] if g.dim() == 2 else [(got[0], g[0]), (got[9], g[9])]):
+        want = ns64(b)
+        err = float((a.double() - want).norm() / want.norm())
+        assert err <= bound(prec, t), (k, err)
+    assert torch.equal(ops.newton_schulz(g), got)
+
+
+@pytest.mark.gpu
+def test_muon_and_linear_on_two_streams_at_once():
+    """two calls in flight: each has its own scratch and job table"""
+    from fneus import ops
+    gs = [torch.randn(8, 256, 256, device="cuda") for _ in range(2)]
+    xs = [torch.randn(4096, 512, device="cuda") for _ in range(2)]
+    w = torch.randn(512, 512, device="cuda")
+    want = [(ops.newton_schulz(g), ops.linear_bwd(x, x, w)) for g, x in zip(gs, xs)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for s, g, x in zip(streams, gs, xs):
+            with torch.cuda.stream(s):
+                got.append((ops.newton_schulz(g), ops.linear_bwd(x, x, w)))
+        torch.cuda.synchronize()
+        for (a, b), (c, d) in zip(got, want):
+            assert torch.equal(a, c) and all(torch.equal(p, q) for p, q in zip(b, d))
+
+
+@pytest.mark.gpu
 def test_newton_schulz_properties():
     """singular values in the polynomial's interval, the singular vectors kept; scale-free; other polynomials and step counts; zero, tiny,
     huge, rank-deficient and NaN matrices"""
@@ -206,6 +241,7 @@ def test_muon_refusals():
     for bad in (lambda: ops.muon_step([p], [g[:5]], [m], 0.1), lambda: ops.muon_step([p], [g], [], 0.1), lambda: ops.muon_step([p], [p], [m], 0.1),
                 lambda: ops.muon_step([p[0]], [g[0]], [m[0]], 0.1), lambda: ops.muon_step([p], [g.half()], [m], 0.1),
                 lambda: ops.muon_step([p.t()], [g.t()], [m.t()], 0.1), lambda: ops.muon_step([p, p], [g, m], [m, g], 0.1),
+                lambda: ops.muon_step([p[:4], p[2:]], [g[:4], g[:4].clone()], [m[:4], m[:4].clone()], 0.1),
                 lambda: ops.muon_step([p], [g], [m], torch.ones(2, device="cuda")), lambda: ops.muon_step([p], [g], [m], 0.1, adjust="other"),
                 lambda: ops.muon_step([p], [g], [m], 0.1, prec=1), lambda: ops.newton_schulz(p.double()), lambda: ops.newton_schulz(p[0])):
         with pytest.raises(ValueError):

@@ -231,6 +231,9 @@ def test_flat_muon_refusals_cpu():
         opt.step()                                                    # no CPU fallback
     with pytest.raises(NotImplementedError):
         opt.step(lambda: None)
+    opt.add_param_group({"params": [nn.Parameter(torch.randn(40, 40))]})
+    with pytest.raises(NotImplementedError):
+        opt.step()
 
 
 def test_indirect_light_residual_cpu():
