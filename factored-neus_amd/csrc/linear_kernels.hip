@@ -474,8 +474,7 @@ static bool lin_aligned(const void* p, long ld, long n, bool k_major) {
 // tile's eight waves have nothing to split (16 x 8192 -> 8192 fp32 683 us), so large ones are tiled from the first row on.
 template <class T>
 static bool lin_direct(const FneusLinear& f, bool backward) {
-    constexpr int V = 16 / (int)sizeof(T);
-    if (f.n_in < V || f.n_out < V || (!backward && f.rows <= 16)) return true;
+    if (!backward && f.rows <= 16) return true;
     const double work = (double)f.rows * f.n_in * f.n_out;
     if (backward) return f.rows <= 1024 && work <= (double)(1L << 27) && (f.rows > 16 || (long)f.n_in * f.n_out <= 1L << 20);
     return work <= (double)(sizeof(T) == 4 ? 1L << 28 : 1L << 27);

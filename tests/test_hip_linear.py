@@ -20,9 +20,10 @@ sys.path.insert(0, os.path.join(ROOT, "factored-neus_amd"))
 TYPES = [torch.float32, torch.bfloat16, torch.float16]
 ACTS = ["none", "relu", "leaky", "sigmoid", "softplus", "gelu", "silu"]
 # (rows, n_in, n_out): one row, the row kernel's last row and the first beyond it, one value, odd sizes, a tile's edges, the tiled kernel's
-# sizes on and off its borders, a long contraction of few columns (split) and few rows with a long contraction
+# sizes on and off its borders, a long contraction of few columns (split) and few rows with a long contraction, many rows of a few values
 SIZES = [(1, 1, 1), (1, 512, 144), (1, 4099, 70), (3, 7, 5), (16, 256, 256), (17, 90, 256), (33, 63, 129), (100, 512, 512), (257, 31, 64),
-         (300, 65, 33), (640, 512, 384), (1000, 777, 1111), (2048, 256, 256), (1025, 520, 1032), (5000, 40, 24), (20000, 256, 128), (64, 4096, 96)]
+         (300, 65, 33), (640, 512, 384), (1000, 777, 1111), (2048, 256, 256), (1025, 520, 1032), (5000, 40, 24), (20000, 256, 128), (64, 4096, 96),
+         (40000, 256, 1), (5000, 3, 257), (30000, 5, 3), (2000, 1, 1)]
 
 
 def act64(z, act):
