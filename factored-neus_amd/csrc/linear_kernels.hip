@@ -468,16 +468,18 @@ static bool lin_aligned(const void* p, long ld, long n, bool k_major) {
 }
 
 // Which form: a direct tile is one launch for a direction and needs no scratch, the tiled kernel shares its operands.  MEASURED (us, forward /
-// backward, direct against tiled): fp32 512^3 9 / 26 against 15 / 35, 2048 x 512 x 512 23 / 88 against 20 / 48, 4096 x 256 x 256 15 / 114 against
-// 14 / 35; bf16 512^3 6 / 19 against 8 / 20, 4096 x 256 x 256 10 / 72 against 7 / 25: up to 2^27 multiplications (forward, fp32: 2^28), and for
-// the weight gradient, which the direct form does not split, up to 1024 rows.  The weight gradient of a few rows is its output: a direct
-// tile's eight waves have nothing to split (16 x 8192 -> 8192 fp32 683 us), so large ones are tiled from the first row on.
+// backward, direct against tiled): fp32 512^3 9 / 26 against 15 / 35, 2048 x 512 x 512 23 / 88 against 20 / 48, 4096 x 256 x 256 15 / 114
+// against 14 / 35; bf16 512^3 6 / 19 against 8 / 20, 4096 x 256 x 256 10 / 72 against 7 / 25: up to 2^27 multiplications (forward, fp32: 2^28),
+// and for the weight gradient, whose contraction the direct form does not split, up to 1024 rows.  Where the contraction is short its eight
+// waves have nothing to split: at most 8192 tiles (65536 x 3 -> 256 fp32, 16384 of them, 60 against 36), and of a few rows' weight gradient at
+// most 1024 (16 x 8192 -> 8192 fp32, 65536 of them, 683 against 86).
 template <class T>
 static bool lin_direct(const FneusLinear& f, bool backward) {
     if (!backward && f.rows <= 16) return true;
     const double work = (double)f.rows * f.n_in * f.n_out;
-    if (backward) return f.rows <= 1024 && work <= (double)(1L << 27) && (f.rows > 16 || (long)f.n_in * f.n_out <= 1L << 20);
-    return work <= (double)(sizeof(T) == 4 ? 1L << 28 : 1L << 27);
+    const long ti = (f.rows + 31) / 32, tj = (f.n_in + 31) / 32, to = (f.n_out + 31) / 32;
+    if (backward) return f.rows <= 1024 && work <= (double)(1L << 27) && (ti + to) * tj <= (f.rows > 16 ? 8192 : 1024);
+    return work <= (double)(sizeof(T) == 4 ? 1L << 28 : 1L << 27) && ti * to <= 8192;
 }
 
 template <class T>
