@@ -1,5 +1,5 @@
 // The Muon update of weight matrices: momentum, orthogonalisation by Newton-Schulz products, step -- every matrix of a model in the same
-// 2 + 3 * steps launches.  For each matrix u, as X [m][n] with m <= n (the transpose where rows > cols):
+// 2 + 3 * steps launches, or three (matrices whose shorter side is at most 64; both where a model has both).  For each matrix u, as X [m][n] with m <= n (the transpose where rows > cols):
 //   X = u / max(|u|_F, eps);   steps times:  A = X X^T,  B = b A + c A A,  X <- a X + B X
 // All three products run on the tiled engine (mm_engine.h): X X^T and A A on operands stored along k, B X with X k-major.
 //
@@ -430,6 +430,268 @@ __global__ void __launch_bounds__(Cfg::THREADS, 2) muon_product_kernel(MuonArgs 
         });
 }
 
+// ---- matrices whose shorter side m is at most 64 ----------------------------------------------------------------------------------
+// Every step multiplies X by a symmetric P = a I + b A + c A A from the left, so with A = X X^T known once the steps need no X:
+//   Q <- P Q,  A <- P (P A);   behind the last  O = Q u / |u|_F,  |u|_F^2 = the trace of u u^T.
+// Three launches instead of 2 + 3 steps: the momentum and parts of u u^T over stretches of the long axis, the steps on m x m matrices (a workgroup
+// a matrix, in LDS), and Q u with the update.  In fp64, on its matrix instructions: a rounding of A grows by up to g' = d(l p(l)^2) / dl a step, 11.9
+// at l = 0 for the usual coefficients, which fp32 has no room for (6e-8 x 11.9^4 = 1e-3); muon_scales() keeps 2^-53 x the growth below fp32's.
+// Bound by the fp64 matrix instructions of one CU: 0.8 us a step at m <= 16, 2 at 32, 9 at 64; the rest of a call 10 - 20.
+typedef double f64x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kFewSide = 64, kFewParts = 64, kFewRun = 64;      // kFewRun: positions along the long axis in LDS at a time
+
+struct MuonFew { int m, n, M, parts; bool trans; long q, total; };
+__host__ __device__ inline MuonFew muon_few_lay(int rows, int cols) {
+    MuonFew L;
+    L.trans = rows > cols;
+    L.m = L.trans ? cols : rows;
+    L.n = L.trans ? rows : cols;
+    L.M = L.m <= 16 ? 16 : (L.m <= 32 ? 32 : 64);
+    L.parts = (L.n + 127) / 128 < kFewParts ? (L.n + 127) / 128 : kFewParts;
+    const long tiles = L.M / 16 * (L.M / 16 + 1) / 2;
+    L.q = L.parts * tiles * 2048;                                // behind the parts of u u^T (the 16 x 16 tiles on and above the diagonal)
+    L.total = (L.q + (long)L.M * L.M * 8 + 255) / 256 * 256;
+    return L;
+}
+// runs of the long axis that part p takes
+FN_DEV int muon_few_run(const MuonFew& L, int p) { return (int)((long)((L.n + kFewRun - 1) / kFewRun) * p / L.parts); }
+
+// u at (i of the short axis, k of the stretch that starts at `at`) in LDS: i along memory's rows where the matrix is stored so (trans)
+template <int M>
+FN_DEV int few_at(bool trans, int i, int k) { return trans ? k * (M + 16) + i : i * (kFewRun + 4) + k; }
+constexpr int kFewTile = kFewRun * (kFewSide + 16);
+
+// UPDATE: the momentum is updated and stored; else it is taken as it is stored (and `zero_grad` clears the gradient)
+template <int M, class T, bool MOM, bool UPDATE>
+FN_DEV void few_load(const MuonJob& J, const MuonFew& L, const MuonNum& P, int at, float* tile, int threads) {
+    constexpr int N = M * kFewRun / 256;
+    float g[N], mo[N];
+    long where[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        const int x = e * threads + threadIdx.x;
+        const int i = L.trans ? x % M : x / kFewRun, k = L.trans ? x / M : x % kFewRun;
+        where[e] = i < L.m && at + k < L.n ? (L.trans ? (long)(at + k) * J.cols + i : (long)i * J.cols + at + k) : -1;
+        const long w = where[e] < 0 ? 0 : where[e];
+        g[e] = (float)((const T*)J.grad)[w];
+        mo[e] = MOM ? (float)((const T*)J.momentum)[w] : 0.0f;
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        const int x = e * threads + threadIdx.x;
+        const int i = L.trans ? x % M : x / kFewRun, k = L.trans ? x / M : x % kFewRun;
+        float u = g[e];
+        if constexpr (MOM) {
+            float m = mo[e];
+            if constexpr (UPDATE) m = (float)(T)(P.mu * m + P.omu * g[e]);
+            u = muon_u<T>(g[e], m, P);
+            if (where[e] >= 0) {
+                if constexpr (UPDATE) ((T*)J.momentum)[where[e]] = (T)m;
+                else if (P.zero_grad) ((T*)J.grad)[where[e]] = (T)0.0f;
+            }
+        }
+        tile[few_at<M>(L.trans, i, k)] = where[e] < 0 ? 0.0f : u;
+    }
+}
+
+// the tiles of an M x M matrix on and above the diagonal, numbered by columns
+FN_DEV constexpr int few_tj(int t) { return t < 1 ? 0 : (t < 3 ? 1 : (t < 6 ? 2 : 3)); }
+FN_DEV constexpr int few_ti(int t) { return t - few_tj(t) * (few_tj(t) + 1) / 2; }
+
+// launch 1: parts of u u^T.  Every wave takes a quarter of a stretch's positions for all tiles; the waves are added in order at the end.
+template <int M, class T, bool MOM>
+FN_DEV void few_gram(const MuonJob& J, const MuonFew& L, const MuonNum& P, int part, double* out, float* tile, f64x4* sums) {
+    constexpr int B = M / 16, TILES = B * (B + 1) / 2;
+    f64x4 acc[TILES];
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) acc[t] = f64x4{0.0, 0.0, 0.0, 0.0};
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int end = muon_few_run(L, part + 1);
+    for (int run = muon_few_run(L, part); run < end; ++run) {
+        few_load<M, T, MOM, true>(J, L, P, run * kFewRun, tile, 256);
+        __syncthreads();
+#pragma unroll
+        for (int s = 0; s < kFewRun / 16; ++s) {
+            double f[B];
+#pragma unroll
+            for (int b = 0; b < B; ++b) f[b] = (double)tile[few_at<M>(L.trans, b * 16 + (lane & 15), wave * 16 + s * 4 + (lane >> 4))];
+#pragma unroll
+            for (int t = 0; t < TILES; ++t) acc[t] = __builtin_amdgcn_mfma_f64_16x16x4f64(f[few_ti(t)], f[few_tj(t)], acc[t], 0, 0, 0);
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        if (wave == w) {
+#pragma unroll
+            for (int t = 0; t < TILES; ++t) {
+                if (w > 0) acc[t] = sums[t * 64 + lane] + acc[t];
+                if (w < 3) sums[t * 64 + lane] = acc[t];
+                else reinterpret_cast<f64x4*>(out)[((long)part * TILES + t) * 64 + lane] = acc[t];
+            }
+        }
+        __syncthreads();
+    }
+}
+template <class T, bool MOM>
+__global__ void __launch_bounds__(256) muon_few_gram_kernel(MuonJobs js, MuonArgs args) {
+    __shared__ float tile[kFewTile];
+    __shared__ f64x4 sums[10 * 64];
+    const int q = muon_find(args, blockIdx.x), part = blockIdx.x - args.first[q];
+    const MuonJob J = js.j[q];
+    if (part == 0 && threadIdx.x == 0) reinterpret_cast<MuonJob*>(js.scratch)[q] = J;
+    const MuonFew L = muon_few_lay(J.rows, J.cols);
+    double* out = reinterpret_cast<double*>(js.scratch + J.off);
+    if (L.M == 16) few_gram<16, T, MOM>(J, L, args.P, part, out, tile, sums);
+    else if (L.M == 32) few_gram<32, T, MOM>(J, L, args.P, part, out, tile, sums);
+    else few_gram<64, T, MOM>(J, L, args.P, part, out, tile, sums);
+}
+
+// launch 2: the steps.  Element (k, i) of an M x M matrix in LDS; odd rows swapped by 16 columns: four rows of 16 on different banks
+template <int M>
+FN_DEV int few_mat(int k, int i) { return k * M + (i ^ ((k & 1) << 4 & (M - 1))); }
+// tile t of U V, both symmetric
+template <int M>
+FN_DEV f64x4 few_product(const double* U, const double* V, int t) {
+    const int lane = threadIdx.x & 63, i = few_ti(t) * 16 + (lane & 15), j = few_tj(t) * 16 + (lane & 15);
+    f64x4 acc = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+    for (int s = 0; s < M / 4; ++s) {
+        const int k = s * 4 + (lane >> 4);
+        acc = __builtin_amdgcn_mfma_f64_16x16x4f64(U[few_mat<M>(k, i)], V[few_mat<M>(k, j)], acc, 0, 0, 0);
+    }
+    return acc;
+}
+// (a lane holds rows 4 r + lane / 16 of the tile, column lane % 16)
+template <int M, class F>
+FN_DEV void few_each(int t, f64x4 v, F&& f) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) f(few_ti(t) * 16 + 4 * r + (lane >> 4), few_tj(t) * 16 + (lane & 15), v[r]);
+}
+template <int M>
+FN_DEV void few_put(double* D, int t, f64x4 v) {
+    few_each<M>(t, v, [&](int i, int j, double x) {
+        D[few_mat<M>(i, j)] = x;
+        if (few_ti(t) != few_tj(t)) D[few_mat<M>(j, i)] = x;
+    });
+}
+constexpr int kFewWaves = 8;
+template <int M>
+FN_DEV void few_steps(const MuonFew& L, const MuonNum& P, int steps, unsigned char* scratch, double* lds) {
+    constexpr int B = M / 16, TILES = B * (B + 1) / 2, HELD = (TILES + kFewWaves - 1) / kFewWaves;
+    double *A = lds, *S = lds + M * M, *W = lds + 2 * M * M, *Q = lds + 3 * M * M;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int other = (wave + kFewWaves - TILES % kFewWaves) % kFewWaves;      // the second product of a phase starts where the first one ends
+    for (int t = wave; t < TILES; t += kFewWaves) {
+        f64x4 v = {0.0, 0.0, 0.0, 0.0};
+        const f64x4* parts = reinterpret_cast<const f64x4*>(scratch) + t * 64 + lane;
+#pragma unroll 8
+        for (int p = 0; p < L.parts; ++p) v += parts[(long)p * TILES * 64];
+        few_put<M>(A, t, v);
+    }
+    __syncthreads();
+    double trace = lane < M ? A[few_mat<M>(lane, lane)] : 0.0;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) trace += __shfl_xor(trace, d, 64);
+    const double root = sqrt(trace), norm = root > (double)P.eps || root != root ? root : (double)P.eps;
+    double s = 1.0 / (norm * norm);                     // (the first step's A is not scaled yet)
+    f64x4 held[HELD];
+    for (int step = 0; step < steps; ++step) {
+        const double b = (double)P.b * s, c = (double)P.c * s * s;
+        for (int t = wave; t < TILES; t += kFewWaves) {
+            const f64x4 v = few_product<M>(A, A, t);
+            few_each<M>(t, v, [&](int i, int j, double x) {
+                const double y = c * x + b * A[few_mat<M>(i, j)] + (i == j ? (double)P.a : 0.0);
+                S[few_mat<M>(i, j)] = y;
+                if (step == 0) Q[few_mat<M>(i, j)] = y;
+                if (few_ti(t) != few_tj(t)) {
+                    S[few_mat<M>(j, i)] = y;
+                    if (step == 0) Q[few_mat<M>(j, i)] = y;
+                }
+            });
+        }
+        __syncthreads();
+        if (step > 0) {
+#pragma unroll
+            for (int h = 0; h < HELD; ++h)
+                if (wave + h * kFewWaves < TILES) held[h] = few_product<M>(S, Q, wave + h * kFewWaves);
+        }
+        const bool more = step + 1 < steps;
+        if (more)
+            for (int t = other; t < TILES; t += kFewWaves) few_put<M>(W, t, few_product<M>(S, A, t));
+        __syncthreads();
+        if (step > 0) {
+#pragma unroll
+            for (int h = 0; h < HELD; ++h)
+                if (wave + h * kFewWaves < TILES) few_put<M>(Q, wave + h * kFewWaves, held[h]);
+        }
+        if (more)
+            for (int t = wave; t < TILES; t += kFewWaves) few_put<M>(A, t, few_product<M>(S, W, t) * s);
+        __syncthreads();
+        s = 1.0;
+    }
+    double* out = reinterpret_cast<double*>(scratch + L.q);
+    for (int e = threadIdx.x; e < M * M; e += 64 * kFewWaves) out[e] = Q[few_mat<M>(e / M, e % M)] / norm;
+}
+__global__ void __launch_bounds__(64 * kFewWaves) muon_few_steps_kernel(MuonArgs args, int steps) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char mm_smem[];
+    double* lds = reinterpret_cast<double*>(mm_smem);
+    const MuonJob J = muon_job(args, blockIdx.x);
+    const MuonFew L = muon_few_lay(J.rows, J.cols);
+    if (L.M == 16) few_steps<16>(L, args.P, steps, args.scratch + J.off, lds);
+    else if (L.M == 32) few_steps<32>(L, args.P, steps, args.scratch + J.off, lds);
+    else few_steps<64>(L, args.P, steps, args.scratch + J.off, lds);
+}
+
+// launch 3: O = Q u, a workgroup a run of the long axis, a wave 16 positions of it; the output's lanes run along memory's rows
+template <int M, class T, bool MOM>
+FN_DEV void few_apply(const MuonJob& J, const MuonFew& L, const MuonNum& P, int run, const double* q, float* tile, double* Q) {
+    constexpr int B = M / 16;
+    for (int e = threadIdx.x; e < M * M; e += 256) Q[few_mat<M>(e / M, e % M)] = q[e];
+    few_load<M, T, MOM, false>(J, L, P, run * kFewRun, tile, 256);
+    __syncthreads();
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    f64x4 acc[B];
+#pragma unroll
+    for (int b = 0; b < B; ++b) acc[b] = f64x4{0.0, 0.0, 0.0, 0.0};
+#pragma unroll 4
+    for (int s = 0; s < M / 4; ++s) {
+        const int k = s * 4 + (lane >> 4);
+        const double x = (double)tile[few_at<M>(L.trans, k, wave * 16 + (lane & 15))];
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            const double w = Q[few_mat<M>(k, b * 16 + (lane & 15))];
+            acc[b] = L.trans ? __builtin_amdgcn_mfma_f64_16x16x4f64(x, w, acc[b], 0, 0, 0) : __builtin_amdgcn_mfma_f64_16x16x4f64(w, x, acc[b], 0, 0, 0);
+        }
+    }
+    const float lr = MOM ? *P.lr : 0.0f, keep = 1.0f - lr * P.wd, step = lr * J.adjust;
+#pragma unroll
+    for (int b = 0; b < B; ++b)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int row = 4 * r + (lane >> 4), col = lane & 15;
+            const int i = b * 16 + (L.trans ? col : row), k = run * kFewRun + wave * 16 + (L.trans ? row : col);
+            if (i >= L.m || k >= L.n) continue;
+            const long at = L.trans ? (long)k * J.cols + i : (long)i * J.cols + k;
+            if constexpr (MOM) ((T*)J.param)[at] = (T)((float)((const T*)J.param)[at] * keep - step * (float)acc[b][r]);
+            else ((T*)J.out)[at] = (T)(float)acc[b][r];
+        }
+}
+template <class T, bool MOM>
+__global__ void __launch_bounds__(256) muon_few_apply_kernel(MuonArgs args) {
+    __shared__ float tile[kFewTile];
+    __shared__ double Q[kFewSide * kFewSide];
+    const int q = muon_find(args, blockIdx.x), run = blockIdx.x - args.first[q];
+    const MuonJob J = muon_job(args, q);
+    const MuonFew L = muon_few_lay(J.rows, J.cols);
+    const double* w = reinterpret_cast<const double*>(args.scratch + J.off + L.q);
+    if (L.M == 16) few_apply<16, T, MOM>(J, L, args.P, run, w, tile, Q);
+    else if (L.M == 32) few_apply<32, T, MOM>(J, L, args.P, run, w, tile, Q);
+    else few_apply<64, T, MOM>(J, L, args.P, run, w, tile, Q);
+}
+
 typedef MmCfg<64, 64, 2, 2, 4, 2> MuonSmall;       // 8 waves, two sharing each stage's 128 k; 128 KiB: three stages in flight
 typedef MmCfg<128, 128, 2, 2, 2> MuonMid;          // 64 KiB, two
 typedef MmCfg<128, 128, 2, 2, 2, 2> MuonMid8;      // 8 waves, 128 KiB: for no more than a workgroup a CU
@@ -443,14 +705,11 @@ static long muon_tiles(long m, long n, bool sym, int b) {
 // whether a symmetric product is shared out evenly: one shape (every tile as long), enough 256-wide tiles and stages that the parts are worth
 // their way through memory, and no more tiles than parts (a part then ends at most one tile).  MEASURED at 4096^2, prec 3 (us a product): 528
 // tiles of 128 x 128 310, shared out 206 and 38 .. 72 to join
-static bool muon_shared(int rows, int cols, int n_jobs, int planes) {
-    const long m = rows < cols ? rows : cols, tiles = muon_tiles(m, m, true, 256) * n_jobs;
+static bool muon_shared(const MuonJobs& js, int planes) {
+    for (int q = 1; q < js.n; ++q)
+        if (js.j[q].rows != js.j[0].rows || js.j[q].cols != js.j[0].cols) return false;
+    const long m = js.j[0].rows < js.j[0].cols ? js.j[0].rows : js.j[0].cols, tiles = muon_tiles(m, m, true, 256) * js.n;
     return tiles >= 96 && tiles <= kMuonParts && m >= 1024 * (3 - planes);
-}
-static bool muon_one_shape(const FneusMuonJob* jobs, int n) {
-    for (int q = 1; q < n; ++q)
-        if (jobs[q].rows != jobs[0].rows || jobs[q].cols != jobs[0].cols) return false;
-    return n > 0;
 }
 constexpr long kMuonPartBytes = (long)kMuonParts * 2 * MuonBig::BM * MuonBig::BN * 4;
 
@@ -507,26 +766,63 @@ static void muon_steps(const MuonJobs& js, MuonArgs& args, int steps, hipStream_
     }
 }
 
+// which form a matrix takes; `few`: whether the polynomial and the steps allow the one for short sides (muon_scales).  MEASURED (us a call, it
+// against the tiled one): fp32 2 x (2038 x 3) 17 / 205, 8 x (32 x 256) 27 / 117, one 64 x 64 63 / 109, 40 of them 129 / 233, 64 x 8192 88 / 537,
+// 32 x (64 x 4096) 166 / 566; bf16 73 / 97 for 8 x (64 x 256), 88 / 234 for 64 x 8192.  Sides beyond 64 do not fit the four matrices in LDS.
+static bool muon_few(const FneusMuonJob& f, bool few) { return few && (f.rows < f.cols ? f.rows : f.cols) <= kFewSide; }
+
+// the next round of launches: up to kMuonMaxJobs matrices of one form, from jobs[at] on; `off`: the scratch it takes
+enum { MU_ALL = 0, MU_TILED = 1, MU_FEW = 2 };       // ALL: every matrix tiled
+static int muon_round(const FneusMuonJob* jobs, int n_jobs, int& at, int form, int planes, MuonJobs& js, long& off) {
+    js.n = 0;
+    off = kMuonTable;
+    for (; at < n_jobs && js.n < kMuonMaxJobs; ++at) {
+        const FneusMuonJob& f = jobs[at];
+        if (f.rows <= 0 || f.cols <= 0 || (form != MU_ALL && muon_few(f, true) != (form == MU_FEW))) continue;
+        MuonJob& J = js.j[js.n++];
+        J.grad = f.grad, J.momentum = f.momentum, J.param = f.param, J.out = f.out;
+        J.rows = f.rows, J.cols = f.cols, J.adjust = f.adjust, J.pad_ = 0, J.off = off;
+        off += form == MU_FEW ? muon_few_lay(f.rows, f.cols).total : muon_lay(f.rows, f.cols, planes).total;
+    }
+    return (int)js.n;
+}
+
+template <class T, bool MOM>
+static void muon_few_run(MuonJobs& js, MuonArgs& args, int steps, hipStream_t stream) {
+    long parts = 0, runs = 0, M = 16;
+    MuonArgs apply = args;
+    for (int q = 0; q < js.n; ++q) {
+        const MuonFew L = muon_few_lay(js.j[q].rows, js.j[q].cols);
+        args.first[q] = (int)parts, apply.first[q] = (int)runs;
+        parts += L.parts, runs += (L.n + kFewRun - 1) / kFewRun;
+        M = L.M > M ? L.M : M;
+    }
+    hipLaunchKernelGGL((muon_few_gram_kernel<T, MOM>), dim3((unsigned)parts), dim3(256), 0, stream, js, args);
+    auto kernel = muon_few_steps_kernel;
+    allow_big_lds(kernel);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)js.n), dim3(64 * kFewWaves), (unsigned)(4 * M * M * 8), stream, args, steps);
+    hipLaunchKernelGGL((muon_few_apply_kernel<T, MOM>), dim3((unsigned)runs), dim3(256), 0, stream, apply);
+}
+
 template <class T, bool MOM, int NP>
-static int muon_run(const FneusMuonJob* jobs, int n_jobs, const MuonNum& P, int steps, unsigned char* scratch, hipStream_t stream) {
-    for (int first = 0; first < n_jobs; first += kMuonMaxJobs) {
-        MuonJobs js;
-        js.n = n_jobs - first < kMuonMaxJobs ? n_jobs - first : kMuonMaxJobs;       // (a local: filled anew for every round)
-        js.scratch = scratch;
-        MuonArgs args;
-        args.P = P, args.cur = 0, args.scratch = scratch;
+static int muon_run(const FneusMuonJob* jobs, int n_jobs, const MuonNum& P, int steps, bool few, unsigned char* scratch, hipStream_t stream) {
+    MuonJobs js;                                        // (a local: filled anew for every round)
+    js.scratch = scratch;
+    long off;
+    MuonArgs args;
+    args.P = P, args.cur = 0, args.scratch = scratch, args.stages = 0, args.pad_ = 0, args.parts = nullptr, args.total = 0;
+    for (int at = 0; few && muon_round(jobs, n_jobs, at, MU_FEW, NP, js, off) > 0;) {
         for (int q = 0; q < kMuonMaxJobs; ++q) args.first[q] = 0x7fffffff;
-        long off = kMuonTable, tiles = 0;
+        muon_few_run<T, MOM>(js, args, steps, stream);
+    }
+    for (int at = 0; muon_round(jobs, n_jobs, at, few ? MU_TILED : MU_ALL, NP, js, off) > 0;) {
+        for (int q = 0; q < kMuonMaxJobs; ++q) args.first[q] = 0x7fffffff;
+        long tiles = 0;
         for (int q = 0; q < js.n; ++q) {
-            const FneusMuonJob& f = jobs[first + q];
-            MuonJob& J = js.j[q];
-            J.grad = f.grad, J.momentum = f.momentum, J.param = f.param, J.out = f.out;
-            J.rows = f.rows, J.cols = f.cols, J.adjust = f.adjust, J.off = off, args.first[q] = (int)tiles;
-            off += muon_lay(f.rows, f.cols, NP).total;
-            tiles += (long)((f.rows + 127) / 128) * ((f.cols + 127) / 128) * 4;
+            args.first[q] = (int)tiles;
+            tiles += (long)((js.j[q].rows + 127) / 128) * ((js.j[q].cols + 127) / 128) * 4;
         }
-        args.stages = 0, args.parts = nullptr;
-        if (muon_one_shape(jobs + first, js.n) && muon_shared(js.j[0].rows, js.j[0].cols, js.n, NP)) args.parts = reinterpret_cast<float*>(scratch + off);
+        args.parts = muon_shared(js, NP) ? reinterpret_cast<float*>(scratch + off) : nullptr;
         hipLaunchKernelGGL((muon_norm_kernel<T, MOM>), dim3((unsigned)(js.n * kMuonChunks)), dim3(256), 0, stream, js, P);
         hipLaunchKernelGGL((muon_init_kernel<T, MOM, NP>), dim3((unsigned)tiles), dim3(256), 0, stream, args);
         muon_steps<NP, T, MOM>(js, args, steps, stream);
@@ -547,14 +843,18 @@ static int muon_exponent(double bound) {
 }
 
 // bounds of the singular values over the steps (from [0, 1]: the Frobenius norm) give the planes' scales
-static bool muon_scales(double a, double b, double c, int steps, MuonNum& P) {
-    double top = 1.0, x = 1.0, poly = 0.0;
+// `few`: whether the form that keeps A = X X^T through the steps may run: an error of A grows by the slope of l p(l)^2 in every step but the last
+static bool muon_scales(double a, double b, double c, int steps, MuonNum& P, bool& few) {
+    double top = 1.0, x = 1.0, poly = 0.0, gain = 1.0, last = 1.0;
     if (!isfinite(a) || !isfinite(b) || !isfinite(c)) return false;
     for (int s = 0; s < steps; ++s) {
         double next = 0.0;
+        gain *= last, last = 1.0;
         for (int k = 0; k <= 512; ++k) {
             const double v = top * k / 512.0, q = v * v;
             const double p = fabs(b * q + c * q * q), w = fabs(a * v + b * v * q + c * v * q * q);
+            const double slope = fabs((a + b * q + c * q * q) * (a + 3.0 * b * q + 5.0 * c * q * q));
+            last = slope > last ? slope : last;
             poly = p > poly ? p : poly;
             next = w > next ? w : next;
         }
@@ -562,6 +862,7 @@ static bool muon_scales(double a, double b, double c, int steps, MuonNum& P) {
         top = next * 1.001 + 1e-6;
         if (!(top <= 16.0)) return false;
     }
+    few = gain <= 1e7;                   // (x 2^-53 x 64: below fp32's half step)
     // (the last step's result is not kept in planes)
     P.ex = muon_exponent(x), P.ea = muon_exponent(x * x), P.eb = muon_exponent(poly > 1e-3 ? poly : 1e-3);
     return true;
@@ -582,11 +883,11 @@ static int muon_check(const FneusMuonJob* jobs, int n_jobs, int steps, int prec,
 }
 
 template <bool MOM>
-static int muon_dispatch(const FneusMuonJob* jobs, int n, const MuonNum& P, int steps, int prec, int dtype, void* scratch, hipStream_t s) {
+static int muon_dispatch(const FneusMuonJob* jobs, int n, const MuonNum& P, int steps, bool few, int prec, int dtype, void* scratch, hipStream_t s) {
     unsigned char* w = (unsigned char*)scratch;
-    if (dtype == DT_F32) return prec == 3 ? muon_run<float, MOM, 2>(jobs, n, P, steps, w, s) : muon_run<float, MOM, 1>(jobs, n, P, steps, w, s);
-    if (dtype == DT_BF16) return prec == 3 ? muon_run<__bf16, MOM, 2>(jobs, n, P, steps, w, s) : muon_run<__bf16, MOM, 1>(jobs, n, P, steps, w, s);
-    return prec == 3 ? muon_run<_Float16, MOM, 2>(jobs, n, P, steps, w, s) : muon_run<_Float16, MOM, 1>(jobs, n, P, steps, w, s);
+    if (dtype == DT_F32) return prec == 3 ? muon_run<float, MOM, 2>(jobs, n, P, steps, few, w, s) : muon_run<float, MOM, 1>(jobs, n, P, steps, few, w, s);
+    if (dtype == DT_BF16) return prec == 3 ? muon_run<__bf16, MOM, 2>(jobs, n, P, steps, few, w, s) : muon_run<__bf16, MOM, 1>(jobs, n, P, steps, few, w, s);
+    return prec == 3 ? muon_run<_Float16, MOM, 2>(jobs, n, P, steps, few, w, s) : muon_run<_Float16, MOM, 1>(jobs, n, P, steps, few, w, s);
 }
 
 }  // namespace fneus
@@ -594,16 +895,15 @@ static int muon_dispatch(const FneusMuonJob* jobs, int n, const MuonNum& P, int 
 using namespace fneus;
 
 extern "C" long fneus_muon_scratch_bytes(const FneusMuonJob* jobs, int n_jobs, int prec) {
-    long most = 0;
+    long most = 0, off;
     if (!jobs) return 0;
-    for (int first = 0; first < n_jobs; first += kMuonMaxJobs) {       // (a further round of launches uses the same memory: one stream)
-        long off = kMuonTable;
-        for (int q = first; q < n_jobs && q < first + kMuonMaxJobs; ++q)
-            if (jobs[q].rows > 0 && jobs[q].cols > 0) off += muon_lay(jobs[q].rows, jobs[q].cols, prec == 3 ? 2 : 1).total;
-        const int n = n_jobs - first < kMuonMaxJobs ? n_jobs - first : kMuonMaxJobs;
-        if (muon_one_shape(jobs + first, n) && muon_shared(jobs[first].rows, jobs[first].cols, n, prec == 3 ? 2 : 1)) off += kMuonPartBytes;
-        most = off > most ? off : most;
-    }
+    const int planes = prec == 3 ? 2 : 1;
+    MuonJobs js;
+    for (int form = MU_ALL; form <= MU_FEW; ++form)       // (a further round of launches uses the same memory: one stream)
+        for (int at = 0; muon_round(jobs, n_jobs, at, form, planes, js, off) > 0;) {
+            if (form != MU_FEW && muon_shared(js, planes)) off += kMuonPartBytes;
+            most = off > most ? off : most;
+        }
     return most;
 }
 
@@ -612,10 +912,11 @@ extern "C" int fneus_newton_schulz(const FneusMuonJob* jobs, int n_jobs, double 
     fneus::clear_status();
     if (int rc = muon_check(jobs, n_jobs, steps, prec, dtype, scratch, scratch_bytes, false)) return rc;
     MuonNum P{};
+    bool few = false;
     P.a = (float)a, P.b = (float)b, P.c = (float)c, P.eps = (float)eps;
-    if (!(eps > 0.0) || !muon_scales(a, b, c, steps, P)) return muon_refuse("fneus_newton_schulz: eps > 0, a polynomial that keeps [0, 1] below 16 over the steps");
+    if (!(P.eps >= 1e-30f) || !muon_scales(a, b, c, steps, P, few)) return muon_refuse("fneus_newton_schulz: eps >= 1e-30, a polynomial that keeps [0, 1] below 16 over the steps");
     if (n_jobs == 0) return 0;
-    return muon_dispatch<false>(jobs, n_jobs, P, steps, prec, dtype, scratch, (hipStream_t)stream);
+    return muon_dispatch<false>(jobs, n_jobs, P, steps, few, prec, dtype, scratch, (hipStream_t)stream);
 }
 
 extern "C" int fneus_muon(const FneusMuonJob* jobs, int n_jobs, const float* lr, double mu, int nesterov, double weight_decay, double a,
@@ -624,9 +925,10 @@ extern "C" int fneus_muon(const FneusMuonJob* jobs, int n_jobs, const float* lr,
     fneus::clear_status();
     if (int rc = muon_check(jobs, n_jobs, steps, prec, dtype, scratch, scratch_bytes, true)) return rc;
     MuonNum P{};
+    bool few = false;
     P.a = (float)a, P.b = (float)b, P.c = (float)c, P.eps = (float)eps;
-    if (!lr || !(eps > 0.0) || !muon_scales(a, b, c, steps, P)) return muon_refuse("fneus_muon: lr, eps > 0, a polynomial that keeps [0, 1] below 16 over the steps");
+    if (!lr || !(P.eps >= 1e-30f) || !muon_scales(a, b, c, steps, P, few)) return muon_refuse("fneus_muon: lr, eps >= 1e-30, a polynomial that keeps [0, 1] below 16 over the steps");
     P.mu = (float)mu, P.omu = (float)(1.0 - mu), P.wd = (float)weight_decay, P.nesterov = nesterov, P.zero_grad = zero_grad, P.lr = lr;
     if (n_jobs == 0) return 0;
-    return muon_dispatch<true>(jobs, n_jobs, P, steps, prec, dtype, scratch, (hipStream_t)stream);
+    return muon_dispatch<true>(jobs, n_jobs, P, steps, few, prec, dtype, scratch, (hipStream_t)stream);
 }

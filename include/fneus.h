@@ -627,7 +627,8 @@ int fneus_composite_bwd(const float* rays_o, const float* rays_d, const float* m
  * Not in the reference.  dtype: 0 fp32, 1 bf16, 2 fp16 (x, y, dy, dx); wtype: the type of weight / bias and of their gradients, dtype or 0.
  * Rows of n values, row strides ld* >= n in elements, any alignment; weight / bias may be NULL (1 / 0).  Statistics and sums in fp32,
  * outputs rounded once.  y = (x - mean) rstd w + b, rstd = 1 / sqrt(var + eps) (var: biased); mean, rstd [rows] are the backward's.
- * rows == 0: nothing is done (forward), refused (backward).  NaN and infinities stay in their row (forward, dx). */
+ * rows == 0: nothing is done (forward), refused (backward).  NaN and infinities stay in their row (forward, dx).
+ * No output may share memory with an input, but y may be x. */
 int fneus_layer_norm_fwd(const void* x, long ldx, const void* weight, const void* bias, void* y, long ldy, float* mean, float* rstd,
                          long rows, int n, float eps, int dtype, int wtype, fneus_stream_t stream);
 /* dx, and dweight / dbias [n] (either may be NULL; OVERWRITTEN) through `scratch` (fneus_layer_norm_bwd_scratch_floats(rows, n) floats):
@@ -645,7 +646,8 @@ long fneus_layer_norm_bwd_scratch_floats(long rows, int n);
  * forward: x, weight, (bias), (residual) -> y and, where z is given, the pre-activation z [rows][n_out] (what the backward of act != 0 reads).
  * backward: dy, x, weight, z -> dx [rows][n_in], dweight [n_out][n_in], dbias [n_out], each where given (OVERWRITTEN); the residual's gradient
  * is dy.  Sums in a fixed order: bit-reproducible.  rows == 0: forward nothing, backward refused.  An fp32 infinity or NaN in an operand
- * gives NaN wherever it takes part.  `scratch`: fneus_linear_scratch_bytes(job, backward) bytes, 16-byte aligned, not shared between calls in flight. */
+ * gives NaN wherever it takes part.  `scratch`: fneus_linear_scratch_bytes(job, backward) bytes, 16-byte aligned, not shared between calls in flight.
+ * No output shares memory with another array (the residual may be x). */
 typedef struct FneusLinear {
     const void *x, *weight, *bias, *residual;
     void *y, *z;
@@ -671,7 +673,8 @@ int fneus_adam(const FneusAdamSegment* segs, int n_segs, const float* lr, float*
 /* ---- optimiser of weight matrices: Muon (beside fneus_adam; not in the reference) ---------------------------------------------------------
  * Newton-Schulz orthogonalisation of each matrix u [rows][cols]: X = u / max(|u|_F, eps), `steps` times  A = X X^T, X <- a X + (b A + c A^2) X
  * (on the transpose where rows > cols).  prec 3: operands as two fp16 terms under power-of-two scales, three products (fp32's accuracy);
- * prec 2: one fp16 product (11 bits; what a 16-bit matrix carries).  Sums in fp32, the norm in fp64.  A zero matrix gives zero.
+ * prec 2: one fp16 product (11 bits; what a 16-bit matrix carries).  Sums in fp32, the norm in fp64.  A shorter side of at most 64: fp64
+ * throughout, whichever prec.  A zero matrix gives zero.  eps >= 1e-30.
  * fneus_newton_schulz: out = NS(grad).  fneus_muon, in place:  momentum <- mu momentum + (1 - mu) grad;  u = (1 - mu) grad + mu momentum
  * (nesterov) or momentum;  param <- param (1 - lr weight_decay) - lr adjust_j NS(u).  lr: device scalar.  dtype: of grad, momentum, param,
  * out (0 fp32, 1 bf16, 2 fp16), all contiguous.  zero_grad != 0 clears each gradient after use.  jobs: HOST array, any number; no two may

@@ -248,3 +248,112 @@ def test_muon_refusals():
             bad()
     with pytest.raises(RuntimeError):
         ops.newton_schulz(p, steps=0)
+
+
+# A side of at most 64: three launches in fp64.  What is left is the rounding of the output: half a step of its type (fp16: of its subnormal
+# values, 2^-25, each), and fp64's of u u^T (2^-53 sqrt(n)) grown by 11.9^4 = 2e4: below 1e-9 for n <= 2^16; 1e-7 covers the fp32 in between.
+def few_bound(t, want):
+    return torch.finfo(t).eps / 2 + 1e-7 + (2.0 ** -25 * want.numel() ** 0.5 / float(want.norm()) if t == torch.float16 else 0.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("size", [(1, 1), (1, 64), (64, 1), (5, 5), (16, 129), (17, 128), (127, 32), (33, 40), (48, 1000), (63, 64), (64, 64), (640, 64),
+                                  (64, 20001), (9999, 15), (2, 65536)], ids=str)
+def test_newton_schulz_of_a_short_side(t, size):
+    from fneus import ops
+    g = (matrix(*size) * (100 if t == torch.float16 else 1)).to(t)
+    want = ns64(g)
+    for prec in (ops.PREC_PARITY, ops.PREC_H16):
+        assert off(ops.newton_schulz(g.cuda(), prec=prec), want) <= few_bound(t, want)
+
+
+@pytest.mark.gpu
+def test_newton_schulz_of_a_short_side_properties():
+    """step counts and polynomials on both sides of the rule for the form; rank-deficient, zero, tiny, huge, NaN matrices; a stack"""
+    from fneus import ops
+    g = matrix(40, 90).cuda()
+    for coef, steps in ((C3, 1), (C3, 2), (C3, 7), ((2.0, -1.5, 0.5), 3), ((1.875, -1.25, 0.375), 12), ((8.28, -23.6, 17.3), 1)):
+        want = ns64(g.cpu(), steps, coef=coef)
+        assert off(ops.newton_schulz(g, coefficients=coef, steps=steps), want) <= few_bound(torch.float32, want)
+    low = (matrix(60, 2) @ matrix(2, 50)).cuda()
+    for steps in (5, 7, 8, 30):                 # (from 8 steps on an error of A has room to grow: the tiled form)
+        s = torch.linalg.svdvals(ops.newton_schulz(low, steps=steps).double())
+        assert bool(torch.isfinite(s).all()) and float(s[0]) < 1.25
+    # rank 2 but for the entries' own fp32 rounding, which the same fp64 polynomial amplifies in both
+    assert off(ops.newton_schulz(low), ns64(low.cpu())) <= few_bound(torch.float32, ns64(low.cpu()))
+    assert float(ops.newton_schulz(torch.zeros(20, 30, device="cuda")).abs().max()) == 0.0
+    for f in (2.0 ** 40, 2.0 ** -40):
+        assert torch.equal(ops.newton_schulz(g * f, eps=1e-30), ops.newton_schulz(g, eps=1e-30))
+    assert off(ops.newton_schulz(g * 1e34), ns64(g.cpu())) <= 1e-6          # (g 1e34: a rounding of every entry)
+    bad = g.clone()
+    bad[3, 4] = float("nan")
+    assert bool(torch.isnan(ops.newton_schulz(bad)).all())
+    stack = torch.stack([matrix(30, 70, seed=k) for k in range(70)]).cuda()
+    out = ops.newton_schulz(stack)
+    for k in (0, 31, 32, 69):
+        assert torch.equal(out[k], ops.newton_schulz(stack[k]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16])
+def test_muon_of_short_and_long_sides_together(t):
+    """more matrices of each form than a round of launches takes, in one call; gradients cleared, neighbours in memory left alone"""
+    from fneus import ops
+    sizes = [((7 + k, 300 - k) if k % 2 else (70 + k, 66 + k)) if k % 3 else (130 + k, 5 + k // 2) for k in range(80)]
+    n = sum(r * c + 1 for r, c in sizes)
+    arenas = [torch.full((n,), 7.0, dtype=t, device="cuda") for _ in range(3)]
+    sets, at = ([], [], []), 0
+    for r, c in sizes:
+        for k, (arena, out) in enumerate(zip(arenas, sets)):
+            out.append(arena[at:at + r * c].view(r, c))
+            out[-1].copy_(matrix(r, c, seed=k).mul(100))
+        at += r * c + 1
+    ps, gs, ms = sets
+    p0, g0, m0 = ([x.cpu().clone() for x in s] for s in sets)
+    lr = torch.full((), 0.03, device="cuda")
+    ops.muon_step(ps, gs, ms, lr, momentum=0.9, weight_decay=0.1, adjust=1.0, zero_grad=True)
+    prec, half = (3 if t == torch.float32 else 2), torch.finfo(t).eps / 2
+    f, lr = torch.float32, 0.03
+    for k in range(len(sizes)):
+        m1 = ms[k].cpu()
+        # (three fp32 roundings in front of the one to t)
+        assert off(m1, 0.9 * m0[k].double() + (1 - 0.9) * g0[k].double()) <= half + 4 * 2.0 ** -24
+        u = (1 - 0.9) * g0[k].double() + 0.9 * m1.double()
+        want = p0[k].double() * (1 - lr * 0.1) - lr * ns64(u)
+        err = lr * bound(prec, f) * float(ns64(u).norm()) / float(want.norm())
+        assert off(ps[k], want) <= half + 4 * 2.0 ** -24 + err, sizes[k]
+        assert float(gs[k].abs().max()) == 0.0
+    at = 0
+    for r, c in sizes:
+        at += r * c + 1
+        assert all(float(a[at - 1]) == 7.0 for a in arenas)
+
+
+@pytest.mark.gpu
+def test_muon_of_a_short_side_in_a_graph():
+    """replayed with new gradients and learning rates and eager work in between, against the eager step, bit for bit"""
+    from fneus import ops
+    sizes = [(64, 300), (40, 17), (1000, 33), (128, 128)]
+    ps, gs, ms = ([matrix(*s, seed=k).cuda() for s in sizes] for k in (1, 2, 3))
+    pe, me = [p.clone() for p in ps], [m.clone() for m in ms]
+    lr = torch.full((), 0.02, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ops.muon_step(ps, gs, ms, lr)
+    torch.cuda.current_stream().wait_stream(side)
+    for dst, src in zip(ps + ms, pe + me):
+        dst.copy_(src)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.muon_step(ps, gs, ms, lr)
+    for k in range(4):
+        for g, s in zip(gs, sizes):
+            g.copy_(matrix(*s, seed=10 + k))
+        lr.fill_(0.01 * (k + 1))
+        graph.replay()
+        torch.cuda.synchronize()
+        ops.muon_step(pe, gs, me, lr)
+        for a, b in zip(ps + ms, pe + me):
+            assert torch.equal(a, b)
