@@ -5,7 +5,8 @@
 // matrix rate the part sustains; an fp32 product is six bf16 ones).  MEASURED (MI355X, us): 1 x 4096 -> 4096 bf16 SiLU + residual 7.9 (4.3 TB/s of
 // W); 512 x 512 -> 512 fp32 forward 9, backward 27; 65536 x 256 -> 256 fp32 softplus + residual forward 102, delta 45, dx 63 (0.82 PFLOP/s of
 // MFMAs), dW 67 + 5 + 5; 8192 x 4096 -> 8192 bf16 dx 465 (1.18 PFLOP/s; the library's 8192^3: 1.34), dW 484, forward with GELU, residual and
-// the stored pre-activation 625 (its epilogue has nothing to run beside at one workgroup a CU), delta 93.
+// the stored pre-activation 625 (its epilogue has nothing to run beside at one workgroup a CU), delta 93.  Heads (up to 16 outputs) have a
+// form of their own each way, bound by reading x: 18135 x 4308 -> 1 fp32 forward 73 (4.3 TB/s), backward 157 (6 TB/s with the caches' help).
 #include <type_traits>
 #include "mm_engine.h"
 #include "fneus_kernels.h"
@@ -161,7 +162,8 @@ __global__ void __launch_bounds__(512) linear_direct_bwd_kernel(LinProduct dx, L
 
 // Up to 16 rows (tokens): reading W once is all there is.  A workgroup owns 16 outputs, its 8 waves split the contraction, a wave's
 // load covers 64 consecutive bytes of each of its 16 weight rows and UNROLL of them are in flight.
-template <class T>
+// HEAD: the same with the operands' places exchanged, for up to 16 outputs: reading x once is all there is, a workgroup owns 16 rows (a = W, b = x).
+template <class T, bool HEAD>
 __global__ void __launch_bounds__(512) linear_row_kernel(LinProduct P) {
     __shared__ float red[8][16][17];
     const int j0 = 16 * (int)blockIdx.x;
@@ -196,17 +198,18 @@ __global__ void __launch_bounds__(512) linear_row_kernel(LinProduct P) {
     for (int e = 0; e < 4; ++e) red[wave][4 * g + e][r] = acc[e];        // row j = 4 g + e, column i = r
     __syncthreads();
     if (threadIdx.x < 256) {
-        const int jj = threadIdx.x & 15, ii = threadIdx.x >> 4;
-        const int gj = j0 + jj;
+        const int lo = threadIdx.x & 15, hi = threadIdx.x >> 4, jj = HEAD ? hi : lo, ii = HEAD ? lo : hi;
         float v = 0.0f;
 #pragma unroll
         for (int w = 0; w < 8; ++w) v += red[w][jj][ii];
-        if (ii < P.ni && gj < P.nj) {
-            if (P.bias) v += (float)((const T*)P.bias)[gj];
-            if (P.z) ((T*)P.z)[ii * P.ldd + gj] = (T)v;
+        if (ii < P.ni && j0 + jj < P.nj) {
+            const long row = HEAD ? j0 + jj : ii;
+            const int col = HEAD ? ii : j0 + jj;
+            if (P.bias) v += (float)((const T*)P.bias)[col];
+            if (P.z) ((T*)P.z)[row * P.ldd + col] = (T)v;
             v = lin_act(v, P.act);
-            if (P.res) v += (float)((const T*)P.res)[ii * P.ldres + gj];
-            ((T*)P.d)[ii * P.ldd + gj] = (T)v;
+            if (P.res) v += (float)((const T*)P.res)[row * P.ldres + col];
+            ((T*)P.d)[row * P.ldd + col] = (T)v;
         }
     }
 }
@@ -337,6 +340,119 @@ __global__ void __launch_bounds__(256) linear_reduce_kernel(LinTiled P) {
     else quad_store<T>((T*)P.d + i * P.ldd + j, valid, v);
 }
 
+// The gradients of a layer with up to 16 outputs (a head): one pass over x and dx, whose bytes are all there is.  A thread owns four columns: their
+// weights and their sums of dW stay in fp32 registers, delta = dy act'(z) of kHeadRows rows lies in LDS (unrounded).  `lanes` threads share a
+// row, the others of a workgroup take further rows; a workgroup leaves its part of dW and of the bias gradient, added in order by
+// linear_reduce_kernel and linear_fold_kernel.  The last columns' thread takes the row's last four (what it shares with its neighbour is written
+// twice, the same).
+constexpr int kHeadRows = 64;
+template <class T>
+struct LinHead {
+    const T *dy, *z, *x, *w;
+    T* dx;
+    float *part, *sums;                 // [parts][n_out][n_in], [parts][n_out]
+    long lddy, ldx, rows, per;          // per: rows a part
+    int n_in, n_out, act, lanes, strips, pad_;
+};
+template <class T, int N, bool DX, bool DW>
+__global__ void __launch_bounds__(256) linear_head_bwd_kernel(LinHead<T> a) {
+    __shared__ __attribute__((aligned(16))) float delta[kHeadRows][N];
+    __shared__ f32x4 fold[256];
+    typedef typename Quad<T>::type Q;
+    const int strip = blockIdx.x % a.strips, part = blockIdx.x / a.strips;
+    const int c = threadIdx.x & (a.lanes - 1), g = threadIdx.x / a.lanes, groups = 256 / a.lanes;
+    const int at = (strip * a.lanes + c) * 4, col = at < a.n_in - 4 ? at : a.n_in - 4;
+    const bool live = at < a.n_in;
+    const long r0 = part * a.per, r1 = r0 + a.per < a.rows ? r0 + a.per : a.rows;
+    float w[N][4], acc[N][4], db = 0.0f;
+#pragma unroll
+    for (int o = 0; o < N; ++o) {
+        Q q = {};
+        if constexpr (DX) q = *reinterpret_cast<const Q*>(a.w + (long)(o < a.n_out ? o : a.n_out - 1) * a.n_in + col);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[o][k] = o < a.n_out ? (float)q[k] : 0.0f, acc[o][k] = 0.0f;
+    }
+    for (long rb = r0; rb < r1; rb += kHeadRows) {
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < kHeadRows * N / 256; ++q) {
+            const int idx = (int)threadIdx.x + 256 * q, o = idx % N;
+            const long row = rb + idx / N;
+            const bool ok = row < r1 && o < a.n_out;
+            const long ra = row < r1 ? row : r1 - 1;
+            const int oa = o < a.n_out ? o : 0;
+            float d = (float)a.dy[ra * a.lddy + oa];
+            if (a.z) d *= lin_dact((float)a.z[ra * a.n_out + oa], a.act);
+            d = ok ? d : 0.0f;
+            delta[idx / N][o] = d;
+            db += d;
+        }
+        __syncthreads();
+        for (int s = g; s < kHeadRows; s += 4 * groups) {
+            if (rb + s >= r1) break;
+            Q x[4];
+            if constexpr (DW) {
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const long row = rb + s + u * groups;
+                    x[u] = *reinterpret_cast<const Q*>(a.x + (row < r1 ? row : r1 - 1) * a.ldx + col);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const long row = rb + s + u * groups;
+                if (row < r1) {
+                    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int o = 0; o < N; o += 4) {
+                        const f32x4 d = *reinterpret_cast<const f32x4*>(&delta[s + u * groups][o]);
+#pragma unroll
+                        for (int p = 0; p < 4; ++p)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                if constexpr (DX) v[k] += d[p] * w[o + p][k];
+                                if constexpr (DW) acc[o + p][k] += d[p] * (float)x[u][k];
+                            }
+                    }
+                    if constexpr (DX) {
+                        Q q;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) q[k] = (T)v[k];
+                        if (live) *reinterpret_cast<Q*>(a.dx + row * a.n_in + col) = q;
+                    }
+                }
+            }
+        }
+    }
+    if constexpr (DW) {
+#pragma unroll
+        for (int o = 0; o < N; ++o) {
+            if (o < a.n_out) {
+                f32x4 v = {acc[o][0], acc[o][1], acc[o][2], acc[o][3]};
+                if (groups > 1) {
+                    __syncthreads();
+                    fold[threadIdx.x] = v;
+                    __syncthreads();
+                    for (int q = 1; q < groups && g == 0; ++q) v += fold[c + q * a.lanes];
+                }
+                if (g == 0 && live) *reinterpret_cast<f32x4_u*>(a.part + ((long)part * a.n_out + o) * a.n_in + col) = v;
+            }
+        }
+    }
+    if (a.sums && strip == 0) {
+        float* red = reinterpret_cast<float*>(fold);
+        __syncthreads();
+        red[threadIdx.x] = db;                       // (of output threadIdx % N)
+        __syncthreads();
+        if ((int)threadIdx.x < a.n_out) {
+            float v = 0.0f;
+#pragma unroll 8
+            for (int q = threadIdx.x; q < 256; q += N) v += red[q];
+            a.sums[(long)part * a.n_out + threadIdx.x] = v;
+        }
+    }
+}
+
 // What a product needs ready, in one launch: matrices whose rows its 16-byte accesses do not fit, copied to rows that do (zeros behind), and
 // delta = dy act'(z) (rounded to T for the products; rows of ldp, zeros behind) with the column sums of delta before that rounding, a
 // partial row of sums for every `sum_parts`-th of the rows.
@@ -452,7 +568,9 @@ static LinShape lin_shape(long ni, long nj, long nk) {
 // Everything a call launches and where its scratch lies.
 struct LinPlan {
     bool tiled;
-    bool pad_x, pad_w, delta;
+    bool pad_x, pad_w, delta, head;            // head: linear_head_bwd_kernel, `parts` parts of `per` rows
+    int parts, lanes, strips;
+    long per;
     int ldx, ldw, ldd, sum_parts;              // padded row lengths
     LinShape fwd, dx, dw;
     long off_x, off_w, off_delta, off_sums, off_part, total;
@@ -473,24 +591,49 @@ static bool lin_aligned(const void* p, long ld, long n, bool k_major) {
 // and for the weight gradient, whose contraction the direct form does not split, up to 1024 rows.  Where the contraction is short its eight
 // waves have nothing to split: at most 8192 tiles (65536 x 3 -> 256 fp32, 16384 of them, 60 against 36), and of a few rows' weight gradient at
 // most 1024 (16 x 8192 -> 8192 fp32, 65536 of them, 683 against 86).
+// Heads (up to 16 outputs) take linear_row_kernel<HEAD>: MEASURED (us, it against the tiled or direct form) fp32 18135 x 4308 -> 1 73 / 106, 23662 x 6183
+// -> 2 141 / 459 (rows that had to be copied), 1444 x 4919 -> 12 19 / 44, 512 x 512 -> 3 5.0 / 7.3, 65536 x 512 -> 3 29 / 36; bf16 36042 x 909 -> 8 33 / 48;
+// but 65536 x 256 -> 16 23 / 21, 65536 x 32 -> 4 11 / 9: not where many rows are short for its eight waves.
+static bool lin_head(const FneusLinear& f) { return f.n_out <= 16 && (f.n_in > 256 || f.rows <= 8192); }
+
 template <class T>
 static bool lin_direct(const FneusLinear& f, bool backward) {
-    if (!backward && f.rows <= 16) return true;
+    if (!backward && (f.rows <= 16 || lin_head(f))) return true;
     const double work = (double)f.rows * f.n_in * f.n_out;
     const long ti = (f.rows + 31) / 32, tj = (f.n_in + 31) / 32, to = (f.n_out + 31) / 32;
     if (backward) return f.rows <= 1024 && work <= (double)(1L << 27) && (ti + to) * tj <= (f.rows > 16 ? 8192 : 1024);
     return work <= (double)(sizeof(T) == 4 ? 1L << 28 : 1L << 27) && ti * to <= 8192;
 }
 
+// Heads, backward: MEASURED (us, dx, dW and db, linear_head_bwd_kernel against the others) fp32 65536 x 256 -> 1 40 / 65, -> 16 43 / 66, 200000 x 96 -> 3
+// 45 / 129, 23662 x 6183 -> 2 333 / 637, 2000 x 2000 -> 4 26 / 37; bf16 32 / 46, 43 / 50, 39 / 105, 201 / 336, 26 / 31; but 512 x 512 -> 3 16 / 16 (bf16 17 / 13),
+// 200 x 4000 -> 6 26 / 15, 8000 x 2000 -> 16 70 / 61 (bf16 74 / 41): many rows, fewer where the outputs are few.
+static bool lin_head_bwd(const FneusLinear& f) { return f.n_out <= 16 && f.n_in >= 16 && f.rows > (f.n_out <= 8 ? 1024 : 32768) && (f.dx || f.dweight); }
+
 template <class T>
 static LinPlan lin_plan(const FneusLinear& f, bool backward) {
     constexpr int V = 16 / (int)sizeof(T);
     LinPlan p;
     memset(&p, 0, sizeof p);
-    p.tiled = !lin_direct<T>(f, backward);
-    if (!p.tiled) return p;
     long o = 0, part = 0;
     auto take = [&](long bytes) { const long at = o; o += lin_up(bytes, 256); return at; };
+    if (backward && lin_head_bwd(f)) {
+        // as many threads a row as it has quads (16 .. 256), 1024 workgroups, and no more parts than keep their sums a small part of x's bytes
+        p.head = true;
+        for (p.lanes = 16; p.lanes < 256 && p.lanes * 4 < f.n_in;) p.lanes *= 2;
+        p.strips = (f.n_in + 4 * p.lanes - 1) / (4 * p.lanes);
+        const long rows = f.n_out * 8 > kHeadRows && f.dweight ? 2 * kHeadRows : kHeadRows;
+        long parts = (1024 + p.strips - 1) / p.strips, most = (f.rows + rows - 1) / rows;
+        parts = parts < most ? parts : most;
+        p.per = lin_up((f.rows + parts - 1) / parts, kHeadRows);
+        p.parts = (int)((f.rows + p.per - 1) / p.per);
+        if (f.dbias) p.off_sums = take((long)p.parts * f.n_out * 4);
+        p.off_part = o;
+        p.total = f.dweight ? o + (long)p.parts * f.n_out * f.n_in * 4 : o;
+        return p;
+    }
+    p.tiled = !lin_direct<T>(f, backward);
+    if (!p.tiled) return p;
     auto partial = [&](const LinShape& s, long ni, long nj) { if (s.splits > 1) { const long b = (long)s.splits * ni * nj * 4; part = b > part ? b : part; } };
     if (!backward) {
         p.pad_x = !lin_aligned<T>(f.x, f.ldx, f.n_in, false);
@@ -556,6 +699,13 @@ static void lin_tiled_with(LinTiled t, long nk, hipStream_t stream) {
     else lin_tiled_whole<Cfg, T, AKM, BKM, FWD>(t, stream);
 }
 
+template <class T, bool FWD>
+static void lin_reduce(const LinTiled& t, hipStream_t stream) {
+    const long quads = t.ni * ((t.nj + 3) / 4);
+    if (t.splits >= 16) hipLaunchKernelGGL((linear_reduce_kernel<T, FWD, 8>), dim3((unsigned)((quads + 31) / 32)), dim3(256), 0, stream, t);
+    else hipLaunchKernelGGL((linear_reduce_kernel<T, FWD, 1>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, stream, t);
+}
+
 template <class T, bool AKM, bool BKM, bool FWD>
 static void lin_tiled_product(LinTiled t, const LinShape& s, long nk, float* partial, hipStream_t stream) {
     const int b = s.tile;
@@ -567,11 +717,7 @@ static void lin_tiled_product(LinTiled t, const LinShape& s, long nk, float* par
     else if (s.tile == 128) lin_tiled_with<LinMid8, T, AKM, BKM, FWD>(t, nk, stream);
     else if (!few) lin_tiled_with<LinSmall, T, AKM, BKM, FWD>(t, nk, stream);
     else lin_tiled_with<LinSmall8, T, AKM, BKM, FWD>(t, nk, stream);
-    if (s.splits > 1) {
-        const long quads = t.ni * ((t.nj + 3) / 4);
-        if (s.splits >= 16) hipLaunchKernelGGL((linear_reduce_kernel<T, FWD, 8>), dim3((unsigned)((quads + 31) / 32)), dim3(256), 0, stream, t);
-        else hipLaunchKernelGGL((linear_reduce_kernel<T, FWD, 1>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, stream, t);
-    }
+    if (s.splits > 1) lin_reduce<T, FWD>(t, stream);
 }
 
 template <class T>
@@ -631,6 +777,33 @@ static void lin_tiled_bwd(const FneusLinear& f, const LinPlan& p, hipStream_t st
     }
 }
 
+template <class T, int N>
+static void lin_head_launch(const LinHead<T>& h, int parts, bool dw, hipStream_t stream) {
+    const dim3 grid((unsigned)(h.strips * parts));
+    if (h.dx && dw) hipLaunchKernelGGL((linear_head_bwd_kernel<T, N, true, true>), grid, dim3(256), 0, stream, h);
+    else if (h.dx) hipLaunchKernelGGL((linear_head_bwd_kernel<T, N, true, false>), grid, dim3(256), 0, stream, h);
+    else hipLaunchKernelGGL((linear_head_bwd_kernel<T, N, false, true>), grid, dim3(256), 0, stream, h);
+}
+
+template <class T>
+static void lin_head_run(const FneusLinear& f, const LinPlan& p, hipStream_t stream) {
+    unsigned char* S = (unsigned char*)f.scratch;
+    LinHead<T> h{};
+    h.dy = (const T*)f.dy, h.z = f.act ? (const T*)f.z : nullptr, h.x = (const T*)f.x, h.w = (const T*)f.weight, h.dx = (T*)f.dx;
+    h.part = (float*)(S + p.off_part), h.sums = f.dbias ? (float*)(S + p.off_sums) : nullptr;
+    h.lddy = f.lddy, h.ldx = f.ldx, h.rows = f.rows, h.per = p.per;
+    h.n_in = f.n_in, h.n_out = f.n_out, h.act = f.act, h.lanes = p.lanes, h.strips = p.strips;
+    if (f.n_out <= 4) lin_head_launch<T, 4>(h, p.parts, f.dweight, stream);
+    else if (f.n_out <= 8) lin_head_launch<T, 8>(h, p.parts, f.dweight, stream);
+    else lin_head_launch<T, 16>(h, p.parts, f.dweight, stream);
+    if (f.dweight) {
+        LinTiled t{};
+        t.d = f.dweight, t.ldd = f.n_in, t.ni = f.n_out, t.nj = f.n_in, t.splits = p.parts, t.partial = h.part;
+        lin_reduce<T, false>(t, stream);
+    }
+    if (f.dbias) hipLaunchKernelGGL((linear_fold_kernel<T>), dim3((unsigned)((f.n_out + 7) / 8)), dim3(1024), 0, stream, h.sums, p.parts, f.n_out, (T*)f.dbias);
+}
+
 static int lin_refuse(const char* msg) {
     set_last_error(msg);
     return -2;
@@ -669,7 +842,12 @@ static int lin_fwd(const FneusLinear& f, hipStream_t stream) {
     p.a = f.x, p.lda = f.ldx, p.b = f.weight, p.ldb = f.n_in, p.bias = f.bias, p.res = f.residual, p.ldres = f.ld_residual;
     p.d = f.y, p.z = f.z, p.ldd = f.n_out, p.ni = f.rows, p.nj = f.n_out, p.nk = f.n_in, p.act = f.act;
     if (f.rows <= 16) {
-        hipLaunchKernelGGL((linear_row_kernel<T>), dim3((unsigned)((f.n_out + 15) / 16)), dim3(512), 0, stream, p);
+        hipLaunchKernelGGL((linear_row_kernel<T, false>), dim3((unsigned)((f.n_out + 15) / 16)), dim3(512), 0, stream, p);
+        return launch_status();
+    }
+    if (lin_head(f)) {
+        p.a = f.weight, p.lda = f.n_in, p.b = f.x, p.ldb = f.ldx, p.ni = f.n_out, p.nj = (int)f.rows;
+        hipLaunchKernelGGL((linear_row_kernel<T, true>), dim3((unsigned)((f.rows + 15) / 16)), dim3(512), 0, stream, p);
         return launch_status();
     }
     p.tiles_j = (p.nj + 31) / 32;
@@ -685,6 +863,11 @@ static int lin_bwd(const FneusLinear& f, hipStream_t stream) {
     if (plan.tiled) {
         if (!lin_scratch_ok(f, plan)) return lin_refuse("fneus_linear_bwd: scratch of fneus_linear_scratch_bytes bytes, 16-byte aligned, must be given");
         lin_tiled_bwd<T>(f, plan, stream);
+        return launch_status();
+    }
+    if (plan.head) {
+        if (!lin_scratch_ok(f, plan)) return lin_refuse("fneus_linear_bwd: scratch of fneus_linear_scratch_bytes bytes, 16-byte aligned, must be given");
+        lin_head_run<T>(f, plan, stream);
         return launch_status();
     }
     LinProduct dx{}, dw{};

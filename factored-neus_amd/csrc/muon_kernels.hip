@@ -4,7 +4,7 @@
 // All three products run on the tiled engine (mm_engine.h): X X^T and A A on operands stored along k, B X with X k-major.
 //
 // Numbers: fp16 planes with fp32 sums.  Every entry of X, A and B is bounded (the polynomial keeps the singular values below about 1.2),
-// entries as small as 1 / n matter, and the fp16 matrix instruction takes subnormal operands as zero, so a plane holds its matrix times a
+// entries as small as 1 / n matter, and fp16 loses digits below 2^-14, so a plane holds its matrix times a
 // power of two that puts the bound just below fp16's largest value (2^14 for the usual coefficients).  prec 2: one plane, 11 bits -- the
 // error that 16-bit gradients bring along, an eighth of what bf16 operands would add.  prec 3: a second plane holds what the first one's
 // rounding left, times another 2^11, so that it is as normal as the first; products hi hi + hi lo + lo hi (22 bits: fp32's accuracy at

@@ -91,8 +91,8 @@ def forward_and_backward(rows, n_in, n_out, t, act, res, bias=True, need=(True, 
             continue
         total = {"dx": d.abs() @ wd.abs(), "dw": d.abs().t() @ xd.abs(), "db": d.abs().sum(0)}[what]
         lim = lim + sums(k) * total
-        flush = tiny * {"dx": wd.abs().sum(0)[None, :], "dw": xd.abs().sum(0)[None, :], "db": torch.zeros_like(want)}[what] * (t == torch.float16)
-        check(got, want, lim + half(t) * (want.abs() + lim) + tiny + flush, what)      # (fp16: operands below its normal range count as zero)
+        flush = 2.0 ** -25 * {"dx": wd.abs().sum(0)[None, :], "dw": xd.abs().sum(0)[None, :], "db": torch.zeros_like(want)}[what] * (t == torch.float16)
+        check(got, want, lim + half(t) * (want.abs() + lim) + tiny + flush, what)      # (fp16: delta below its normal range, half a step of 2^-24)
     assert [g is not None for g in (dx, dw, db)] == list(need)
     return y, z, dx, dw, db
 
@@ -285,3 +285,76 @@ def test_linear_refusals():
                 lambda: ops.linear_fwd(x, w[:0])):
         with pytest.raises(ValueError):
             bad()
+
+
+# Heads: up to 16 outputs (their own form each way), on both sides of the rules for it and of its blocks: 64 rows, lanes of 4 columns, strips of
+# 1024 columns, the last four columns shared; more parts than one
+HEADS = [(1025, 16, 1), (1024, 64, 8), (1100, 17, 4), (3000, 63, 5), (2049, 257, 3), (5000, 1031, 8), (9000, 4100, 2), (70001, 18, 7), (33000, 260, 16),
+         (40000, 41, 9), (8200, 300, 16), (100, 5001, 16), (17, 300, 12), (1026, 15, 4)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("size", HEADS, ids=str)
+def test_linear_heads(t, size):
+    forward_and_backward(*size, t, "sigmoid", True)
+    forward_and_backward(*size, t, "none", False, bias=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("need", [(True, False, False), (False, True, False), (False, False, True), (True, True, False), (False, True, True),
+                                  (True, False, True)], ids=str)
+def test_linear_heads_one_gradient_at_a_time(need):
+    for size in ((3000, 90, 3), (3000, 1500, 8), (34000, 100, 16)):
+        forward_and_backward(*size, torch.bfloat16, "silu", False, need=need)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", TYPES)
+def test_linear_heads_strided_rows_and_neighbours(t):
+    """rows apart, unaligned starts; nothing outside the outputs is written; the same bits twice; an infinite x stays in its own row and column"""
+    from fneus import ops
+    rows, n_in, n_out = 3001, 517, 6
+    x, w, b, r, dy = inputs(rows, n_in, n_out, t)
+    wide = torch.zeros(rows, n_in + 9, dtype=t, device="cuda")
+    wide[:, 3:3 + n_in] = x
+    dwide = torch.zeros(rows, n_out + 5, dtype=t, device="cuda")
+    dwide[:, 1:1 + n_out] = dy
+    y, z = ops.linear_fwd(x, w, b, act="silu", residual=r, train=True)
+    y2, z2 = ops.linear_fwd(wide[:, 3:3 + n_in], w, b, act="silu", residual=r, train=True)
+    assert torch.equal(y, y2) and torch.equal(z, z2)
+    g = ops.linear_bwd(dy, x, w, z, act="silu")
+    g2 = ops.linear_bwd(dwide[:, 1:1 + n_out], wide[:, 3:3 + n_in], w, z, act="silu")
+    assert all(torch.equal(p, q) for p, q in zip(g, g2))
+    assert float(wide[:, :3].abs().max()) == 0.0 and float(wide[:, 3 + n_in:].abs().max()) == 0.0
+    bad = x.clone()
+    bad[rows - 1, 7] = float("inf")
+    dx, dw, db = ops.linear_bwd(dy, bad, w, z, act="silu")
+    assert torch.equal(dx, g[0]) and torch.equal(db, g[2])
+    keep = [c for c in range(n_in) if c != 7]
+    assert torch.equal(dw[:, keep], g[1][:, keep]) and not bool(torch.isfinite(dw[:, 7]).any())
+
+
+@pytest.mark.gpu
+def test_linear_heads_in_a_graph():
+    """replayed with other inputs and eager work in between, against the eager calls, bit for bit"""
+    from fneus import ops
+    x, w, b, r, dy = inputs(5000, 300, 3, torch.float32)
+
+    def run():
+        y, z = ops.linear_fwd(x, w, b, act="softplus", residual=r, train=True)
+        return (y,) + ops.linear_bwd(dy, x, w, z, act="softplus")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for k in range(4):
+        for t, s in zip((x, w, b, r, dy), inputs(5000, 300, 3, torch.float32, seed=k + 1)):
+            t.copy_(s)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(out, run()))
