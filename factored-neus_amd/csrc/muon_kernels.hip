@@ -54,7 +54,7 @@ struct MuonArgs {
     unsigned char* scratch;
     int first[kMuonMaxJobs];
     // a symmetric product whose contractions are shared out evenly: `stages` a tile, parts of tiles at `parts`
-    int stages, pad_;
+    int stages, shares, narrow, pad_;        // narrow: X X^T alone, in 64-wide tiles
     float* parts;
 };
 constexpr long kMuonTable = kMuonMaxJobs * sizeof(MuonJob);
@@ -241,7 +241,7 @@ FN_DEV void muon_upper(int t, int& ti, int& tj) {
 constexpr int kMuonParts = 256;
 template <class Cfg>
 FN_DEV float* muon_part(const MuonArgs& a, int wg, int which) { return a.parts + ((long)wg * 2 + which) * (Cfg::BM * Cfg::BN) + threadIdx.x * 4; }
-FN_DEV long muon_part_begin(const MuonArgs& a, long wg) { return wg * a.total * a.stages / kMuonParts; }
+FN_DEV long muon_part_begin(const MuonArgs& a, long wg) { return wg * a.total * a.stages / a.shares; }
 
 template <class Cfg>
 FN_DEV void muon_join(const MuonArgs& a, int tile, f32x16 (&acc)[Cfg::MI][Cfg::NJ]) {
@@ -252,10 +252,10 @@ FN_DEV void muon_join(const MuonArgs& a, int tile, f32x16 (&acc)[Cfg::MI][Cfg::N
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[m][n][e] = 0.0f;
     const long lo = (long)tile * a.stages, hi = lo + a.stages, all = (long)a.total * a.stages;
-    int w = (int)(lo * kMuonParts / all);
+    int w = (int)(lo * a.shares / all);
     while (w > 0 && muon_part_begin(a, w) > lo) --w;
     while (muon_part_begin(a, w + 1) <= lo) ++w;              // the part that holds the tile's first stage
-    for (; w < kMuonParts && muon_part_begin(a, w) < hi; ++w) {
+    for (; w < a.shares && muon_part_begin(a, w) < hi; ++w) {
         const float* p = muon_part<Cfg>(a, w, muon_part_begin(a, w) < lo ? 1 : 0);
 #pragma unroll
         for (int m = 0; m < Cfg::MI; ++m)
@@ -273,7 +273,7 @@ FN_DEV void muon_join(const MuonArgs& a, int tile, f32x16 (&acc)[Cfg::MI][Cfg::N
 template <class Cfg, int NP, int KIND>
 __global__ void __launch_bounds__(Cfg::THREADS, 2) muon_part_kernel(MuonArgs args) {
     extern __shared__ __attribute__((aligned(16))) unsigned char mm_smem[];
-    const int wg = (int)mm_spread(blockIdx.x, kMuonParts);
+    const int wg = (int)mm_spread(blockIdx.x, args.shares);
     long at = muon_part_begin(args, wg);
     const long end = muon_part_begin(args, wg + 1);
 #pragma unroll 1
@@ -705,13 +705,31 @@ static long muon_tiles(long m, long n, bool sym, int b) {
 // whether a symmetric product is shared out evenly: one shape (every tile as long), enough 256-wide tiles and stages that the parts are worth
 // their way through memory, and no more tiles than parts (a part then ends at most one tile).  MEASURED at 4096^2, prec 3 (us a product): 528
 // tiles of 128 x 128 310, shared out 206 and 38 .. 72 to join
-static bool muon_shared(const MuonJobs& js, int planes) {
+static bool muon_one_shape(const MuonJobs& js) {
     for (int q = 1; q < js.n; ++q)
         if (js.j[q].rows != js.j[0].rows || js.j[q].cols != js.j[0].cols) return false;
+    return true;
+}
+static bool muon_shared(const MuonJobs& js, int planes) {
+    if (!muon_one_shape(js)) return false;
     const long m = js.j[0].rows < js.j[0].cols ? js.j[0].rows : js.j[0].cols, tiles = muon_tiles(m, m, true, 256) * js.n;
     return tiles >= 96 && tiles <= kMuonParts && m >= 1024 * (3 - planes);
 }
-constexpr long kMuonPartBytes = (long)kMuonParts * 2 * MuonBig::BM * MuonBig::BN * 4;
+// The same with 64-wide tiles for X X^T of a few rows that are long: tiles and stages such that what the other CUs take over, at 0.4 us a stage, is
+// worth the launch that joins.  MEASURED (us a call, shared out against not; in brackets the stages taken over): fp32 65 x 65536 505 / 3540
+// [3036], 256 x 4096 247 / 358 [185], 2975 x 422 300 / 383 [128], 3 x (188 x 1436) 215 / 226 [67], 4 x (512 x 2048) 363 / 343 [42], 2 x (128 x 640)
+// 156 / 147 [29]; bf16 256 x 4096 180 / 190 [62], 2975 x 422 221 / 216 [43]
+typedef MmCfg<64, 64, 2, 2, 4> MuonPart;
+static bool muon_gram_shared(const MuonJobs& js, int planes) {
+    if (!muon_one_shape(js)) return false;
+    const long m = js.j[0].rows < js.j[0].cols ? js.j[0].rows : js.j[0].cols, n = js.j[0].rows < js.j[0].cols ? js.j[0].cols : js.j[0].rows;
+    const long tiles = muon_tiles(m, m, true, 64) * js.n, stages = (planes == 2 ? 3 : 1) * ((n + 127) / 128 * 2);
+    return muon_tiles(m, m, true, 128) * js.n < 128 && tiles < kMuonParts && stages * (kMuonParts - tiles) >= 56L * kMuonParts;
+}
+static long muon_part_bytes(const MuonJobs& js, int planes) {
+    return muon_shared(js, planes) ? (long)kMuonParts * 2 * MuonBig::BM * MuonBig::BN * 4
+                                   : (muon_gram_shared(js, planes) ? (long)kMuonParts * 2 * MuonPart::BM * MuonPart::BN * 4 : 0);
+}
 
 template <class Cfg, int NP, int KIND, class T, bool MOM, bool JOIN = false>
 static void muon_product_launch(const MuonJobs& js, MuonArgs& args, hipStream_t stream) {
@@ -725,9 +743,10 @@ static void muon_product_launch(const MuonJobs& js, MuonArgs& args, hipStream_t 
     if constexpr (JOIN) {
         const MuonLay L = muon_lay(js.j[0].rows, js.j[0].cols, NP);
         args.stages = (NP == 2 ? 3 : 1) * (int)((KIND == MU_GRAM ? L.ldx : L.lda) / Cfg::ROW);
+        args.shares = (int)(tiles * args.stages / 4 < kMuonParts ? tiles * args.stages / 4 : kMuonParts);       // (four stages at least: none empty)
         auto part = muon_part_kernel<Cfg, NP, KIND>;
         allow_big_lds(part);
-        hipLaunchKernelGGL(part, dim3(kMuonParts), dim3(Cfg::THREADS), Cfg::LDS, stream, args);
+        hipLaunchKernelGGL(part, dim3((unsigned)args.shares), dim3(Cfg::THREADS), Cfg::LDS, stream, args);
     }
     auto kernel = muon_product_kernel<Cfg, NP, KIND, T, MOM, JOIN>;
     allow_big_lds(kernel);
@@ -744,8 +763,12 @@ static void muon_product(const MuonJobs& js, MuonArgs& args, hipStream_t stream)
         big += muon_tiles(m, n, KIND <= MU_POLY, 256), mid += muon_tiles(m, n, KIND <= MU_POLY, 128);
     }
     if constexpr (KIND <= MU_POLY) {
-        if (args.parts) {
+        if (args.parts && !args.narrow) {
             muon_product_launch<MuonBig, NP, KIND, T, MOM, true>(js, args, stream);
+            return;
+        }
+        if (KIND == MU_GRAM && args.parts) {
+            muon_product_launch<MuonPart, NP, MU_GRAM, T, MOM, true>(js, args, stream);
             return;
         }
     }
@@ -810,7 +833,7 @@ static int muon_run(const FneusMuonJob* jobs, int n_jobs, const MuonNum& P, int 
     js.scratch = scratch;
     long off;
     MuonArgs args;
-    args.P = P, args.cur = 0, args.scratch = scratch, args.stages = 0, args.pad_ = 0, args.parts = nullptr, args.total = 0;
+    args.P = P, args.cur = 0, args.scratch = scratch, args.stages = 0, args.shares = 0, args.narrow = 0, args.pad_ = 0, args.parts = nullptr, args.total = 0;
     for (int at = 0; few && muon_round(jobs, n_jobs, at, MU_FEW, NP, js, off) > 0;) {
         for (int q = 0; q < kMuonMaxJobs; ++q) args.first[q] = 0x7fffffff;
         muon_few_run<T, MOM>(js, args, steps, stream);
@@ -822,7 +845,8 @@ static int muon_run(const FneusMuonJob* jobs, int n_jobs, const MuonNum& P, int 
             args.first[q] = (int)tiles;
             tiles += (long)((js.j[q].rows + 127) / 128) * ((js.j[q].cols + 127) / 128) * 4;
         }
-        args.parts = muon_shared(js, NP) ? reinterpret_cast<float*>(scratch + off) : nullptr;
+        args.parts = muon_part_bytes(js, NP) > 0 ? reinterpret_cast<float*>(scratch + off) : nullptr;
+        args.narrow = !muon_shared(js, NP);
         hipLaunchKernelGGL((muon_norm_kernel<T, MOM>), dim3((unsigned)(js.n * kMuonChunks)), dim3(256), 0, stream, js, P);
         hipLaunchKernelGGL((muon_init_kernel<T, MOM, NP>), dim3((unsigned)tiles), dim3(256), 0, stream, args);
         muon_steps<NP, T, MOM>(js, args, steps, stream);
@@ -901,7 +925,7 @@ extern "C" long fneus_muon_scratch_bytes(const FneusMuonJob* jobs, int n_jobs, i
     MuonJobs js;
     for (int form = MU_ALL; form <= MU_FEW; ++form)       // (a further round of launches uses the same memory: one stream)
         for (int at = 0; muon_round(jobs, n_jobs, at, form, planes, js, off) > 0;) {
-            if (form != MU_FEW && muon_shared(js, planes)) off += kMuonPartBytes;
+            if (form != MU_FEW) off += muon_part_bytes(js, planes);
             most = off > most ? off : most;
         }
     return most;

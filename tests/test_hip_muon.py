@@ -357,3 +357,18 @@ def test_muon_of_a_short_side_in_a_graph():
         ops.muon_step(pe, gs, me, lr)
         for a, b in zip(ps + ms, pe + me):
             assert torch.equal(a, b)
+
+
+# X X^T of a few long rows: its contraction shared out over the CUs
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("size", [(1, 130, 5000), (1, 2975, 422), (3, 65, 3001), (1, 4160, 66), (2, 1500, 257), (1, 100, 30000)], ids=str)
+def test_newton_schulz_of_long_rows(t, size):
+    from fneus import ops
+    count, rows, cols = size
+    g = torch.stack([matrix(rows, cols, seed=k) for k in range(count)]).to(t)
+    out = ops.newton_schulz(g.cuda())
+    again = ops.newton_schulz(g.cuda())
+    assert torch.equal(out, again)
+    for k in range(count):
+        assert off(out[k], ns64(g[k])) <= bound(3 if t == torch.float32 else 2, t)
