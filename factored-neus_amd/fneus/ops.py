@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from typing import Optional
 
 import numpy as np
@@ -1407,6 +1408,8 @@ def linear_bwd(dy, x, weight, z=None, act="none", need=(True, True, True)):
 
 # ---- Muon: momentum, orthogonalisation by Newton-Schulz products, step (csrc/muon_kernels.hip) -------------------------------------------
 NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+_MUON_JOB = struct.Struct("PPPPiifi")          # _lib.FneusMuonJob
+assert _MUON_JOB.size == C.sizeof(_lib.FneusMuonJob)
 
 
 def _muon_prec(prec, dtype) -> int:
@@ -1416,18 +1419,6 @@ def _muon_prec(prec, dtype) -> int:
     if prec not in (PREC_PARITY, PREC_H16):
         raise ValueError("muon: prec must be PREC_PARITY or PREC_H16")
     return prec
-
-
-def _muon_matrices(ts, name, like=None):
-    ts = list(ts)
-    for k, t in enumerate(ts):
-        ref = like[k] if like is not None else ts[0]
-        if not torch.is_tensor(t) or t.dim() != 2 or not t.is_cuda or t.dtype not in _DTYPES or t.dtype != ref.dtype or t.device != ref.device \
-                or not t.is_contiguous() or t.numel() == 0:
-            raise ValueError(f"muon: {name} must be contiguous, non-empty CUDA matrices of one supported type on one device")
-        if like is not None and t.shape != ref.shape:
-            raise ValueError(f"muon: {name}[{k}] is {tuple(t.shape)}, its parameter {tuple(ref.shape)}")
-    return ts
 
 
 def muon_adjust(adjust, rows: int, cols: int) -> float:
@@ -1444,19 +1435,36 @@ def muon_adjust(adjust, rows: int, cols: int) -> float:
 
 def muon_jobs(params, grads, momenta, adjust="match_rms"):
     """the table of muon_step for lists that stay: a caller that keeps it skips the checks of its tensors in every step"""
-    params = _muon_matrices(params, "params")
-    grads, momenta = _muon_matrices(grads, "grads", params), _muon_matrices(momenta, "momenta", params)
-    if not len(params) == len(grads) == len(momenta):
+    params, grads, momenta = list(params), list(grads), list(momenta)
+    n = len(params)
+    if not n == len(grads) == len(momenta):
         raise ValueError("muon: params, grads and momenta must be lists of one length")
-    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in params + grads + momenta)
-    if any(b[0] < a[1] for a, b in zip(spans, spans[1:])):
-        raise ValueError("muon: two of params, grads and momenta share memory")
-    jobs = (_lib.FneusMuonJob * max(1, len(params)))()
-    for j, p, g, m in zip(jobs, params, grads, momenta):
-        j.grad, j.momentum, j.param = g.data_ptr(), m.data_ptr(), p.data_ptr()
-        j.rows, j.cols = p.shape
-        j.adjust = muon_adjust(adjust, *p.shape)
-    return jobs, len(params), (params[0] if params else None)
+    table = bytearray(max(1, n) * _MUON_JOB.size)
+    spans, first = [], params[0] if n else None
+    for k in range(n):
+        p, g, m = params[k], grads[k], momenta[k]
+        for t, name in ((p, "params"), (g, "grads"), (m, "momenta")):
+            if not torch.is_tensor(t) or not t.is_cuda or t.dtype not in _DTYPES or t.dtype != first.dtype or t.get_device() != first.get_device() \
+                    or not t.is_contiguous() or len(t.shape) != 2:
+                raise ValueError(f"muon: {name} must be contiguous CUDA matrices of one supported type on one device")
+        shape = p.shape
+        if g.shape != shape or m.shape != shape:
+            raise ValueError(f"muon: grads[{k}] is {tuple(g.shape)}, momenta[{k}] {tuple(m.shape)}, their parameter {tuple(shape)}")
+        rows, cols = shape
+        size = rows * cols * p.element_size()
+        if size == 0:
+            raise ValueError(f"muon: params[{k}] has no elements")
+        at = p.data_ptr(), g.data_ptr(), m.data_ptr()
+        spans += (at[0], at[0] + size), (at[1], at[1] + size), (at[2], at[2] + size)
+        _MUON_JOB.pack_into(table, k * _MUON_JOB.size, at[1], at[2], at[0], 0, rows, cols, muon_adjust(adjust, rows, cols), 0)
+    spans.sort()
+    end = 0
+    for lo, hi in spans:
+        if lo < end:
+            raise ValueError("muon: two of params, grads and momenta share memory")
+        end = hi
+    jobs = (_lib.FneusMuonJob * max(1, n)).from_buffer(table)
+    return jobs, n, first
 
 
 def muon_launch(table, lr, momentum, nesterov, weight_decay, coefficients, steps, eps, prec, zero_grad):
