@@ -645,8 +645,8 @@ long fneus_layer_norm_bwd_scratch_floats(long rows, int n);
  * act: 0 none, 1 ReLU, 2 LeakyReLU(0.2), 3 sigmoid, 4 softplus(beta 100), 5 GELU (erf), 6 SiLU.
  * forward: x, weight, (bias), (residual) -> y and, where z is given, the pre-activation z [rows][n_out] (what the backward of act != 0 reads).
  * backward: dy, x, weight, z -> dx [rows][n_in], dweight [n_out][n_in], dbias [n_out], each where given (OVERWRITTEN); the residual's gradient
- * is dy.  Sums in a fixed order: bit-reproducible.  rows == 0: forward nothing, backward refused.  An fp32 infinity or NaN in an operand
- * gives NaN wherever it takes part.  `scratch`: fneus_linear_scratch_bytes(job, backward) bytes, 16-byte aligned, not shared between calls in flight.
+ * is dy.  Sums in a fixed order: bit-reproducible.  rows == 0: forward nothing, backward refused.  An fp32 infinity in an operand
+ * may give NaN where it takes part.  `scratch`: fneus_linear_scratch_bytes(job, backward) bytes, 16-byte aligned, not shared between calls in flight.
  * No output shares memory with another array (the residual may be x). */
 typedef struct FneusLinear {
     const void *x, *weight, *bias, *residual;
