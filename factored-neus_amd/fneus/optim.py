@@ -261,6 +261,7 @@ class FlatMuon(torch.optim.Optimizer):
                     if torch.is_tensor(v):
                         st[k] = v.clone()              # (torch shares tensors with the dict it is given)
         if self.adam is not None:
+            self.adam.state.clear()                    # (a parameter that the loaded state does not hold starts anew)
             for p in self.adam.param_groups[0]["params"]:
                 if p in self.state:
                     self.adam.state[p] = dict(self.state[p])

@@ -287,3 +287,32 @@ def test_stage_trainers_with_muon_and_residual_trunk(stage, use_graph):
     assert tr.train_step(data) is not None
     with pytest.raises(ValueError):
         (Stage2Trainer if stage == 2 else Stage3Trainer)(dev, optimizer="sgd")
+
+
+def _stepped_adam_state(opt, value):
+    """what FlatAdam's step leaves for its parameters, without a GPU"""
+    for p in opt.adam.param_groups[0]["params"]:
+        opt.adam.state[p] = {"step": torch.tensor(float(value)), "exp_avg": torch.full_like(p, value), "exp_avg_sq": torch.full_like(p, value)}
+
+
+def test_flat_muon_load_replaces_adam_state_cpu():
+    """a loaded state takes the place of all that the optimiser had: what it does not hold (a fresh optimiser's, a parameter that had no
+    gradient) starts anew, for Adam's parameters too"""
+    from fneus.optim import FlatMuon
+    make = lambda: FlatMuon([nn.Parameter(torch.zeros(40, 50)), nn.Parameter(torch.zeros(3)), nn.Parameter(torch.zeros(5))])  # noqa: E731
+    a = make()
+    w, b, c = a.param_groups[0]["params"]
+    _stepped_adam_state(a, 100.0)
+    a.state[w] = {"momentum_buffer": torch.ones(40, 50)}
+    a.adam._segs = object()
+    a.load_state_dict(make().state_dict())                            # an empty state
+    assert len(a.state.get(w, {})) == len(a.adam.state.get(b, {})) == len(a.adam.state.get(c, {})) == 0 and a.adam._segs is None
+    assert not a.state_dict()["state"]
+    partial = make()
+    _stepped_adam_state(partial, 7.0)
+    del partial.adam.state[partial.param_groups[0]["params"][2]]      # one of the two has no state
+    sd = partial.state_dict()
+    _stepped_adam_state(a, 100.0)
+    a.load_state_dict(sd)
+    assert float(a.adam.state[b]["step"]) == 7.0 and float(a.adam.state[b]["exp_avg"][0]) == 7.0 and len(a.adam.state.get(c, {})) == 0
+    assert sorted(a.state_dict()["state"]) == [1]
