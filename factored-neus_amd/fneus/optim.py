@@ -193,6 +193,14 @@ class FlatMuon(torch.optim.Optimizer):
     def _live(self):
         return [p for p in self.matrices if p.requires_grad and p.grad is not None]
 
+    def _table_keys(self, ps):
+        """all that the table of jobs holds or was checked for: it is built anew where any of it differs"""
+        keys = [self.param_groups[0]["adjust"]]
+        for p in ps:
+            m = self.state[p].get("momentum_buffer")
+            keys.append((p.data_ptr(), p.grad.data_ptr(), 0 if m is None else m.data_ptr(), p.dtype, p.shape, p.stride(), p.grad.stride()))
+        return keys
+
     def _build(self, ps):
         from . import ops
         for p in ps:
@@ -201,7 +209,7 @@ class FlatMuon(torch.optim.Optimizer):
                 st["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
         self._table = ops.muon_jobs([p.detach() for p in ps], [p.grad for p in ps], [self.state[p]["momentum_buffer"] for p in ps],
                                     self.param_groups[0]["adjust"])
-        self._keys = [(p.data_ptr(), p.grad.data_ptr(), self.state[p]["momentum_buffer"].data_ptr()) for p in ps]
+        self._keys = self._table_keys(ps)
         if self._lr_dev is None or self._lr_dev.device != ps[0].device:
             self._lr_host = float(self.param_groups[0]["lr"])
             self._lr_dev = torch.full((), self._lr_host, dtype=torch.float32, device=ps[0].device)
@@ -222,8 +230,7 @@ class FlatMuon(torch.optim.Optimizer):
                 self.adam.step()
         if not ps:
             return
-        if self._keys != [(p.data_ptr(), p.grad.data_ptr(), self.state[p]["momentum_buffer"].data_ptr() if "momentum_buffer" in self.state[p] else 0)
-                          for p in ps]:
+        if self._keys != self._table_keys(ps):
             self._build(ps)
         if float(g["lr"]) != self._lr_host:
             self._lr_dev.fill_(float(g["lr"]))

@@ -316,3 +316,53 @@ def test_flat_muon_load_replaces_adam_state_cpu():
     a.load_state_dict(sd)
     assert float(a.adam.state[b]["step"]) == 7.0 and float(a.adam.state[b]["exp_avg"][0]) == 7.0 and len(a.adam.state.get(c, {})) == 0
     assert sorted(a.state_dict()["state"]) == [1]
+
+
+def test_flat_muon_table_follows_what_it_was_built_from_cpu(monkeypatch):
+    """the table of jobs is built anew where something it holds has changed at the same addresses: adjust, a matrix's shape, a gradient's layout"""
+    from fneus import ops
+    from fneus.optim import FlatMuon
+    built = []
+    monkeypatch.setattr(ops, "muon_jobs", lambda ps, gs, ms, adjust: built.append((adjust, [tuple(p.shape) for p in ps], [g.stride() for g in gs])))
+    monkeypatch.setattr(ops, "muon_launch", lambda *a: None)
+    p = nn.Parameter(torch.zeros(40, 40))
+    p.grad = torch.ones(40, 40)
+    opt = FlatMuon([p], lr=1e-2)
+    opt.step(), opt.step()
+    assert len(built) == 1
+    opt.param_groups[0]["adjust"] = "original"
+    opt.step(), opt.step()
+    assert len(built) == 2 and built[-1][0] == "original"
+    p.grad.t_()                                                       # the same memory, transposed
+    opt.step()
+    assert len(built) == 3 and built[-1][2] == [(1, 40)]
+    with torch.no_grad():
+        p.grad = None
+        m = opt.state[p]["momentum_buffer"]
+        g = torch.ones(1600)
+        p.grad = g.view(40, 40)
+        opt.step()
+        p.grad = None
+        p.data, opt.state[p]["momentum_buffer"] = p.data.view(50, 32), m.view(50, 32)
+        p.grad = g.view(50, 32)
+    opt.step()
+    assert built[-1][1] == [(50, 32)]
+
+
+@pytest.mark.gpu
+def test_flat_muon_adjust_between_steps():
+    """the factor on the learning rate, assigned between steps, is the one the next step takes"""
+    from fneus.optim import FlatMuon
+    p = nn.Parameter(torch.zeros(64, 100, device="cuda"))
+    grad = torch.randn(64, 100, device="cuda")
+    moved = []
+    opt = FlatMuon([p], lr=1e-2, adjust=1.0, momentum=0.0)
+    p.grad = torch.zeros_like(p)
+    for adjust in (1.0, 3.0):
+        opt.param_groups[0]["adjust"] = adjust
+        with torch.no_grad():
+            p.zero_(), p.grad.copy_(grad)
+        opt.step()
+        moved.append(p.detach().double().clone())
+    # the same orthogonalised gradient, times lr adjust: one fp32 product and one difference from 0 each (2^-24 both), lr adjust itself 2^-24
+    assert float((moved[1] - 3.0 * moved[0]).abs().max()) <= 4 * 2.0 ** -24 * float(moved[1].abs().max())
