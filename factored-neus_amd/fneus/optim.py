@@ -155,11 +155,19 @@ class FlatAdam(torch.optim.Adam):
         return 0 if self._segs is None else len(self._segs)
 
 
+def _capturing(device) -> bool:
+    if device.type != "cuda":
+        return False
+    with torch.cuda.device(device):
+        return torch.cuda.is_current_stream_capturing()
+
+
 class FlatMuon(torch.optim.Optimizer):
     """Muon for a model's weight matrices, FlatAdam for everything else, one learning rate for both (adjust="match_rms" gives a matrix's
     update Adam's rms).  Every matrix of the model takes part in the same launches of fneus_muon (momentum, Newton-Schulz
     orthogonalisation, step); learning rate and step count are device scalars, gradients are cleared by the kernels: capturable in a
-    hipGraph like FlatAdam, with its methods (set_lr, state_dict / load_state_dict).
+    hipGraph like FlatAdam, behind an eager step that allocates the state (else refused), with its methods (set_lr, state_dict /
+    load_state_dict).
 
     params: parameters; the 2-D ones with no side shorter than `min_side` are Muon's (a layer with a handful of outputs has no spectrum to
     level), the others Adam's.  State: `momentum_buffer` a matrix, torch.optim.Adam's of the others.  A parameter without a gradient is
@@ -214,6 +222,15 @@ class FlatMuon(torch.optim.Optimizer):
             self._lr_host = float(self.param_groups[0]["lr"])
             self._lr_dev = torch.full((), self._lr_host, dtype=torch.float32, device=ps[0].device)
 
+    def _capturable(self, ps):
+        """refuses a captured step that would clear its state or write its learning rate: a replay would do so again every time"""
+        lr, adam = float(self.param_groups[0]["lr"]), self.adam
+        if self._lr_dev is None or self._lr_dev.device != ps[0].device or any("momentum_buffer" not in self.state[p] for p in ps) or \
+                (adam is not None and adam._params() and adam._stale()):
+            raise RuntimeError("FlatMuon.step(): take an eager step (it allocates the state) before the step is captured")
+        if lr != self._lr_host or (adam is not None and adam._params() and lr != adam._lr_host):
+            raise RuntimeError("FlatMuon.step(): use set_lr() before the capture, not param_groups: a captured step does not change its learning rate")
+
     @torch.no_grad()
     def step(self, closure=None):
         if closure is not None:
@@ -223,6 +240,8 @@ class FlatMuon(torch.optim.Optimizer):
             raise NotImplementedError("FlatMuon supports a single parameter group")
         g = self.param_groups[0]
         ps = self._live()
+        if ps and _capturing(ps[0].device):
+            self._capturable(ps)
         if self.adam is not None:
             if self.adam.param_groups[0]["lr"] != g["lr"]:       # someone assigned param_groups[0]["lr"] directly
                 self.adam.set_lr(g["lr"])

@@ -366,3 +366,57 @@ def test_flat_muon_adjust_between_steps():
         moved.append(p.detach().double().clone())
     # the same orthogonalised gradient, times lr adjust: one fp32 product and one difference from 0 each (2^-24 both), lr adjust itself 2^-24
     assert float((moved[1] - 3.0 * moved[0]).abs().max()) <= 4 * 2.0 ** -24 * float(moved[1].abs().max())
+
+
+def test_flat_muon_refuses_its_first_step_in_a_capture_cpu(monkeypatch):
+    """buffers cleared, or a learning rate written, inside a captured step would be so again in every replay: the state has to be there before"""
+    from fneus import ops, optim
+    from fneus.optim import FlatMuon
+    launched = []
+    monkeypatch.setattr(ops, "muon_jobs", lambda *a: None)
+    monkeypatch.setattr(ops, "muon_launch", lambda *a: launched.append(a))
+    capturing = [True]
+    monkeypatch.setattr(optim, "_capturing", lambda device: capturing[0])
+    p, v = nn.Parameter(torch.zeros(40, 40)), nn.Parameter(torch.zeros(5))
+    p.grad, v.grad = torch.ones(40, 40), torch.ones(5)
+    opt = FlatMuon([p], lr=1e-2)
+    with pytest.raises(RuntimeError, match="eager step"):
+        opt.step()
+    assert not launched and not opt.state[p]
+    capturing[0] = False
+    opt.step()
+    capturing[0] = True
+    opt.step()
+    p.grad = torch.ones(40, 40)                                       # (another gradient: host work alone)
+    opt.step()
+    assert len(launched) == 3
+    opt.param_groups[0]["lr"] = 0.5                                   # (would be written by the captured step, in every replay)
+    with pytest.raises(RuntimeError, match="set_lr"):
+        opt.step()
+    opt.param_groups[0]["lr"] = 1e-2
+    opt.load_state_dict(FlatMuon([nn.Parameter(torch.zeros(40, 40))], lr=1e-2).state_dict())
+    with pytest.raises(RuntimeError, match="eager step"):
+        opt.step()
+    both = FlatMuon([p, v], lr=1e-2)                                  # Adam's parameters alone are stale
+    both.state[p]["momentum_buffer"], both._lr_dev, both._lr_host = torch.zeros(40, 40), torch.zeros(()), 1e-2
+    with pytest.raises(RuntimeError, match="eager step"):
+        both.step()
+
+
+@pytest.mark.gpu
+def test_flat_muon_refuses_its_first_step_in_a_capture():
+    from fneus.optim import FlatMuon
+    p = nn.Parameter(torch.randn(40, 50, device="cuda"))
+    p.grad = torch.randn_like(p)
+    old = p.detach().clone()
+    opt = FlatMuon([p], lr=1e-2)
+    graph, other = torch.cuda.CUDAGraph(), torch.zeros(8, device="cuda")
+    with torch.cuda.graph(graph):
+        other.add_(1.0)
+        with pytest.raises(RuntimeError, match="eager step"):
+            opt.step()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert float(other[0]) == 1.0 and torch.equal(p, old) and not opt.state[p]
+    opt.step()
+    assert not torch.equal(p, old)
