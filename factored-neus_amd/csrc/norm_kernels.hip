@@ -4,7 +4,8 @@
 // Memory bound: the forward reads x and writes y, the backward reads dy and x and writes dx.  A TEAM of TPR threads owns a row and
 // holds it in registers (EPT values a thread, 16-byte chunks): one pass over memory, the variance from the centred values (two
 // passes over registers: a row with a large mean keeps its digits).  TPR = 16 (sums by DPP), 64, 256 or 512 threads; wider rows
-// take the streaming kernels, which read a row from the caches again.
+// take the streaming kernels, which read a row from the caches again; rows of fewer than 8 values a thread each.  A launch takes fewer than 2^32
+// threads, so every grid is capped and its workgroups go on to further rows.
 // The weight gradients: a team keeps its columns' sums of dy xh and dy in registers over all the rows it takes, the teams of a
 // workgroup are added in LDS, every workgroup writes ONE partial row, and a second launch adds the partial rows in a fixed order: no
 // atomics, the same bits in every run.
@@ -115,13 +116,99 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) layer_norm_fwd_kernel(N
     }
 }
 
-// rows wider than a team's registers: a workgroup a row, three passes (the second and third from the caches)
+// Rows of fewer than 8 values: a thread a row (a row is a few bytes, less than one chunk), rows blockIdx * 256 + thread, then a grid's further
+constexpr int kThin = 8;
+template <class T>
+FN_DEV void load_thin(const T* p, int n, float (&v)[kThin - 1]) {
+    T q[kThin - 1];
+#pragma unroll
+    for (int k = 0; k < kThin - 1; ++k) q[k] = p[k < n ? k : n - 1];
+#pragma unroll
+    for (int k = 0; k < kThin - 1; ++k) v[k] = k < n ? (float)q[k] : 0.0f;
+}
 template <class T, class P>
-__global__ void __launch_bounds__(1024) layer_norm_fwd_stream_kernel(NormArgs<T, P> a) {
+__global__ void __launch_bounds__(256) layer_norm_fwd_thin_kernel(NormArgs<T, P> a) {
+    float w[kThin - 1], b[kThin - 1];
+#pragma unroll
+    for (int k = 0; k < kThin - 1; ++k) {
+        w[k] = a.w && k < a.n ? (float)a.w[k] : 1.0f;
+        b[k] = a.b && k < a.n ? (float)a.b[k] : 0.0f;
+    }
+    const float len = (float)a.n;
+    for (long row = (long)blockIdx.x * 256 + threadIdx.x; row < a.rows; row += (long)gridDim.x * 256) {
+        float v[kThin - 1], s = 0.0f, q = 0.0f;
+        load_thin<T>(a.x + row * a.ldx, a.n, v);
+#pragma unroll
+        for (int k = 0; k < kThin - 1; ++k) s += v[k];
+        const float mu = s / len;
+#pragma unroll
+        for (int k = 0; k < kThin - 1; ++k) {
+            v[k] -= mu;
+            q += k < a.n ? v[k] * v[k] : 0.0f;
+        }
+        const float r = 1.0f / sqrtf(q / len + a.eps);
+        T* y = a.y + row * a.ldy;
+#pragma unroll
+        for (int k = 0; k < kThin - 1; ++k)
+            if (k < a.n) y[k] = (T)(v[k] * r * w[k] + b[k]);
+        a.mean[row] = mu;
+        a.rstd[row] = r;
+    }
+}
+
+// dx, and with PARAMS this workgroup's partial row of (dw, db): a thread's sums over its rows, the wave's, the four waves' in order
+template <class T, class P, bool PARAMS>
+__global__ void __launch_bounds__(256) layer_norm_bwd_thin_kernel(NormArgs<T, P> a) {
+    float w[kThin - 1], sum[2][kThin - 1];
+#pragma unroll
+    for (int k = 0; k < kThin - 1; ++k) {
+        w[k] = a.w && k < a.n ? (float)a.w[k] : 1.0f;
+        sum[0][k] = sum[1][k] = 0.0f;
+    }
+    const float inv_n = 1.0f / (float)a.n;
+    for (long row = (long)blockIdx.x * 256 + threadIdx.x; row < a.rows; row += (long)gridDim.x * 256) {
+        float h[kThin - 1], g[kThin - 1], s1 = 0.0f, s2 = 0.0f;
+        load_thin<T>(a.x + row * a.ldx, a.n, h);
+        load_thin<T>(a.dy + row * a.lddy, a.n, g);
+        const float mu = a.mean[row], r = a.rstd[row];
+#pragma unroll
+        for (int k = 0; k < kThin - 1; ++k) {
+            h[k] = k < a.n ? (h[k] - mu) * r : 0.0f;
+            if constexpr (PARAMS) {
+                sum[0][k] += g[k] * h[k];
+                sum[1][k] += g[k];
+            }
+            g[k] *= w[k];
+            s1 += g[k];
+            s2 += g[k] * h[k];
+        }
+        s1 *= inv_n;
+        s2 *= inv_n;
+        T* dx = a.dx + row * a.lddx;
+#pragma unroll
+        for (int k = 0; k < kThin - 1; ++k)
+            if (k < a.n) dx[k] = (T)(r * (g[k] - s1 - h[k] * s2));
+    }
+    if constexpr (PARAMS) {
+        __shared__ float red[4][2][kThin];
+#pragma unroll
+        for (int which = 0; which < 2; ++which)
+#pragma unroll
+            for (int k = 0; k < kThin - 1; ++k) {
+                const float s = wave_sum(sum[which][k]);
+                if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6][which][k] = s;
+            }
+        __syncthreads();
+        const int which = threadIdx.x / kThin, k = threadIdx.x % kThin;
+        if (which < 2 && k < a.n)
+            a.partial[((long)blockIdx.x * 2 + which) * a.n + k] = red[0][which][k] + red[1][which][k] + red[2][which][k] + red[3][which][k];
+    }
+}
+
+// rows wider than a team's registers: a workgroup a row (blockIdx, blockIdx + grid, ...), three passes (the second and third from the caches)
+template <class T, class P>
+FN_DEV void layer_norm_fwd_stream_row(const NormArgs<T, P>& a, long row, float* red, int& flip) {
     constexpr int V = Chunk<T>::N;
-    __shared__ float red[32];
-    int flip = 0;
-    const long row = blockIdx.x;
     const T* x = a.x + row * a.ldx;
     const float len = (float)a.n;
     float s = 0.0f, v[V];
@@ -151,6 +238,12 @@ __global__ void __launch_bounds__(1024) layer_norm_fwd_stream_kernel(NormArgs<T,
         a.mean[row] = mu;
         a.rstd[row] = r;
     }
+}
+template <class T, class P>
+__global__ void __launch_bounds__(1024) layer_norm_fwd_stream_kernel(NormArgs<T, P> a) {
+    __shared__ float red[32];
+    int flip = 0;
+    for (long row = blockIdx.x; row < a.rows; row += gridDim.x) layer_norm_fwd_stream_row(a, row, red, flip);
 }
 
 // dx of the rows blockIdx, blockIdx + grid, ... and, PARAMS, this workgroup's partial row of (dw, db)
@@ -250,11 +343,8 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) layer_norm_bwd_kernel(N
 }
 
 template <class T, class P>
-__global__ void __launch_bounds__(1024) layer_norm_bwd_stream_kernel(NormArgs<T, P> a) {
+FN_DEV void layer_norm_bwd_stream_row(const NormArgs<T, P>& a, long row, float* red, int& flip) {
     constexpr int V = Chunk<T>::N;
-    __shared__ float red[32];
-    int flip = 0;
-    const long row = blockIdx.x;
     const T *x = a.x + row * a.ldx, *dy = a.dy + row * a.lddy;
     const float mu = a.mean[row], r = a.rstd[row], inv_n = 1.0f / (float)a.n;
     float s1 = 0.0f, s2 = 0.0f, v[V], d[V];
@@ -281,6 +371,12 @@ __global__ void __launch_bounds__(1024) layer_norm_bwd_stream_kernel(NormArgs<T,
             if (k < left) v[k] = r * (d[k] * (a.w ? (float)a.w[col + k] : 1.0f) - s1 - (v[k] - mu) * r * s2);
         store_chunk<T>(a.dx + row * a.lddx + col, left, v);
     }
+}
+template <class T, class P>
+__global__ void __launch_bounds__(1024) layer_norm_bwd_stream_kernel(NormArgs<T, P> a) {
+    __shared__ float red[32];
+    int flip = 0;
+    for (long row = blockIdx.x; row < a.rows; row += gridDim.x) layer_norm_bwd_stream_row(a, row, red, flip);
 }
 
 // the streaming form's partial rows: a thread a column, the rows blockIdx.y, blockIdx.y + gridDim.y, ...
@@ -315,12 +411,12 @@ __global__ void __launch_bounds__(1024) layer_norm_fold_kernel(const float* __re
     }
 }
 
-struct NormShape { int tpr, ept; };      // tpr 0: streaming
+struct NormShape { int tpr, ept; };      // tpr 0: streaming, 1: a thread a row
 
 // The narrowest team whose threads hold the row in at most 32 values each (the backward keeps five registers a value); 16 threads up to
 // 256 values (sums by DPP, four rows a wave), one wave up to 2048 (no barrier), four and eight waves up to 8192 and 16384
 static NormShape norm_shape(int n) {
-    if (n < 8) return {0, 0};             // (a chunk does not fit the row: the streaming form)
+    if (n < kThin) return {1, 0};         // (a chunk does not fit the row)
     if (n <= 256) return {16, 16};
     if (n <= 2048) return {64, 8 * ((n + 511) / 512)};
     if (n <= 8192) return {256, 8 * ((n + 2047) / 2048)};
@@ -355,13 +451,17 @@ static int norm_grid(long rows, int n) {
 template <class T, class P>
 static void norm_fwd_launch(const NormArgs<T, P>& a, hipStream_t stream) {
     const NormShape s = norm_shape(a.n);
-    if (s.tpr == 0) {
-        hipLaunchKernelGGL((layer_norm_fwd_stream_kernel<T, P>), dim3((unsigned)a.rows), dim3(1024), 0, stream, a);
-        return;
-    }
     const int threads = s.tpr > 256 ? s.tpr : 256, teams = norm_teams(s);
     const long need = (a.rows + teams - 1) / teams;
     const dim3 grid((unsigned)(need < kNormFwdGrid ? need : kNormFwdGrid));
+    if (s.tpr == 0) {
+        hipLaunchKernelGGL((layer_norm_fwd_stream_kernel<T, P>), grid, dim3(1024), 0, stream, a);
+        return;
+    }
+    if (s.tpr == 1) {
+        hipLaunchKernelGGL((layer_norm_fwd_thin_kernel<T, P>), grid, dim3(256), 0, stream, a);
+        return;
+    }
 #define CALL(TPR, EPT) hipLaunchKernelGGL((layer_norm_fwd_kernel<T, P, TPR, EPT>), grid, dim3(threads), 0, stream, a)
     FN_NORM_SHAPES(CALL)
 #undef CALL
@@ -372,8 +472,12 @@ static void norm_bwd_launch(const NormArgs<T, P>& a, P* dw, P* db, hipStream_t s
     const NormShape s = norm_shape(a.n);
     const int grid = norm_grid(a.rows, a.n);
     const bool params = dw || db;
-    if (s.tpr == 0) {
-        hipLaunchKernelGGL((layer_norm_bwd_stream_kernel<T, P>), dim3((unsigned)a.rows), dim3(1024), 0, stream, a);
+    if (s.tpr == 1) {
+        if (params) hipLaunchKernelGGL((layer_norm_bwd_thin_kernel<T, P, true>), dim3((unsigned)grid), dim3(256), 0, stream, a);
+        else hipLaunchKernelGGL((layer_norm_bwd_thin_kernel<T, P, false>), dim3((unsigned)grid), dim3(256), 0, stream, a);
+    } else if (s.tpr == 0) {
+        const dim3 most((unsigned)(a.rows < kNormFwdGrid ? a.rows : kNormFwdGrid));
+        hipLaunchKernelGGL((layer_norm_bwd_stream_kernel<T, P>), most, dim3(1024), 0, stream, a);
         if (params) hipLaunchKernelGGL((layer_norm_params_kernel<T, P>), dim3((unsigned)((a.n + 255) / 256), (unsigned)grid), dim3(256), 0, stream, a);
     } else {
         const int threads = s.tpr > 256 ? s.tpr : 256, teams = threads / s.tpr;

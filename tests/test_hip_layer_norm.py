@@ -193,3 +193,59 @@ def test_layer_norm_refusals():
                 lambda: ops.layer_norm_bwd(x, x, w, w[:3], w[:4])):
         with pytest.raises(ValueError):
             bad()
+
+
+# Rows below 8 values (a thread a row) and beyond 16384 (a workgroup a row): more rows than one launch has threads or workgroups for
+def many(rows, n, t, seed):
+    """spread over [-5.5, 6.5] in each row's values, weights of at most 1.5, eps 0.1 (r <= 3.17): with max |x| = 6.5, the mean of n <= 7 values is
+    off by (n + 1) 2^-24 6.5 = 3.1e-6, xh by 1e-5, y by 1.5e-5; dx by r (2 x 1e-5 mean |g xh| + 8 x 2^-24 |g|) < 5e-4 of values that reach r |g| > 10.
+    close() allows 2e-5 of the largest y (> 1.5) and of the largest dx, hence the slack given to dx"""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = (torch.randn(rows, n, generator=g, device="cuda").clamp(-5, 5) + 0.5).to(t)
+    w = torch.linspace(0.8, 1.5, n, device="cuda").to(t)
+    b = torch.linspace(-0.5, 0.5, n, device="cuda").to(t)
+    return x, w, b, torch.randn(rows, n, generator=g, device="cuda").to(t)
+
+
+def compare(got, ref, t, slacks):
+    for a, want, tt, what, slack in zip(got, ref, (t, torch.float32, torch.float32, t, t, t), ("y", "mean", "rstd", "dx", "dw", "db"), slacks):
+        if a is None:
+            continue
+        lim = want.abs() * (torch.finfo(tt).eps / 2) * 1.01 + slack * float(want.abs().max())
+        err = (a.double() - want).abs()
+        assert bool((err <= lim).all()), (what, float((err - lim).max()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("rows,n", [((1 << 22) + 5, 3), ((1 << 22) + 300, 7), (300000, 1), (262145, 2), (255, 5), (2051, 16411)], ids=str)
+def test_layer_norm_more_rows_than_a_launch_takes(t, rows, n):
+    """dw, db: sums of N terms of about unit size by blocks (at most 256 of them in series, then trees): the roundings of all levels add up to
+    sqrt(256 / 3) 2^-24 sqrt(N) rms, 2e-5 of the sum's own sqrt(N)"""
+    from fneus import ops
+    x, w, b, dy = many(rows, n, t, rows)
+    y, mean, rstd = ops.layer_norm_fwd(x, w, b, 0.1)
+    dx, dw, db = ops.layer_norm_bwd(dy, x, w, mean, rstd)
+    ref = formula(x, w, b, 0.1, dy)
+    compare((y, mean, rstd, dx, dw if n > 1 else None, db), ref, t, (2e-5, 2e-5, 2e-5, 5e-5, 2e-5, 2e-5))
+    if n == 1:
+        assert float(dx.abs().max()) == 0.0 and float(dw.abs().max()) == 0.0
+    assert torch.equal(ops.layer_norm_bwd(dy, x, w, mean, rstd, need_params=False)[0], dx)
+    again = ops.layer_norm_bwd(dy, x, w, mean, rstd)
+    assert all(torch.equal(p, q) for p, q in zip(again, (dx, dw, db)))
+    # strided rows from an unaligned start: the same bits, and nothing beside them is written
+    if rows < 400000:
+        wide = torch.full((rows, n + 3), 9.0, dtype=t, device="cuda")
+        wide[:, 1:1 + n] = x
+        assert torch.equal(ops.layer_norm_fwd(wide[:, 1:1 + n], w, b, 0.1)[0], y)
+        assert all(torch.equal(p, q) for p, q in zip(ops.layer_norm_bwd(dy, wide[:, 1:1 + n], w, mean, rstd), (dx, dw, db)))
+
+
+def test_layer_norm_scratch_stays_bounded_cpu():
+    """partial rows of the weight gradients: one a workgroup, 1024 at most however many rows there are"""
+    from fneus._lib import lib
+    for n in (1, 3, 7, 8, 256, 300, 2049, 16384, 16385):
+        for rows in (1, 1000, 1 << 22, (1 << 23) + 5, (1 << 31) - 1):
+            parts = lib.fneus_layer_norm_bwd_scratch_floats(rows, n) // (2 * n)
+            assert 1 <= parts <= 1024, (n, rows)
+    assert lib.fneus_layer_norm_bwd_scratch_floats(256, 3) == 6 and lib.fneus_layer_norm_bwd_scratch_floats(257, 3) == 12
