@@ -19,6 +19,7 @@ namespace fneus {
 
 constexpr int kNormMaxGrid = 1024;       // workgroups of the backward at most
 constexpr long kNormFwdGrid = 2048;      // of the forward: 8 a CU
+constexpr long kNormBwdGrid = 1L << 20;  // of the backward without weight gradients: the launch's limit alone
 
 // sums of v over the team, in every thread of it.  `red`: LDS floats, 2 * TPR / 64 (TPR > 64); `flip` alternates the half used, so
 // one barrier a sum is enough
@@ -481,7 +482,8 @@ static void norm_bwd_launch(const NormArgs<T, P>& a, P* dw, P* db, hipStream_t s
         if (params) hipLaunchKernelGGL((layer_norm_params_kernel<T, P>), dim3((unsigned)((a.n + 255) / 256), (unsigned)grid), dim3(256), 0, stream, a);
     } else {
         const int threads = s.tpr > 256 ? s.tpr : 256, teams = threads / s.tpr;
-        const unsigned all = (unsigned)((a.rows + teams - 1) / teams);
+        const long need = (a.rows + teams - 1) / teams;
+        const unsigned all = (unsigned)(need < kNormBwdGrid ? need : kNormBwdGrid);
         if (params) {
 #define CALL(TPR, EPT) hipLaunchKernelGGL((layer_norm_bwd_kernel<T, P, TPR, EPT, true>), dim3((unsigned)grid), dim3(threads), 0, stream, a)
             FN_NORM_SHAPES(CALL)

@@ -249,3 +249,21 @@ def test_layer_norm_scratch_stays_bounded_cpu():
             parts = lib.fneus_layer_norm_bwd_scratch_floats(rows, n) // (2 * n)
             assert 1 <= parts <= 1024, (n, rows)
     assert lib.fneus_layer_norm_bwd_scratch_floats(256, 3) == 6 and lib.fneus_layer_norm_bwd_scratch_floats(257, 3) == 12
+
+
+@pytest.mark.gpu
+def test_layer_norm_input_gradient_of_many_rows():
+    """2^28 + 40 rows of 8 values without weight gradients: 2^32 threads were a launch's.  All rows but the last hundred are one row seen again"""
+    from fneus import ops
+    rows, n = (1 << 28) + 40, 8
+    near = torch.randn(100, n, generator=torch.Generator().manual_seed(4)).cuda().bfloat16()
+    x = torch.empty(rows, n, dtype=torch.bfloat16, device="cuda")
+    x[:-100] = near[:1]
+    x[-100:] = near
+    y, mean, rstd = ops.layer_norm_fwd(x)
+    ry, rmean, rrstd = ops.layer_norm_fwd(near)
+    assert torch.equal(y[-100:], ry) and torch.equal(mean[-100:], rmean) and bool((y[:-100] == ry[0]).all())
+    del y
+    dx = ops.layer_norm_bwd(x, x, None, mean, rstd, need_params=False)[0]
+    want = ops.layer_norm_bwd(near, near, None, rmean, rrstd, need_params=False)[0]
+    assert torch.equal(dx[-100:], want) and bool((dx[:-100] == want[0]).all())
