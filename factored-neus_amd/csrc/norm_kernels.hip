@@ -19,7 +19,7 @@ namespace fneus {
 
 constexpr int kNormMaxGrid = 1024;       // workgroups of the backward at most
 constexpr long kNormFwdGrid = 2048;      // of the forward: 8 a CU
-constexpr long kNormBwdGrid = 1L << 20;  // of the backward without weight gradients: the launch's limit alone
+constexpr long kNormBwdGrid = 1L << 20;  // of the backward without weight gradients, and of the fold: the launch's limit alone
 
 // sums of v over the team, in every thread of it.  `red`: LDS floats, 2 * TPR / 64 (TPR > 64); `flip` alternates the half used, so
 // one barrier a sum is enough
@@ -401,14 +401,17 @@ template <class P>
 __global__ void __launch_bounds__(1024) layer_norm_fold_kernel(const float* __restrict__ partial, int parts, int n, P* __restrict__ dw,
                                                                P* __restrict__ db) {
     __shared__ float red[128][9];
-    const long col0 = 8L * blockIdx.x, col = col0 + threadIdx.x;          // of the 2 n columns
-    const float s = fold_rows8(partial, parts, 2L * n, col0, 2L * n, red);
-    if (threadIdx.x < 8 && col < 2L * n) {
-        if (col < n) {
-            if (dw) dw[col] = (P)s;
-        } else if (db) {
-            db[col - n] = (P)s;
+    for (long col0 = 8L * blockIdx.x; col0 < 2L * n; col0 += 8L * gridDim.x) {          // of the 2 n columns
+        const long col = col0 + threadIdx.x;
+        const float s = fold_rows8(partial, parts, 2L * n, col0, 2L * n, red);
+        if (threadIdx.x < 8 && col < 2L * n) {
+            if (col < n) {
+                if (dw) dw[col] = (P)s;
+            } else if (db) {
+                db[col - n] = (P)s;
+            }
         }
+        __syncthreads();                 // (the next columns' sums go to the same cells)
     }
 }
 
@@ -494,8 +497,11 @@ static void norm_bwd_launch(const NormArgs<T, P>& a, P* dw, P* db, hipStream_t s
 #undef CALL
         }
     }
-    if (params)
-        hipLaunchKernelGGL((layer_norm_fold_kernel<P>), dim3((unsigned)((2L * a.n + 7) / 8)), dim3(1024), 0, stream, a.partial, grid, a.n, dw, db);
+    if (params) {
+        const long folds = (2L * a.n + 7) / 8;
+        hipLaunchKernelGGL((layer_norm_fold_kernel<P>), dim3((unsigned)(folds < kNormBwdGrid ? folds : kNormBwdGrid)), dim3(1024), 0, stream, a.partial,
+                           grid, a.n, dw, db);
+    }
 }
 
 static int norm_check(const char* what, const void* x, const void* out, const void* mean, const void* rstd, long rows, int n, int dtype,

@@ -267,3 +267,19 @@ def test_layer_norm_input_gradient_of_many_rows():
     dx = ops.layer_norm_bwd(x, x, None, mean, rstd, need_params=False)[0]
     want = ops.layer_norm_bwd(near, near, None, rmean, rrstd, need_params=False)[0]
     assert torch.equal(dx[-100:], want) and bool((dx[:-100] == want[0]).all())
+
+
+@pytest.mark.gpu
+def test_layer_norm_of_a_row_beyond_2_to_24():
+    """one row of 2^24 + 8 values: the fold of its weight gradients has more columns than a launch has threads for.  Sums of 2^14 values a thread in
+    series: sqrt(2^14 / 3) 2^-24 = 4e-6 of a thread's own sum, 1024 threads' errors add at random"""
+    from fneus import ops
+    n = (1 << 24) + 8
+    g = torch.Generator(device="cuda").manual_seed(3)
+    r = lambda: torch.randn(1, n, generator=g, device="cuda")  # noqa: E731
+    x, dy, w, b = r(), r(), 1 + 0.2 * r()[0], 0.2 * r()[0]
+    y, mean, rstd = ops.layer_norm_fwd(x, w, b)
+    dx, dw, db = ops.layer_norm_bwd(dy, x, w, mean, rstd)
+    ref = formula(x, w, b, 1e-5, dy)
+    assert abs(float(mean) - float(ref[1])) <= 2e-6 and abs(float(rstd) / float(ref[2]) - 1) <= 2e-6
+    compare((y, None, None, dx, dw, db), ref, torch.float32, (2e-5,) * 6)
