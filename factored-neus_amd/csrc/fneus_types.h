@@ -155,4 +155,12 @@ FN_DEV float wave_sum(float v) {
     return v;
 }
 
+// A launch takes fewer than 2^32 threads along a dimension: more than kWideGrid workgroups go along two.  wide_block() is a workgroup's number,
+// of which the last may lie beyond the count.
+constexpr long kWideGrid = 1L << 15;
+inline dim3 wide_grid(long groups) {
+    return groups <= kWideGrid ? dim3((unsigned)groups) : dim3((unsigned)kWideGrid, (unsigned)((groups + kWideGrid - 1) / kWideGrid));
+}
+FN_DEV long wide_block() { return (long)blockIdx.y * gridDim.x + blockIdx.x; }
+
 }  // namespace fneus

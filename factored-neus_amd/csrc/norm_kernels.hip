@@ -5,11 +5,11 @@
 // holds it in registers (EPT values a thread, 16-byte chunks): one pass over memory, the variance from the centred values (two
 // passes over registers: a row with a large mean keeps its digits).  TPR = 16 (sums by DPP), 64, 256 or 512 threads; wider rows
 // take the streaming kernels, which read a row from the caches again; rows of fewer than 8 values a thread each.  A launch takes fewer than 2^32
-// threads, so every grid is capped and its workgroups go on to further rows.
+// threads along a dimension, so grids are capped and their workgroups go on to further rows (the streaming kernels': a grid along two).
 // The weight gradients: a team keeps its columns' sums of dy xh and dy in registers over all the rows it takes, the teams of a
 // workgroup are added in LDS, every workgroup writes ONE partial row, and a second launch adds the partial rows in a fixed order: no
 // atomics, the same bits in every run.
-// MEASURED (MI355X, us): forward 8192 x 8192 bf16 46 (5.8 TB/s with the caches' help; a copy of 1 GiB: 5.1), 65536 x 256 fp32 23 (5.8); backward
+// MEASURED (MI355X, us): 4M x 3 fp32 forward 26, backward 43; forward 8192 x 8192 bf16 46 (5.8 TB/s with the caches' help; a copy of 1 GiB: 5.1), 65536 x 256 fp32 23 (5.8); backward
 // of the latter 33 (5.8) + 4.6 for the fold; 4099 x 1031 fp16 11 / 15 / 5: latency, unaligned rows; one row of 4096 3.4.  A workgroup of 1024
 // threads a row took 140 at 8192 x 8192: two rows a CU in flight, two barriers each.
 #include "fneus_types.h"
@@ -206,10 +206,15 @@ __global__ void __launch_bounds__(256) layer_norm_bwd_thin_kernel(NormArgs<T, P>
     }
 }
 
-// rows wider than a team's registers: a workgroup a row (blockIdx, blockIdx + grid, ...), three passes (the second and third from the caches)
+// rows wider than a team's registers: a workgroup a row, three passes (the second and third from the caches).  (Workgroups that go on to
+// further rows: 442 us against 374 at 8192 x 20000 bf16.)
 template <class T, class P>
-FN_DEV void layer_norm_fwd_stream_row(const NormArgs<T, P>& a, long row, float* red, int& flip) {
+__global__ void __launch_bounds__(1024) layer_norm_fwd_stream_kernel(NormArgs<T, P> a) {
     constexpr int V = Chunk<T>::N;
+    __shared__ float red[32];
+    int flip = 0;
+    const long row = wide_block();
+    if (row >= a.rows) return;
     const T* x = a.x + row * a.ldx;
     const float len = (float)a.n;
     float s = 0.0f, v[V];
@@ -239,12 +244,6 @@ FN_DEV void layer_norm_fwd_stream_row(const NormArgs<T, P>& a, long row, float* 
         a.mean[row] = mu;
         a.rstd[row] = r;
     }
-}
-template <class T, class P>
-__global__ void __launch_bounds__(1024) layer_norm_fwd_stream_kernel(NormArgs<T, P> a) {
-    __shared__ float red[32];
-    int flip = 0;
-    for (long row = blockIdx.x; row < a.rows; row += gridDim.x) layer_norm_fwd_stream_row(a, row, red, flip);
 }
 
 // dx of the rows blockIdx, blockIdx + grid, ... and, PARAMS, this workgroup's partial row of (dw, db)
@@ -344,8 +343,12 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) layer_norm_bwd_kernel(N
 }
 
 template <class T, class P>
-FN_DEV void layer_norm_bwd_stream_row(const NormArgs<T, P>& a, long row, float* red, int& flip) {
+__global__ void __launch_bounds__(1024) layer_norm_bwd_stream_kernel(NormArgs<T, P> a) {
     constexpr int V = Chunk<T>::N;
+    __shared__ float red[32];
+    int flip = 0;
+    const long row = wide_block();
+    if (row >= a.rows) return;
     const T *x = a.x + row * a.ldx, *dy = a.dy + row * a.lddy;
     const float mu = a.mean[row], r = a.rstd[row], inv_n = 1.0f / (float)a.n;
     float s1 = 0.0f, s2 = 0.0f, v[V], d[V];
@@ -372,12 +375,6 @@ FN_DEV void layer_norm_bwd_stream_row(const NormArgs<T, P>& a, long row, float* 
             if (k < left) v[k] = r * (d[k] * (a.w ? (float)a.w[col + k] : 1.0f) - s1 - (v[k] - mu) * r * s2);
         store_chunk<T>(a.dx + row * a.lddx + col, left, v);
     }
-}
-template <class T, class P>
-__global__ void __launch_bounds__(1024) layer_norm_bwd_stream_kernel(NormArgs<T, P> a) {
-    __shared__ float red[32];
-    int flip = 0;
-    for (long row = blockIdx.x; row < a.rows; row += gridDim.x) layer_norm_bwd_stream_row(a, row, red, flip);
 }
 
 // the streaming form's partial rows: a thread a column, the rows blockIdx.y, blockIdx.y + gridDim.y, ...
@@ -459,7 +456,7 @@ static void norm_fwd_launch(const NormArgs<T, P>& a, hipStream_t stream) {
     const long need = (a.rows + teams - 1) / teams;
     const dim3 grid((unsigned)(need < kNormFwdGrid ? need : kNormFwdGrid));
     if (s.tpr == 0) {
-        hipLaunchKernelGGL((layer_norm_fwd_stream_kernel<T, P>), grid, dim3(1024), 0, stream, a);
+        hipLaunchKernelGGL((layer_norm_fwd_stream_kernel<T, P>), wide_grid(a.rows), dim3(1024), 0, stream, a);
         return;
     }
     if (s.tpr == 1) {
@@ -480,8 +477,7 @@ static void norm_bwd_launch(const NormArgs<T, P>& a, P* dw, P* db, hipStream_t s
         if (params) hipLaunchKernelGGL((layer_norm_bwd_thin_kernel<T, P, true>), dim3((unsigned)grid), dim3(256), 0, stream, a);
         else hipLaunchKernelGGL((layer_norm_bwd_thin_kernel<T, P, false>), dim3((unsigned)grid), dim3(256), 0, stream, a);
     } else if (s.tpr == 0) {
-        const dim3 most((unsigned)(a.rows < kNormFwdGrid ? a.rows : kNormFwdGrid));
-        hipLaunchKernelGGL((layer_norm_bwd_stream_kernel<T, P>), most, dim3(1024), 0, stream, a);
+        hipLaunchKernelGGL((layer_norm_bwd_stream_kernel<T, P>), wide_grid(a.rows), dim3(1024), 0, stream, a);
         if (params) hipLaunchKernelGGL((layer_norm_params_kernel<T, P>), dim3((unsigned)((a.n + 255) / 256), (unsigned)grid), dim3(256), 0, stream, a);
     } else {
         const int threads = s.tpr > 256 ? s.tpr : 256, teams = threads / s.tpr;

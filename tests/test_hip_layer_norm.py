@@ -283,3 +283,20 @@ def test_layer_norm_of_a_row_beyond_2_to_24():
     ref = formula(x, w, b, 1e-5, dy)
     assert abs(float(mean) - float(ref[1])) <= 2e-6 and abs(float(rstd) / float(ref[2]) - 1) <= 2e-6
     compare((y, None, None, dx, dw, db), ref, torch.float32, (2e-5,) * 6)
+
+
+@pytest.mark.gpu
+def test_layer_norm_stream_rows_along_two_grid_dimensions():
+    """rows beyond the registers' form, more than the 2^15 that a launch has along its first dimension"""
+    from fneus import ops
+    rows, n = (1 << 15) + 3, 16387
+    near = torch.randn(5, n, generator=torch.Generator().manual_seed(4)).cuda().half()
+    x = torch.empty(rows, n, dtype=torch.float16, device="cuda")
+    x[:-5] = near[:1]
+    x[-5:] = near
+    y, mean, rstd = ops.layer_norm_fwd(x)
+    ry, rmean, rrstd = ops.layer_norm_fwd(near)
+    assert torch.equal(y[-5:], ry) and bool((y[:-5] == ry[0]).all()) and torch.equal(mean[-5:], rmean) and bool((rstd[:-5] == rrstd[0]).all())
+    dx = ops.layer_norm_bwd(x, x, None, mean, rstd, need_params=False)[0]
+    want = ops.layer_norm_bwd(near, near, None, rmean, rrstd, need_params=False)[0]
+    assert torch.equal(dx[-5:], want) and bool((dx[:-5] == want[0]).all())
