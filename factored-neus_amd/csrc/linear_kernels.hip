@@ -166,7 +166,8 @@ __global__ void __launch_bounds__(512) linear_direct_bwd_kernel(LinProduct dx, L
 template <class T, bool HEAD>
 __global__ void __launch_bounds__(512) linear_row_kernel(LinProduct P) {
     __shared__ float red[8][16][17];
-    const int j0 = 16 * (int)blockIdx.x;
+    const long j0 = 16 * wide_block();
+    if (j0 >= P.nj) return;
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const long part = ((P.nk + 7) / 8 + 31) / 32 * 32;
@@ -204,7 +205,7 @@ __global__ void __launch_bounds__(512) linear_row_kernel(LinProduct P) {
         for (int w = 0; w < 8; ++w) v += red[w][jj][ii];
         if (ii < P.ni && j0 + jj < P.nj) {
             const long row = HEAD ? j0 + jj : ii;
-            const int col = HEAD ? ii : j0 + jj;
+            const int col = HEAD ? ii : (int)j0 + jj;
             if (P.bias) v += (float)((const T*)P.bias)[col];
             if (P.z) ((T*)P.z)[row * P.ldd + col] = (T)v;
             v = lin_act(v, P.act);
@@ -253,7 +254,9 @@ template <class Cfg, class T, bool AKM, bool BKM, int EPI, int CLASS>
 __global__ void __launch_bounds__(Cfg::THREADS, 2) linear_tiled_kernel(LinTiled P) {
     extern __shared__ __attribute__((aligned(16))) unsigned char mm_smem[];
     const long tiles = (long)P.tiles_i * P.tiles_j;
-    const long t = mm_spread(blockIdx.x, tiles * P.splits);
+    const long wg = wide_block();
+    if (wg >= tiles * P.splits) return;
+    const long t = mm_spread(wg, tiles * P.splits);
     const int split = (int)(t / tiles);
     int ti, tj;
     mm_tile(t - split * tiles, P.tiles_i, P.tiles_j, ti, tj);
@@ -674,7 +677,7 @@ template <class Cfg, class T, bool AKM, bool BKM, int EPI, int CLASS>
 static void lin_tiled_launch(const LinTiled& t, hipStream_t stream) {
     auto kernel = linear_tiled_kernel<Cfg, T, AKM, BKM, EPI, CLASS>;
     allow_big_lds(kernel);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((long)t.tiles_i * t.tiles_j * t.splits)), dim3(Cfg::THREADS), Cfg::LDS, stream, t);
+    hipLaunchKernelGGL(kernel, wide_grid((long)t.tiles_i * t.tiles_j * t.splits), dim3(Cfg::THREADS), Cfg::LDS, stream, t);
 }
 
 template <class Cfg, class T, bool AKM, bool BKM, bool FWD>
@@ -847,7 +850,7 @@ static int lin_fwd(const FneusLinear& f, hipStream_t stream) {
     }
     if (lin_head(f)) {
         p.a = f.weight, p.lda = f.n_in, p.b = f.x, p.ldb = f.ldx, p.ni = f.n_out, p.nj = (int)f.rows;
-        hipLaunchKernelGGL((linear_row_kernel<T, true>), dim3((unsigned)((f.rows + 15) / 16)), dim3(512), 0, stream, p);
+        hipLaunchKernelGGL((linear_row_kernel<T, true>), wide_grid((f.rows + 15) / 16), dim3(512), 0, stream, p);
         return launch_status();
     }
     p.tiles_j = (p.nj + 31) / 32;

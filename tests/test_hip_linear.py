@@ -358,3 +358,34 @@ def test_linear_heads_in_a_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(out, run()))
+
+
+# More workgroups than 2^32 threads hold, which is what a launch takes along its first dimension
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,n_in,n_out", [((1 << 27) + 37, 264, 2), ((1 << 30) + 70, 8, 1)], ids=["head", "tiled"])
+def test_linear_more_rows_than_a_launch_takes(rows, n_in, n_out):
+    """heads of 2^27 rows (512 threads per 16 of them), few outputs of 2^30 rows (256 threads per 64): forward, and the tiled input gradient.  All
+    rows but the last hundred are one row seen again: the same bits in every place (a row's sums do not depend on its place)"""
+    from fneus import ops
+    g = torch.Generator().manual_seed(6)
+    near = torch.randn(100, n_in, generator=g).bfloat16().cuda()
+    w = (torch.randn(n_out, n_in, generator=g) / math.sqrt(n_in)).bfloat16().cuda()
+    x = torch.empty(rows, n_in, dtype=torch.bfloat16, device="cuda")
+    x[:-100] = near[:1]
+    x[-100:] = near
+    y = ops.linear_fwd(x, w, act="silu")[0]
+    zd = near.double() @ w.double().t()
+    want = act64(zd, "silu")
+    lim = (1.13 * sums(n_in) + 4 * 2.0 ** -23) * (near.double().abs() @ w.double().abs().t()) + half(torch.bfloat16) * want.abs()
+    check(y[-100:], want, lim + torch.finfo(torch.bfloat16).smallest_normal, "y")
+    check(y[:1], want[:1], lim[:1] + torch.finfo(torch.bfloat16).smallest_normal, "y")
+    same = y[0].clone()
+    assert bool((y[:-100] == same).all())
+    if n_in == 8:
+        del y
+        dy = torch.empty(rows, n_out, dtype=torch.bfloat16, device="cuda")
+        dy[:-100], dy[-100:] = 0.5, near[:, :n_out]
+        dx = ops.linear_bwd(dy, x, w, need=(True, False, False))[0]
+        want = near[:, :n_out].double() @ w.double()
+        check(dx[-100:], want, (half(torch.bfloat16) + sums(n_out)) * want.abs() + torch.finfo(torch.bfloat16).smallest_normal, "dx")
+        assert bool((dx[:-100] == (0.5 * w.float()).bfloat16()[0]).all())
