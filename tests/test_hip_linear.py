@@ -389,3 +389,24 @@ def test_linear_more_rows_than_a_launch_takes(rows, n_in, n_out):
         want = near[:, :n_out].double() @ w.double()
         check(dx[-100:], want, (half(torch.bfloat16) + sums(n_out)) * want.abs() + torch.finfo(torch.bfloat16).smallest_normal, "dx")
         assert bool((dx[:-100] == (0.5 * w.float()).bfloat16()[0]).all())
+
+
+@pytest.mark.gpu
+def test_linear_gelu_keeps_its_digits_in_the_tail():
+    """fp32 GELU and its derivative relative to their own size, through identity weights (z = x and dx = delta to the last bit: three bf16 terms hold 24).
+    exp(-z^2 / 2): the argument is off by six roundings (1 / sqrt 2, the product, the square twice over, log2 e, the product) of z^2 / 2 each, 3 z^2 2^-24;
+    the instructions' ulp, nine steps of the polynomial and four products: at most 16 + 8 x 2^-24 more"""
+    from fneus import ops
+    z = torch.linspace(-8.0, 8.0, 4096 * 64, device="cuda").reshape(-1, 64).contiguous()
+    eye = torch.eye(64, device="cuda")
+    for rows in (8, 500, 4096):                     # (each form of the product)
+        x = z[:: 4096 // rows].contiguous()
+        y, zz = ops.linear_fwd(x, eye, act="gelu", train=True)
+        assert torch.equal(zz, x)
+        d = x.double()
+        want = act64(d, "gelu")
+        rel = (3 * d * d + 24) * 2.0 ** -24
+        check(y, want, rel * want.abs(), "gelu")
+        dx = ops.linear_bwd(torch.ones_like(x), x, eye, zz, act="gelu", need=(True, False, False))[0]
+        pdf = torch.exp(-d * d / 2) / math.sqrt(2 * math.pi)
+        check(dx, dact64(d, "gelu"), rel * (0.5 * torch.special.erfc(-d * math.sqrt(0.5)) + d.abs() * pdf), "gelu'")
