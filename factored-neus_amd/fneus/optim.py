@@ -114,6 +114,13 @@ class FlatAdam(torch.optim.Adam):
         lr = self.param_groups[0]["lr"]
         if float(lr) != self._lr_host:       # someone assigned param_groups[0]["lr"] directly (reference style)
             self.set_lr(float(lr))
+        device = self._lr_dev.device
+        if device.index != torch.cuda.current_device():      # the launch goes to the device of the parameters, whichever is current
+            with torch.cuda.device(device):
+                return self._launch()
+        self._launch()
+
+    def _launch(self):
         b1, b2 = self.param_groups[0]["betas"]
         check(lib.fneus_adam(self._segs, len(self._segs), C.c_void_p(self._lr_dev.data_ptr()),
                              C.c_void_p(self._step_dev.data_ptr()), float(b1), float(b2), float(self.param_groups[0]["eps"]),

@@ -420,3 +420,29 @@ def test_flat_muon_refuses_its_first_step_in_a_capture():
     assert float(other[0]) == 1.0 and torch.equal(p, old) and not opt.state[p]
     opt.step()
     assert not torch.equal(p, old)
+
+
+@pytest.mark.gpu
+def test_optimizers_launch_on_the_device_of_their_parameters(monkeypatch):
+    """another device is current when step() is called: the launch is made with the parameters' device current, on that device's stream (here the
+    runtime is made to say that device 1 is current until somebody selects device 0)"""
+    from fneus.optim import FlatAdam, FlatMuon
+    p = nn.Parameter(torch.randn(7, device="cuda:0"))
+    p.grad = torch.ones_like(p)
+    entered = []
+
+    class select(torch.cuda.device):
+        def __enter__(self):
+            entered.append(self.idx)
+            return super().__enter__()
+
+    for opt in (FlatAdam([p], lr=1e-2), FlatMuon([p], lr=1e-2)):
+        start = p.detach().clone()
+        p.grad.fill_(1.0)
+        del entered[:]
+        with monkeypatch.context() as m:
+            m.setattr(torch.cuda, "current_device", lambda: entered[-1] if entered else 1)
+            m.setattr(torch.cuda, "device", select)
+            opt.step()
+        assert entered and set(entered) == {0}
+        assert float((p.detach() - start).abs().min()) > 0.0
