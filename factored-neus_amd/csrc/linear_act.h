@@ -58,15 +58,17 @@ FN_DEV float lin_act_of(float z, float slope, bool times) {
     else return lin_act(z, CLASS);
 }
 
-// act'(z); at 0 the ReLUs take the slope of the negative side
+FN_DEV float lin_near(float z) { return fabsf(z) > 128.0f ? 0.0f : z; }
+// act'(z); at 0 the ReLUs take the slope of the negative side.  An infinite z has the limit (an fp16 z beyond 65504 is stored as infinity, its output
+// may be finite): GELU's and SiLU's z times a factor that is 0 from |z| = 128 on is formed with z = 0 there, not as infinity times 0.
 FN_DEV float lin_dact(float z, int act) {
     switch (act) {
         case 1: return z > 0.0f ? 1.0f : 0.0f;
         case 2: return z > 0.0f ? 1.0f : 0.2f;
         case 3: { const float s = lin_sigmoid(z); return s * (1.0f - s); }
         case 4: return lin_sigmoid(100.0f * z);
-        case 5: { float e; const float p = lin_phi(z, e); return p + z * (0.39894228040143268f * e); }
-        case 6: { const float s = lin_sigmoid(z); return s * (1.0f + z * (1.0f - s)); }
+        case 5: { float e; const float p = lin_phi(z, e); return p + lin_near(z) * (0.39894228040143268f * e); }
+        case 6: { const float s = lin_sigmoid(z); return s * (1.0f + lin_near(z) * (1.0f - s)); }
         default: return 1.0f;
     }
 }

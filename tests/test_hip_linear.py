@@ -410,3 +410,25 @@ def test_linear_gelu_keeps_its_digits_in_the_tail():
         dx = ops.linear_bwd(torch.ones_like(x), x, eye, zz, act="gelu", need=(True, False, False))[0]
         pdf = torch.exp(-d * d / 2) / math.sqrt(2 * math.pi)
         check(dx, dact64(d, "gelu"), rel * (0.5 * torch.special.erfc(-d * math.sqrt(0.5)) + d.abs() * pdf), "gelu'")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["sigmoid", "softplus", "gelu", "silu"])
+def test_linear_gradient_at_pre_activations_beyond_fp16(act):
+    """z = -160000 and +160000 in fp16 rows: stored as infinities; the derivative there is its limit (0, and 1 or 0), not NaN; a NaN stays one"""
+    from fneus import ops
+    for rows, n_out in ((4, 24), (500, 24), (9000, 24), (9000, 3)):        # (each form)
+        x = torch.full((rows, 8), 200.0, dtype=torch.float16, device="cuda")
+        x[1] = -200.0
+        x[2, 0] = float("nan")
+        w = torch.full((n_out, 8), -100.0, dtype=torch.float16, device="cuda")
+        y, z = ops.linear_fwd(x, w, act=act, train=True)
+        assert bool(torch.isinf(z[0]).all()) and bool(torch.isfinite(y[0]).all()) and bool((y[0] == 0).all())
+        dy = torch.full((rows, n_out), 2.0 ** -7, dtype=torch.float16, device="cuda")
+        dx, dw, db = ops.linear_bwd(dy, x, w, z, act=act)
+        assert bool((dx[0] == 0).all()) and bool((dx[3:] == 0).all()) and bool(torch.isnan(dx[2]).all())
+        up = 0.0 if act == "sigmoid" else -100.0 * n_out * 2.0 ** -7
+        assert bool((dx[1] == up).all()), (rows, n_out, dx[1])
+        clean = [k for k in range(rows) if k != 2]
+        db = ops.linear_bwd(dy[clean], x[clean], w, z[clean], act=act)[2]
+        assert bool((db == (0.0 if act == "sigmoid" else 2.0 ** -7)).all())
