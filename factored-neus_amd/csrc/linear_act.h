@@ -7,7 +7,8 @@ namespace fneus {
 
 constexpr int kLinActs = 7;
 
-// exp by the base-2 instruction, 1 / x by the reciprocal instruction (1 ulp each): sigmoid to 2e-8 absolute
+// exp by the base-2 instruction, 1 / x by the reciprocal instruction (1 ulp each): sigmoid to 1e-7 absolute (its largest values lie next to 1, where an
+// ulp is 6e-8)
 FN_DEV float lin_exp(float x) { return fast_exp2(x * kLog2e); }
 FN_DEV float lin_sigmoid(float z) { return fast_rcp(1.0f + lin_exp(-z)); }
 
@@ -74,9 +75,10 @@ FN_DEV float lin_dact(float z, int act) {
 }
 
 // Operands of the 32x32x16 / 16x16x32 matrix instructions: 8 consecutive values of the contraction a lane.  bf16 and fp16 enter as
-// they are.  An fp32 value enters as THREE bf16 terms x = t0 + t1 + t2 (each the rounding of what is left: 24 bits, the whole range of
-// fp32), a product as the six term pairs down to 2^-24 of it, smallest first: fp32's accuracy at 6 bf16 MFMAs (16 k in 192 cycles; the
-// fp32 MFMA takes 512).  An infinity has NaN as its second term, so it comes out as NaN.
+// they are.  An fp32 value enters as THREE bf16 terms x = t0 + t1 + t2 (each the rounding of what is left: 24 bits for 2^-110 <= |x| < 3.39e38;
+// below, the last terms' bits fall under bf16's smallest value, 2^-133), a product as the six term pairs down to 2^-24 of it, smallest first:
+// fp32's accuracy at 6 bf16 MFMAs (16 k in 192 cycles; the fp32 MFMA takes 512).  An infinity, and a finite value that rounds above bf16's
+// largest (3.39e38), has NaN as its second term, so it comes out as NaN.
 template <class T> struct LinFrag;
 template <> struct LinFrag<__bf16> { bf16x8 t; };
 template <> struct LinFrag<_Float16> { fn_f16x8 t; };

@@ -3,10 +3,15 @@
 // The three products are one form, D(i, j) = sum_k A(i, k) B(j, k), with either operand stored along k or along its rows.
 // Three forms of it: one for up to 16 rows (bound by reading W), direct tiles (bound by latency), tiles through LDS (mm_engine.h: bound by the
 // matrix rate the part sustains; an fp32 product is six bf16 ones).  MEASURED (MI355X, us): 1 x 4096 -> 4096 bf16 SiLU + residual 7.9 (4.3 TB/s of
-// W); 512 x 512 -> 512 fp32 forward 9, backward 27; 65536 x 256 -> 256 fp32 softplus + residual forward 102, delta 45, dx 63 (0.82 PFLOP/s of
-// MFMAs), dW 67 + 5 + 5; 8192 x 4096 -> 8192 bf16 dx 465 (1.18 PFLOP/s; the library's 8192^3: 1.34), dW 484, forward with GELU, residual and
-// the stored pre-activation 625 (its epilogue has nothing to run beside at one workgroup a CU), delta 93.  Heads (up to 16 outputs) have a
-// form of their own each way, bound by reading x: 18135 x 4308 -> 1 fp32 forward 73 (4.3 TB/s), backward 157 (6 TB/s with the caches' help).
+// W); 512 x 512 -> 512 fp32 forward 9, backward 27; 65536 x 256 -> 256 fp32 softplus + residual forward 102, delta 46, dx 66 (0.78 PFLOP/s of
+// MFMAs), dW 69 + 5 + 5; 8192 x 4096 -> 8192 bf16 dx 465 (1.18 PFLOP/s; the library's 8192^3: 1.34), dW 499, forward with GELU, residual and
+// the stored pre-activation 625 (its epilogue has nothing to run beside at one workgroup a CU), delta 95.  Heads (up to 16 outputs) have a
+// form of their own each way, bound by reading x: 18135 x 4308 -> 1 fp32 forward 68 (4.6 TB/s), backward 155 (6 TB/s with the caches' help).
+// Roundings beside the outputs': 16-bit rows store z in their own type, and act' is taken at that z (as a module that keeps its pre-activation in the
+// rows' type does: an fp32 z would double what the forward writes beside y); their products take delta rounded to the rows' type (one matrix
+// product instead of the two that a second term of delta needs).  Against 64 bits that leaves dx and dW with 1.4 roundings of the type instead of one
+// (relative, bf16 8192 x 4096 -> 8192: 2.4e-3 / 1.7e-3; fp16 1999 x 777 -> 1111: 3.0e-4 / 2.1e-4).  The bias gradient and the heads' form take delta
+// unrounded.  fp32 rows have neither.
 #include <type_traits>
 #include "mm_engine.h"
 #include "fneus_kernels.h"

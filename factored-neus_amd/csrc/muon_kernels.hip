@@ -10,9 +10,9 @@
 // rounding left, times another 2^11, so that it is as normal as the first; products hi hi + hi lo + lo hi (22 bits: fp32's accuracy at
 // half the matrix work of three bf16 terms).
 //
-// What bounds it (MI355X, us): one fp32 4096^2 matrix 4600, of which matrix products 4470 at 1.0 - 1.1 PFLOP/s of fp16 MFMAs (a bare stream
-// of them: 1.6), the momentum and norm 56 (5 x 64 MiB: 6 TB/s); four bf16 4096 x 1024 531 (X X^T 41, A A 18, B X 48 a step); eight fp32
-// 256^2 145 = 17 launches of 8 .. 10: 1.3 until the job is read, 2.7 until the first stage has arrived from the other XCDs' writes, 0.4 a stage.
+// What bounds it (MI355X, us): one fp32 4096^2 matrix 4600, of which matrix products 3950 at 1.0 - 1.1 PFLOP/s of fp16 MFMAs (a bare stream
+// of them: 1.6), the joins of the shared-out ones 550, the momentum and norm 56 (5 x 64 MiB: 6 TB/s); four bf16 4096 x 1024 544 (X X^T 41, A A 18, B X 48 a step); eight fp32
+// 256^2 142 = 17 launches of 8 .. 10: 1.3 until the job is read, 2.7 until the first stage has arrived from the other XCDs' writes, 0.4 a stage.
 #include <math.h>
 #include "mm_engine.h"
 #include "fneus_kernels.h"

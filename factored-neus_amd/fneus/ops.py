@@ -1346,7 +1346,7 @@ def _linear_scratch(job, backward: int, x):
 def linear_fwd(x, weight, bias=None, act="none", residual=None, train: bool = False):
     """(y, z): y = act(x weight^T + bias) + residual of x [rows, n_in], weight [n_out, n_in], bias [n_out], residual [rows, n_out], all of one
     type (float32, bfloat16, float16); act: a key of LINEAR_ACTS or its code.  z: with train and an activation, the pre-activation
-    linear_bwd takes, else None."""
+    linear_bwd takes (in x's type, rounded once), else None."""
     code = _act_code(act)
     x = _rows(x, "linear: x")
     device = x.device.index
@@ -1373,7 +1373,8 @@ def linear_fwd(x, weight, bias=None, act="none", residual=None, train: bool = Fa
 
 def linear_bwd(dy, x, weight, z=None, act="none", need=(True, True, True)):
     """(dx, dweight, dbias) of linear_fwd(..., train=True), each where `need` asks for it, else None; the residual's gradient is dy.
-    dbias [n_out] comes in the one type of the other arrays."""
+    dbias [n_out] comes in the one type of the other arrays.  16-bit arrays: act' is taken at the rounded z, and dx and dweight are products of
+    dy act'(z) rounded to that type, as those of a 16-bit module are; float32 arrays carry both in full."""
     code = _act_code(act)
     x = _rows(x, "linear: x")
     device = x.device.index
@@ -1486,7 +1487,8 @@ def muon_step(params, grads, momenta, lr, momentum: float = 0.95, nesterov: bool
               coefficients=NS_COEFFICIENTS, steps: int = 5, eps: float = 1e-7, prec: Optional[int] = None, zero_grad: bool = False):
     """One Muon update of every matrix, in place: m <- mu m + (1 - mu) g;  u = (1 - mu) g + mu m (nesterov) or m;
     p <- p (1 - lr weight_decay) - lr adjust NS(u), NS as in newton_schulz.  params, grads, momenta: lists of contiguous matrices of one
-    type; lr: float32 device scalar (a captured step sees its changes) or a number; zero_grad clears the gradients after use."""
+    type; lr: float32 device scalar (a captured step sees its changes) or a number; zero_grad clears the gradients after use; prec as in
+    newton_schulz."""
     table = muon_jobs(params, grads, momenta, adjust)
     if table[1] == 0:
         return
@@ -1500,7 +1502,9 @@ def muon_step(params, grads, momenta, lr, momentum: float = 0.95, nesterov: bool
 
 def newton_schulz(g, coefficients=NS_COEFFICIENTS, steps: int = 5, eps: float = 1e-7, prec: Optional[int] = None):
     """The matrix g [rows, cols], or each of a stack [count, rows, cols], with its singular values taken towards 1: X = g / max(|g|_F, eps), then
-    `steps` times X <- a X + (b A + c A^2) X, A = X X^T (for rows > cols on the transpose).  -> a tensor of g's shape and type"""
+    `steps` times X <- a X + (b A + c A^2) X, A = X X^T (for rows > cols on the transpose).  -> a tensor of g's shape and type.
+    prec: how many bits the products carry, PREC_H16 11 (the default of 16-bit matrices: it adds less than their own rounding does) or PREC_PARITY
+    22 at three times the matrix work (the default of float32)."""
     if g.dim() not in (2, 3) or not g.is_cuda or g.dtype not in _DTYPES:
         raise ValueError("newton_schulz: a CUDA matrix, or a stack of them, of float32, bfloat16 or float16")
     device = g.device.index

@@ -177,7 +177,7 @@ class FlatMuon(torch.optim.Optimizer):
     load_state_dict).
 
     params: parameters; the 2-D ones with no side shorter than `min_side` are Muon's (a layer with a handful of outputs has no spectrum to
-    level), the others Adam's.  State: `momentum_buffer` a matrix, torch.optim.Adam's of the others.  A parameter without a gradient is
+    level), the others Adam's (fp32, as FlatAdam's are; weight_decay is Muon's alone).  State: `momentum_buffer` a matrix, torch.optim.Adam's of the others.  A parameter without a gradient is
     skipped."""
 
     def __init__(self, params, lr=1e-3, momentum=0.95, nesterov=True, weight_decay=0.0, adjust="match_rms", coefficients=None, steps=5,

@@ -627,7 +627,7 @@ int fneus_composite_bwd(const float* rays_o, const float* rays_d, const float* m
  * Not in the reference.  dtype: 0 fp32, 1 bf16, 2 fp16 (x, y, dy, dx); wtype: the type of weight / bias and of their gradients, dtype or 0.
  * Rows of n values, row strides ld* >= n in elements, any alignment; weight / bias may be NULL (1 / 0).  Statistics and sums in fp32,
  * outputs rounded once.  y = (x - mean) rstd w + b, rstd = 1 / sqrt(var + eps) (var: biased); mean, rstd [rows] are the backward's.
- * rows == 0: nothing is done (forward), refused (backward).  NaN and infinities stay in their row (forward, dx).
+ * Up to 2^31 - 1 rows, any n.  rows == 0: nothing is done (forward), refused (backward).  NaN and infinities stay in their row (forward, dx).
  * No output may share memory with an input, but y may be x. */
 int fneus_layer_norm_fwd(const void* x, long ldx, const void* weight, const void* bias, void* y, long ldy, float* mean, float* rstd,
                          long rows, int n, float eps, int dtype, int wtype, fneus_stream_t stream);
@@ -641,12 +641,15 @@ long fneus_layer_norm_bwd_scratch_floats(long rows, int n);
 /* ---- linear layer with bias, activation and residual in its epilogue (beside fneus_mlp_*: those take fp32 stacks of a few hundred rows) --
  * Not in the reference.  y = act(x W^T + b) + residual for any row count, fp32, bf16 or fp16 (one type for every array), products on the
  * matrix cores with fp32 sums (fp32 operands as three bf16 terms, six products: fp32's accuracy), rounded once.  Row-major; x, residual and dy
- * have row strides in elements, any alignment; weight [n_out][n_in], y, z, dx, dweight are contiguous.
+ * have row strides in elements, any alignment; weight [n_out][n_in], y, z, dx, dweight are contiguous.  Up to 2^31 - 1 rows, 2^22 columns.
  * act: 0 none, 1 ReLU, 2 LeakyReLU(0.2), 3 sigmoid, 4 softplus(beta 100), 5 GELU (erf), 6 SiLU.
  * forward: x, weight, (bias), (residual) -> y and, where z is given, the pre-activation z [rows][n_out] (what the backward of act != 0 reads).
  * backward: dy, x, weight, z -> dx [rows][n_in], dweight [n_out][n_in], dbias [n_out], each where given (OVERWRITTEN); the residual's gradient
- * is dy.  Sums in a fixed order: bit-reproducible.  rows == 0: forward nothing, backward refused.  An fp32 infinity in an operand
- * may give NaN where it takes part.  `scratch`: fneus_linear_scratch_bytes(job, backward) bytes, 16-byte aligned, not shared between calls in flight.
+ * is dy.  Sums in a fixed order: bit-reproducible.  rows == 0: forward nothing, backward refused.  An fp32 infinity in an operand, or a value
+ * above bf16's largest (3.39e38), may give NaN where it takes part; operands below 2^-110 lose digits.
+ * Accuracy beside the rounding of the outputs: activations to 4 x 2^-23 of |z| + |act(z)|, GELU's tail to z^2 x 2e-7 of itself.  bf16 / fp16: z is kept
+ * in that type and act' taken at it, and dx and dweight are products of delta = dy act'(z) rounded to it (dbias is not); an infinite z has act's
+ * limit.  `scratch`: fneus_linear_scratch_bytes(job, backward) bytes, 16-byte aligned, not shared between calls in flight.
  * No output shares memory with another array (the residual may be x). */
 typedef struct FneusLinear {
     const void *x, *weight, *bias, *residual;
@@ -673,8 +676,9 @@ int fneus_adam(const FneusAdamSegment* segs, int n_segs, const float* lr, float*
 /* ---- optimiser of weight matrices: Muon (beside fneus_adam; not in the reference) ---------------------------------------------------------
  * Newton-Schulz orthogonalisation of each matrix u [rows][cols]: X = u / max(|u|_F, eps), `steps` times  A = X X^T, X <- a X + (b A + c A^2) X
  * (on the transpose where rows > cols).  prec 3: operands as two fp16 terms under power-of-two scales, three products (fp32's accuracy);
- * prec 2: one fp16 product (11 bits; what a 16-bit matrix carries).  Sums in fp32, the norm in fp64.  A shorter side of at most 64: fp64
- * throughout, whichever prec.  A zero matrix gives zero.  eps >= 1e-30.
+ * prec 2: one fp16 product (11 bits; what a 16-bit matrix carries: of bf16 4096 x 1024 the result is 2.0e-3 off 64 bits, 1.7e-3 of which is bf16's
+ * own rounding).  Sums in fp32, the norm in fp64.  A shorter side of at most 64: fp64 throughout, whichever prec.  A zero matrix gives zero.
+ * eps >= 1e-30, 1 to 64 steps, matrices of 1 to 65536 rows and columns.
  * fneus_newton_schulz: out = NS(grad).  fneus_muon, in place:  momentum <- mu momentum + (1 - mu) grad;  u = (1 - mu) grad + mu momentum
  * (nesterov) or momentum;  param <- param (1 - lr weight_decay) - lr adjust_j NS(u).  lr: device scalar.  dtype: of grad, momentum, param,
  * out (0 fp32, 1 bf16, 2 fp16), all contiguous.  zero_grad != 0 clears each gradient after use.  jobs: HOST array, any number; no two may
