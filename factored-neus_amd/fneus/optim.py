@@ -165,6 +165,8 @@ class FlatAdam(torch.optim.Adam):
 def _capturing(device) -> bool:
     if device.type != "cuda":
         return False
+    if device.index == torch.cuda.current_device():
+        return torch.cuda.is_current_stream_capturing()
     with torch.cuda.device(device):
         return torch.cuda.is_current_stream_capturing()
 
